@@ -55,7 +55,8 @@ enum {
     M27Q_TYPE_Q4_K = 12,
     M27Q_TYPE_Q5_K = 13,
     M27Q_TYPE_Q6_K = 14,
-    M27Q_TYPE_IQ4_XS = 23
+    M27Q_TYPE_IQ4_XS = 23,
+    M27Q_TYPE_BF16 = 30       /* activations and caches of the token mixers only */
 };
 
 /* Weight layouts in device memory.
@@ -338,6 +339,168 @@ M27Q_API m27q_status m27q_topk_noalloc(const float *logits, int n, int k, int32_
  * order, as the reference's loop. */
 M27Q_API m27q_status m27q_sample(const int32_t *idx, const float *val, int k, float temperature, float min_p,
                                  float top_p, const float *u, int32_t *token, hipStream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Token mixers: rotary positions, attention over a paged cache, the gated
+ * delta rule.  What stands between the projections of a decoder layer.
+ *
+ * Lengths, places and page tables live in device memory (a step can be
+ * replayed as a graph with new ones); the host gives their bounds.  A length
+ * or an index outside its bound is never followed: what each call does
+ * instead is said there.  Values are F32, F16 or BF16; sums, softmax
+ * statistics and states are fp32.
+ * ---------------------------------------------------------------------- */
+
+/* Rows [tokens][heads][dim] in device memory, the dim values of a head side by
+ * side, tokens and heads any (non-negative) number of values apart: a head's
+ * query can be read from a projection that gives query and gate side by side. */
+typedef struct m27q_rows {
+    void *ptr;
+    uint32_t type;          /* M27Q_TYPE_F32, _F16 or _BF16 */
+    uint32_t heads;
+    uint32_t dim;
+    uint32_t pad;
+    int64_t token_stride;   /* values from a token to the next */
+    int64_t head_stride;    /* values from a head to the next */
+} m27q_rows;
+
+/* The pages of a cache: K and V are [pages][heads][page_size][dim] each, pages
+ * page_stride values apart (K and V alike; >= heads * page_size * dim, so K
+ * and V pages may alternate in one buffer). */
+typedef struct m27q_cache {
+    void *k;
+    void *v;
+    uint32_t type;          /* M27Q_TYPE_F16 or _BF16 */
+    uint32_t pages;
+    uint32_t heads;
+    uint32_t page_size;     /* tokens a page, a power of two, 16 .. 4096 */
+    uint32_t dim;
+    uint32_t pad;
+    int64_t page_stride;
+} m27q_cache;
+
+/* The sequences of a call.  Sequence s has the rows start[s] .. start[s + 1] - 1
+ * of the call's rows (none is fine) as its newest tokens and kv_len[s] tokens
+ * in its cache with them: row t stands at place kv_len[s] - (start[s + 1] - t).
+ * Place j is in page table[s][j / page_size].  start does not descend and stays
+ * within 0 .. tokens; every sequence has at most max_q rows and max_kv tokens
+ * (bounds of the launch: rows and tokens past them are not worked on). */
+typedef struct m27q_seqs {
+    const int32_t *start;   /* device, n + 1 */
+    const int32_t *kv_len;  /* device, n */
+    const int32_t *table;   /* device, [n][table_stride] */
+    uint32_t n;
+    uint32_t table_stride;
+    uint32_t tokens;        /* rows of the call */
+    uint32_t max_q;
+    uint32_t max_kv;
+    uint32_t pad;
+} m27q_seqs;
+
+/* Which values of a head turn together: j and j + rot / 2, or 2 j and 2 j + 1. */
+enum { M27Q_ROPE_HALF = 0, M27Q_ROPE_PAIRS = 1 };
+/* How the frequencies of a trained context are stretched by `factor`. */
+enum { M27Q_ROPE_PLAIN = 0, M27Q_ROPE_LINEAR = 1, M27Q_ROPE_NTK = 2, M27Q_ROPE_YARN = 3 };
+
+/* Rotary positions: pair j < rot / 2 of a head at position p turns by p f_j,
+ * the rest of the head stays.  The frequencies are given as turns per position,
+ * f_j / (2 pi) as a 64-bit fraction of a turn, so that a position's phase is
+ * p * turns[j] modulo 2^64: exact at any position, where fp32 angles lose
+ * 2^-24 of a product that passes 10^5 radians in a long context. */
+typedef struct m27q_rope_plan {
+    const uint64_t *turns;  /* device, rot / 2, 8-byte aligned */
+    uint32_t rot;           /* even, 2 .. dim */
+    uint32_t layout;        /* M27Q_ROPE_HALF or _PAIRS */
+    float mscale;           /* cosines and sines are multiplied by it (1 for none) */
+    uint32_t pad;
+} m27q_rope_plan;
+
+/* Host, once per model: turns[rot / 2] and *mscale of f_j = base^(-2 j / rot),
+ * stretched: LINEAR f / factor; NTK base * factor^(rot / (rot - 2)) for base
+ * (rot > 2); YARN (Peng et al. 2023) f / factor for pairs that turn less than
+ * once in the `trained` tokens, f for those that turn more than 32 times, a
+ * linear blend over j between, and mscale 0.1 ln(factor) + 1.  factor >= 1;
+ * PLAIN ignores factor and trained, the others of them what they do not use.
+ * f_0 <= 1, so base >= 1.  rot even, 2 .. 1024. */
+M27Q_API m27q_status m27q_rope_turns(uint32_t rot, double base, int scaling, double factor, double trained,
+                                     uint64_t *turns, float *mscale);
+
+/* out = x rotated by pos[t] (device, tokens of them, any int32).  x and out are
+ * of one shape, in any of the types; out may be x itself (same type and
+ * strides).  Computed in fp32, rounded once.  Replaces k_mrope (exec:1147-1178)
+ * for text, where its position axes agree. */
+M27Q_API m27q_status m27q_rope(const m27q_rope_plan *rope, const int32_t *pos, int tokens, const m27q_rows *x,
+                               const m27q_rows *out, hipStream_t stream);
+
+/* One launch in front of attention: q rotated into q_out, k rotated and v as it
+ * is into their places in the cache (rounded to the cache's type).  q and q_out
+ * as in m27q_rope; k and v have the cache's heads and dim, any type.  A row of no
+ * sequence, or whose place is negative or past table_stride * page_size, or
+ * whose table entry is outside 0 .. pages - 1, is not written to the cache (its
+ * query is rotated all the same).  Replaces k_mrope_and_cache (exec:1180-1229),
+ * whose cache is one fp32 buffer per layer. */
+M27Q_API m27q_status m27q_rope_append(const m27q_rope_plan *rope, const int32_t *pos, const m27q_seqs *seqs,
+                                      const m27q_cache *cache, const m27q_rows *q, const m27q_rows *q_out,
+                                      const m27q_rows *k, const m27q_rows *v, hipStream_t stream);
+
+/* Attention of every sequence's rows over its pages: row t at place i, head h of
+ * q.heads, with the keys and values of cache head h / (q.heads / cache.heads)
+ * at the places j <= i (window > 0: and j > i - window):
+ *   out = sum_j p_j v_j / sum_j p_j,  p_j = e^(scale q.k_j - max).
+ * q has the cache's type and dim (64, 128 or 256), out that type or F32; q.heads
+ * is a multiple of cache.heads, at most 64 for each.  A row that sees no key
+ * gives zeros; rows of no sequence are not written.  Keys whose table entry is
+ * outside 0 .. pages - 1 are left out, as if masked; nothing of a masked key or
+ * value is used, be it NaN.  Products are MFMA on the cache's type with fp32
+ * sums; the weights p are rounded to it for the second product, for an F32
+ * output as the sum of two (F16) or three (BF16) such values.
+ * scratch (16-byte aligned) >= m27q_attn_scratch_bytes, whose bound holds for
+ * any lengths within the seqs' bounds; what it holds is of no matter.
+ * Replaces k_attn_decode_split_partial / _reduce (exec:1339-1484), one token
+ * over one sequence. */
+M27Q_API size_t m27q_attn_scratch_bytes(const m27q_seqs *seqs, uint32_t q_heads, const m27q_cache *cache);
+M27Q_API m27q_status m27q_attn_paged(const m27q_seqs *seqs, const m27q_cache *cache, const m27q_rows *q,
+                                     const m27q_rows *out, float scale, int window, void *scratch,
+                                     size_t scratch_bytes, hipStream_t stream);
+
+/* Which key head a value head of the delta rule goes with: h / (heads / k heads),
+ * or h modulo k heads (the order of GGUF files). */
+enum { M27Q_HEADS_GROUPED = 0, M27Q_HEADS_CYCLED = 1 };
+
+/* The gated delta rule.  For each sequence (rows start[s] .. start[s + 1] - 1, in
+ * order) and each head h of v, on a state S[dv][dk]:
+ *   S <- e^g S;  u = beta (v - S k);  S <- S + u k^T;  out = scale S q.
+ * q and k: k_heads of dk (64 or 128); v and out: heads (a multiple of k_heads) of
+ * dv (a multiple of 16, 16 .. 256); q, k, v and out of one type; g and beta fp32
+ * [tokens][heads] without gaps.  States are fp32 [slots][heads][dv][dk]; sequence s starts
+ * from slot slots[s] (slots NULL: s) of state_in and ends in that slot of
+ * state_out, which may be state_in.  state_in NULL, or a slot outside
+ * 0 .. n_slots - 1, starts from zeros; such a slot is not written, nor is
+ * anything where state_out is NULL.  Two sequences of a call need two slots.  A sequence without
+ * rows keeps its state (copied where state_out is another buffer).
+ * g = -infinity clears the state.  Replaces k_deltanet_ggml (exec:1525-1670). */
+typedef struct m27q_delta {
+    const int32_t *start;   /* device, n + 1; ascending within 0 .. tokens */
+    const int32_t *slots;   /* device, n, or NULL */
+    const float *g;
+    const float *beta;
+    const float *state_in;
+    float *state_out;
+    m27q_rows q, k, v, out;
+    uint32_t n;
+    uint32_t tokens;
+    uint32_t max_len;       /* rows of the longest sequence, at least */
+    uint32_t n_slots;
+    uint32_t head_map;      /* M27Q_HEADS_* */
+    float scale;
+} m27q_delta;
+
+/* scratch (16-byte aligned) >= m27q_delta_scratch_bytes; what it holds is of no
+ * matter.  Few rows go through the rule row by row, more in chunks of 64 as
+ * triangular systems, with fp32-accurate products throughout. */
+M27Q_API size_t m27q_delta_scratch_bytes(uint32_t n, uint32_t tokens, uint32_t max_len, uint32_t heads, uint32_t dk,
+                                         uint32_t dv);
+M27Q_API m27q_status m27q_delta_rule(const m27q_delta *d, void *scratch, size_t scratch_bytes, hipStream_t stream);
 
 #ifdef __cplusplus
 }

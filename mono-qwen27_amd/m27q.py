@@ -18,8 +18,11 @@ ROOT = os.path.dirname(PKG_DIR)
 LIB_PATH = os.path.join(PKG_DIR, "libm27q.so")
 HEADER = os.path.join(ROOT, "include", "m27q.h")
 
-F32, F16, Q8_0, Q4_K, Q5_K, Q6_K, IQ4_XS = 0, 1, 8, 12, 13, 14, 23
+F32, F16, Q8_0, Q4_K, Q5_K, Q6_K, IQ4_XS, BF16 = 0, 1, 8, 12, 13, 14, 23, 30
 GGUF, TILED = 0, 1
+ROPE_HALF, ROPE_PAIRS = 0, 1
+ROPE_PLAIN, ROPE_LINEAR, ROPE_NTK, ROPE_YARN = 0, 1, 2, 3
+HEADS_GROUPED, HEADS_CYCLED = 0, 1
 BLOCK_ELEMS = {F32: 1, F16: 1, Q8_0: 32, Q4_K: 256, Q5_K: 256, Q6_K: 256, IQ4_XS: 256}
 BLOCK_BYTES = {F32: 4, F16: 2, Q8_0: 34, Q4_K: 144, Q5_K: 176, Q6_K: 210, IQ4_XS: 136}
 
@@ -44,6 +47,40 @@ class BlobTensor(C.Structure):
                 ("role", C.c_uint32), ("row_elems", C.c_uint32), ("row_count", C.c_uint32),
                 ("layout", C.c_uint32), ("row_blocks", C.c_uint32), ("pad", C.c_uint32),
                 ("file_offset", C.c_uint64), ("bytes", C.c_uint64)]
+
+
+class Rows(C.Structure):
+    """m27q_rows: [tokens][heads][dim] values, tokens and heads any distance apart."""
+    _fields_ = [("ptr", C.c_void_p), ("type", C.c_uint32), ("heads", C.c_uint32), ("dim", C.c_uint32),
+                ("pad", C.c_uint32), ("token_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
+class RopePlan(C.Structure):
+    """m27q_rope_plan"""
+    _fields_ = [("turns", C.c_void_p), ("rot", C.c_uint32), ("layout", C.c_uint32), ("mscale", C.c_float),
+                ("pad", C.c_uint32)]
+
+
+class CacheDesc(C.Structure):
+    """m27q_cache"""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("type", C.c_uint32), ("pages", C.c_uint32),
+                ("heads", C.c_uint32), ("page_size", C.c_uint32), ("dim", C.c_uint32), ("pad", C.c_uint32),
+                ("page_stride", C.c_int64)]
+
+
+class SeqsDesc(C.Structure):
+    """m27q_seqs"""
+    _fields_ = [("start", C.c_void_p), ("kv_len", C.c_void_p), ("table", C.c_void_p), ("n", C.c_uint32),
+                ("table_stride", C.c_uint32), ("tokens", C.c_uint32), ("max_q", C.c_uint32), ("max_kv", C.c_uint32),
+                ("pad", C.c_uint32)]
+
+
+class DeltaDesc(C.Structure):
+    """m27q_delta"""
+    _fields_ = [("start", C.c_void_p), ("slots", C.c_void_p), ("g", C.c_void_p), ("beta", C.c_void_p),
+                ("state_in", C.c_void_p), ("state_out", C.c_void_p), ("q", Rows), ("k", Rows), ("v", Rows),
+                ("out", Rows), ("n", C.c_uint32), ("tokens", C.c_uint32), ("max_len", C.c_uint32),
+                ("n_slots", C.c_uint32), ("head_map", C.c_uint32), ("scale", C.c_float)]
 
 
 _P, _I, _SZ, _U32 = C.c_void_p, C.c_int, C.c_size_t, C.c_uint32
@@ -77,7 +114,18 @@ _SIGS = {
     "m27q_topk": (_I, [_P, _I, _I, _P, _P, _P, _SZ, _P]),
     "m27q_topk_noalloc": (_I, [_P, _I, _I, _P, _P, _P]),
     "m27q_sample": (_I, [_P, _P, _I, C.c_float, C.c_float, C.c_float, _P, _P, _P]),
+    "m27q_rope_turns": (_I, [_U32, C.c_double, _I, C.c_double, C.c_double, _P, C.POINTER(C.c_float)]),
+    "m27q_rope": (_I, [C.POINTER(RopePlan), _P, _I, C.POINTER(Rows), C.POINTER(Rows), _P]),
+    "m27q_rope_append": (_I, [C.POINTER(RopePlan), _P, C.POINTER(SeqsDesc), C.POINTER(CacheDesc)]
+                         + [C.POINTER(Rows)] * 4 + [_P]),
+    "m27q_attn_scratch_bytes": (_SZ, [C.POINTER(SeqsDesc), _U32, C.POINTER(CacheDesc)]),
+    "m27q_attn_paged": (_I, [C.POINTER(SeqsDesc), C.POINTER(CacheDesc), C.POINTER(Rows), C.POINTER(Rows), C.c_float,
+                             _I, _P, _SZ, _P]),
+    "m27q_delta_scratch_bytes": (_SZ, [_U32] * 6),
+    "m27q_delta_rule": (_I, [C.POINTER(DeltaDesc), _P, _SZ, _P]),
 }
+# What the wrappers pass as packed bytes.
+_PACKED = tuple(C.POINTER(t) for t in (WeightDesc, C.c_void_p, Rows, RopePlan, CacheDesc, SeqsDesc, DeltaDesc))
 
 _lib = _fast = None
 
@@ -103,16 +151,16 @@ class _Calls:
 
 
 def _calls() -> _Calls:
-    """The entry points as the wrappers below call them: where lib() takes weight
-    records or arrays of pointers by type, these take any pointer (c_void_p), so
-    that the wrappers can pass packed bytes."""
+    """The entry points as the wrappers below call them: where lib() takes records
+    or arrays of pointers by type, these take any pointer (c_void_p), so that the
+    wrappers can pass packed bytes."""
     global _fast
     if _fast is None:
         L, c = lib(), _Calls()
         for name, (res, args) in _SIGS.items():
             f = L[name]  # a function object of its own, not lib()'s
             f.restype = res
-            f.argtypes = [_P if a in (C.POINTER(WeightDesc), C.POINTER(_P)) else a for a in args]
+            f.argtypes = [_P if a in _PACKED else a for a in args]
             setattr(c, name, f)
         _fast = c
     return _fast
@@ -416,3 +464,154 @@ def topk_noalloc(logits, k: int, idx, val, stream=None) -> None:
     """m27q_topk on the library's static scratch (no scratch argument)."""
     check((_fast or _calls()).m27q_topk_noalloc(_ptr(logits), logits.numel(), k, _ptr(idx), _ptr(val),
                                                 _stream(stream)), "m27q_topk_noalloc")
+
+
+# ---------------------------------------------------------- token mixers --
+
+_pack_rows = struct.Struct("=QIIIIqq").pack   # m27q_rows
+_pack_delta = struct.Struct("=6Q40s40s40s40s5If").pack  # m27q_delta
+_value_types = None
+
+
+def _type_of(t) -> int:
+    global _value_types
+    if _value_types is None:
+        torch = _torch()
+        _value_types = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+    return _value_types.get(t.dtype, 0xffffffff)  # others: for the library to refuse
+
+
+def _rows(t, tokens: int, what: str):
+    """A [tokens, heads, dim] tensor as its m27q_rows record."""
+    n, h, d = t.shape
+    a, b, c = t.stride()
+    if n != tokens or (c != 1 and d != 1):
+        raise M27QError(2, what)
+    return _pack_rows(t.data_ptr(), _type_of(t), h, d, 0, a, b)
+
+
+def _int32(t, what: str):
+    torch = _torch()
+    if t.dtype != torch.int32 or not t.is_contiguous():
+        raise M27QError(4, what)
+    return t.data_ptr()
+
+
+def rope_turns(rot: int, base: float, scaling: int = ROPE_PLAIN, factor: float = 1.0, trained: float = 0.0):
+    """Turns per position of each pair as 64-bit fractions (numpy uint64), and mscale (host only)."""
+    out, m = np.empty(max(1, rot // 2), np.uint64), C.c_float()
+    check(lib().m27q_rope_turns(rot, base, scaling, factor, trained, out.ctypes.data, C.byref(m)), "m27q_rope_turns")
+    return out, m.value
+
+
+class Rope:
+    """A model's rotary positions (m27q_rope_plan): turns as a device tensor of rot / 2 int64 values."""
+
+    def __init__(self, turns, rot: int, layout: int = ROPE_HALF, mscale: float = 1.0):
+        torch = _torch()
+        if turns.dtype != torch.int64 or not turns.is_contiguous() or 2 * turns.numel() < rot:
+            raise M27QError(4, "Rope")
+        self.turns = turns
+        self.packed = bytes(RopePlan(turns.data_ptr(), rot, layout, mscale, 0))
+
+    @staticmethod
+    def make(rot: int, base: float, layout: int = ROPE_HALF, scaling: int = ROPE_PLAIN, factor: float = 1.0,
+             trained: float = 0.0, device="cuda"):
+        turns, mscale = rope_turns(rot, base, scaling, factor, trained)
+        return Rope(_torch().from_numpy(turns.view(np.int64)).to(device), rot, layout, mscale)
+
+
+class KVCache:
+    """The pages of a layer's cache: k and v [pages, heads, page_size, dim], float16 or bfloat16.  Pages may lie
+    further apart than they are long."""
+
+    def __init__(self, k, v):
+        pages, heads, size, dim = k.shape
+        if v.shape != k.shape or v.stride() != k.stride() or v.dtype != k.dtype:
+            raise M27QError(2, "KVCache")
+        if k.stride()[1:] != (size * dim, dim, 1):
+            raise M27QError(4, "KVCache")
+        self.k, self.v, self.page_size = k, v, size
+        self.packed = bytes(CacheDesc(k.data_ptr(), v.data_ptr(), _type_of(k), pages, heads, size, dim, 0,
+                                      k.stride(0)))
+
+
+class Seqs:
+    """The sequences of a call (m27q_seqs): start [n + 1], kv_len [n], table [n, pages a sequence], int32 device
+    tensors whose contents may change from call to call; the rows of the call and the bounds max_q and max_kv."""
+
+    def __init__(self, start, kv_len, table, tokens: int, max_q: int, max_kv: int):
+        n, stride = table.shape
+        if start.numel() != n + 1 or kv_len.numel() != n:
+            raise M27QError(2, "Seqs")
+        self.start, self.kv_len, self.table, self.tokens = start, kv_len, table, tokens
+        self.packed = bytes(SeqsDesc(_int32(start, "Seqs"), _int32(kv_len, "Seqs"), _int32(table, "Seqs"), n, stride,
+                                     tokens, max_q, max_kv, 0))
+
+
+def rope(rope: Rope, pos, x, out, stream=None) -> None:
+    """out <- x rotated by pos; x and out [tokens, heads, dim]."""
+    n = pos.numel()
+    st = (_fast or _calls()).m27q_rope(rope.packed, _int32(pos, "m27q_rope"), n, _rows(x, n, "m27q_rope"),
+                                       _rows(out, n, "m27q_rope"), _stream(stream))
+    if st:
+        check(st, "m27q_rope")
+
+
+def rope_append(rope: Rope, pos, seqs: Seqs, cache: KVCache, q, q_out, k, v, stream=None) -> None:
+    """q_out <- q rotated; k rotated and v into the cache; q, k, v [tokens, heads, dim]."""
+    n = seqs.tokens
+    if pos.numel() != n:
+        raise M27QError(2, "m27q_rope_append")
+    st = (_fast or _calls()).m27q_rope_append(
+        rope.packed, _int32(pos, "m27q_rope_append"), seqs.packed, cache.packed, _rows(q, n, "m27q_rope_append"),
+        _rows(q_out, n, "m27q_rope_append"), _rows(k, n, "m27q_rope_append"), _rows(v, n, "m27q_rope_append"),
+        _stream(stream))
+    if st:
+        check(st, "m27q_rope_append")
+
+
+def attn_scratch_bytes(seqs: Seqs, q_heads: int, cache: KVCache) -> int:
+    return (_fast or _calls()).m27q_attn_scratch_bytes(seqs.packed, q_heads, cache.packed)
+
+
+def attn_paged(seqs: Seqs, cache: KVCache, q, out, scratch, scale: float, window: int = 0, stream=None) -> None:
+    """out <- attention of the rows q [tokens, heads, dim] over their sequences' pages."""
+    n = seqs.tokens
+    st = (_fast or _calls()).m27q_attn_paged(
+        seqs.packed, cache.packed, _rows(q, n, "m27q_attn_paged"), _rows(out, n, "m27q_attn_paged"), scale, window,
+        scratch.data_ptr(), scratch.numel() * scratch.element_size(), _stream(stream))
+    if st:
+        check(st, "m27q_attn_paged")
+
+
+def delta_scratch_bytes(n: int, tokens: int, max_len: int, heads: int, dk: int, dv: int) -> int:
+    return lib().m27q_delta_scratch_bytes(n, tokens, max_len, heads, dk, dv)
+
+
+def delta_rule(start, q, k, v, g, beta, state, state_out, out, scratch, scale: float, max_len: int, slots=None,
+               head_map: int = HEADS_GROUPED, stream=None) -> None:
+    """The gated delta rule over each sequence's rows: out and state_out <- rows from state [slots, heads, dv, dk]
+    (state or state_out may be None, state_out may be state)."""
+    what = "m27q_delta_rule"
+    torch = _torch()
+    n, h, dv = v.shape
+    held = state if state is not None else state_out
+    shape = (held.shape[0] if held is not None else 0, h, dv, k.shape[2])
+    for s in (state, state_out):
+        if s is not None and (s.shape != shape or s.dtype != torch.float32 or not s.is_contiguous()):
+            raise M27QError(2, what)
+    for x in (g, beta):
+        if x.shape != (n, h) or x.dtype != torch.float32 or not x.is_contiguous():
+            raise M27QError(2, what)
+    seqs = start.numel() - 1
+    if slots is not None and slots.numel() != seqs:
+        raise M27QError(2, what)
+    d = _pack_delta(_int32(start, what), 0 if slots is None else _int32(slots, what), g.data_ptr(), beta.data_ptr(),
+                    0 if state is None else state.data_ptr(), 0 if state_out is None else state_out.data_ptr(),
+                    _rows(q, n, what), _rows(k, n, what), _rows(v, n, what), _rows(out, n, what), seqs, n, max_len,
+                    shape[0], head_map, scale)
+    st = (_fast or _calls()).m27q_delta_rule(d, scratch.data_ptr(), scratch.numel() * scratch.element_size(),
+                                             _stream(stream))
+    if st:
+        check(st, what)
