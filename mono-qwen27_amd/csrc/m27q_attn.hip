@@ -289,16 +289,17 @@ __global__ __launch_bounds__(kWaves * 64, 2) void k_attn(const AttnParams p) {
     __shared__ __attribute__((aligned(1024))) char kt0[kKeys * D * 2], vt0[kKeys * D * 2];
     __shared__ __attribute__((aligned(1024))) char kt1[kKeys * D * 2], vt1[kKeys * D * 2];
     const int group = (int)(p.q.heads / p.cache.heads);
-    // workgroups of one (sequence, head) are gridDim.x apart in dispatch order, so that
+    // workgroups of one (sequence, head) are seqs * heads apart in dispatch order, so that
     // where that is a multiple of the XCDs they share an L2; the last rows see the most keys
     // and go first
-    const int s = blockIdx.x / p.cache.heads;
+    const unsigned pairs = p.seqs.n * p.cache.heads, fromlast = blockIdx.x / pairs, pair = blockIdx.x - fromlast * pairs;
+    const int s = pair / p.cache.heads;
     Work w;
     w.s = s;
-    w.head = blockIdx.x - s * p.cache.heads;
+    w.head = pair - s * p.cache.heads;
     const SeqRows sr = seq_rows(p.seqs.start, s, (int)p.seqs.tokens, (int)p.seqs.max_q);
     w.rows = sr.count * group;
-    w.row0 = (int)(gridDim.y - 1 - blockIdx.y) * kWaves * kRows;
+    w.row0 = (int)(gridDim.x / pairs - 1 - fromlast) * kWaves * kRows;
     if (w.row0 >= w.rows) return;
     const int kv = min(max(p.seqs.kv_len[s], 0), (int)p.seqs.max_kv);
     const int place0 = p.seqs.kv_len[s] - (sr.end - sr.first);  // of the sequence's first row
@@ -309,7 +310,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void k_attn(const AttnParams p) {
     if (p.splits > 1) {
         const int tiles = max(0, hi - lo + kKeys - 1) / kKeys;
         const int each = (tiles + p.splits - 1) / p.splits;
-        lo += (int)blockIdx.z * each * kKeys;
+        lo += (int)blockIdx.y * each * kKeys;
         hi = min(hi, lo + each * kKeys);
     }
     w.lo = lo;
@@ -405,7 +406,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void k_attn(const AttnParams p) {
     x.l = sum_halves(x.l);
     if (!live) return;
     if (p.splits > 1) {
-        const long long at = ((long long)token * p.q.heads + qh) * p.splits + blockIdx.z;
+        const long long at = ((long long)token * p.q.heads + qh) * p.splits + blockIdx.y;
         if (h == 0) p.stat[at] = make_float2(x.m * sc, x.l);
         if (x.l == 0) return;
         float *o = p.part + at * D;
@@ -461,10 +462,18 @@ __global__ __launch_bounds__(256) void k_attn_join(const AttnParams p) {
     else *(f16x4 *)((_Float16 *)p.out.ptr + to) = __builtin_convertvector(o, f16x4);
 }
 
+}  // namespace
+
+long long attn_groups(const m27q_seqs &seqs, uint32_t q_heads, const m27q_cache &cache) {
+    const long long rows = (long long)seqs.max_q * (q_heads / cache.heads);
+    return (rows + kWaves * kRows - 1) / (kWaves * kRows) * seqs.n * cache.heads;
+}
+
+namespace {
+
 template <int D, bool BF>
 hipError_t launch_t(const AttnParams &p, const AttnPlan &plan, hipStream_t s) {
-    const int group = (int)(p.q.heads / p.cache.heads);
-    const dim3 grid(p.seqs.n * p.cache.heads, (p.seqs.max_q * group + kWaves * kRows - 1) / (kWaves * kRows), p.splits);
+    const dim3 grid((unsigned)attn_groups(p.seqs, p.q.heads, p.cache), p.splits);
     constexpr int NP = BF ? 3 : 2;
     if (p.out.type == M27Q_TYPE_F32) hipLaunchKernelGGL((k_attn<D, BF, NP>), grid, dim3(kWaves * 64), 0, s, p);
     else hipLaunchKernelGGL((k_attn<D, BF, 1>), grid, dim3(kWaves * 64), 0, s, p);
@@ -480,8 +489,7 @@ hipError_t launch_t(const AttnParams &p, const AttnPlan &plan, hipStream_t s) {
 
 // Parts of the keys: enough workgroups for two on each CU, parts of 256 keys at least.
 AttnPlan attn_plan(const m27q_seqs &seqs, uint32_t q_heads, const m27q_cache &cache, int cus) {
-    const long long rows = (long long)seqs.max_q * (q_heads / cache.heads);
-    const long long wgs = (rows + kWaves * kRows - 1) / (kWaves * kRows) * seqs.n * cache.heads;
+    const long long wgs = attn_groups(seqs, q_heads, cache);
     const long long want = (2ll * cus + wgs - 1) / wgs, most = (seqs.max_kv + 255) / 256;
     long long splits = want < most ? want : most;
     if (splits > kMaxSplits) splits = kMaxSplits;

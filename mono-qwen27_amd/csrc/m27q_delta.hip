@@ -92,16 +92,444 @@ __global__ __launch_bounds__(64) void k_delta_rows(const m27q_delta d) {
     }
 }
 
+// ---------------------------------------------------------------- chunks --
+//
+// C = 64 rows at a time.  With G_i the sum of g over the chunk's rows up to i,
+// the rule within a chunk that starts from S is
+//   (I + A) U = diag(beta) (V - diag(e^G) K S^T),
+//       A_ij = beta_i e^(G_i - G_j) k_i.k_j   for j < i,
+//   out = scale diag(e^G) Q S^T + P U,  P_ij = scale e^(G_i - G_j) q_i.k_j  for j <= i,
+//   S <- e^(G_C) S + (diag(e^(G_C - G)) U)^T K.
+// A first launch, parallel over chunks, makes T = (I + A)^-1 diag(beta), P and the
+// factors; a second one walks the chunks of a sequence with 32 rows of a head's
+// state, 4 waves: three products that wait for each other a chunk, the state in
+// accumulators throughout.
+//
+// Products are fp32-accurate on the bf16 matrix units, 16 times the rate of the
+// fp32 ones: a value is the sum of three bf16 values (8 + 8 + 8 bits; F16 takes
+// two, BF16 one) and a product the six partial products above 2^-24 of it, which
+// is 6 / 16 of the fp32 instructions' time.
+
+constexpr int kC = 64;       // rows of a chunk
+constexpr int kSlice = 32;   // state rows of a workgroup
+
+template <typename T>
+struct In;  // an input type's values as bf16 pieces
+template <>
+struct In<float> {
+    static constexpr int N = 3;
+    typedef f32x8a raw;
+};
+template <>
+struct In<_Float16> {
+    static constexpr int N = 2;
+    typedef f16x8 raw;
+};
+template <>
+struct In<__bf16> {
+    static constexpr int N = 1;
+    typedef bf16x8 raw;
+};
+
+// x as N bf16 values each, rounded to nearest: what the ones before leave over.
+template <int N>
+__device__ __forceinline__ void split(f32x8 x, bf16x8 (&p)[N]) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        p[j] = __builtin_convertvector(x, bf16x8);
+        if (j + 1 < N) x -= __builtin_convertvector(p[j], f32x8);
+    }
+}
+template <int N>
+__device__ __forceinline__ void split(f32x4 x, bf16x4 (&p)[N]) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        p[j] = __builtin_convertvector(x, bf16x4);
+        if (j + 1 < N) x -= __builtin_convertvector(p[j], f32x4);
+    }
+}
+
+// c += a b over a 16x16 tile and 32 of the contraction, the smallest parts first.
+template <int NA, int NB>
+__device__ __forceinline__ f32x4 mma(const bf16x8 (&a)[NA], const bf16x8 (&b)[NB], f32x4 c) {
+#pragma unroll
+    for (int o = 2; o >= 0; --o)
+#pragma unroll
+        for (int i = 0; i < NA; ++i)
+            if (o - i >= 0 && o - i < NB) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[o - i], c, 0, 0, 0);
+    return c;
+}
+
+#define LDS_AS __attribute__((address_space(3)))
+
+// What the first launch leaves for a chunk and a head, in floats.
+constexpr int kT = 0, kP = kC * kC, kEg = 2 * kC * kC, kEc = kEg + kC, kLast = kEc + kC, kRecord = kLast + 64;
+
+// The place of a sequence's first chunk among all: places do not meet, as a
+// sequence has at most one chunk more than whole ones.
+__device__ __forceinline__ long long chunk_place(int first, int s) { return first / kC + s; }
+
+// The sequence's 16 rows from t0 as operand rows: lane m = lane % 16, values
+// 32 i + 8 (lane / 16) + 0 .. 7 of row t0 + m; zeros past the end.
+template <int DK, typename T>
+__device__ __forceinline__ void load_rows(const m27q_rows &r, long long first, int head, int t0, int count,
+                                          typename In<T>::raw (&x)[DK / 32]) {
+    const int lane = threadIdx.x & 63, t = t0 + (lane & 15);
+    const T *p = (const T *)r.ptr + (first + t) * r.token_stride + (long long)head * r.head_stride + 8 * (lane >> 4);
+#pragma unroll
+    for (int i = 0; i < DK / 32; ++i) {
+        x[i] = typename In<T>::raw{};
+        if (t < count) x[i] = *(const typename In<T>::raw *)(p + 32 * i);
+    }
+}
+template <typename T>
+__device__ __forceinline__ void pieces(typename In<T>::raw x, bf16x8 (&p)[In<T>::N]) {
+    if constexpr (In<T>::N == 1) p[0] = x;
+    else split<In<T>::N>(__builtin_convertvector(x, f32x8), p);
+}
+
+template <int DK, typename T>
+__global__ __launch_bounds__(256) void k_delta_prepare(const m27q_delta d, float *scratch) {
+    constexpr int N = In<T>::N, KS = DK / 32, LD = DK + 16, LM = kC + 1;
+    constexpr size_t planes = sizeof(__bf16) * N * kC * LD, mats = sizeof(float) * 2 * kC * LM;
+    __shared__ __attribute__((aligned(16))) char mem[planes > mats ? planes : mats];
+    __shared__ double G[kC];
+    __shared__ float B[kC];
+    __bf16 *kp = (__bf16 *)mem;                          // K's pieces, [N][kC][LD]
+    float *Am = (float *)mem, *Xm = Am + kC * LM;        // then A and the inverse of I + A
+    const int s = blockIdx.z, head = blockIdx.y, t0 = blockIdx.x * kC;
+    const SeqRows sr = seq_rows(d.start, s, (int)d.tokens, (int)d.max_len);
+    if (t0 >= sr.count) return;
+    const int kh = d.head_map == M27Q_HEADS_CYCLED ? head % (int)d.k.heads : head / (int)(d.v.heads / d.k.heads);
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    float *rec = scratch + ((chunk_place(sr.first, s) + blockIdx.x) * d.v.heads + head) * (long long)kRecord;
+
+    bf16x8 ka[KS][N], qa[KS][N];
+    {
+        typename In<T>::raw x[KS], y[KS];
+        load_rows<DK, T>(d.k, sr.first, kh, t0 + 16 * wave, sr.count, x);
+        load_rows<DK, T>(d.q, sr.first, kh, t0 + 16 * wave, sr.count, y);
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+            pieces<T>(x[i], ka[i]);
+            pieces<T>(y[i], qa[i]);
+#pragma unroll
+            for (int j = 0; j < N; ++j) *(bf16x8 *)(kp + (j * kC + 16 * wave + n) * LD + 32 * i + 8 * g) = ka[i][j];
+        }
+    }
+    if (wave == 0) {  // sums of g in 64 bits: differences of them are taken below
+        const bool in = t0 + lane < sr.count;
+        const long long at = (long long)(sr.first + t0 + lane) * d.v.heads + head;
+        const float gf = in ? d.g[at] : 0.0f;
+        double x = gf < -1e4f ? -1e4 : (double)gf;  // e^-10000 is 0 as e^-inf is, and no inf - inf
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const double y = __shfl_up(x, o);
+            x += lane >= o ? y : 0.0;
+        }
+        const double last = __shfl(x, 63);
+        G[lane] = x;
+        B[lane] = in ? d.beta[at] : 0.0f;
+        rec[kEg + lane] = expf((float)x);
+        rec[kEc + lane] = expf((float)(last - x));
+        if (lane == 0) rec[kLast] = expf((float)last);
+    }
+    __syncthreads();
+
+    f32x4 kk[4], qk[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        kk[j] = qk[j] = f32x4{};
+        if (j > wave) continue;
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+            bf16x8 b[N];
+#pragma unroll
+            for (int u = 0; u < N; ++u) b[u] = *(const bf16x8 *)(kp + (u * kC + 16 * j + n) * LD + 32 * i + 8 * g);
+            kk[j] = mma<N, N>(ka[i], b, kk[j]);
+            qk[j] = mma<N, N>(qa[i], b, qk[j]);
+        }
+    }
+    __syncthreads();  // K's pieces make room
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int row = 16 * wave + 4 * g + i, col = 16 * j + n;
+            float a = 0, p = 0;
+            if (col <= row) {
+                const float e = expf((float)(G[row] - G[col]));
+                p = d.scale * e * qk[j][i];
+                if (col < row) a = B[row] * e * kk[j][i];
+            }
+            Am[row * LM + col] = a;
+            Xm[row * LM + col] = 0;
+            rec[kP + row * kC + col] = p;
+        }
+    __syncthreads();
+    // the inverse's 16x16 blocks: on the diagonal by forward substitution, a column a lane
+    const int r0 = 16 * wave;
+    if (lane < 16) {
+        float x[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            float v = i == lane ? 1.0f : 0.0f;
+#pragma unroll
+            for (int k = 0; k < i; ++k) v = __builtin_fmaf(-Am[(r0 + i) * LM + r0 + k], x[k], v);
+            x[i] = v;
+            Xm[(r0 + i) * LM + r0 + lane] = v;
+        }
+    }
+    // below it by diagonals: X_ij = -X_ii sum_(j <= k < i) A_ik X_kj.  The sum's rows lie
+    // in the lanes as 4 g + t, so the second product takes X_ii's columns in that order.
+#pragma unroll
+    for (int o = 1; o < 4; ++o) {
+        __syncthreads();
+        if (wave < o) continue;
+        const int c0 = 16 * (wave - o);
+        f32x4 y = {}, x = {};
+        for (int k0 = c0; k0 < r0; k0 += 4)
+            y = __builtin_amdgcn_mfma_f32_16x16x4f32(Am[(r0 + n) * LM + k0 + g], Xm[(k0 + g) * LM + c0 + n], y, 0, 0, 0);
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+            x = __builtin_amdgcn_mfma_f32_16x16x4f32(-Xm[(r0 + n) * LM + r0 + 4 * g + t], y[t], x, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) Xm[(r0 + 4 * g + i) * LM + c0 + n] = x[i];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < kC * kC; i += 256) rec[kT + i] = Xm[(i / kC) * LM + i % kC] * B[i % kC];
+}
+
+// One chunk's inputs in the registers of its lanes.
+template <int DK, typename T>
+struct Chunk {
+    typename In<T>::raw k[DK / 32], q[DK / 32];
+    f32x8 t[2], p[2];     // rows 16 wave + lane % 16 of T and P
+    float v[2][4];        // V at rows 16 wave + 4 (lane / 16) + i, values lane % 16 and 16 + that of the slice
+    float eg[4], ec[4], last;
+
+    __device__ __forceinline__ void load(const m27q_delta &d, const float *rec, const SeqRows &sr, int head, int kh,
+                                         int t0, int v0) {
+        const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+        load_rows<DK, T>(d.k, sr.first, kh, t0 + 16 * wave, sr.count, k);
+        load_rows<DK, T>(d.q, sr.first, kh, t0 + 16 * wave, sr.count, q);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            t[i] = *(const f32x8a *)(rec + kT + (16 * wave + n) * kC + 32 * i + 8 * g);
+            p[i] = *(const f32x8a *)(rec + kP + (16 * wave + n) * kC + 32 * i + 8 * g);
+        }
+        const int row = 16 * wave + 4 * g;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            eg[i] = rec[kEg + row + i];
+            ec[i] = rec[kEc + row + i];
+            const T *x = (const T *)d.v.ptr + (long long)(sr.first + t0 + row + i) * d.v.token_stride +
+                         (long long)head * d.v.head_stride + v0 + n;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) v[j][i] = t0 + row + i < sr.count && v0 + 16 * j < (int)d.v.dim ? (float)x[16 * j] : 0.0f;
+        }
+        last = rec[kLast];
+    }
+};
+
+template <int DK, typename T>
+__global__ __launch_bounds__(256, 1) void k_delta_chunks(const m27q_delta d, const float *scratch) {
+    constexpr int N = In<T>::N, KS = DK / 32, MT = DK / 64;
+    constexpr int LK = DK + 16, LS = DK + 8, LU = kC + 8;
+    __shared__ __attribute__((aligned(16))) __bf16 kp[N * kC * LK];       // K's pieces [N][row][dk]
+    __shared__ __attribute__((aligned(16))) __bf16 sb[3 * kSlice * LS];   // the state's [3][dv][dk]
+    __shared__ __attribute__((aligned(16))) __bf16 rb[3 * kSlice * LU];   // the right-hand sides' [3][dv][row]
+    __shared__ __attribute__((aligned(16))) __bf16 ub[3 * kSlice * LU];   // U's
+    __shared__ __attribute__((aligned(16))) __bf16 wb[3 * kSlice * LU];   // diag(e^(G_C - G)) U's
+    // workgroups of one key head and sequence are gridDim.x apart, so that where that is a
+    // multiple of the XCDs they share an L2
+    const int kheads = (int)d.k.heads, per = (int)d.v.heads / kheads, slices = (int)(d.v.dim + kSlice - 1) / kSlice;
+    const int s = blockIdx.x / kheads, kh = blockIdx.x - s * kheads;
+    const int which = blockIdx.y / slices, v0 = (blockIdx.y - which * slices) * kSlice;
+    const int head = d.head_map == M27Q_HEADS_CYCLED ? which * kheads + kh : kh * per + which;
+    const SeqRows sr = seq_rows(d.start, s, (int)d.tokens, (int)d.max_len);
+    const int slot = d.slots ? d.slots[s] : s;
+    const bool held = slot >= 0 && (uint32_t)slot < d.n_slots;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    const float *rec = scratch + (chunk_place(sr.first, s) * d.v.heads + head) * (long long)kRecord;
+    const long long step = (long long)d.v.heads * kRecord;
+
+    // the state: dk = 16 (MT wave + m) + 4 g + i of rows v0 + 16 j + n
+    f32x4 S[MT][2];
+    const long long at = (((long long)slot * d.v.heads + head) * d.v.dim + v0 + n) * DK + 16 * MT * wave + 4 * g;
+    const bool in[2] = {v0 < (int)d.v.dim, v0 + 16 < (int)d.v.dim};
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            S[m][j] = f32x4{};
+            if (held && d.state_in && in[j]) S[m][j] = *(const f32x4 *)(d.state_in + at + 16 * j * DK + 16 * m);
+        }
+    auto put_state = [&]() {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                bf16x4 p[3];
+                split<3>(S[m][j], p);
+#pragma unroll
+                for (int u = 0; u < 3; ++u)
+                    *(bf16x4 *)(sb + (u * kSlice + 16 * j + n) * LS + 16 * (MT * wave + m) + 4 * g) = p[u];
+            }
+    };
+    // rows 16 wave + 4 g + 0 .. 3 of value 16 j + n of the slice
+    auto put_rows = [&](__bf16 *to, int j, f32x4 x) {
+        bf16x4 p[3];
+        split<3>(x, p);
+#pragma unroll
+        for (int u = 0; u < 3; ++u) *(bf16x4 *)(to + (u * kSlice + 16 * j + n) * LU + 16 * wave + 4 * g) = p[u];
+    };
+    auto get_rows = [&](const __bf16 *from, int j, int i, bf16x8(&b)[3]) {
+#pragma unroll
+        for (int u = 0; u < 3; ++u) b[u] = *(const bf16x8 *)(from + (u * kSlice + 16 * j + n) * LU + 32 * i + 8 * g);
+    };
+
+    Chunk<DK, T> next;
+    if (sr.count > 0) next.load(d, rec, sr, head, kh, 0, v0);
+    put_state();
+    for (int t0 = 0; t0 < sr.count; t0 += kC) {
+        const Chunk<DK, T> c = next;
+        rec += step;
+        if (t0 + kC < sr.count) next.load(d, rec, sr, head, kh, t0 + kC, v0);
+        bf16x8 ka[KS][N];
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+            pieces<T>(c.k[i], ka[i]);
+#pragma unroll
+            for (int u = 0; u < N; ++u) *(bf16x8 *)(kp + (u * kC + 16 * wave + n) * LK + 32 * i + 8 * g) = ka[i][u];
+        }
+        __syncthreads();  // the state's pieces are there
+        f32x4 xk[2] = {}, xq[2] = {};
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+            bf16x8 qa[N];
+            pieces<T>(c.q[i], qa);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                bf16x8 b[3];
+#pragma unroll
+                for (int u = 0; u < 3; ++u)
+                    b[u] = *(const bf16x8 *)(sb + (u * kSlice + 16 * j + n) * LS + 32 * i + 8 * g);
+                xk[j] = mma<N, 3>(ka[i], b, xk[j]);
+                xq[j] = mma<N, 3>(qa, b, xq[j]);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            f32x4 r;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r[i] = c.v[j][i] - c.eg[i] * xk[j][i];
+            put_rows(rb, j, r);
+        }
+        bf16x8 a[2][3];
+        split<3>(c.t[0], a[0]);
+        split<3>(c.t[1], a[1]);
+        __syncthreads();
+        f32x4 u[2] = {};
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            if (i == 1 && wave < 2) break;  // above the diagonal
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                bf16x8 b[3];
+                get_rows(rb, j, i, b);
+                u[j] = mma<3, 3>(a[i], b, u[j]);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            f32x4 w;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = u[j][i] * c.ec[i];
+            put_rows(ub, j, u[j]);
+            put_rows(wb, j, w);
+        }
+        split<3>(c.p[0], a[0]);
+        split<3>(c.p[1], a[1]);
+        __syncthreads();
+        f32x4 o[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[j][i] = d.scale * c.eg[i] * xq[j][i];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int m = 0; m < MT; ++m) S[m][j] *= c.last;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            bf16x8 kt[MT][N];  // K^T: dk = 16 (MT wave + m) + n, rows 32 i + 8 g + 0 .. 7
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int w = 0; w < N; ++w) {
+                    typedef short s4 __attribute__((ext_vector_type(4)));
+                    const __bf16 *from = kp + (w * kC + 32 * i + 8 * g + (n >> 2)) * LK + 16 * (MT * wave + m) + 4 * (n & 3);
+                    const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS s4 *)from);
+                    const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS s4 *)(from + 4 * LK));
+                    kt[m][w] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+                }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                bf16x8 b[3];
+                if (i == 0 || wave >= 2) {
+                    get_rows(ub, j, i, b);
+                    o[j] = mma<3, 3>(a[i], b, o[j]);
+                }
+                get_rows(wb, j, i, b);
+#pragma unroll
+                for (int m = 0; m < MT; ++m) S[m][j] = mma<N, 3>(kt[m], b, S[m][j]);
+            }
+        }
+        put_state();  // read again behind the next barrier; nobody reads the old ones any more
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int t = t0 + 16 * wave + 4 * g + i;
+            if (t >= sr.count) break;
+            T *out = (T *)d.out.ptr + (long long)(sr.first + t) * d.out.token_stride +
+                     (long long)head * d.out.head_stride + v0 + n;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                if (in[j]) out[16 * j] = (T)o[j][i];
+        }
+        __syncthreads();  // K's pieces have been read
+    }
+    if (held && d.state_out) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+                if (in[j]) *(f32x4 *)(d.state_out + at + 16 * j * DK + 16 * m) = S[m][j];
+    }
+}
+
+// Rows from which the chunks are faster.
+constexpr uint32_t kChunkRows = 17;
+
 template <int DK, typename T>
 hipError_t launch_t(const m27q_delta &d, void *scratch, hipStream_t s) {
-    hipLaunchKernelGGL((k_delta_rows<DK, T>), dim3(d.v.heads * (d.v.dim / 16), d.n), dim3(64), 0, s, d);
+    if (d.max_len < kChunkRows) {
+        hipLaunchKernelGGL((k_delta_rows<DK, T>), dim3(d.v.heads * (d.v.dim / 16), d.n), dim3(64), 0, s, d);
+        return hipGetLastError();
+    }
+    hipLaunchKernelGGL((k_delta_prepare<DK, T>), dim3((d.max_len + kC - 1) / kC, d.v.heads, d.n), dim3(256), 0, s, d,
+                       (float *)scratch);
+    const unsigned slices = (d.v.dim + kSlice - 1) / kSlice;
+    hipLaunchKernelGGL((k_delta_chunks<DK, T>), dim3(d.n * d.k.heads, d.v.heads / d.k.heads * slices), dim3(256), 0, s, d,
+                       (const float *)scratch);
     return hipGetLastError();
 }
 
 }  // namespace
 
 size_t delta_scratch(uint32_t n, uint32_t tokens, uint32_t max_len, uint32_t heads, uint32_t dk, uint32_t dv) {
-    return 16;
+    if (max_len < kChunkRows) return 16;
+    return ((size_t)tokens / kC + n + 1) * heads * kRecord * sizeof(float);
 }
 
 hipError_t launch_delta(const m27q_delta &d, void *scratch, hipStream_t s) {

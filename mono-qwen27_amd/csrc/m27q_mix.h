@@ -41,6 +41,8 @@ struct AttnPlan {
     int few;        // the kernel for few rows
     int splits;
 };
+// Workgroups of a part of the keys.
+long long attn_groups(const m27q_seqs &seqs, uint32_t q_heads, const m27q_cache &cache);
 AttnPlan attn_plan(const m27q_seqs &seqs, uint32_t q_heads, const m27q_cache &cache, int cus);
 size_t attn_scratch(const m27q_seqs &seqs, uint32_t q_heads, uint32_t dim, int splits);
 hipError_t launch_attn(const AttnParams &p, const AttnPlan &plan, hipStream_t s);

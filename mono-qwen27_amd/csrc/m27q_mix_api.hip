@@ -14,6 +14,7 @@ constexpr uint32_t kMaxTokens = 1u << 24;   // rows of a call
 constexpr uint32_t kMaxSeqs = 65535;        // a grid's y
 constexpr uint32_t kMaxKv = 1u << 30;
 constexpr uint32_t kMaxHeads = 1024;
+constexpr long long kMaxGroups = (1ll << 24) - 1;  // workgroups of 256 in a grid's x: below 2^32 work-items
 
 bool aligned(const void *p, size_t a) { return ((uintptr_t)p % a) == 0; }
 
@@ -92,7 +93,7 @@ bool attn_shape(const m27q_seqs *s, uint32_t q_heads, const m27q_cache *c) {
     if (check_seqs(s) != M27Q_OK || check_cache(c) != M27Q_OK) return false;
     if (c->dim != 64 && c->dim != 128 && c->dim != 256) return false;
     if (q_heads < 1 || q_heads > kMaxHeads || q_heads % c->heads || q_heads / c->heads > 64) return false;
-    return true;
+    return attn_groups(*s, q_heads, *c) <= kMaxGroups;
 }
 
 }  // namespace
@@ -227,7 +228,7 @@ M27Q_API m27q_status m27q_delta_rule(const m27q_delta *d, void *scratch, size_t 
     if (d->q.type != d->v.type || d->k.type != d->v.type || d->out.type != d->v.type) return M27Q_ERR_TYPE;
     if (!same_shape(d->q, d->k) || !same_shape(d->v, d->out) || d->v.heads % d->k.heads) return M27Q_ERR_SHAPE;
     const size_t need = m27q_delta_scratch_bytes(d->n, d->tokens, d->max_len, d->v.heads, d->k.dim, d->v.dim);
-    if (!need || d->n_slots > (1u << 24)) return M27Q_ERR_SHAPE;
+    if (!need || d->n_slots > (1u << 24) || (long long)d->n * d->k.heads > kMaxGroups) return M27Q_ERR_SHAPE;
     if (!std::isfinite(d->scale) || d->head_map > M27Q_HEADS_CYCLED) return M27Q_ERR_RANGE;
     if (!rows_aligned(d->q, 16) || !rows_aligned(d->k, 16) || !rows_aligned(d->v, 16) || !rows_aligned(d->out, 16))
         return M27Q_ERR_LAYOUT;
