@@ -352,8 +352,9 @@ M27Q_API m27q_status m27q_sample(const int32_t *idx, const float *val, int k, fl
  * ---------------------------------------------------------------------- */
 
 /* Rows [tokens][heads][dim] in device memory, the dim values of a head side by
- * side, tokens and heads any (non-negative) number of values apart: a head's
- * query can be read from a projection that gives query and gate side by side. */
+ * side, tokens (below 2^31 values) and heads any distance apart that is not
+ * negative: a head's query can be read from a projection that gives query and
+ * gate side by side. */
 typedef struct m27q_rows {
     void *ptr;
     uint32_t type;          /* M27Q_TYPE_F32, _F16 or _BF16 */

@@ -102,7 +102,7 @@ __global__ __launch_bounds__(64) void k_delta_rows(const m27q_delta d) {
 //   S <- e^(G_C) S + (diag(e^(G_C - G)) U)^T K.
 // A first launch, parallel over chunks, makes T = (I + A)^-1 diag(beta), P and the
 // factors; a second one walks the chunks of a sequence with 32 rows of a head's
-// state, 4 waves: three products that wait for each other a chunk, the state in
+// state, 8 waves: three products that wait for each other a chunk, the state in
 // accumulators throughout.
 //
 // Products are fp32-accurate on the bf16 matrix units, 16 times the rate of the
@@ -131,56 +131,84 @@ struct In<__bf16> {
     typedef bf16x8 raw;
 };
 
-// x as N bf16 values each, rounded to nearest: what the ones before leave over.
+// x as N bf16 values each, rounded to nearest: what the ones before leave over.  Two values
+// at a time, their fp32 forms taken from the packed word (one conversion for both).
 template <int N>
-__device__ __forceinline__ void split(f32x8 x, bf16x8 (&p)[N]) {
+__device__ __forceinline__ void split2(float x, float y, uint32_t (&p)[N]) {
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-        p[j] = __builtin_convertvector(x, bf16x8);
-        if (j + 1 < N) x -= __builtin_convertvector(p[j], f32x8);
+        p[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{x, y}, bf16x2));
+        if (j + 1 < N) {
+            asm("" : "+v"(p[j]));  // one conversion, not one more for each half
+            x -= __builtin_bit_cast(float, p[j] << 16);
+            y -= __builtin_bit_cast(float, p[j] & 0xffff0000u);
+        }
     }
+}
+template <int N>
+__device__ __forceinline__ void split(f32x8 x, bf16x8 (&p)[N]) {
+    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+    u4 w[N];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t t[N];
+        split2<N>(x[2 * i], x[2 * i + 1], t);
+#pragma unroll
+        for (int j = 0; j < N; ++j) w[j][i] = t[j];
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) p[j] = __builtin_bit_cast(bf16x8, w[j]);
 }
 template <int N>
 __device__ __forceinline__ void split(f32x4 x, bf16x4 (&p)[N]) {
+    typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+    uint32_t a[N], b[N];
+    split2<N>(x[0], x[1], a);
+    split2<N>(x[2], x[3], b);
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-        p[j] = __builtin_convertvector(x, bf16x4);
-        if (j + 1 < N) x -= __builtin_convertvector(p[j], f32x4);
-    }
+    for (int j = 0; j < N; ++j) p[j] = __builtin_bit_cast(bf16x4, u2{a[j], b[j]});
 }
 
-// c += a b over a 16x16 tile and 32 of the contraction, the smallest parts first.
-template <int NA, int NB>
-__device__ __forceinline__ f32x4 mma(const bf16x8 (&a)[NA], const bf16x8 (&b)[NB], f32x4 c) {
+// c[j] += a[j] b over 16x16 tiles and 32 of the contraction, the smallest parts first; the
+// tiles in turn, so that a product does not wait for the one before.
+template <int NC, int NA, int NB>
+__device__ __forceinline__ void mma(const bf16x8 (&a)[NC][NA], const bf16x8 (&b)[NB], f32x4 (&c)[NC]) {
 #pragma unroll
     for (int o = 2; o >= 0; --o)
 #pragma unroll
         for (int i = 0; i < NA; ++i)
-            if (o - i >= 0 && o - i < NB) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[o - i], c, 0, 0, 0);
-    return c;
+            if (o - i >= 0 && o - i < NB)
+#pragma unroll
+                for (int j = 0; j < NC; ++j)
+                    c[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[j][i], b[o - i], c[j], 0, 0, 0);
 }
 
 #define LDS_AS __attribute__((address_space(3)))
 
-// What the first launch leaves for a chunk and a head, in floats.
-constexpr int kT = 0, kP = kC * kC, kEg = 2 * kC * kC, kEc = kEg + kC, kLast = kEc + kC, kRecord = kLast + 64;
+// What the first launch leaves for a chunk and a head: the pieces of T and of P as operand
+// rows, six blocks of 16 rows and 32 columns (row tile m's first, and its second where that
+// is not above the diagonal) of [3][64 lanes][8]; then the factors.
+constexpr int kBlocks = 6, kBlockHalves = 3 * 64 * 8;
+constexpr int kT = 0, kP = kBlocks * kBlockHalves / 2, kEg = 2 * kP, kEc = kEg + kC, kLast = kEc + kC,
+              kRecord = kLast + 64;  // in floats
+__device__ __forceinline__ int block_of(int m, int i) { return m < 2 ? m : 2 * m - 2 + i; }
 
 // The place of a sequence's first chunk among all: places do not meet, as a
 // sequence has at most one chunk more than whole ones.
 __device__ __forceinline__ long long chunk_place(int first, int s) { return first / kC + s; }
 
-// The sequence's 16 rows from t0 as operand rows: lane m = lane % 16, values
-// 32 i + 8 (lane / 16) + 0 .. 7 of row t0 + m; zeros past the end.
-template <int DK, typename T>
-__device__ __forceinline__ void load_rows(const m27q_rows &r, long long first, int head, int t0, int count,
-                                          typename In<T>::raw (&x)[DK / 32]) {
-    const int lane = threadIdx.x & 63, t = t0 + (lane & 15);
-    const T *p = (const T *)r.ptr + (first + t) * r.token_stride + (long long)head * r.head_stride + 8 * (lane >> 4);
+// NI steps of the sequence's 16 rows from t0 as operand rows: lane m = lane % 16, values
+// 32 (i0 + i) + 8 (lane / 16) + 0 .. 7 of row t0 + m.  Past the end it is the last row again,
+// without a branch (a load under one would keep later waits from telling it from others):
+// beta is 0 there, which keeps such rows out of U and of the state.
+template <int NI, typename T>
+__device__ __forceinline__ void load_rows(const m27q_rows &r, long long first, int head, int t0, int count, int i0,
+                                          typename In<T>::raw (&x)[NI]) {
+    const int lane = threadIdx.x & 63, t = min(t0 + (lane & 15), count - 1);
+    const T *p = (const T *)r.ptr + first * r.token_stride + (long long)head * r.head_stride + 32 * i0;
+    const unsigned long long at = (unsigned long long)(uint32_t)t * (uint32_t)r.token_stride + 8 * (lane >> 4);
 #pragma unroll
-    for (int i = 0; i < DK / 32; ++i) {
-        x[i] = typename In<T>::raw{};
-        if (t < count) x[i] = *(const typename In<T>::raw *)(p + 32 * i);
-    }
+    for (int i = 0; i < NI; ++i) x[i] = *(const typename In<T>::raw *)(p + at + 32 * i);
 }
 template <typename T>
 __device__ __forceinline__ void pieces(typename In<T>::raw x, bf16x8 (&p)[In<T>::N]) {
@@ -188,152 +216,177 @@ __device__ __forceinline__ void pieces(typename In<T>::raw x, bf16x8 (&p)[In<T>:
     else split<In<T>::N>(__builtin_convertvector(x, f32x8), p);
 }
 
+// A chunk of a key head: K K^T and Q K^T once, then for its value heads (every `parts`-th
+// of them) the triangular inverse.
 template <int DK, typename T>
-__global__ __launch_bounds__(256) void k_delta_prepare(const m27q_delta d, float *scratch) {
-    constexpr int N = In<T>::N, KS = DK / 32, LD = DK + 16, LM = kC + 1;
-    constexpr size_t planes = sizeof(__bf16) * N * kC * LD, mats = sizeof(float) * 2 * kC * LM;
+__global__ __launch_bounds__(256) void k_delta_prepare(const m27q_delta d, float *scratch, int parts) {
+    constexpr int N = In<T>::N, KS = DK / 32, LD = DK + 16, LM = kC + 4;
+    constexpr size_t planes = sizeof(__bf16) * N * kC * LD, mats = sizeof(float) * 3 * kC * LM;
     __shared__ __attribute__((aligned(16))) char mem[planes > mats ? planes : mats];
     __shared__ double G[kC];
     __shared__ float B[kC];
-    __bf16 *kp = (__bf16 *)mem;                          // K's pieces, [N][kC][LD]
-    float *Am = (float *)mem, *Xm = Am + kC * LM;        // then A and the inverse of I + A
-    const int s = blockIdx.z, head = blockIdx.y, t0 = blockIdx.x * kC;
+    __bf16 *kp = (__bf16 *)mem;                                        // K's pieces, [N][kC][LD]
+    float *Am = (float *)mem, *Xm = Am + kC * LM, *Pm = Xm + kC * LM;  // then A, the inverse of I + A, and P
+    const int s = blockIdx.z, kh = blockIdx.y / parts, part = blockIdx.y - kh * parts, t0 = blockIdx.x * kC;
     const SeqRows sr = seq_rows(d.start, s, (int)d.tokens, (int)d.max_len);
     if (t0 >= sr.count) return;
-    const int kh = d.head_map == M27Q_HEADS_CYCLED ? head % (int)d.k.heads : head / (int)(d.v.heads / d.k.heads);
+    const int kheads = (int)d.k.heads, per = (int)d.v.heads / kheads;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-    float *rec = scratch + ((chunk_place(sr.first, s) + blockIdx.x) * d.v.heads + head) * (long long)kRecord;
 
-    bf16x8 ka[KS][N], qa[KS][N];
+    bf16x8 a[KS][2][N];  // K's and Q's
     {
         typename In<T>::raw x[KS], y[KS];
-        load_rows<DK, T>(d.k, sr.first, kh, t0 + 16 * wave, sr.count, x);
-        load_rows<DK, T>(d.q, sr.first, kh, t0 + 16 * wave, sr.count, y);
+        load_rows<KS, T>(d.k, sr.first, kh, t0 + 16 * wave, sr.count, 0, x);
+        load_rows<KS, T>(d.q, sr.first, kh, t0 + 16 * wave, sr.count, 0, y);
 #pragma unroll
         for (int i = 0; i < KS; ++i) {
-            pieces<T>(x[i], ka[i]);
-            pieces<T>(y[i], qa[i]);
+            pieces<T>(x[i], a[i][0]);
+            pieces<T>(y[i], a[i][1]);
 #pragma unroll
-            for (int j = 0; j < N; ++j) *(bf16x8 *)(kp + (j * kC + 16 * wave + n) * LD + 32 * i + 8 * g) = ka[i][j];
+            for (int j = 0; j < N; ++j) *(bf16x8 *)(kp + (j * kC + 16 * wave + n) * LD + 32 * i + 8 * g) = a[i][0][j];
         }
-    }
-    if (wave == 0) {  // sums of g in 64 bits: differences of them are taken below
-        const bool in = t0 + lane < sr.count;
-        const long long at = (long long)(sr.first + t0 + lane) * d.v.heads + head;
-        const float gf = in ? d.g[at] : 0.0f;
-        double x = gf < -1e4f ? -1e4 : (double)gf;  // e^-10000 is 0 as e^-inf is, and no inf - inf
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const double y = __shfl_up(x, o);
-            x += lane >= o ? y : 0.0;
-        }
-        const double last = __shfl(x, 63);
-        G[lane] = x;
-        B[lane] = in ? d.beta[at] : 0.0f;
-        rec[kEg + lane] = expf((float)x);
-        rec[kEc + lane] = expf((float)(last - x));
-        if (lane == 0) rec[kLast] = expf((float)last);
     }
     __syncthreads();
-
-    f32x4 kk[4], qk[4];
+    f32x4 prod[4][2];  // tiles of K K^T and Q K^T at rows 16 wave, columns 16 j
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        kk[j] = qk[j] = f32x4{};
+        prod[j][0] = prod[j][1] = f32x4{};
         if (j > wave) continue;
 #pragma unroll
         for (int i = 0; i < KS; ++i) {
             bf16x8 b[N];
 #pragma unroll
             for (int u = 0; u < N; ++u) b[u] = *(const bf16x8 *)(kp + (u * kC + 16 * j + n) * LD + 32 * i + 8 * g);
-            kk[j] = mma<N, N>(ka[i], b, kk[j]);
-            qk[j] = mma<N, N>(qa[i], b, qk[j]);
+            mma<2, N, N>(a[i], b, prod[j]);
         }
     }
-    __syncthreads();  // K's pieces make room
+
+    for (int which = part; which < per; which += parts) {
+        const int head = d.head_map == M27Q_HEADS_CYCLED ? which * kheads + kh : kh * per + which;
+        float *rec = scratch + ((chunk_place(sr.first, s) + blockIdx.x) * d.v.heads + head) * (long long)kRecord;
+        __syncthreads();  // K's pieces, or the last head's matrices, make room
+        if (wave == 0) {  // sums of g in 64 bits: differences of them are taken below
+            const bool in = t0 + lane < sr.count;
+            const long long at = (long long)(sr.first + t0 + lane) * d.v.heads + head;
+            const float gf = in ? d.g[at] : 0.0f;
+            double x = gf < -1e4f ? -1e4 : (double)gf;  // e^-10000 is 0 as e^-inf is, and no inf - inf
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int row = 16 * wave + 4 * g + i, col = 16 * j + n;
-            float a = 0, p = 0;
-            if (col <= row) {
-                const float e = expf((float)(G[row] - G[col]));
-                p = d.scale * e * qk[j][i];
-                if (col < row) a = B[row] * e * kk[j][i];
+            for (int o = 1; o < 64; o <<= 1) {
+                const double y = __shfl_up(x, o);
+                x += lane >= o ? y : 0.0;
             }
-            Am[row * LM + col] = a;
-            Xm[row * LM + col] = 0;
-            rec[kP + row * kC + col] = p;
+            const double last = __shfl(x, 63);
+            G[lane] = x;
+            B[lane] = in ? d.beta[at] : 0.0f;
+            rec[kEg + lane] = expf((float)x);
+            rec[kEc + lane] = expf((float)(last - x));
+            if (lane == 0) rec[kLast] = expf((float)last);
         }
-    __syncthreads();
-    // the inverse's 16x16 blocks: on the diagonal by forward substitution, a column a lane
-    const int r0 = 16 * wave;
-    if (lane < 16) {
-        float x[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            float v = i == lane ? 1.0f : 0.0f;
-#pragma unroll
-            for (int k = 0; k < i; ++k) v = __builtin_fmaf(-Am[(r0 + i) * LM + r0 + k], x[k], v);
-            x[i] = v;
-            Xm[(r0 + i) * LM + r0 + lane] = v;
-        }
-    }
-    // below it by diagonals: X_ij = -X_ii sum_(j <= k < i) A_ik X_kj.  The sum's rows lie
-    // in the lanes as 4 g + t, so the second product takes X_ii's columns in that order.
-#pragma unroll
-    for (int o = 1; o < 4; ++o) {
         __syncthreads();
-        if (wave < o) continue;
-        const int c0 = 16 * (wave - o);
-        f32x4 y = {}, x = {};
-        for (int k0 = c0; k0 < r0; k0 += 4)
-            y = __builtin_amdgcn_mfma_f32_16x16x4f32(Am[(r0 + n) * LM + k0 + g], Xm[(k0 + g) * LM + c0 + n], y, 0, 0, 0);
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
-            x = __builtin_amdgcn_mfma_f32_16x16x4f32(-Xm[(r0 + n) * LM + r0 + 4 * g + t], y[t], x, 0, 0, 0);
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) Xm[(r0 + 4 * g + i) * LM + c0 + n] = x[i];
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < kC * kC; i += 256) rec[kT + i] = Xm[(i / kC) * LM + i % kC] * B[i % kC];
-}
-
-// One chunk's inputs in the registers of its lanes.
-template <int DK, typename T>
-struct Chunk {
-    typename In<T>::raw k[DK / 32], q[DK / 32];
-    f32x8 t[2], p[2];     // rows 16 wave + lane % 16 of T and P
-    float v[2][4];        // V at rows 16 wave + 4 (lane / 16) + i, values lane % 16 and 16 + that of the slice
-    float eg[4], ec[4], last;
-
-    __device__ __forceinline__ void load(const m27q_delta &d, const float *rec, const SeqRows &sr, int head, int kh,
-                                         int t0, int v0) {
-        const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-        load_rows<DK, T>(d.k, sr.first, kh, t0 + 16 * wave, sr.count, k);
-        load_rows<DK, T>(d.q, sr.first, kh, t0 + 16 * wave, sr.count, q);
+            for (int i = 0; i < 4; ++i) {
+                const int row = 16 * wave + 4 * g + i, col = 16 * j + n;
+                float x = 0, p = 0;
+                if (col <= row) {
+                    const float e = expf((float)(G[row] - G[col]));
+                    p = d.scale * e * prod[j][1][i];
+                    if (col < row) x = B[row] * e * prod[j][0][i];
+                }
+                Am[row * LM + col] = x;
+                Xm[row * LM + col] = 0;
+                Pm[row * LM + col] = p;
+            }
+        __syncthreads();
+        // the inverse's 16x16 blocks: on the diagonal by forward substitution, a column a lane
+        const int r0 = 16 * wave;
+        if (lane < 16) {
+            float x[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                float v = i == lane ? 1.0f : 0.0f;
+#pragma unroll
+                for (int k = 0; k < i; ++k) v = __builtin_fmaf(-Am[(r0 + i) * LM + r0 + k], x[k], v);
+                x[i] = v;
+                Xm[(r0 + i) * LM + r0 + lane] = v;
+            }
+        }
+        // below it by diagonals: X_ij = -X_ii sum_(j <= k < i) A_ik X_kj.  The sum's rows lie
+        // in the lanes as 4 g + t, so the second product takes X_ii's columns in that order.
+#pragma unroll
+        for (int o = 1; o < 4; ++o) {
+            __syncthreads();
+            if (wave < o) continue;
+            const int c0 = 16 * (wave - o);
+            f32x4 y[4] = {}, x = {};
+#pragma unroll
+            for (int k = 0; k < 4 * o; ++k)
+                y[k & 3] = __builtin_amdgcn_mfma_f32_16x16x4f32(Am[(r0 + n) * LM + c0 + 4 * k + g],
+                                                                Xm[(c0 + 4 * k + g) * LM + c0 + n], y[k & 3], 0, 0, 0);
+            y[0] = (y[0] + y[1]) + (y[2] + y[3]);
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+                x = __builtin_amdgcn_mfma_f32_16x16x4f32(-Xm[(r0 + n) * LM + r0 + 4 * g + t], y[0][t], x, 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) Xm[(r0 + 4 * g + i) * LM + c0 + n] = x[i];
+        }
+        __syncthreads();
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            t[i] = *(const f32x8a *)(rec + kT + (16 * wave + n) * kC + 32 * i + 8 * g);
-            p[i] = *(const f32x8a *)(rec + kP + (16 * wave + n) * kC + 32 * i + 8 * g);
-        }
-        const int row = 16 * wave + 4 * g;
+            if (i == 1 && wave < 2) break;
+            const int at = (r0 + n) * LM + 32 * i + 8 * g;
+            __bf16 *to = (__bf16 *)(rec + kT) + block_of(wave, i) * kBlockHalves + lane * 8;
+            bf16x8 x[3], y[3];
+            split<3>(*(const f32x8a *)(Xm + at) * *(const f32x8a *)(B + 32 * i + 8 * g), x);
+            split<3>(*(const f32x8a *)(Pm + at), y);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            eg[i] = rec[kEg + row + i];
-            ec[i] = rec[kEc + row + i];
-            const T *x = (const T *)d.v.ptr + (long long)(sr.first + t0 + row + i) * d.v.token_stride +
-                         (long long)head * d.v.head_stride + v0 + n;
-#pragma unroll
-            for (int j = 0; j < 2; ++j) v[j][i] = t0 + row + i < sr.count && v0 + 16 * j < (int)d.v.dim ? (float)x[16 * j] : 0.0f;
+            for (int u = 0; u < 3; ++u) {
+                *(bf16x8 *)(to + u * 512) = x[u];
+                *(bf16x8 *)(to + 2 * (kP - kT) + u * 512) = y[u];
+            }
         }
-        last = rec[kLast];
+    }
+}
+
+// A chunk's inputs in the registers of its lanes: wave m + 4 j of eight has rows 16 m ..
+// of the chunk and 16 j .. of the slice's state rows.  Each part is asked for again, for the
+// next chunk, as soon as it has been used.
+template <int DK, typename T>
+struct Chunk {
+    typename In<T>::raw k[DK / 64], q[DK / 32];  // of K's rows half the values, the j-th
+    bf16x8 t[2][3], p[2][3];
+    T v[4];               // V at rows 16 m + 4 (lane / 16) + i, value 16 j + lane % 16 of the slice
+    f32x4 eg, ec;
+    float last;
+
+    __device__ __forceinline__ void load_k(const m27q_delta &d, const SeqRows &sr, int kh, int t0, int m, int j) {
+        load_rows<DK / 64, T>(d.k, sr.first, kh, t0 + 16 * m, sr.count, j * (DK / 64), k);
+    }
+    __device__ __forceinline__ void load_q(const m27q_delta &d, const SeqRows &sr, int kh, int t0, int m) {
+        load_rows<DK / 32, T>(d.q, sr.first, kh, t0 + 16 * m, sr.count, 0, q);
+    }
+    __device__ __forceinline__ void load_v(const m27q_delta &d, const SeqRows &sr, int head, int t0, int v0, int m, int j) {
+        const int lane = threadIdx.x & 63, row = t0 + 16 * m + 4 * (lane >> 4);
+        const T *x = (const T *)d.v.ptr + (long long)sr.first * d.v.token_stride + (long long)head * d.v.head_stride +
+                     min(v0 + 16 * j, (int)d.v.dim - 16);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            v[i] = x[(unsigned long long)(uint32_t)min(row + i, sr.count - 1) * (uint32_t)d.v.token_stride + (lane & 15)];
+    }
+    __device__ __forceinline__ void load_blocks(const float *from, int m, bf16x8 (&x)[2][3]) {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const __bf16 *b = (const __bf16 *)from + block_of(m, m < 2 ? 0 : i) * kBlockHalves + lane * 8;
+#pragma unroll
+            for (int u = 0; u < 3; ++u) x[i][u] = *(const bf16x8 *)(b + u * 512);
+        }
     }
 };
 
 template <int DK, typename T>
-__global__ __launch_bounds__(256, 1) void k_delta_chunks(const m27q_delta d, const float *scratch) {
+__global__ __launch_bounds__(512) void k_delta_chunks(const m27q_delta d, const float *scratch) {
     constexpr int N = In<T>::N, KS = DK / 32, MT = DK / 64;
     constexpr int LK = DK + 16, LS = DK + 8, LU = kC + 8;
     __shared__ __attribute__((aligned(16))) __bf16 kp[N * kC * LK];       // K's pieces [N][row][dk]
@@ -350,161 +403,147 @@ __global__ __launch_bounds__(256, 1) void k_delta_chunks(const m27q_delta d, con
     const SeqRows sr = seq_rows(d.start, s, (int)d.tokens, (int)d.max_len);
     const int slot = d.slots ? d.slots[s] : s;
     const bool held = slot >= 0 && (uint32_t)slot < d.n_slots;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), mt = wave & 3, nt = wave >> 2;
+    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     const float *rec = scratch + (chunk_place(sr.first, s) * d.v.heads + head) * (long long)kRecord;
     const long long step = (long long)d.v.heads * kRecord;
 
-    // the state: dk = 16 (MT wave + m) + 4 g + i of rows v0 + 16 j + n
-    f32x4 S[MT][2];
-    const long long at = (((long long)slot * d.v.heads + head) * d.v.dim + v0 + n) * DK + 16 * MT * wave + 4 * g;
-    const bool in[2] = {v0 < (int)d.v.dim, v0 + 16 < (int)d.v.dim};
+    // the state: dk = 16 (MT mt + m) + 4 g + i of row v0 + 16 nt + n
+    f32x4 S[MT];
+    const long long at = (((long long)slot * d.v.heads + head) * d.v.dim + v0 + 16 * nt + n) * DK + 16 * MT * mt + 4 * g;
+    const bool in = v0 + 16 * nt < (int)d.v.dim;
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            S[m][j] = f32x4{};
-            if (held && d.state_in && in[j]) S[m][j] = *(const f32x4 *)(d.state_in + at + 16 * j * DK + 16 * m);
-        }
+    for (int m = 0; m < MT; ++m) {
+        S[m] = f32x4{};
+        if (held && d.state_in && in) S[m] = *(const f32x4 *)(d.state_in + at + 16 * m);
+    }
     auto put_state = [&]() {
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int m = 0; m < MT; ++m) {
+            bf16x4 p[3];
+            split<3>(S[m], p);
 #pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                bf16x4 p[3];
-                split<3>(S[m][j], p);
-#pragma unroll
-                for (int u = 0; u < 3; ++u)
-                    *(bf16x4 *)(sb + (u * kSlice + 16 * j + n) * LS + 16 * (MT * wave + m) + 4 * g) = p[u];
-            }
+            for (int u = 0; u < 3; ++u)
+                *(bf16x4 *)(sb + (u * kSlice + 16 * nt + n) * LS + 16 * (MT * mt + m) + 4 * g) = p[u];
+        }
     };
-    // rows 16 wave + 4 g + 0 .. 3 of value 16 j + n of the slice
-    auto put_rows = [&](__bf16 *to, int j, f32x4 x) {
+    // rows 16 mt + 4 g + 0 .. 3 of value 16 nt + n of the slice
+    auto put_rows = [&](__bf16 *to, f32x4 x) {
         bf16x4 p[3];
         split<3>(x, p);
 #pragma unroll
-        for (int u = 0; u < 3; ++u) *(bf16x4 *)(to + (u * kSlice + 16 * j + n) * LU + 16 * wave + 4 * g) = p[u];
+        for (int u = 0; u < 3; ++u) *(bf16x4 *)(to + (u * kSlice + 16 * nt + n) * LU + 16 * mt + 4 * g) = p[u];
     };
-    auto get_rows = [&](const __bf16 *from, int j, int i, bf16x8(&b)[3]) {
+    auto get_rows = [&](const __bf16 *from, int i, bf16x8(&b)[3]) {
 #pragma unroll
-        for (int u = 0; u < 3; ++u) b[u] = *(const bf16x8 *)(from + (u * kSlice + 16 * j + n) * LU + 32 * i + 8 * g);
+        for (int u = 0; u < 3; ++u) b[u] = *(const bf16x8 *)(from + (u * kSlice + 16 * nt + n) * LU + 32 * i + 8 * g);
     };
 
-    Chunk<DK, T> next;
-    if (sr.count > 0) next.load(d, rec, sr, head, kh, 0, v0);
+    Chunk<DK, T> c;
+    const int row = 16 * mt + 4 * g;
+    T *const out = (T *)d.out.ptr + (long long)sr.first * d.out.token_stride + (long long)head * d.out.head_stride + v0 + 16 * nt;
+    auto load_factors = [&]() {
+        c.eg = *(const f32x4 *)(rec + kEg + row);
+        c.ec = *(const f32x4 *)(rec + kEc + row);
+        c.last = rec[kLast];
+    };
+    if (sr.count > 0) {
+        c.load_k(d, sr, kh, 0, mt, nt);
+        c.load_q(d, sr, kh, 0, mt);
+        c.load_v(d, sr, head, 0, v0, mt, nt);
+        c.load_blocks(rec + kT, mt, c.t);
+        c.load_blocks(rec + kP, mt, c.p);
+        load_factors();
+    }
     put_state();
     for (int t0 = 0; t0 < sr.count; t0 += kC) {
-        const Chunk<DK, T> c = next;
-        rec += step;
-        if (t0 + kC < sr.count) next.load(d, rec, sr, head, kh, t0 + kC, v0);
-        bf16x8 ka[KS][N];
+        rec += step;  // behind the last chunk's there is room for one more (of no matter)
+#pragma unroll
+        for (int i = 0; i < KS / 2; ++i) {
+            bf16x8 x[N];
+            pieces<T>(c.k[i], x);
+#pragma unroll
+            for (int u = 0; u < N; ++u)
+                *(bf16x8 *)(kp + (u * kC + 16 * mt + n) * LK + 32 * (nt * (KS / 2) + i) + 8 * g) = x[u];
+        }
+        c.load_k(d, sr, kh, t0 + kC, mt, nt);
+        __syncthreads();  // K's and the state's pieces are there
+        f32x4 x[2] = {};  // K S^T and Q S^T
 #pragma unroll
         for (int i = 0; i < KS; ++i) {
-            pieces<T>(c.k[i], ka[i]);
+            bf16x8 a[2][N], b[3];
 #pragma unroll
-            for (int u = 0; u < N; ++u) *(bf16x8 *)(kp + (u * kC + 16 * wave + n) * LK + 32 * i + 8 * g) = ka[i][u];
+            for (int u = 0; u < N; ++u) a[0][u] = *(const bf16x8 *)(kp + (u * kC + 16 * mt + n) * LK + 32 * i + 8 * g);
+            pieces<T>(c.q[i], a[1]);
+#pragma unroll
+            for (int u = 0; u < 3; ++u) b[u] = *(const bf16x8 *)(sb + (u * kSlice + 16 * nt + n) * LS + 32 * i + 8 * g);
+            mma<2, N, 3>(a, b, x);
         }
-        __syncthreads();  // the state's pieces are there
-        f32x4 xk[2] = {}, xq[2] = {};
+        f32x4 r;
 #pragma unroll
-        for (int i = 0; i < KS; ++i) {
-            bf16x8 qa[N];
-            pieces<T>(c.q[i], qa);
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                bf16x8 b[3];
-#pragma unroll
-                for (int u = 0; u < 3; ++u)
-                    b[u] = *(const bf16x8 *)(sb + (u * kSlice + 16 * j + n) * LS + 32 * i + 8 * g);
-                xk[j] = mma<N, 3>(ka[i], b, xk[j]);
-                xq[j] = mma<N, 3>(qa, b, xq[j]);
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            f32x4 r;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) r[i] = c.v[j][i] - c.eg[i] * xk[j][i];
-            put_rows(rb, j, r);
-        }
-        bf16x8 a[2][3];
-        split<3>(c.t[0], a[0]);
-        split<3>(c.t[1], a[1]);
+        for (int i = 0; i < 4; ++i) r[i] = (float)c.v[i] - c.eg[i] * x[0][i];
+        put_rows(rb, r);
+        c.load_q(d, sr, kh, t0 + kC, mt);
+        c.load_v(d, sr, head, t0 + kC, v0, mt, nt);
         __syncthreads();
-        f32x4 u[2] = {};
+        f32x4 u[1] = {};
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            if (i == 1 && wave < 2) break;  // above the diagonal
+            if (i == 1 && mt < 2) break;  // above the diagonal
+            bf16x8 a[1][3], b[3];
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                bf16x8 b[3];
-                get_rows(rb, j, i, b);
-                u[j] = mma<3, 3>(a[i], b, u[j]);
-            }
+            for (int w = 0; w < 3; ++w) a[0][w] = c.t[i][w];
+            get_rows(rb, i, b);
+            mma<1, 3, 3>(a, b, u);
         }
+        f32x4 w;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            f32x4 w;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = u[j][i] * c.ec[i];
-            put_rows(ub, j, u[j]);
-            put_rows(wb, j, w);
-        }
-        split<3>(c.p[0], a[0]);
-        split<3>(c.p[1], a[1]);
+        for (int i = 0; i < 4; ++i) w[i] = u[0][i] * c.ec[i];
+        put_rows(ub, u[0]);
+        put_rows(wb, w);
+        c.load_blocks(rec + kT, mt, c.t);
         __syncthreads();
-        f32x4 o[2];
+        f32x4 o[1];
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int i = 0; i < 4; ++i) o[0][i] = d.scale * c.eg[i] * x[1][i];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[j][i] = d.scale * c.eg[i] * xq[j][i];
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int m = 0; m < MT; ++m) S[m][j] *= c.last;
+        for (int m = 0; m < MT; ++m) S[m] *= c.last;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            bf16x8 kt[MT][N];  // K^T: dk = 16 (MT wave + m) + n, rows 32 i + 8 g + 0 .. 7
+            bf16x8 kt[MT][N], b[3];  // K^T: dk = 16 (MT mt + m) + n, rows 32 i + 8 g + 0 .. 7
 #pragma unroll
             for (int m = 0; m < MT; ++m)
 #pragma unroll
-                for (int w = 0; w < N; ++w) {
+                for (int z = 0; z < N; ++z) {
                     typedef short s4 __attribute__((ext_vector_type(4)));
-                    const __bf16 *from = kp + (w * kC + 32 * i + 8 * g + (n >> 2)) * LK + 16 * (MT * wave + m) + 4 * (n & 3);
-                    const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS s4 *)from);
-                    const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS s4 *)(from + 4 * LK));
-                    kt[m][w] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+                    const __bf16 *from = kp + (z * kC + 32 * i + 8 * g + (n >> 2)) * LK + 16 * (MT * mt + m) + 4 * (n & 3);
+                    const s4 y0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS s4 *)from);
+                    const s4 y1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS s4 *)(from + 4 * LK));
+                    kt[m][z] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(y0, y1, 0, 1, 2, 3, 4, 5, 6, 7));
                 }
+            get_rows(wb, i, b);
+            mma<MT, N, 3>(kt, b, S);
+            if (i == 0 || mt >= 2) {
+                bf16x8 a[1][3];
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                bf16x8 b[3];
-                if (i == 0 || wave >= 2) {
-                    get_rows(ub, j, i, b);
-                    o[j] = mma<3, 3>(a[i], b, o[j]);
-                }
-                get_rows(wb, j, i, b);
-#pragma unroll
-                for (int m = 0; m < MT; ++m) S[m][j] = mma<N, 3>(kt[m], b, S[m][j]);
+                for (int z = 0; z < 3; ++z) a[0][z] = c.p[i][z];
+                get_rows(ub, i, b);
+                mma<1, 3, 3>(a, b, o);
             }
         }
-        put_state();  // read again behind the next barrier; nobody reads the old ones any more
+        c.load_blocks(rec + kP, mt, c.p);
+        load_factors();
+        put_state();  // read again behind the next barrier but one; nobody reads the old ones any more
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int t = t0 + 16 * wave + 4 * g + i;
-            if (t >= sr.count) break;
-            T *out = (T *)d.out.ptr + (long long)(sr.first + t) * d.out.token_stride +
-                     (long long)head * d.out.head_stride + v0 + n;
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-                if (in[j]) out[16 * j] = (T)o[j][i];
+            const int t = t0 + row + i;
+            if (in && t < sr.count) out[(unsigned long long)(uint32_t)t * (uint32_t)d.out.token_stride + n] = (T)o[0][i];
         }
         __syncthreads();  // K's pieces have been read
     }
-    if (held && d.state_out) {
+    if (held && d.state_out && in) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-                if (in[j]) *(f32x4 *)(d.state_out + at + 16 * j * DK + 16 * m) = S[m][j];
+        for (int m = 0; m < MT; ++m) *(f32x4 *)(d.state_out + at + 16 * m) = S[m];
     }
 }
 
@@ -517,10 +556,13 @@ hipError_t launch_t(const m27q_delta &d, void *scratch, hipStream_t s) {
         hipLaunchKernelGGL((k_delta_rows<DK, T>), dim3(d.v.heads * (d.v.dim / 16), d.n), dim3(64), 0, s, d);
         return hipGetLastError();
     }
-    hipLaunchKernelGGL((k_delta_prepare<DK, T>), dim3((d.max_len + kC - 1) / kC, d.v.heads, d.n), dim3(256), 0, s, d,
-                       (float *)scratch);
+    const unsigned chunks = (d.max_len + kC - 1) / kC, per = d.v.heads / d.k.heads;
+    // a workgroup makes all value heads of a key head where that still leaves two for each CU
+    const unsigned parts = (unsigned long long)chunks * d.k.heads * d.n >= 512 ? 1 : per;
+    hipLaunchKernelGGL((k_delta_prepare<DK, T>), dim3(chunks, d.k.heads * parts, d.n), dim3(256), 0, s, d,
+                       (float *)scratch, (int)parts);
     const unsigned slices = (d.v.dim + kSlice - 1) / kSlice;
-    hipLaunchKernelGGL((k_delta_chunks<DK, T>), dim3(d.n * d.k.heads, d.v.heads / d.k.heads * slices), dim3(256), 0, s, d,
+    hipLaunchKernelGGL((k_delta_chunks<DK, T>), dim3(d.n * d.k.heads, per * slices), dim3(512), 0, s, d,
                        (const float *)scratch);
     return hipGetLastError();
 }

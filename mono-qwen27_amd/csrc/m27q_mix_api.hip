@@ -14,7 +14,7 @@ constexpr uint32_t kMaxTokens = 1u << 24;   // rows of a call
 constexpr uint32_t kMaxSeqs = 65535;        // a grid's y
 constexpr uint32_t kMaxKv = 1u << 30;
 constexpr uint32_t kMaxHeads = 1024;
-constexpr long long kMaxGroups = (1ll << 24) - 1;  // workgroups of 256 in a grid's x: below 2^32 work-items
+constexpr long long kMaxGroups = (1ll << 23) - 1;  // workgroups of up to 512 in a grid's x: below 2^32 work-items
 
 bool aligned(const void *p, size_t a) { return ((uintptr_t)p % a) == 0; }
 
@@ -24,7 +24,7 @@ m27q_status check_rows(const m27q_rows &r, uint32_t max_dim) {
     if (!r.ptr) return M27Q_ERR_NULL;
     if (!value_type(r.type)) return M27Q_ERR_TYPE;
     if (r.heads < 1 || r.heads > kMaxHeads || r.dim < 1 || r.dim > max_dim) return M27Q_ERR_SHAPE;
-    if (r.token_stride < 0 || r.head_stride < 0) return M27Q_ERR_SHAPE;
+    if (r.token_stride < 0 || r.head_stride < 0 || r.token_stride > INT32_MAX) return M27Q_ERR_SHAPE;
     if (!aligned(r.ptr, (size_t)type_bytes(r.type))) return M27Q_ERR_LAYOUT;
     return M27Q_OK;
 }
