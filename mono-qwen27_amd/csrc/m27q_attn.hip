@@ -35,6 +35,9 @@ struct Num<false> {
     static __device__ __forceinline__ f32x16 mma(t8 a, t8 b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
     }
+    static __device__ __forceinline__ f32x4 mma(t8 a, t8 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    }
 };
 template <>
 struct Num<true> {
@@ -45,16 +48,30 @@ struct Num<true> {
     static __device__ __forceinline__ f32x16 mma(t8 a, t8 b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
     }
+    static __device__ __forceinline__ f32x4 mma(t8 a, t8 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    }
 };
 
-// The maximum of a value over the wave's two halves (lane l and l ^ 32).
-__device__ __forceinline__ float max_halves(float x) {
-    const unsigned u = __builtin_bit_cast(unsigned, x);
+// The maximum and the sum of a value over the lanes of a row: l and l ^ 32, for rows of a
+// 16-row tile l ^ 16 and l ^ 48 as well.
+template <int RW>
+__device__ __forceinline__ float max_row(float x) {
+    unsigned u = __builtin_bit_cast(unsigned, x);
+    if constexpr (RW == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+        u = __builtin_bit_cast(unsigned, fmaxf(__builtin_bit_cast(float, (unsigned)r[0]), __builtin_bit_cast(float, (unsigned)r[1])));
+    }
     const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
     return fmaxf(__builtin_bit_cast(float, (unsigned)r[0]), __builtin_bit_cast(float, (unsigned)r[1]));
 }
-__device__ __forceinline__ float sum_halves(float x) {
-    const unsigned u = __builtin_bit_cast(unsigned, x);
+template <int RW>
+__device__ __forceinline__ float sum_row(float x) {
+    unsigned u = __builtin_bit_cast(unsigned, x);
+    if constexpr (RW == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+        u = __builtin_bit_cast(unsigned, __builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]));
+    }
     const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
     return __builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]);
 }
@@ -129,17 +146,17 @@ __device__ __forceinline__ void tile_barrier() {
     __syncthreads();
 }
 
-// Puts zeros for the values of V that are not finite, in the rows that this
-// wave brought into the tile: some row of queries may not see their key, and
+// Puts zeros for the values of V that are not finite, in ROWS rows that this
+// wave brought into LDS: some row of queries may not see their key, and
 // its weight of 0 would make NaN of them.  Returns whether there were any.
-template <int D, bool BF>
-__device__ __forceinline__ bool clear_odd(LDS_AS char *vt) {
+template <int D, bool BF, int ROWS>
+__device__ __forceinline__ bool clear_odd(LDS_AS char *at) {
     typedef uint32_t u4 __attribute__((ext_vector_type(4)));
     constexpr uint32_t E = BF ? 0x7f80u : 0x7c00u;
     bool odd = false;
-    LDS_AS char *at = vt + (threadIdx.x >> 6) * (kKeys / kWaves) * D * 2 + (threadIdx.x & 63) * 16;
+    at += (threadIdx.x & 63) * 16;
 #pragma unroll
-    for (int i = 0; i < kKeys / kWaves * D / 512; ++i) {
+    for (int i = 0; i < ROWS * D / 512; ++i) {
         u4 v = *(LDS_AS u4 *)(at + i * 1024);
         bool here = false;
 #pragma unroll
@@ -154,80 +171,150 @@ __device__ __forceinline__ bool clear_odd(LDS_AS char *vt) {
     return odd;
 }
 
-// One wave's rows: the statistics and sums of a softmax in one pass.
-template <int D, bool BF, int NP>
+// One wave's rows, RW of them (32, or 16 where there are no more): the statistics and sums
+// of a softmax in one pass.  Lane l has row l % RW and, as part g = l / RW of 64 / RW, four
+// consecutive keys of every 4 * 64 / RW, and likewise of the values of a sum.
+template <int D, bool BF, int NP, int RW>
 struct Rows {
     typedef Num<BF> N;
     typedef typename N::t T;
     typedef typename N::t4 T4;
     typedef typename N::t8 T8;
-    T8 q[D / 16];
-    f32x16 o[D / 32];
-    float m, l;      // maximum of the scores (before scale) that weights are taken from; this half's sum of weights
+    static constexpr int G = 64 / RW, STEP = 4 * G;   // parts, and the keys that they share out
+    static constexpr int NS = kKeys / G;              // scores of a tile in a lane
+    static constexpr int KD = 8 * G;                  // values of a product's step
+    static constexpr int NV = NS / 8;                 // steps of the keys in the second product
+    template <int W, int X = 0>
+    struct Acc {
+        typedef f32x16 t;
+    };
+    template <int X>
+    struct Acc<16, X> {
+        typedef f32x4 t;
+    };
+    typedef typename Acc<RW>::t acc;
+    static constexpr int NA = RW * RW / 64;           // values of an accumulator
+    T8 q[D / KD];
+    acc o[D / RW];
+    float m, l;      // maximum of the scores (before scale) that weights are taken from; this part's sum of weights
     int place;       // of this lane's row (-1: none)
+
+    static __device__ __forceinline__ int part() { return (threadIdx.x & 63) / RW; }
+    // the i-th of this lane's keys in a tile; the j-th value of accumulator t
+    static __device__ __forceinline__ int key_at(int i) { return STEP * (i / 4) + 4 * part() + i % 4; }
+    static __device__ __forceinline__ int value_at(int t, int j) { return RW * t + STEP * (j / 4) + 4 * part() + j % 4; }
+
+    __device__ __forceinline__ void clear() {
+        m = -__builtin_inff();
+        l = 0;
+#pragma unroll
+        for (int i = 0; i < D / RW; ++i) o[i] = acc{};
+    }
+
+    // token and head: a row of the call's, also for a lane that has none (and takes zeros)
+    __device__ __forceinline__ void load_q(const AttnParams &p, int token, int head, bool live) {
+        const T *from =
+            (const T *)p.q.ptr + (long long)token * p.q.token_stride + (long long)head * p.q.head_stride + 8 * part();
+        typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+        // a negative scale goes into q, exactly: scores are then compared before scaling
+        const uint32_t flip = p.scale < 0 ? 0x80008000u : 0, keep = live ? ~0u : 0u;
+        u4 v[D / KD];
+#pragma unroll
+        for (int i = 0; i < D / KD; ++i) v[i] = *(const u4 *)(from + KD * i);
+#pragma unroll
+        for (int i = 0; i < D / KD; ++i) q[i] = __builtin_bit_cast(T8, (v[i] ^ flip) & keep);
+    }
 
     // The tile in LDS.  MASK: some of its keys may be hidden from some row, or missing.
     template <bool MASK>
     __device__ __forceinline__ void tile(const AttnParams &p, const Work &w, float sc, int k0, const LDS_AS char *kt,
                                          const LDS_AS char *vt) {
-        const int lane = threadIdx.x & 63, h = lane >> 5, r = lane & 31;
-        f32x16 s = {};
-        // K: row r, chunks 2 i + h
+        float s[NS];
+        T8 pc[NV][NP];
+        scores(kt, s);
+        weights<MASK>(p, w, sc, s, k0, pc);
+        values(vt, pc);
+    }
+
+    __device__ __forceinline__ void scores(const LDS_AS char *kt, float (&s)[NS]) const {
+        const int r = threadIdx.x & (RW - 1);
+        // chunk G i + part of key row r (and r + 16): k_chunk of it is (y ^ (G i & 7)) + (G i & ~7),
+        // a few addresses, the rest offsets
         const LDS_AS char *kr = kt + r * D * 2;
-        const int y = (r & 7) ^ h;  // k_chunk(r, 2 i + h) = (y ^ (2 i & 6)) + (2 i & ~7): four addresses, the rest offsets
+        const int y = (r & 7) ^ part();
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-            const T8 a = *(const LDS_AS T8 *)(kr + (y ^ (2 * i & 6)) * 16 + (2 * i & ~7) * 16);
-            s = N::mma(a, q[i], s);
+        for (int b = 0; b < kKeys / RW; ++b) {
+            acc c = {};
+#pragma unroll
+            for (int i = 0; i < D / KD; ++i) {
+                const T8 a = *(const LDS_AS T8 *)(kr + b * RW * D * 2 + (y ^ (G * i & 7)) * 16 + (G * i & ~7) * 16);
+                c = N::mma(a, q[i], c);
+            }
+#pragma unroll
+            for (int i = 0; i < NA; ++i) s[b * NA + i] = c[i];
         }
+    }
+
+    // Their weights, as NP pieces of the cache's type, each what the ones before left over.
+    template <bool MASK>
+    __device__ __forceinline__ void weights(const AttnParams &p, const Work &w, float sc, float (&s)[NS], int k0,
+                                            T8 (&pc)[NV][NP]) {
         if constexpr (MASK) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                s[i] = sees(p, w, k0 + 8 * (i / 4) + 4 * h + i % 4) ? s[i] : -__builtin_inff();
+            for (int i = 0; i < NS; ++i) s[i] = sees(p, w, k0 + key_at(i)) ? s[i] : -__builtin_inff();
         }
         float top = s[0];
 #pragma unroll
-        for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
-        top = max_halves(top);
+        for (int i = 1; i < NS; ++i) top = fmaxf(top, s[i]);
+        top = max_row<RW>(top);
         // The maximum that weights are taken from follows the rows' own only
         // when one has grown by 2^8: weights reach 2^(6 + 8) then, and lie 2^6
         // above the type's small values otherwise.  (m = -inf: no key yet.)
         if (__any(!((top - m) * sc <= 8.0f) && top != m)) {
             const float next = fmaxf(m, top);
-            const float f = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((m - next) * sc);
+            const bool none = m == -__builtin_inff();
+            const float f = none ? 1.0f : __builtin_amdgcn_exp2f((m - next) * sc);
             m = next;
-            l *= f;
+            if (__any(!none)) {
+                l *= f;
 #pragma unroll
-            for (int i = 0; i < D / 32; ++i) o[i] *= f;
+                for (int i = 0; i < D / RW; ++i) o[i] *= f;
+            }
         }
         const float off = 6.0f - (m == -__builtin_inff() ? 0.0f : m) * sc;
         float part = 0;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
+        for (int i = 0; i < NS; ++i) {
             s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], sc, off));
             part += s[i];
         }
         l += part;
-        // P as NP pieces of the cache's type, each what the ones before left over
-        T8 pc[2][NP];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            f32x8 x = i ? __builtin_shufflevector(s, s, 8, 9, 10, 11, 12, 13, 14, 15)
-                        : __builtin_shufflevector(s, s, 0, 1, 2, 3, 4, 5, 6, 7);
+        for (int i = 0; i < NV; ++i) {
+            f32x8 x;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = s[8 * i + j];
 #pragma unroll
             for (int j = 0; j < NP; ++j) {
                 pc[i][j] = __builtin_convertvector(x, T8);
                 if (j + 1 < NP) x -= __builtin_convertvector(pc[i][j], f32x8);
             }
         }
-        // V^T: lane (d = 32 t + lane % 32, half h) takes keys 16 i + 8 e + 4 h + 0 .. 3
-        const int x = 4 * h + ((lane & 15) >> 2);  // key mod 8 of the row this lane reads
+    }
+
+    // O += weights times values.  V^T: lane (value RW t + lane % RW, part g) takes the keys of its
+    // weights, STEP (2 i + e) + 4 g + 0 .. 3.
+    __device__ __forceinline__ void values(const LDS_AS char *vt, const T8 (&pc)[NV][NP]) {
+        const int lane = threadIdx.x & 63, x = 4 * part() + ((lane & 15) >> 2);  // the key this lane's 16 lanes read for
         const LDS_AS char *vr = vt + x * D * 2 + (lane & 3) * 8;
+        constexpr int M = D >= 128 ? 7 : 3, U = RW / 16;
+        const int y = (x & M) ^ ((lane >> 4) & (U - 1));  // 32-byte unit U t + .. of a row, exchanged as in v_chunk
 #pragma unroll
-        for (int t = 0; t < D / 32; ++t)
+        for (int t = 0; t < D / RW; ++t)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const T8 v = values(vr + 16 * i * D * 2, x, t);
+            for (int i = 0; i < NV; ++i) {
+                const LDS_AS char *at = vr + 2 * i * STEP * D * 2 + ((U * t & M) ^ y) * 32 + (U * t & ~M) * 32;
+                const T8 v = __builtin_shufflevector(tr4(at), tr4(at + STEP * D * 2), 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
                 for (int j = 0; j < NP; ++j) o[t] = N::mma(v, pc[i][j], o[t]);
             }
@@ -244,14 +331,6 @@ struct Rows {
         return ok;
     }
 
-    // This lane's eight values of V^T in the 16 keys at vr: d = 32 t + lane % 32.
-    static __device__ __forceinline__ T8 values(const LDS_AS char *vr, int x, int t) {
-        constexpr int M = D >= 128 ? 7 : 3;
-        const int y = (x & M) ^ ((threadIdx.x >> 4) & 1);  // its 32-byte unit, exchanged as in v_chunk
-        const int c = ((2 * t & (M - 1)) ^ y) * 32 + (2 * t & ~M) * 32;
-        return __builtin_shufflevector(tr4(vr + c), tr4(vr + c + 8 * D * 2), 0, 1, 2, 3, 4, 5, 6, 7);
-    }
-
     static __device__ __forceinline__ T4 tr4(const LDS_AS char *at) {
         typedef short s4 __attribute__((ext_vector_type(4)));
         return __builtin_bit_cast(T4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS s4 *)at));
@@ -260,7 +339,7 @@ struct Rows {
     // O += the values of V that are not finite, where they are seen: the whole of
     // their effect, as a weight is positive.
     __device__ __forceinline__ void add_odd(const AttnParams &p, const Work &w, int k0, const LDS_AS char *vt) {
-        const int lane = threadIdx.x & 63, h = lane >> 5;
+        const int lane = threadIdx.x & 63;
         for (int key = 0; key < kKeys; ++key) {
             const LDS_AS char *vk = vt + key * D * 2;
             bool odd = false;
@@ -268,24 +347,34 @@ struct Rows {
             if (!__any(odd)) continue;
             const bool ok = sees(p, w, k0 + key);
 #pragma unroll
-            for (int t = 0; t < D / 32; ++t) {
+            for (int t = 0; t < D / RW; ++t) {
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const int d = 32 * t + 8 * (j / 4) + 4 * h + j % 4;
+                for (int j = 0; j < NA; ++j) {
+                    const int d = value_at(t, j);
                     const float v = (float)*(const LDS_AS T *)(vk + (v_chunk<D>(key, d / 8) * 8 + d % 8) * 2);
                     o[t][j] += ok && !__builtin_isfinite(v) ? v : 0.0f;
                 }
-                __builtin_amdgcn_sched_barrier(0);
+                __builtin_amdgcn_sched_barrier(0);  // one step's registers at a time
             }
         }
     }
 };
 
+// Looks at every page of the keys once, for the whole workgroup: tiles trust them then.
+__device__ __forceinline__ bool any_gaps(const AttnParams &p, const Work &w) {
+    const int shift = __builtin_ctz(p.cache.page_size);
+    const int32_t *table = p.seqs.table + (long long)w.s * p.seqs.table_stride;
+    bool bad = false;
+    if (w.lo < w.hi)
+        for (int i = (w.lo >> shift) + (int)threadIdx.x; i <= (w.hi - 1) >> shift; i += kWaves * 64)
+            bad |= (uint32_t)table[i] >= p.cache.pages;
+    return __syncthreads_or(bad);
+}
+
 template <int D, bool BF, int NP>
 __global__ __launch_bounds__(kWaves * 64, 2) void k_attn(const AttnParams p) {
-    typedef Rows<D, BF, NP> R;
+    typedef Rows<D, BF, NP, kRows> R;
     typedef typename R::T T;
-    typedef typename R::T8 T8;
     __shared__ __attribute__((aligned(1024))) char kt0[kKeys * D * 2], vt0[kKeys * D * 2];
     __shared__ __attribute__((aligned(1024))) char kt1[kKeys * D * 2], vt1[kKeys * D * 2];
     const int group = (int)(p.q.heads / p.cache.heads);
@@ -318,41 +407,17 @@ __global__ __launch_bounds__(kWaves * 64, 2) void k_attn(const AttnParams p) {
 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
     const int wrow = w.row0 + wave * kRows;  // this wave's first row
-    const int row = wrow + (lane & 31);
-    const bool live = row < w.rows;
+    const bool live = wrow + (lane & 31) < w.rows;
+    const int row = min(wrow + (lane & 31), w.rows - 1);
     const int token = sr.first + row / group, qh = w.head * group + row % group;
     R x;
     x.place = live ? place0 + row / group : -1;
-    x.m = -__builtin_inff();
-    x.l = 0;
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) x.o[i] = f32x16{};
-    {
-        const T *q = (const T *)p.q.ptr + (long long)token * p.q.token_stride + (long long)qh * p.q.head_stride;
-        typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-        // a negative scale goes into q, exactly: scores are then compared before scaling
-        const uint32_t flip = p.scale < 0 ? 0x80008000u : 0;
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-            u4 v = {0, 0, 0, 0};
-            if (live) v = *(const u4 *)(q + 16 * i + 8 * h);
-            x.q[i] = __builtin_bit_cast(T8, v ^ flip);
-        }
-    }
+    x.clear();
+    x.load_q(p, token, qh, live);
     // (a scale of 0 would make NaN of a masked score's -inf)
     const float sc = fmaxf(fabsf(p.scale) * kLog2e, 1e-37f);
 
-    // every page of the keys, looked at once: the tiles below trust them
-    w.gaps = false;
-    {
-        const int shift = __builtin_ctz(p.cache.page_size);
-        const int32_t *table = p.seqs.table + (long long)s * p.seqs.table_stride;
-        bool bad = false;
-        if (w.lo < w.hi)
-            for (int i = (w.lo >> shift) + (int)threadIdx.x; i <= (w.hi - 1) >> shift; i += kWaves * 64)
-                bad |= (uint32_t)table[i] >= p.cache.pages;
-        w.gaps = __syncthreads_or(bad);
-    }
+    w.gaps = any_gaps(p, w);
     // tiles [ta, tb) are seen whole by every row of the workgroup: the next one is
     // on its way while one is worked on; the others, at the ends, go one by one
     const int tiles = max(0, w.hi - w.lo + kKeys - 1) / kKeys;
@@ -390,7 +455,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void k_attn(const AttnParams p) {
         __syncthreads();
         load_tile<D, true>(p, w, k0, tile_page(p, w, k0), ka, va);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        odd |= clear_odd<D, BF>(va);
+        odd |= clear_odd<D, BF, kKeys / kWaves>(va + wave * (kKeys / kWaves) * D * 2);
         __syncthreads();
         if (any) x.template tile<true>(p, w, sc, k0, ka, va);
     }
@@ -403,7 +468,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void k_attn(const AttnParams p) {
             if (any) x.add_odd(p, w, k0, va);
         }
 
-    x.l = sum_halves(x.l);
+    x.l = sum_row<kRows>(x.l);
     if (!live) return;
     if (p.splits > 1) {
         const long long at = ((long long)token * p.q.heads + qh) * p.splits + blockIdx.y;
@@ -432,30 +497,253 @@ __global__ __launch_bounds__(kWaves * 64, 2) void k_attn(const AttnParams p) {
         }
 }
 
-// Joins the parts of each row, in order of the parts: D / 4 lanes a row.
+// Few rows (up to 32 of a sequence and cache head): the cache's bytes bound it.  The waves
+// of a workgroup take tiles in turn, each for itself with K and V tiles of its own: K of
+// its next tile is on its way from the moment its scores are there, V from when its values
+// are added, and nothing waits for another wave.  At the end the four sums are joined.
+template <int D, bool BF, int NP, int RW>
+__global__ __launch_bounds__(kWaves * 64, 1) void k_attn_few(const AttnParams p) {
+    typedef Rows<D, BF, NP, RW> R;
+    typedef typename R::T T;
+    constexpr int TB = kKeys * D * 2;  // bytes of a tile
+    __shared__ __attribute__((aligned(1024))) char kts[kWaves * TB], vts[kWaves * TB];
+    __shared__ float ms[kWaves][RW], ls[kWaves][RW];
+    const int group = (int)(p.q.heads / p.cache.heads);
+    const int s = blockIdx.x / p.cache.heads;
+    Work w;
+    w.s = s;
+    w.head = blockIdx.x - s * p.cache.heads;
+    const SeqRows sr = seq_rows(p.seqs.start, s, (int)p.seqs.tokens, (int)p.seqs.max_q);
+    w.rows = sr.count * group;
+    if (w.rows == 0) return;
+    const int kv = min(max(p.seqs.kv_len[s], 0), (int)p.seqs.max_kv);
+    const int first = p.seqs.kv_len[s] - (sr.end - sr.first), last = first + sr.count - 1;
+    w.lo = p.window ? max(0, first - p.window + 1) & ~(kKeys - 1) : 0;
+    w.hi = min(kv, last + 1);
+    if (p.splits > 1) {
+        const int tiles = max(0, w.hi - w.lo + kKeys - 1) / kKeys;
+        const int each = (tiles + p.splits - 1) / p.splits;
+        w.lo += (int)blockIdx.y * each * kKeys;
+        w.hi = min(w.hi, w.lo + each * kKeys);
+    }
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const bool live = (lane & (RW - 1)) < w.rows;
+    const int row = min(lane & (RW - 1), w.rows - 1);
+    LDS_AS char *const kt = (LDS_AS char *)kts + wave * TB, *const vt = (LDS_AS char *)vts + wave * TB;
+    const int32_t *table = p.seqs.table + (long long)s * p.seqs.table_stride;
+    const int shift = __builtin_ctz(p.cache.page_size);
+    // the pages of a tile's two halves
+    auto page = [&](int k0, int half) {
+        int at = min(k0 + 16 * half, w.hi - 1) >> shift;
+        asm("" : "+v"(at));
+        return table[at];
+    };
+    constexpr int RPI = 512 / D, CPR = D / 8;
+    const int r0 = lane / CPR, pc = lane % CPR;
+    const uint32_t ko = r0 * D * 2 + k_chunk<D>(r0, pc) * 16, vo = r0 * D * 2 + v_chunk<D>(r0, pc) * 16;
+    constexpr int KF = 16, VF = D >= 128 ? 32 : 0;  // how rows exchange chunks (D = 64: loads of 8 whole rows)
+    // K (or V) of the tile at k0; `checked` as in load_tile, otherwise a page that is none is
+    // read as the first (and what it gives is not used)
+    auto load = [&](const void *from, LDS_AS char *to, uint32_t off, int flips, int k0, const int (&pages)[2], bool checked,
+                    bool clear) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int id = __builtin_amdgcn_readfirstlane(pages[half]), key = k0 + 16 * half;
+            const bool ok = (uint32_t)id < p.cache.pages;
+            const int rows = checked ? (ok ? w.hi - key : 0) : 16;
+            const long long at = ((long long)(ok && rows > 0 ? id : 0) * p.cache.page_stride +
+                                  ((long long)w.head * p.cache.page_size + (key & (int)(p.cache.page_size - 1))) * D) * 2;
+            const __amdgpu_buffer_rsrc_t rs = buf_rsrc((const char *)from + at, 16 * D * 2);
+#pragma unroll
+            for (int i = 0; i < 16 / RPI; ++i) {
+                LDS_AS char *d = to + (16 * half + i * RPI) * D * 2;
+                const uint32_t o = off ^ ((i * RPI & 7) * flips);
+                if (!checked || i * RPI + r0 < rows)
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (LDS_AS void *)d, 16, o, i * 1024, 0, 0);
+                else if (clear) *(LDS_AS f32x4 *)(d + lane * 16) = f32x4{0, 0, 0, 0};
+            }
+        }
+    };
+
+    // tiles [ta, tb): seen whole by every row (if no page is missing, which is found out
+    // while the first of them is on its way)
+    const int tiles = max(0, w.hi - w.lo + kKeys - 1) / kKeys;
+    int tb = max(0, min(first + 1, w.hi) - w.lo) / kKeys;
+    int ta = p.window ? min(tb, (max(0, last - p.window + 1 - w.lo) + kKeys - 1) / kKeys) : 0;
+    int t = ta + ((wave - ta) & (kWaves - 1));  // this wave's first
+    int ids[2];
+    if (t < tb) {
+        ids[0] = page(w.lo + t * kKeys, 0);
+        ids[1] = page(w.lo + t * kKeys, 1);
+        load(p.cache.k, kt, ko, KF, w.lo + t * kKeys, ids, false, false);
+        load(p.cache.v, vt, vo, VF, w.lo + t * kKeys, ids, false, false);
+    }
+    R x;
+    x.place = live ? first + row / group : -1;
+    x.clear();
+    x.load_q(p, sr.first + row / group, w.head * group + row % group, live);
+    const float sc = fmaxf(fabsf(p.scale) * kLog2e, 1e-37f);
+    w.gaps = any_gaps(p, w);
+    if (w.gaps) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        ta = tb = 0;
+    }
+    typename R::T8 pcs[R::NV][NP];
+    float sco[R::NS];
+    for (; t < tb; t += kWaves) {
+        const int k0 = w.lo + t * kKeys, k1 = k0 + kWaves * kKeys;
+        ids[0] = page(k1, 0);
+        ids[1] = page(k1, 1);
+        // K is there when no more than V's loads are on their way
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(32 / RPI) : "memory");
+        x.scores(kt, sco);
+        x.template weights<false>(p, w, sc, sco, k0, pcs);
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        if (t + kWaves < tb) load(p.cache.k, kt, ko, KF, k1, ids, false, false);
+        x.values(vt, pcs);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // V has been read
+        if (t + kWaves < tb) load(p.cache.v, vt, vo, VF, k1, ids, false, false);
+    }
+    bool odd = false;
+    for (int t = wave; t < tiles; t += kWaves) {
+        if (t >= ta && t < tb) continue;
+        const int k0 = w.lo + t * kKeys, ids[2] = {page(k0, 0), page(k0, 1)};
+        load(p.cache.k, kt, ko, KF, k0, ids, true, false);
+        load(p.cache.v, vt, vo, VF, k0, ids, true, true);
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        odd |= clear_odd<D, BF, kKeys>(vt);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        x.template tile<true>(p, w, sc, k0, kt, vt);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+    if (__builtin_expect(__any(odd), 0))
+        for (int t = wave; t < tiles; t += kWaves) {
+            if (t >= ta && t < tb) continue;
+            const int k0 = w.lo + t * kKeys, ids[2] = {page(k0, 0), page(k0, 1)};
+            load(p.cache.v, vt, vo, VF, k0, ids, true, true);
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            x.add_odd(p, w, k0, vt);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        }
+
+    // the waves' sums: to a common maximum, into LDS (a quadruple of values of the rows side by
+    // side; the first TB bytes in the wave's K tile, what is more in its V tile), then added in order
+    const int col = lane & (RW - 1);
+    x.l = sum_row<RW>(x.l);
+    if (lane < RW) {
+        ms[wave][col] = x.m;
+        ls[wave][col] = x.l;
+    }
+    __syncthreads();
+    float m = ms[0][col];
+#pragma unroll
+    for (int i = 1; i < kWaves; ++i) m = fmaxf(m, ms[i][col]);
+    constexpr int HALF = TB / (RW * 16);  // quadruples of a tile's room
+    if (x.l != 0) {
+        const float f = __builtin_amdgcn_exp2f((x.m - m) * sc);
+#pragma unroll
+        for (int t = 0; t < D / RW; ++t)
+#pragma unroll
+            for (int j = 0; j < R::NA / 4; ++j) {
+                const int quad = R::value_at(t, 4 * j) / 4;
+                f32x4 v;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = x.o[t][4 * j + i] * f;
+                *(LDS_AS f32x4 *)((RW * t < 4 * HALF ? kt : vt - TB) + (quad * RW + col) * 16) = v;
+            }
+    }
+    __syncthreads();
+    float fs[kWaves], l = 0;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+        fs[i] = ls[i][col];
+        const float e = ms[i][col] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((ms[i][col] - m) * sc);
+        l += ls[i][col] * e;
+    }
+    if (!live) return;
+    const int token = sr.first + row / group, qh = w.head * group + row % group;
+    const long long part = ((long long)token * p.q.heads + qh) * p.splits + blockIdx.y;
+    if (p.splits > 1 && threadIdx.x < RW) p.stat[part] = make_float2(m * sc, l);
+    if (p.splits > 1 && l == 0) return;
+    const long long to = (long long)token * p.out.token_stride + (long long)qh * p.out.head_stride;
+    const float inv = l == 0 ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int u = 0; u < D / 4 * RW / (kWaves * 64); ++u) {
+        const int quad = threadIdx.x / RW + u * (kWaves * 64 / RW);
+        f32x4 o = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i)
+            if (fs[i] != 0)
+                o += *(const LDS_AS f32x4 *)((LDS_AS char *)(quad < HALF ? kts : vts - TB) + i * TB + (quad * RW + col) * 16);
+        if (p.splits > 1) {
+            *(f32x4 *)(p.part + part * D + 4 * quad) = o;
+            continue;
+        }
+        o = l == 0 ? f32x4{0, 0, 0, 0} : o * inv;
+        if (p.out.type == M27Q_TYPE_F32) *(f32x4 *)((float *)p.out.ptr + to + 4 * quad) = o;
+        else *(typename R::T4 *)((T *)p.out.ptr + to + 4 * quad) = __builtin_convertvector(o, typename R::T4);
+    }
+}
+
+// Joins the parts of each row, in order of the parts: a wave a row (two for D = 128, four
+// for 64), each part's statistics in a lane (at most 64 parts), then the sums, several on
+// their way at a time.
 template <int D, bool BF>
 __global__ __launch_bounds__(256) void k_attn_join(const AttnParams p) {
-    constexpr int L = D / 4, RPB = 256 / L;
+    constexpr int L = D / 4, RPW = 64 / L;
     const SeqRows sr = seq_rows(p.seqs.start, blockIdx.y, (int)p.seqs.tokens, (int)p.seqs.max_q);
-    const int row = blockIdx.x * RPB + threadIdx.x / L, d = 4 * (threadIdx.x % L);
-    if (row >= sr.count * (int)p.q.heads) return;
-    const int token = sr.first + row / (int)p.q.heads, qh = row % (int)p.q.heads;
-    const long long at = ((long long)token * p.q.heads + qh) * p.splits;
-    float m = -__builtin_inff();
-    for (int i = 0; i < p.splits; ++i) {
-        const float2 st = p.stat[at + i];
-        if (st.y != 0) m = fmaxf(m, st.x);
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int first = (blockIdx.x * 4 + wave) * RPW, d = 4 * (lane % L), rows = sr.count * (int)p.q.heads;
+    if (first >= rows) return;
+    const long long base = (long long)sr.first * p.q.heads;
+    const int mine = lane / L, row = first + mine;
+    const bool live = row < rows;
+    const float *from = p.part + (base + (live ? row : first)) * p.splits * D + d;
+    constexpr int AT = 8;  // parts on their way at a time, the first before the statistics are there
+    f32x4 v[AT];
+#pragma unroll
+    for (int i = 0; i < AT; ++i) v[i] = *(const f32x4 *)(from + (long long)min(i, p.splits - 1) * D);
+    float f[RPW], inv[RPW];  // lane i: part i's factor of each of the wave's rows
+#pragma unroll
+    for (int r = 0; r < RPW; ++r) {
+        float2 st = p.stat[(base + min(first + r, rows - 1)) * p.splits + min(lane, p.splits - 1)];
+        if (lane >= p.splits) st.y = 0;
+        float m = st.y != 0 ? st.x : -__builtin_inff();
+#pragma unroll
+        for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+        f[r] = st.y != 0 ? __builtin_amdgcn_exp2f(st.x - m) : 0.0f;
+        float l = st.y * f[r];
+        f[r] = st.y != 0 ? f[r] : -1.0f;  // no key: its sums were not written
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) l += __shfl_xor(l, o);
+        inv[r] = l == 0 ? 0.0f : 1.0f / l;
     }
-    float l = 0;
     f32x4 o = {};
-    for (int i = 0; i < p.splits; ++i) {
-        const float2 st = p.stat[at + i];
-        if (st.y == 0) continue;  // no key: its sums were not written
-        const float f = __builtin_amdgcn_exp2f(st.x - m);
-        l += st.y * f;
-        o += *(const f32x4 *)(p.part + (at + i) * D + d) * f;
+    for (int i0 = 0; i0 < p.splits; i0 += AT) {
+        f32x4 u[AT];
+#pragma unroll
+        for (int i = 0; i < AT; ++i) u[i] = v[i];
+        if (i0 + AT < p.splits) {
+#pragma unroll
+            for (int i = 0; i < AT; ++i) v[i] = *(const f32x4 *)(from + (long long)min(i0 + AT + i, p.splits - 1) * D);
+        }
+#pragma unroll
+        for (int i = 0; i < AT; ++i) {
+            float w = __shfl(f[0], (i0 + i) & 63);
+#pragma unroll
+            for (int r = 1; r < RPW; ++r) {
+                const float y = __shfl(f[r], (i0 + i) & 63);
+                w = mine == r ? y : w;
+            }
+            o = i0 + i >= p.splits || w == -1.0f ? o : o + u[i] * w;
+        }
     }
-    o = l == 0 ? f32x4{0, 0, 0, 0} : o * (1.0f / l);
+    if (!live) return;
+    float scale = inv[0];
+#pragma unroll
+    for (int r = 1; r < RPW; ++r) scale = mine == r ? inv[r] : scale;
+    o = scale == 0 ? f32x4{0, 0, 0, 0} : o * scale;
+    const int token = sr.first + row / (int)p.q.heads, qh = row % (int)p.q.heads;
     const long long to = (long long)token * p.out.token_stride + (long long)qh * p.out.head_stride + d;
     if (p.out.type == M27Q_TYPE_F32) *(f32x4 *)((float *)p.out.ptr + to) = o;
     else if constexpr (BF) *(bf16x4 *)((__bf16 *)p.out.ptr + to) = __builtin_convertvector(o, bf16x4);
@@ -473,12 +761,22 @@ namespace {
 
 template <int D, bool BF>
 hipError_t launch_t(const AttnParams &p, const AttnPlan &plan, hipStream_t s) {
-    const dim3 grid((unsigned)attn_groups(p.seqs, p.q.heads, p.cache), p.splits);
     constexpr int NP = BF ? 3 : 2;
-    if (p.out.type == M27Q_TYPE_F32) hipLaunchKernelGGL((k_attn<D, BF, NP>), grid, dim3(kWaves * 64), 0, s, p);
-    else hipLaunchKernelGGL((k_attn<D, BF, 1>), grid, dim3(kWaves * 64), 0, s, p);
+    const bool full = p.out.type == M27Q_TYPE_F32;
+    if (plan.few) {
+        const dim3 grid(p.seqs.n * p.cache.heads, p.splits);
+        const bool half = p.seqs.max_q * (p.q.heads / p.cache.heads) <= 16;
+        if (full && half) hipLaunchKernelGGL((k_attn_few<D, BF, NP, 16>), grid, dim3(kWaves * 64), 0, s, p);
+        else if (full) hipLaunchKernelGGL((k_attn_few<D, BF, NP, kRows>), grid, dim3(kWaves * 64), 0, s, p);
+        else if (half) hipLaunchKernelGGL((k_attn_few<D, BF, 1, 16>), grid, dim3(kWaves * 64), 0, s, p);
+        else hipLaunchKernelGGL((k_attn_few<D, BF, 1, kRows>), grid, dim3(kWaves * 64), 0, s, p);
+    } else {
+        const dim3 grid((unsigned)attn_groups(p.seqs, p.q.heads, p.cache), p.splits);
+        if (full) hipLaunchKernelGGL((k_attn<D, BF, NP>), grid, dim3(kWaves * 64), 0, s, p);
+        else hipLaunchKernelGGL((k_attn<D, BF, 1>), grid, dim3(kWaves * 64), 0, s, p);
+    }
     if (p.splits > 1) {
-        constexpr int RPB = 256 / (D / 4);
+        constexpr int RPB = 4 * 64 / (D / 4);
         const dim3 g2((p.seqs.max_q * p.q.heads + RPB - 1) / RPB, p.seqs.n);
         hipLaunchKernelGGL((k_attn_join<D, BF>), g2, dim3(256), 0, s, p);
     }
@@ -487,13 +785,16 @@ hipError_t launch_t(const AttnParams &p, const AttnPlan &plan, hipStream_t s) {
 
 }  // namespace
 
-// Parts of the keys: enough workgroups for two on each CU, parts of 256 keys at least.
+// Parts of the keys.  Rows of several tiles: enough workgroups for two on each CU, parts of
+// 256 keys at least.  Few rows: four on each CU, for ragged sequences to even out, parts of
+// 128 keys at least, a tile for each wave.
 AttnPlan attn_plan(const m27q_seqs &seqs, uint32_t q_heads, const m27q_cache &cache, int cus) {
-    const long long wgs = attn_groups(seqs, q_heads, cache);
-    const long long want = (2ll * cus + wgs - 1) / wgs, most = (seqs.max_kv + 255) / 256;
+    const bool few = (long long)seqs.max_q * (q_heads / cache.heads) <= kRows;
+    const long long wgs = attn_groups(seqs, q_heads, cache), least = few ? 128 : 256;
+    const long long want = ((few ? 4ll : 2ll) * cus + wgs - 1) / wgs, most = (seqs.max_kv + least - 1) / least;
     long long splits = want < most ? want : most;
     if (splits > kMaxSplits) splits = kMaxSplits;
-    return {0, splits < 1 ? 1 : (int)splits};
+    return {few, splits < 1 ? 1 : (int)splits};
 }
 
 size_t attn_scratch(const m27q_seqs &seqs, uint32_t q_heads, uint32_t dim, int splits) {
