@@ -578,6 +578,17 @@ __global__ __launch_bounds__(kWaves * 64, 1) void k_attn_few(const AttnParams p)
         load(p.cache.k, kt, ko, KF, w.lo + t * kKeys, ids, false, false);
         load(p.cache.v, vt, vo, VF, w.lo + t * kKeys, ids, false, false);
     }
+    // a wave that has none of them asks for its first one of the others
+    int there = -1;
+    if (t >= tb) {
+        for (there = wave; there >= ta && there < tb;) there += kWaves;
+        if (there < tiles) {
+            ids[0] = page(w.lo + there * kKeys, 0);
+            ids[1] = page(w.lo + there * kKeys, 1);
+            load(p.cache.k, kt, ko, KF, w.lo + there * kKeys, ids, true, false);
+            load(p.cache.v, vt, vo, VF, w.lo + there * kKeys, ids, true, true);
+        }
+    }
     R x;
     x.place = live ? first + row / group : -1;
     x.clear();
@@ -607,9 +618,14 @@ __global__ __launch_bounds__(kWaves * 64, 1) void k_attn_few(const AttnParams p)
     bool odd = false;
     for (int t = wave; t < tiles; t += kWaves) {
         if (t >= ta && t < tb) continue;
-        const int k0 = w.lo + t * kKeys, ids[2] = {page(k0, 0), page(k0, 1)};
-        load(p.cache.k, kt, ko, KF, k0, ids, true, false);
-        load(p.cache.v, vt, vo, VF, k0, ids, true, true);
+        const int k0 = w.lo + t * kKeys;
+        if (t != there) {
+            ids[0] = page(k0, 0);
+            ids[1] = page(k0, 1);
+            load(p.cache.k, kt, ko, KF, k0, ids, true, false);
+            load(p.cache.v, vt, vo, VF, k0, ids, true, true);
+        }
+        there = -1;
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         odd |= clear_odd<D, BF, kKeys>(vt);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -786,12 +802,16 @@ hipError_t launch_t(const AttnParams &p, const AttnPlan &plan, hipStream_t s) {
 }  // namespace
 
 // Parts of the keys.  Rows of several tiles: enough workgroups for two on each CU, parts of
-// 256 keys at least.  Few rows: four on each CU, for ragged sequences to even out, parts of
-// 128 keys at least, a tile for each wave.
+// 256 keys at least.  Few rows: one workgroup on each CU (dim 256: its tiles take the LDS),
+// or two, and twice that from 64 pairs of sequence and head on, for ragged ones to even out,
+// unless the pairs fill the CUs; parts of 128 keys at least, a tile for each wave.  Measured
+// at one, two and four times the CUs: dim 256, 2 sequences of 32768 keys 63 / 74 / 75 us, 32
+// of 16381 301 / 294 / 297, 64 of 3000 117 / 123 / 129; dim 128, 2 of 16384 31 / 30 / 37.
 AttnPlan attn_plan(const m27q_seqs &seqs, uint32_t q_heads, const m27q_cache &cache, int cus) {
     const bool few = (long long)seqs.max_q * (q_heads / cache.heads) <= kRows;
     const long long wgs = attn_groups(seqs, q_heads, cache), least = few ? 128 : 256;
-    const long long want = ((few ? 4ll : 2ll) * cus + wgs - 1) / wgs, most = (seqs.max_kv + least - 1) / least;
+    const long long once = few ? (long long)cus * (cache.dim == 256 ? 1 : 2) * (wgs < 64 || wgs >= cus ? 1 : 2) : 2ll * cus;
+    const long long want = (once + wgs - 1) / wgs, most = (seqs.max_kv + least - 1) / least;
     long long splits = want < most ? want : most;
     if (splits > kMaxSplits) splits = kMaxSplits;
     return {few, splits < 1 ? 1 : (int)splits};
