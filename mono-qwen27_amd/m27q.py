@@ -468,31 +468,39 @@ def topk_noalloc(logits, k: int, idx, val, stream=None) -> None:
 
 # ---------------------------------------------------------- token mixers --
 
-_pack_rows = struct.Struct("=QIIIIqq").pack   # m27q_rows
-_pack_delta = struct.Struct("=6Q40s40s40s40s5If").pack  # m27q_delta
-_value_types = None
+# These calls go through m27q_torch.so (csrc/m27q_torch.cpp), which reads the
+# tensors itself: through ctypes the reading took 2 to 5 us a call, as long as the
+# launch.  Records of plans, caches and sequences, which a program keeps, are packed
+# when they are made.
+
+_mixers_so = None
 
 
-def _type_of(t) -> int:
-    global _value_types
-    if _value_types is None:
-        torch = _torch()
-        _value_types = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
-    return _value_types.get(t.dtype, 0xffffffff)  # others: for the library to refuse
+def _mixers():
+    """The module of the token mixers' calls."""
+    global _mixers_so
+    if _mixers_so is None:
+        import importlib.util
+        _torch()  # its libraries are the module's
+        lib()
+        path = os.path.join(PKG_DIR, "m27q_torch.so")
+        if not os.path.exists(path):
+            raise RuntimeError(f"{path} is not built: run __graft_entry__.build()")
+        spec = importlib.util.spec_from_file_location("m27q_torch", path)
+        m = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(m)
+        m.streams(_stream)
+        _mixers_so = m
+    return _mixers_so
 
 
-def _rows(t, tokens: int, what: str):
-    """A [tokens, heads, dim] tensor as its m27q_rows record."""
-    n, h, d = t.shape
-    a, b, c = t.stride()
-    if n != tokens or (c != 1 and d != 1):
-        raise M27QError(2, what)
-    return _pack_rows(t.data_ptr(), _type_of(t), h, d, 0, a, b)
+def _value_type(t) -> int:
+    torch = _torch()
+    return {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}.get(t.dtype, 0xffffffff)
 
 
 def _int32(t, what: str):
-    torch = _torch()
-    if t.dtype != torch.int32 or not t.is_contiguous():
+    if t.dtype != _torch().int32 or not t.is_contiguous():
         raise M27QError(4, what)
     return t.data_ptr()
 
@@ -508,8 +516,7 @@ class Rope:
     """A model's rotary positions (m27q_rope_plan): turns as a device tensor of rot / 2 int64 values."""
 
     def __init__(self, turns, rot: int, layout: int = ROPE_HALF, mscale: float = 1.0):
-        torch = _torch()
-        if turns.dtype != torch.int64 or not turns.is_contiguous() or 2 * turns.numel() < rot:
+        if turns.dtype != _torch().int64 or not turns.is_contiguous() or 2 * turns.numel() < rot:
             raise M27QError(4, "Rope")
         self.turns = turns
         self.packed = bytes(RopePlan(turns.data_ptr(), rot, layout, mscale, 0))
@@ -532,7 +539,7 @@ class KVCache:
         if k.stride()[1:] != (size * dim, dim, 1):
             raise M27QError(4, "KVCache")
         self.k, self.v, self.page_size = k, v, size
-        self.packed = bytes(CacheDesc(k.data_ptr(), v.data_ptr(), _type_of(k), pages, heads, size, dim, 0,
+        self.packed = bytes(CacheDesc(k.data_ptr(), v.data_ptr(), _value_type(k), pages, heads, size, dim, 0,
                                       k.stride(0)))
 
 
@@ -551,22 +558,14 @@ class Seqs:
 
 def rope(rope: Rope, pos, x, out, stream=None) -> None:
     """out <- x rotated by pos; x and out [tokens, heads, dim]."""
-    n = pos.numel()
-    st = (_fast or _calls()).m27q_rope(rope.packed, _int32(pos, "m27q_rope"), n, _rows(x, n, "m27q_rope"),
-                                       _rows(out, n, "m27q_rope"), _stream(stream))
+    st = (_mixers_so or _mixers()).rope(rope.packed, pos, x, out, stream)
     if st:
         check(st, "m27q_rope")
 
 
 def rope_append(rope: Rope, pos, seqs: Seqs, cache: KVCache, q, q_out, k, v, stream=None) -> None:
     """q_out <- q rotated; k rotated and v into the cache; q, k, v [tokens, heads, dim]."""
-    n = seqs.tokens
-    if pos.numel() != n:
-        raise M27QError(2, "m27q_rope_append")
-    st = (_fast or _calls()).m27q_rope_append(
-        rope.packed, _int32(pos, "m27q_rope_append"), seqs.packed, cache.packed, _rows(q, n, "m27q_rope_append"),
-        _rows(q_out, n, "m27q_rope_append"), _rows(k, n, "m27q_rope_append"), _rows(v, n, "m27q_rope_append"),
-        _stream(stream))
+    st = (_mixers_so or _mixers()).rope_append(rope.packed, pos, seqs.packed, cache.packed, q, q_out, k, v, stream)
     if st:
         check(st, "m27q_rope_append")
 
@@ -577,10 +576,7 @@ def attn_scratch_bytes(seqs: Seqs, q_heads: int, cache: KVCache) -> int:
 
 def attn_paged(seqs: Seqs, cache: KVCache, q, out, scratch, scale: float, window: int = 0, stream=None) -> None:
     """out <- attention of the rows q [tokens, heads, dim] over their sequences' pages."""
-    n = seqs.tokens
-    st = (_fast or _calls()).m27q_attn_paged(
-        seqs.packed, cache.packed, _rows(q, n, "m27q_attn_paged"), _rows(out, n, "m27q_attn_paged"), scale, window,
-        scratch.data_ptr(), scratch.numel() * scratch.element_size(), _stream(stream))
+    st = (_mixers_so or _mixers()).attn_paged(seqs.packed, cache.packed, q, out, scratch, scale, window, stream)
     if st:
         check(st, "m27q_attn_paged")
 
@@ -593,25 +589,7 @@ def delta_rule(start, q, k, v, g, beta, state, state_out, out, scratch, scale: f
                head_map: int = HEADS_GROUPED, stream=None) -> None:
     """The gated delta rule over each sequence's rows: out and state_out <- rows from state [slots, heads, dv, dk]
     (state or state_out may be None, state_out may be state)."""
-    what = "m27q_delta_rule"
-    torch = _torch()
-    n, h, dv = v.shape
-    held = state if state is not None else state_out
-    shape = (held.shape[0] if held is not None else 0, h, dv, k.shape[2])
-    for s in (state, state_out):
-        if s is not None and (s.shape != shape or s.dtype != torch.float32 or not s.is_contiguous()):
-            raise M27QError(2, what)
-    for x in (g, beta):
-        if x.shape != (n, h) or x.dtype != torch.float32 or not x.is_contiguous():
-            raise M27QError(2, what)
-    seqs = start.numel() - 1
-    if slots is not None and slots.numel() != seqs:
-        raise M27QError(2, what)
-    d = _pack_delta(_int32(start, what), 0 if slots is None else _int32(slots, what), g.data_ptr(), beta.data_ptr(),
-                    0 if state is None else state.data_ptr(), 0 if state_out is None else state_out.data_ptr(),
-                    _rows(q, n, what), _rows(k, n, what), _rows(v, n, what), _rows(out, n, what), seqs, n, max_len,
-                    shape[0], head_map, scale)
-    st = (_fast or _calls()).m27q_delta_rule(d, scratch.data_ptr(), scratch.numel() * scratch.element_size(),
-                                             _stream(stream))
+    st = (_mixers_so or _mixers()).delta_rule(start, q, k, v, g, beta, state, state_out, out, scratch, scale, max_len,
+                                              slots, head_map, stream)
     if st:
-        check(st, what)
+        check(st, "m27q_delta_rule")
