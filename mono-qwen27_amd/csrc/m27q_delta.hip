@@ -102,8 +102,7 @@ __global__ __launch_bounds__(64) void k_delta_rows(const m27q_delta d) {
 //   S <- e^(G_C) S + (diag(e^(G_C - G)) U)^T K.
 // A first launch, parallel over chunks, makes T = (I + A)^-1 diag(beta), P and the
 // factors; a second one walks the chunks of a sequence with 32 rows of a head's
-// state, 8 waves: three products that wait for each other a chunk, the state in
-// accumulators throughout.
+// state, three products that wait for each other a chunk.
 //
 // Products are fp32-accurate on the bf16 matrix units, 16 times the rate of the
 // fp32 ones: a value is the sum of three bf16 values (8 + 8 + 8 bits; F16 takes
@@ -277,8 +276,9 @@ __global__ __launch_bounds__(256) void k_delta_prepare(const m27q_delta d, float
             }
             const double last = __shfl(x, 63);
             G[lane] = x;
-            B[lane] = in ? d.beta[at] : 0.0f;
-            rec[kEg + lane] = expf((float)x);
+            const float beta = in ? d.beta[at] : 0.0f;
+            B[lane] = beta;
+            rec[kEg + lane] = __builtin_isfinite(beta) ? expf((float)x) : __builtin_nanf("");  // to be seen by the walk
             rec[kEc + lane] = expf((float)(last - x));
             if (lane == 0) rec[kLast] = expf((float)last);
         }
@@ -349,51 +349,121 @@ __global__ __launch_bounds__(256) void k_delta_prepare(const m27q_delta d, float
     }
 }
 
-// A chunk's inputs in the registers of its lanes: wave m + 4 j of eight has rows 16 m ..
-// of the chunk and 16 j .. of the slice's state rows.  Each part is asked for again, for the
-// next chunk, as soon as it has been used.
-template <int DK, typename T>
-struct Chunk {
-    typename In<T>::raw k[DK / 64], q[DK / 32];  // of K's rows half the values, the j-th
-    bf16x8 t[2][3], p[2][3];
-    T v[4];               // V at rows 16 m + 4 (lane / 16) + i, value 16 j + lane % 16 of the slice
-    f32x4 eg, ec;
-    float last;
+// c[j] += a b[j], as above with one left operand.
+template <int NC, int NA, int NB>
+__device__ __forceinline__ void mma(const bf16x8 (&a)[NA], const bf16x8 (&b)[NC][NB], f32x4 (&c)[NC]) {
+#pragma unroll
+    for (int o = 2; o >= 0; --o)
+#pragma unroll
+        for (int i = 0; i < NA; ++i)
+            if (o - i >= 0 && o - i < NB)
+#pragma unroll
+                for (int j = 0; j < NC; ++j)
+                    c[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[j][o - i], c[j], 0, 0, 0);
+}
 
-    __device__ __forceinline__ void load_k(const m27q_delta &d, const SeqRows &sr, int kh, int t0, int m, int j) {
-        load_rows<DK / 64, T>(d.k, sr.first, kh, t0 + 16 * m, sr.count, j * (DK / 64), k);
-    }
-    __device__ __forceinline__ void load_q(const m27q_delta &d, const SeqRows &sr, int kh, int t0, int m) {
-        load_rows<DK / 32, T>(d.q, sr.first, kh, t0 + 16 * m, sr.count, 0, q);
-    }
-    __device__ __forceinline__ void load_v(const m27q_delta &d, const SeqRows &sr, int head, int t0, int v0, int m, int j) {
-        const int lane = threadIdx.x & 63, row = t0 + 16 * m + 4 * (lane >> 4);
-        const T *x = (const T *)d.v.ptr + (long long)sr.first * d.v.token_stride + (long long)head * d.v.head_stride +
-                     min(v0 + 16 * j, (int)d.v.dim - 16);
+// Place of a value in LDS, rows of W values: the 32-byte units of a row are exchanged by the row,
+// so that 8 rows' reads of a column of 16 bytes, and a transposing read's 4 rows of a unit, meet
+// different banks.
+template <int W>
+__device__ __forceinline__ int lds_at(int row, int col) {
+    const int unit = W == 128 ? ((col >> 4) ^ row) & 7 : ((col >> 4) ^ (row >> 1)) & 3;
+    return row * W + unit * 16 + (col & 15);
+}
+
+// A record's operand blocks of row tile m (see kT): its first, and its second or the first again.
+__device__ __forceinline__ void load_blocks(const float *from, int m, bf16x8 (&x)[2][3]) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            v[i] = x[(unsigned long long)(uint32_t)min(row + i, sr.count - 1) * (uint32_t)d.v.token_stride + (lane & 15)];
+    for (int i = 0; i < 2; ++i) {
+        const __bf16 *b = (const __bf16 *)from + block_of(m, m < 2 ? 0 : i) * kBlockHalves + (threadIdx.x & 63) * 8;
+#pragma unroll
+        for (int u = 0; u < 3; ++u) x[i][u] = *(const bf16x8 *)(b + u * 512);
     }
-    __device__ __forceinline__ void load_blocks(const float *from, int m, bf16x8 (&x)[2][3]) {
-        const int lane = threadIdx.x & 63;
+}
+
+// A chunk's rows one by one, for a chunk with a value that is not finite: its products would
+// carry it, times zeros, to the rows before it.  The four waves that hold the state (as in
+// k_delta_chunks) sum over their columns and, through `sums`, over each other's; two barriers
+// a row.
+template <int DK, typename T>
+__device__ __forceinline__ void row_by_row(const m27q_delta &d, const SeqRows &sr, int kh, int head, int t0, int v0,
+                                                     int mt, f32x4 (&S)[DK / 64][2], float *sums, T *out) {
+    constexpr int MT = DK / 64;
+    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    auto total = [&](float x) {  // over the lanes of a state row
+        x += __shfl_xor(x, 16);
+        return x + __shfl_xor(x, 32);
+    };
+    for (int t = t0; t < min(t0 + kC, sr.count); ++t) {
+        const long long row = sr.first + t;
+        const T *k = (const T *)d.k.ptr + row * d.k.token_stride + (long long)kh * d.k.head_stride + 16 * MT * mt + 4 * g;
+        const T *q = (const T *)d.q.ptr + row * d.q.token_stride + (long long)kh * d.q.head_stride + 16 * MT * mt + 4 * g;
+        const T *v = (const T *)d.v.ptr + row * d.v.token_stride + (long long)head * d.v.head_stride;
+        const float e = expf(d.g[row * d.v.heads + head]), beta = d.beta[row * d.v.heads + head];
+        float kk[MT][4], part[2] = {};
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const __bf16 *b = (const __bf16 *)from + block_of(m, m < 2 ? 0 : i) * kBlockHalves + lane * 8;
+        for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int u = 0; u < 3; ++u) x[i][u] = *(const bf16x8 *)(b + u * 512);
+            for (int i = 0; i < 4; ++i) {
+                kk[m][i] = (float)k[16 * m + i];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    S[m][j][i] *= e;
+                    part[j] += S[m][j][i] * kk[m][i];
+                }
+            }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const float x = total(part[j]);
+            if (g == 0) sums[mt * kSlice + 16 * j + n] = x;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            float x = 0;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) x += sums[w * kSlice + 16 * j + n];
+            const float u = beta * ((float)v[min(v0 + 16 * j, (int)d.v.dim - 16) + n] - x);
+            part[j] = 0;
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    S[m][j][i] += u * kk[m][i];
+                    part[j] += S[m][j][i] * (float)q[16 * m + i];
+                }
+            const float y = total(part[j]);
+            if (g == 0) sums[(4 + mt) * kSlice + 16 * j + n] = y;
+        }
+        __syncthreads();
+        if (mt == 0 && lane < kSlice && v0 + lane < (int)d.v.dim) {
+            float o = 0;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) o += sums[(4 + w) * kSlice + lane];
+            out[(long long)t * d.out.token_stride + lane] = (T)(d.scale * o);
         }
     }
-};
+}
 
+// The walk over a sequence's chunks, 32 state rows of a head a workgroup.  Four waves carry
+// the state (16 MT of its columns each, in accumulators) through the three products that wait
+// for each other; four more, one on each SIMD beside them, do what nothing waits for: Q S^T
+// and P U, the outputs, and the next chunk's K in pieces.  Wave m of either four has rows
+// 16 m .. of the chunk.  Three barriers a chunk part
+//   1  X = K S^T, R = V - diag(e^G) X        | K of the next chunk into pieces
+//   2  U = T R                               | Q S^T
+//   3  S <- e^(G_C) S + K^T diag(..) U       | K's pieces to LDS, out = .. Q S^T + P U
+// Operands that come from memory are asked for again, for the next chunk, as soon as they have
+// been used, without branches (a load under one would keep later waits from telling it apart).
 template <int DK, typename T>
 __global__ __launch_bounds__(512) void k_delta_chunks(const m27q_delta d, const float *scratch) {
     constexpr int N = In<T>::N, KS = DK / 32, MT = DK / 64;
-    constexpr int LK = DK + 16, LS = DK + 8, LU = kC + 8;
-    __shared__ __attribute__((aligned(16))) __bf16 kp[N * kC * LK];       // K's pieces [N][row][dk]
-    __shared__ __attribute__((aligned(16))) __bf16 sb[3 * kSlice * LS];   // the state's [3][dv][dk]
-    __shared__ __attribute__((aligned(16))) __bf16 rb[3 * kSlice * LU];   // the right-hand sides' [3][dv][row]
-    __shared__ __attribute__((aligned(16))) __bf16 ub[3 * kSlice * LU];   // U's
-    __shared__ __attribute__((aligned(16))) __bf16 wb[3 * kSlice * LU];   // diag(e^(G_C - G)) U's
+    __shared__ __attribute__((aligned(16))) __bf16 kp[N * kC * DK];         // K's pieces [N][row][dk]
+    __shared__ __attribute__((aligned(16))) __bf16 sb[3 * kSlice * DK];     // the state's [3][dv][dk]
+    __shared__ __attribute__((aligned(16))) __bf16 rb[3 * kSlice * kC];     // the right-hand sides' [3][dv][row]
+    __shared__ __attribute__((aligned(16))) __bf16 ub[3 * kSlice * kC];     // U's
+    __shared__ __attribute__((aligned(16))) __bf16 wb[3 * kSlice * kC];     // diag(e^(G_C - G)) U's
+    __shared__ int odd;                                                     // some right-hand side is not finite
     // workgroups of one key head and sequence are gridDim.x apart, so that where that is a
     // multiple of the XCDs they share an L2
     const int kheads = (int)d.k.heads, per = (int)d.v.heads / kheads, slices = (int)(d.v.dim + kSlice - 1) / kSlice;
@@ -403,147 +473,249 @@ __global__ __launch_bounds__(512) void k_delta_chunks(const m27q_delta d, const 
     const SeqRows sr = seq_rows(d.start, s, (int)d.tokens, (int)d.max_len);
     const int slot = d.slots ? d.slots[s] : s;
     const bool held = slot >= 0 && (uint32_t)slot < d.n_slots;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), mt = wave & 3, nt = wave >> 2;
-    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), mt = wave & 3;
+    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, row = 16 * mt + 4 * g;
     const float *rec = scratch + (chunk_place(sr.first, s) * d.v.heads + head) * (long long)kRecord;
-    const long long step = (long long)d.v.heads * kRecord;
+    const long long step = (long long)d.v.heads * kRecord;  // behind the last chunk's there is room for one more
+    const bool in[2] = {v0 < (int)d.v.dim, v0 + 16 < (int)d.v.dim};
+    const long long at = (((long long)slot * d.v.heads + head) * d.v.dim + v0 + n) * DK + 16 * MT * mt + 4 * g;
+    T *const out = (T *)d.out.ptr + (long long)sr.first * d.out.token_stride + (long long)head * d.out.head_stride + v0;
 
-    // the state: dk = 16 (MT mt + m) + 4 g + i of row v0 + 16 nt + n
-    f32x4 S[MT];
-    const long long at = (((long long)slot * d.v.heads + head) * d.v.dim + v0 + 16 * nt + n) * DK + 16 * MT * mt + 4 * g;
-    const bool in = v0 + 16 * nt < (int)d.v.dim;
+    if (sr.count == 0) {  // its state stays
+        if (wave < 4 && held && d.state_out)
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        S[m] = f32x4{};
-        if (held && d.state_in && in) S[m] = *(const f32x4 *)(d.state_in + at + 16 * m);
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+                    if (in[j])
+                        *(f32x4 *)(d.state_out + at + 16 * j * DK + 16 * m) =
+                            d.state_in ? *(const f32x4 *)(d.state_in + at + 16 * j * DK + 16 * m) : f32x4{};
+        return;
     }
-    auto put_state = [&]() {
+    if (threadIdx.x == 0) odd = 0;
+
+    auto get_rows = [&](const __bf16 *from, int j, int i, bf16x8(&b)[3]) {
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            bf16x4 p[3];
-            split<3>(S[m], p);
+        for (int u = 0; u < 3; ++u)
+            b[u] = *(const bf16x8 *)(from + u * kSlice * kC + lds_at<kC>(16 * j + n, 32 * i + 8 * g));
+    };
+    auto get_state = [&](int i, bf16x8(&b)[2][3]) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int u = 0; u < 3; ++u)
-                *(bf16x4 *)(sb + (u * kSlice + 16 * nt + n) * LS + 16 * (MT * mt + m) + 4 * g) = p[u];
-        }
-    };
-    // rows 16 mt + 4 g + 0 .. 3 of value 16 nt + n of the slice
-    auto put_rows = [&](__bf16 *to, f32x4 x) {
-        bf16x4 p[3];
-        split<3>(x, p);
-#pragma unroll
-        for (int u = 0; u < 3; ++u) *(bf16x4 *)(to + (u * kSlice + 16 * nt + n) * LU + 16 * mt + 4 * g) = p[u];
-    };
-    auto get_rows = [&](const __bf16 *from, int i, bf16x8(&b)[3]) {
-#pragma unroll
-        for (int u = 0; u < 3; ++u) b[u] = *(const bf16x8 *)(from + (u * kSlice + 16 * nt + n) * LU + 32 * i + 8 * g);
+                b[j][u] = *(const bf16x8 *)(sb + u * kSlice * DK + lds_at<DK>(16 * j + n, 32 * i + 8 * g));
     };
 
-    Chunk<DK, T> c;
-    const int row = 16 * mt + 4 * g;
-    T *const out = (T *)d.out.ptr + (long long)sr.first * d.out.token_stride + (long long)head * d.out.head_stride + v0 + 16 * nt;
-    auto load_factors = [&]() {
-        c.eg = *(const f32x4 *)(rec + kEg + row);
-        c.ec = *(const f32x4 *)(rec + kEc + row);
-        c.last = rec[kLast];
-    };
-    if (sr.count > 0) {
-        c.load_k(d, sr, kh, 0, mt, nt);
-        c.load_q(d, sr, kh, 0, mt);
-        c.load_v(d, sr, head, 0, v0, mt, nt);
-        c.load_blocks(rec + kT, mt, c.t);
-        c.load_blocks(rec + kP, mt, c.p);
-        load_factors();
-    }
-    put_state();
-    for (int t0 = 0; t0 < sr.count; t0 += kC) {
-        rec += step;  // behind the last chunk's there is room for one more (of no matter)
+    if (wave < 4) {
+        // dk = 16 (MT mt + m) + 4 g + i of row v0 + 16 j + n
+        f32x4 S[MT][2];
 #pragma unroll
-        for (int i = 0; i < KS / 2; ++i) {
-            bf16x8 x[N];
-            pieces<T>(c.k[i], x);
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                S[m][j] = f32x4{};
+                if (held && d.state_in && in[j]) S[m][j] = *(const f32x4 *)(d.state_in + at + 16 * j * DK + 16 * m);
+            }
+        auto put_state = [&]() {
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    bf16x4 p[3];
+                    split<3>(S[m][j], p);
+#pragma unroll
+                    for (int u = 0; u < 3; ++u)
+                        *(bf16x4 *)(sb + u * kSlice * DK + lds_at<DK>(16 * j + n, 16 * (MT * mt + m) + 4 * g)) = p[u];
+                }
+        };
+        // rows `row` .. of value 16 j + n of the slice
+        auto put_rows = [&](__bf16 *to, int j, f32x4 x) {
+            bf16x4 p[3];
+            split<3>(x, p);
+#pragma unroll
+            for (int u = 0; u < 3; ++u) *(bf16x4 *)(to + u * kSlice * kC + lds_at<kC>(16 * j + n, row)) = p[u];
+        };
+        bf16x8 t[2][3];
+        T v[2][4];
+        f32x4 eg, ec;
+        float last;
+        auto load_v = [&](int t0) {
+            const T *x = (const T *)d.v.ptr + (long long)sr.first * d.v.token_stride + (long long)head * d.v.head_stride;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const unsigned long long o =
+                    (unsigned long long)(uint32_t)min(t0 + row + i, sr.count - 1) * (uint32_t)d.v.token_stride + n;
+#pragma unroll
+                for (int j = 0; j < 2; ++j) v[j][i] = x[min(v0 + 16 * j, (int)d.v.dim - 16) + o];
+            }
+        };
+        load_v(0);
+        eg = *(const f32x4 *)(rec + kEg + row);
+        load_blocks(rec + kT, mt, t);
+        ec = *(const f32x4 *)(rec + kEc + row);
+        last = rec[kLast];
+        put_state();
+        __syncthreads();
+        for (int t0 = 0; t0 < sr.count; t0 += kC) {
+            rec += step;
+            f32x4 x[2] = {};
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {
+                bf16x8 a[N], b[2][3];
+#pragma unroll
+                for (int u = 0; u < N; ++u)
+                    a[u] = *(const bf16x8 *)(kp + u * kC * DK + lds_at<DK>(16 * mt + n, 32 * i + 8 * g));
+                get_state(i, b);
+                mma<2, N, 3>(a, b, x);
+            }
+            bf16x8 kt[2][MT][N];  // K^T: dk = 16 (MT mt + m) + n, rows 32 i + 8 g + 0 .. 7
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int u = 0; u < N; ++u) {
+                        typedef short s4 __attribute__((ext_vector_type(4)));
+                        const int r = 32 * i + 8 * g + (n >> 2), c = 16 * (MT * mt + m) + 4 * (n & 3);
+                        const s4 y0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                            (LDS_AS s4 *)(kp + u * kC * DK + lds_at<DK>(r, c)));
+                        const s4 y1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                            (LDS_AS s4 *)(kp + u * kC * DK + lds_at<DK>(r + 4, c)));
+                        kt[i][m][u] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(y0, y1, 0, 1, 2, 3, 4, 5, 6, 7));
+                    }
+            bool bad = false;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                f32x4 r;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    r[i] = (float)v[j][i] - eg[i] * x[j][i];
+                    bad |= !__builtin_isfinite(r[i]);
+                }
+                put_rows(rb, j, r);
+            }
+            if (bad) odd = 1;
+            load_v(t0 + kC);
+            eg = *(const f32x4 *)(rec + kEg + row);
+            __syncthreads();
+            const bool slow = odd;
+            if (__builtin_expect(slow, 0)) {
+                row_by_row<DK, T>(d, sr, kh, head, t0, v0, mt, S, (float *)ub, out);
+            } else {
+                f32x4 u[2] = {};
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    if (i == 1 && mt < 2) break;  // above the diagonal
+                    bf16x8 b[2][3];
+                    get_rows(rb, 0, i, b[0]);
+                    get_rows(rb, 1, i, b[1]);
+                    mma<2, 3, 3>(t[i], b, u);
+                }
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    put_rows(ub, j, u[j]);
+                    put_rows(wb, j, u[j] * ec);
+                }
+            }
+            load_blocks(rec + kT, mt, t);
+            const float decay = last;
+            ec = *(const f32x4 *)(rec + kEc + row);
+            last = rec[kLast];
+            __syncthreads();
+            if (threadIdx.x == 0) odd = 0;  // every wave has read it, and sets it behind the next barrier
+            if (!slow) {
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) S[m][j] *= decay;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    bf16x8 b[2][3];
+                    get_rows(wb, 0, i, b[0]);
+                    get_rows(wb, 1, i, b[1]);
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) mma<2, N, 3>(kt[i][m], b, S[m]);
+                }
+            }
+            put_state();
+            __syncthreads();
+        }
+        if (held && d.state_out)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+                    if (in[j]) *(f32x4 *)(d.state_out + at + 16 * j * DK + 16 * m) = S[m][j];
+        return;
+    }
+
+    typename In<T>::raw k[KS], q[KS];
+    bf16x8 p[2][3], ka[KS][N];
+    auto cut = [&]() {
+#pragma unroll
+        for (int i = 0; i < KS; ++i) pieces<T>(k[i], ka[i]);
+    };
+    auto put_k = [&]() {
+#pragma unroll
+        for (int i = 0; i < KS; ++i)
 #pragma unroll
             for (int u = 0; u < N; ++u)
-                *(bf16x8 *)(kp + (u * kC + 16 * mt + n) * LK + 32 * (nt * (KS / 2) + i) + 8 * g) = x[u];
-        }
-        c.load_k(d, sr, kh, t0 + kC, mt, nt);
-        __syncthreads();  // K's and the state's pieces are there
-        f32x4 x[2] = {};  // K S^T and Q S^T
-#pragma unroll
-        for (int i = 0; i < KS; ++i) {
-            bf16x8 a[2][N], b[3];
-#pragma unroll
-            for (int u = 0; u < N; ++u) a[0][u] = *(const bf16x8 *)(kp + (u * kC + 16 * mt + n) * LK + 32 * i + 8 * g);
-            pieces<T>(c.q[i], a[1]);
-#pragma unroll
-            for (int u = 0; u < 3; ++u) b[u] = *(const bf16x8 *)(sb + (u * kSlice + 16 * nt + n) * LS + 32 * i + 8 * g);
-            mma<2, N, 3>(a, b, x);
-        }
-        f32x4 r;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) r[i] = (float)c.v[i] - c.eg[i] * x[0][i];
-        put_rows(rb, r);
-        c.load_q(d, sr, kh, t0 + kC, mt);
-        c.load_v(d, sr, head, t0 + kC, v0, mt, nt);
+                *(bf16x8 *)(kp + u * kC * DK + lds_at<DK>(16 * mt + n, 32 * i + 8 * g)) = ka[i][u];
+    };
+    load_rows<KS, T>(d.k, sr.first, kh, 16 * mt, sr.count, 0, k);
+    load_rows<KS, T>(d.q, sr.first, kh, 16 * mt, sr.count, 0, q);
+    load_blocks(rec + kP, mt, p);
+    f32x4 eg = *(const f32x4 *)(rec + kEg + row);
+    cut();
+    load_rows<KS, T>(d.k, sr.first, kh, kC + 16 * mt, sr.count, 0, k);
+    put_k();
+    __syncthreads();
+    for (int t0 = 0; t0 < sr.count; t0 += kC) {
+        rec += step;
+        cut();
+        load_rows<KS, T>(d.k, sr.first, kh, t0 + 2 * kC + 16 * mt, sr.count, 0, k);
         __syncthreads();
-        f32x4 u[1] = {};
+        const bool slow = odd;
+        f32x4 x[2] = {};
+        if (__builtin_expect(slow, 0)) {
+            for (int i = 0; i < 2 * min(kC, sr.count - t0); ++i) __syncthreads();  // those of row_by_row
+        } else {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            if (i == 1 && mt < 2) break;  // above the diagonal
-            bf16x8 a[1][3], b[3];
-#pragma unroll
-            for (int w = 0; w < 3; ++w) a[0][w] = c.t[i][w];
-            get_rows(rb, i, b);
-            mma<1, 3, 3>(a, b, u);
-        }
-        f32x4 w;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = u[0][i] * c.ec[i];
-        put_rows(ub, u[0]);
-        put_rows(wb, w);
-        c.load_blocks(rec + kT, mt, c.t);
-        __syncthreads();
-        f32x4 o[1];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[0][i] = d.scale * c.eg[i] * x[1][i];
-#pragma unroll
-        for (int m = 0; m < MT; ++m) S[m] *= c.last;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            bf16x8 kt[MT][N], b[3];  // K^T: dk = 16 (MT mt + m) + n, rows 32 i + 8 g + 0 .. 7
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int z = 0; z < N; ++z) {
-                    typedef short s4 __attribute__((ext_vector_type(4)));
-                    const __bf16 *from = kp + (z * kC + 32 * i + 8 * g + (n >> 2)) * LK + 16 * (MT * mt + m) + 4 * (n & 3);
-                    const s4 y0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS s4 *)from);
-                    const s4 y1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS s4 *)(from + 4 * LK));
-                    kt[m][z] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(y0, y1, 0, 1, 2, 3, 4, 5, 6, 7));
-                }
-            get_rows(wb, i, b);
-            mma<MT, N, 3>(kt, b, S);
-            if (i == 0 || mt >= 2) {
-                bf16x8 a[1][3];
-#pragma unroll
-                for (int z = 0; z < 3; ++z) a[0][z] = c.p[i][z];
-                get_rows(ub, i, b);
-                mma<1, 3, 3>(a, b, o);
+            for (int i = 0; i < KS; ++i) {
+                bf16x8 a[N], b[2][3];
+                pieces<T>(q[i], a);
+                get_state(i, b);
+                mma<2, N, 3>(a, b, x);
             }
         }
-        c.load_blocks(rec + kP, mt, c.p);
-        load_factors();
-        put_state();  // read again behind the next barrier but one; nobody reads the old ones any more
+        load_rows<KS, T>(d.q, sr.first, kh, t0 + kC + 16 * mt, sr.count, 0, q);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int t = t0 + row + i;
-            if (in && t < sr.count) out[(unsigned long long)(uint32_t)t * (uint32_t)d.out.token_stride + n] = (T)o[0][i];
+        for (int j = 0; j < 2; ++j) x[j] *= eg * d.scale;
+        eg = *(const f32x4 *)(rec + kEg + row);
+        __syncthreads();
+        put_k();
+        if (!slow) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if (i == 1 && mt < 2) break;
+                bf16x8 b[2][3];
+                get_rows(ub, 0, i, b[0]);
+                get_rows(ub, 1, i, b[1]);
+                mma<2, 3, 3>(p[i], b, x);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int t = t0 + row + i;
+                if (t >= sr.count) break;
+                T *o = out + (unsigned long long)(uint32_t)t * (uint32_t)d.out.token_stride + n;
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                    if (in[j]) o[16 * j] = (T)x[j][i];
+            }
         }
-        __syncthreads();  // K's pieces have been read
-    }
-    if (held && d.state_out && in) {
-#pragma unroll
-        for (int m = 0; m < MT; ++m) *(f32x4 *)(d.state_out + at + 16 * m) = S[m];
+        load_blocks(rec + kP, mt, p);
+        __syncthreads();
     }
 }
 

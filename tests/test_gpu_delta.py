@@ -241,3 +241,36 @@ def test_same_result_every_time_on_any_stream_and_in_a_graph(m27q, dev, lens):
         call()
         torch.cuda.synchronize()
         assert torch.equal(b, out) and torch.equal(sb, so)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("lens,row", [([9], 4), ([150], 0), ([150], 70), ([70, 200], 133), ([64], 63)])
+@pytest.mark.parametrize("where", ["v", "k", "q", "g", "beta", "state"])
+@pytest.mark.parametrize("what", [float("nan"), float("inf")])
+def test_values_that_are_not_finite(m27q, dev, lens, row, where, what, t):
+    """They show in the rows, heads and values that the definition carries them to, and nowhere before."""
+    say("delta odd values", lens, row, where, what, t)
+    p = Problem(m27q, dev, lens, 1, 2, 64, 48, t)
+    x = getattr(p, where)
+    if where == "state":
+        x[-1, 1, 17, 3] = what
+    elif where in ("g", "beta"):
+        x[row, 1] = what
+    else:
+        x[row, x.shape[1] - 1, 5] = what
+    got, state = p.run()
+    with np.errstate(all="ignore"):
+        want, ends, size, sizes = p.want()
+    assert np.array_equal(np.isfinite(got), np.isfinite(want))
+    ok, at = np.isfinite(want), 0
+    for s, n in enumerate(lens):
+        rows = slice(at, at + n)
+        tol = 8 * np.sqrt(max(n, 1) * 128) * 2.0 ** -24 * 64 ** -0.5 * 1.01 * np.where(np.isfinite(size[rows]), size[rows], 0) \
+            + OUT[t] * np.abs(np.where(ok[rows], want[rows], 0))
+        assert np.all(np.abs(got[rows] - want[rows])[ok[rows]] <= tol[ok[rows]])
+        fine = np.isfinite(ends[s])
+        assert np.array_equal(np.isfinite(state[s]), fine)
+        tol = 8 * np.sqrt(max(n, 1) * 128) * 2.0 ** -24 * np.where(np.isfinite(sizes[s]), sizes[s], np.inf)[..., None]
+        assert np.all((np.abs(state[s] - ends[s]) <= tol)[fine])
+        at += n
