@@ -86,18 +86,22 @@ struct Work {
     bool gaps;          // some page of them is not one
 };
 
-// Tiles of K and V in LDS: kKeys rows of D values, 16-byte chunks exchanged
-// within a row so that neither kind of read meets bank conflicts: K's chunk c
-// of row r lies at c ^ (r & 7) (a read takes one chunk column of 32 rows), V's
-// 32-byte unit u at u ^ (r & 7) (D = 64: r & 3; a transposing read takes one
-// unit of 4 rows per 16 lanes).
+// Tiles of K and V in LDS: kKeys rows of D values, 16-byte chunks exchanged within a row so
+// that no kind of read meets bank conflicts (64 banks, 16 lanes of 16 bytes or 32 of 8 at a
+// time): K's chunk c of row r lies at c ^ (r & 15) (a read takes one chunk column of 16 rows;
+// D = 64, two rows to the banks: c ^ (r / 2 & 7)), V's 32-byte unit u at u ^ v_swap(r) (a
+// transposing read takes two units of 4 rows, or one of 8).  Exchanges of row bits add up.
 template <int D>
 __device__ __forceinline__ int k_chunk(int row, int c) {
-    return c ^ (row & 7);
+    return c ^ (D >= 128 ? row & 15 : (row >> 1) & 7);
+}
+template <int D>
+__device__ __forceinline__ int v_swap(int row) {
+    return D >= 128 ? ((row & 3) << 1) ^ ((row >> 2) & 1) : (row & 2) ^ ((row >> 2) & 1);
 }
 template <int D>
 __device__ __forceinline__ int v_chunk(int row, int c) {
-    return c ^ ((row & (D >= 128 ? 7 : 3)) << 1);
+    return c ^ (v_swap<D>(row) << 1);
 }
 
 // The page of the keys that this wave brings into the tile at k0 (a multiple
@@ -125,14 +129,15 @@ __device__ __forceinline__ void load_tile(const AttnParams &p, const Work &w, in
                           ((long long)w.head * p.cache.page_size + (key & (int)(p.cache.page_size - 1))) * D) * 2;
     const __amdgpu_buffer_rsrc_t kg = buf_rsrc((const char *)p.cache.k + at, RPW * D * 2);
     const __amdgpu_buffer_rsrc_t vg = buf_rsrc((const char *)p.cache.v + at, RPW * D * 2);
-    const int r0 = lane / CPR, pc = lane % CPR;
-    const uint32_t ko = r0 * D * 2 + k_chunk<D>(r0, pc) * 16, vo = r0 * D * 2 + v_chunk<D>(r0, pc) * 16;
+    const int r0 = lane / CPR, pc = lane % CPR, first = wave * RPW + r0;
+    const uint32_t ko = r0 * D * 2 + k_chunk<D>(first, pc) * 16, vo = r0 * D * 2 + v_chunk<D>(first, pc) * 16;
 #pragma unroll
-    for (int i = 0; i < RPW / RPI; ++i) {  // row i RPI + r0: its chunks are r0's with i RPI exchanged as well
+    for (int i = 0; i < RPW / RPI; ++i) {  // row first + i RPI: its chunks are the first's with i RPI exchanged as well
         LDS_AS char *kd = kt + (wave * RPW + i * RPI) * D * 2, *vd = vt + (wave * RPW + i * RPI) * D * 2;
         if (!CHECKED || i * RPI + r0 < rows) {
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(kg, (LDS_AS void *)kd, 16, ko ^ (i * RPI * 16), i * 1024, 0, 0);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(vg, (LDS_AS void *)vd, 16, vo ^ (i * RPI * 32), i * 1024, 0, 0);
+            const uint32_t ka = ko ^ (k_chunk<D>(i * RPI, 0) * 16), va = vo ^ (v_chunk<D>(i * RPI, 0) * 16);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(kg, (LDS_AS void *)kd, 16, ka, i * 1024, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(vg, (LDS_AS void *)vd, 16, va, i * 1024, 0, 0);
         } else {
             *(LDS_AS f32x4 *)(vd + lane * 16) = f32x4{0, 0, 0, 0};
         }
@@ -238,16 +243,18 @@ struct Rows {
 
     __device__ __forceinline__ void scores(const LDS_AS char *kt, float (&s)[NS]) const {
         const int r = threadIdx.x & (RW - 1);
-        // chunk G i + part of key row r (and r + 16): k_chunk of it is (y ^ (G i & 7)) + (G i & ~7),
+        // chunk G i + part of key row r (and r + 16): k_chunk of it is (y ^ (G i & M)) + (G i & ~M),
         // a few addresses, the rest offsets
+        constexpr int M = D >= 128 ? 15 : 7;
         const LDS_AS char *kr = kt + r * D * 2;
-        const int y = (r & 7) ^ part();
+        int y = k_chunk<D>(r, part());
+        asm("" : "+v"(y));  // addresses are made here, not kept
 #pragma unroll
         for (int b = 0; b < kKeys / RW; ++b) {
             acc c = {};
 #pragma unroll
             for (int i = 0; i < D / KD; ++i) {
-                const T8 a = *(const LDS_AS T8 *)(kr + b * RW * D * 2 + (y ^ (G * i & 7)) * 16 + (G * i & ~7) * 16);
+                const T8 a = *(const LDS_AS T8 *)(kr + b * RW * D * 2 + (y ^ (G * i & M)) * 16 + (G * i & ~M) * 16);
                 c = N::mma(a, q[i], c);
             }
 #pragma unroll
@@ -308,7 +315,7 @@ struct Rows {
         const int lane = threadIdx.x & 63, x = 4 * part() + ((lane & 15) >> 2);  // the key this lane's 16 lanes read for
         const LDS_AS char *vr = vt + x * D * 2 + (lane & 3) * 8;
         constexpr int M = D >= 128 ? 7 : 3, U = RW / 16;
-        const int y = (x & M) ^ ((lane >> 4) & (U - 1));  // 32-byte unit U t + .. of a row, exchanged as in v_chunk
+        const int y = v_swap<D>(x) ^ ((lane >> 4) & (U - 1));  // 32-byte unit U t + .. of a row, exchanged
 #pragma unroll
         for (int t = 0; t < D / RW; ++t)
 #pragma unroll
@@ -541,10 +548,9 @@ __global__ __launch_bounds__(kWaves * 64, 1) void k_attn_few(const AttnParams p)
     constexpr int RPI = 512 / D, CPR = D / 8;
     const int r0 = lane / CPR, pc = lane % CPR;
     const uint32_t ko = r0 * D * 2 + k_chunk<D>(r0, pc) * 16, vo = r0 * D * 2 + v_chunk<D>(r0, pc) * 16;
-    constexpr int KF = 16, VF = D >= 128 ? 32 : 0;  // how rows exchange chunks (D = 64: loads of 8 whole rows)
     // K (or V) of the tile at k0; `checked` as in load_tile, otherwise a page that is none is
     // read as the first (and what it gives is not used)
-    auto load = [&](const void *from, LDS_AS char *to, uint32_t off, int flips, int k0, const int (&pages)[2], bool checked,
+    auto load = [&](const void *from, LDS_AS char *to, bool keys, int k0, const int (&pages)[2], bool checked,
                     bool clear) {
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
@@ -557,7 +563,7 @@ __global__ __launch_bounds__(kWaves * 64, 1) void k_attn_few(const AttnParams p)
 #pragma unroll
             for (int i = 0; i < 16 / RPI; ++i) {
                 LDS_AS char *d = to + (16 * half + i * RPI) * D * 2;
-                const uint32_t o = off ^ ((i * RPI & 7) * flips);
+                const uint32_t o = keys ? ko ^ (k_chunk<D>(i * RPI, 0) * 16) : vo ^ (v_chunk<D>(i * RPI, 0) * 16);
                 if (!checked || i * RPI + r0 < rows)
                     __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (LDS_AS void *)d, 16, o, i * 1024, 0, 0);
                 else if (clear) *(LDS_AS f32x4 *)(d + lane * 16) = f32x4{0, 0, 0, 0};
@@ -575,8 +581,8 @@ __global__ __launch_bounds__(kWaves * 64, 1) void k_attn_few(const AttnParams p)
     if (t < tb) {
         ids[0] = page(w.lo + t * kKeys, 0);
         ids[1] = page(w.lo + t * kKeys, 1);
-        load(p.cache.k, kt, ko, KF, w.lo + t * kKeys, ids, false, false);
-        load(p.cache.v, vt, vo, VF, w.lo + t * kKeys, ids, false, false);
+        load(p.cache.k, kt, true, w.lo + t * kKeys, ids, false, false);
+        load(p.cache.v, vt, false, w.lo + t * kKeys, ids, false, false);
     }
     // a wave that has none of them asks for its first one of the others
     int there = -1;
@@ -585,8 +591,8 @@ __global__ __launch_bounds__(kWaves * 64, 1) void k_attn_few(const AttnParams p)
         if (there < tiles) {
             ids[0] = page(w.lo + there * kKeys, 0);
             ids[1] = page(w.lo + there * kKeys, 1);
-            load(p.cache.k, kt, ko, KF, w.lo + there * kKeys, ids, true, false);
-            load(p.cache.v, vt, vo, VF, w.lo + there * kKeys, ids, true, true);
+            load(p.cache.k, kt, true, w.lo + there * kKeys, ids, true, false);
+            load(p.cache.v, vt, false, w.lo + there * kKeys, ids, true, true);
         }
     }
     R x;
@@ -610,10 +616,10 @@ __global__ __launch_bounds__(kWaves * 64, 1) void k_attn_few(const AttnParams p)
         x.scores(kt, sco);
         x.template weights<false>(p, w, sc, sco, k0, pcs);
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        if (t + kWaves < tb) load(p.cache.k, kt, ko, KF, k1, ids, false, false);
+        if (t + kWaves < tb) load(p.cache.k, kt, true, k1, ids, false, false);
         x.values(vt, pcs);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // V has been read
-        if (t + kWaves < tb) load(p.cache.v, vt, vo, VF, k1, ids, false, false);
+        if (t + kWaves < tb) load(p.cache.v, vt, false, k1, ids, false, false);
     }
     bool odd = false;
     for (int t = wave; t < tiles; t += kWaves) {
@@ -622,8 +628,8 @@ __global__ __launch_bounds__(kWaves * 64, 1) void k_attn_few(const AttnParams p)
         if (t != there) {
             ids[0] = page(k0, 0);
             ids[1] = page(k0, 1);
-            load(p.cache.k, kt, ko, KF, k0, ids, true, false);
-            load(p.cache.v, vt, vo, VF, k0, ids, true, true);
+            load(p.cache.k, kt, true, k0, ids, true, false);
+            load(p.cache.v, vt, false, k0, ids, true, true);
         }
         there = -1;
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
@@ -636,7 +642,7 @@ __global__ __launch_bounds__(kWaves * 64, 1) void k_attn_few(const AttnParams p)
         for (int t = wave; t < tiles; t += kWaves) {
             if (t >= ta && t < tb) continue;
             const int k0 = w.lo + t * kKeys, ids[2] = {page(k0, 0), page(k0, 1)};
-            load(p.cache.v, vt, vo, VF, k0, ids, true, true);
+            load(p.cache.v, vt, false, k0, ids, true, true);
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
             x.add_odd(p, w, k0, vt);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");

@@ -362,13 +362,14 @@ __device__ __forceinline__ void mma(const bf16x8 (&a)[NA], const bf16x8 (&b)[NC]
                     c[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[j][o - i], c[j], 0, 0, 0);
 }
 
-// Place of a value in LDS, rows of W values: the 32-byte units of a row are exchanged by the row,
-// so that 8 rows' reads of a column of 16 bytes, and a transposing read's 4 rows of a unit, meet
-// different banks.
+// Place of a value in LDS, rows of W values: the 16-byte chunks of a row are exchanged by the row,
+// so that 16 rows' reads of a column of chunks, and two groups of a transposing read (32-byte
+// units of rows r .. r + 3 and r + 8 .. r + 11), meet different ones of the 64 banks.
 template <int W>
 __device__ __forceinline__ int lds_at(int row, int col) {
-    const int unit = W == 128 ? ((col >> 4) ^ row) & 7 : ((col >> 4) ^ (row >> 1)) & 3;
-    return row * W + unit * 16 + (col & 15);
+    const int x = (W == 128 ? row : row >> 1) & (W == 128 ? 15 : 7), top = x >> (W == 128 ? 3 : 2);
+    const int swap = W == 128 ? ((x & 7) << 1) ^ (top * 9) : ((x & 3) << 1) ^ (top * 5);
+    return row * W + (((col >> 3) ^ swap) << 3) + (col & 7);
 }
 
 // A record's operand blocks of row tile m (see kT): its first, and its second or the first again.
