@@ -705,6 +705,10 @@ __global__ __launch_bounds__(512) void k_delta_chunks(const m27q_delta d, const 
                 get_rows(ub, 1, i, b[1]);
                 mma<2, 3, 3>(p[i], b, x);
             }
+        }
+        load_blocks(rec + kP, mt, p);
+        // last, behind all loads: a wait for one of those would be one for these too
+        if (!slow) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int t = t0 + row + i;
@@ -715,7 +719,6 @@ __global__ __launch_bounds__(512) void k_delta_chunks(const m27q_delta d, const 
                     if (in[j]) o[16 * j] = (T)x[j][i];
             }
         }
-        load_blocks(rec + kP, mt, p);
         __syncthreads();
     }
 }
