@@ -215,89 +215,125 @@ __device__ __forceinline__ void pieces(typename In<T>::raw x, bf16x8 (&p)[In<T>:
     else split<In<T>::N>(__builtin_convertvector(x, f32x8), p);
 }
 
+// Place of a value in LDS, rows of W values: the 16-byte chunks of a row are exchanged by the row,
+// so that 16 rows' reads of a column of chunks, and two groups of a transposing read (32-byte
+// units of rows r .. r + 3 and r + 8 .. r + 11), meet different ones of the 64 banks.
+template <int W>
+__device__ __forceinline__ int lds_at(int row, int col) {
+    const int x = (W == 128 ? row : row >> 1) & (W == 128 ? 15 : 7), top = x >> (W == 128 ? 3 : 2);
+    const int swap = W == 128 ? ((x & 7) << 1) ^ (top * 9) : ((x & 3) << 1) ^ (top * 5);
+    return row * W + (((col >> 3) ^ swap) << 3) + (col & 7);
+}
+
 // A chunk of a key head: K K^T and Q K^T once, then for its value heads (every `parts`-th
 // of them) the triangular inverse.
 template <int DK, typename T>
-__global__ __launch_bounds__(256) void k_delta_prepare(const m27q_delta d, float *scratch, int parts) {
-    constexpr int N = In<T>::N, KS = DK / 32, LD = DK + 16, LM = kC + 4;
-    constexpr size_t planes = sizeof(__bf16) * N * kC * LD, mats = sizeof(float) * 3 * kC * LM;
+__global__ __launch_bounds__(256, 4) void k_delta_prepare(const m27q_delta d, float *scratch, int parts) {
+    constexpr int N = In<T>::N, LM = kC + 4;
+    constexpr size_t planes = sizeof(__bf16) * N * kC * 64, mats = sizeof(float) * 2 * kC * LM;
     __shared__ __attribute__((aligned(16))) char mem[planes > mats ? planes : mats];
-    __shared__ double G[kC];
-    __shared__ float B[kC];
-    __bf16 *kp = (__bf16 *)mem;                                        // K's pieces, [N][kC][LD]
-    float *Am = (float *)mem, *Xm = Am + kC * LM, *Pm = Xm + kC * LM;  // then A, the inverse of I + A, and P
+    __shared__ double Gs[3][kC];
+    __shared__ float Bs[3][kC];
+    __bf16 *kp = (__bf16 *)mem;                                        // K's pieces, 64 columns at a time, [N][kC][64]
+    float *Am = (float *)mem, *Xm = Am + kC * LM;  // then A, P after it, and the inverse of I + A
     const int s = blockIdx.z, kh = blockIdx.y / parts, part = blockIdx.y - kh * parts, t0 = blockIdx.x * kC;
     const SeqRows sr = seq_rows(d.start, s, (int)d.tokens, (int)d.max_len);
     if (t0 >= sr.count) return;
     const int kheads = (int)d.k.heads, per = (int)d.v.heads / kheads;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
 
-    bf16x8 a[KS][2][N];  // K's and Q's
-    {
-        typename In<T>::raw x[KS], y[KS];
-        load_rows<KS, T>(d.k, sr.first, kh, t0 + 16 * wave, sr.count, 0, x);
-        load_rows<KS, T>(d.q, sr.first, kh, t0 + 16 * wave, sr.count, 0, y);
+    const auto head_of = [&](int which) {
+        return d.head_map == M27Q_HEADS_CYCLED ? which * kheads + kh : kh * per + which;
+    };
+    const auto record = [&](int which) {
+        return scratch + ((chunk_place(sr.first, s) + blockIdx.x) * d.v.heads + head_of(which)) * (long long)kRecord;
+    };
+    // A head's factors, three heads at a time, a wave each.  The sums of g are in 64 bits, as
+    // differences of them are taken.
+    const auto factors = [&](int which) {
+        if (wave == 3 || which >= per) return;
+        float *rec = record(which);
+        const bool in = t0 + lane < sr.count;
+        const long long at = (long long)(sr.first + t0 + lane) * d.v.heads + head_of(which);
+        const float gf = in ? d.g[at] : 0.0f, beta = in ? d.beta[at] : 0.0f;
+        double x = gf < -1e4f ? -1e4 : (double)gf;  // e^-10000 is 0 as e^-inf is, and no inf - inf
 #pragma unroll
-        for (int i = 0; i < KS; ++i) {
+        for (int o = 1; o < 64; o <<= 1) {
+            const double y = __shfl_up(x, o);
+            x += lane >= o ? y : 0.0;
+        }
+        const double last = __shfl(x, 63);
+        Gs[wave][lane] = x;
+        Bs[wave][lane] = beta;
+        rec[kEg + lane] = __builtin_isfinite(beta) ? expf((float)x) : __builtin_nanf("");  // to be seen by the walk
+        rec[kEc + lane] = expf((float)(last - x));
+        if (lane == 0) rec[kLast] = expf((float)last);
+    };
+
+    typename In<T>::raw x[2], y[2];
+    load_rows<2, T>(d.k, sr.first, kh, t0 + 16 * wave, sr.count, 0, x);
+    load_rows<2, T>(d.q, sr.first, kh, t0 + 16 * wave, sr.count, 0, y);
+    factors(part + wave * parts);
+    f32x4 prod[4][2] = {};  // tiles of K K^T and Q K^T at rows 16 wave, columns 16 j
+#pragma unroll
+    for (int h = 0; h < DK / 64; ++h) {
+        bf16x8 a[2][2][N];  // K's and Q's
+        if (h) __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
             pieces<T>(x[i], a[i][0]);
             pieces<T>(y[i], a[i][1]);
 #pragma unroll
-            for (int j = 0; j < N; ++j) *(bf16x8 *)(kp + (j * kC + 16 * wave + n) * LD + 32 * i + 8 * g) = a[i][0][j];
+            for (int j = 0; j < N; ++j)
+                *(bf16x8 *)(kp + j * kC * 64 + lds_at<64>(16 * wave + n, 32 * i + 8 * g)) = a[i][0][j];
         }
-    }
-    __syncthreads();
-    f32x4 prod[4][2];  // tiles of K K^T and Q K^T at rows 16 wave, columns 16 j
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        prod[j][0] = prod[j][1] = f32x4{};
-        if (j > wave) continue;
-#pragma unroll
-        for (int i = 0; i < KS; ++i) {
-            bf16x8 b[N];
-#pragma unroll
-            for (int u = 0; u < N; ++u) b[u] = *(const bf16x8 *)(kp + (u * kC + 16 * j + n) * LD + 32 * i + 8 * g);
-            mma<2, N, N>(a[i], b, prod[j]);
-        }
-    }
-
-    for (int which = part; which < per; which += parts) {
-        const int head = d.head_map == M27Q_HEADS_CYCLED ? which * kheads + kh : kh * per + which;
-        float *rec = scratch + ((chunk_place(sr.first, s) + blockIdx.x) * d.v.heads + head) * (long long)kRecord;
-        __syncthreads();  // K's pieces, or the last head's matrices, make room
-        if (wave == 0) {  // sums of g in 64 bits: differences of them are taken below
-            const bool in = t0 + lane < sr.count;
-            const long long at = (long long)(sr.first + t0 + lane) * d.v.heads + head;
-            const float gf = in ? d.g[at] : 0.0f;
-            double x = gf < -1e4f ? -1e4 : (double)gf;  // e^-10000 is 0 as e^-inf is, and no inf - inf
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const double y = __shfl_up(x, o);
-                x += lane >= o ? y : 0.0;
-            }
-            const double last = __shfl(x, 63);
-            G[lane] = x;
-            const float beta = in ? d.beta[at] : 0.0f;
-            B[lane] = beta;
-            rec[kEg + lane] = __builtin_isfinite(beta) ? expf((float)x) : __builtin_nanf("");  // to be seen by the walk
-            rec[kEc + lane] = expf((float)(last - x));
-            if (lane == 0) rec[kLast] = expf((float)last);
+        if (h + 1 < DK / 64) {
+            load_rows<2, T>(d.k, sr.first, kh, t0 + 16 * wave, sr.count, 2, x);
+            load_rows<2, T>(d.q, sr.first, kh, t0 + 16 * wave, sr.count, 2, y);
         }
         __syncthreads();
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < 4; ++j) {
+            if (j > wave) break;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                bf16x8 b[N];
+#pragma unroll
+                for (int u = 0; u < N; ++u)
+                    b[u] = *(const bf16x8 *)(kp + u * kC * 64 + lds_at<64>(16 * j + n, 32 * i + 8 * g));
+                mma<2, N, N>(a[i], b, prod[j]);
+            }
+        }
+    }
+
+    for (int which = part, slot = 0; which < per; which += parts, ++slot) {
+        __syncthreads();  // K's pieces, or the last head's matrices, make room
+        if (slot == 3) {
+            slot = 0;
+            factors(which + wave * parts);
+            __syncthreads();
+        }
+        const double *G = Gs[slot];
+        const float *B = Bs[slot];
+        float *rec = record(which);
+        f32x4 P[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (j > (wave | 1)) break;  // read by nothing
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int row = 16 * wave + 4 * g + i, col = 16 * j + n;
-                float x = 0, p = 0;
+                float x = 0;
+                P[j][i] = 0;
                 if (col <= row) {
                     const float e = expf((float)(G[row] - G[col]));
-                    p = d.scale * e * prod[j][1][i];
+                    P[j][i] = d.scale * e * prod[j][1][i];
                     if (col < row) x = B[row] * e * prod[j][0][i];
                 }
                 Am[row * LM + col] = x;
                 Xm[row * LM + col] = 0;
-                Pm[row * LM + col] = p;
             }
+        }
         __syncthreads();
         // the inverse's 16x16 blocks: on the diagonal by forward substitution, a column a lane
         const int r0 = 16 * wave;
@@ -333,13 +369,19 @@ __global__ __launch_bounds__(256) void k_delta_prepare(const m27q_delta d, float
         }
         __syncthreads();
 #pragma unroll
+        for (int j = 0; j < 4; ++j) {  // a wave's own rows: written and read without a barrier
+            if (j > (wave | 1)) break;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) Am[(r0 + 4 * g + i) * LM + 16 * j + n] = P[j][i];
+        }
+#pragma unroll
         for (int i = 0; i < 2; ++i) {
             if (i == 1 && wave < 2) break;
             const int at = (r0 + n) * LM + 32 * i + 8 * g;
             __bf16 *to = (__bf16 *)(rec + kT) + block_of(wave, i) * kBlockHalves + lane * 8;
             bf16x8 x[3], y[3];
             split<3>(*(const f32x8a *)(Xm + at) * *(const f32x8a *)(B + 32 * i + 8 * g), x);
-            split<3>(*(const f32x8a *)(Pm + at), y);
+            split<3>(*(const f32x8a *)(Am + at), y);
 #pragma unroll
             for (int u = 0; u < 3; ++u) {
                 *(bf16x8 *)(to + u * 512) = x[u];
@@ -360,16 +402,6 @@ __device__ __forceinline__ void mma(const bf16x8 (&a)[NA], const bf16x8 (&b)[NC]
 #pragma unroll
                 for (int j = 0; j < NC; ++j)
                     c[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[j][o - i], c[j], 0, 0, 0);
-}
-
-// Place of a value in LDS, rows of W values: the 16-byte chunks of a row are exchanged by the row,
-// so that 16 rows' reads of a column of chunks, and two groups of a transposing read (32-byte
-// units of rows r .. r + 3 and r + 8 .. r + 11), meet different ones of the 64 banks.
-template <int W>
-__device__ __forceinline__ int lds_at(int row, int col) {
-    const int x = (W == 128 ? row : row >> 1) & (W == 128 ? 15 : 7), top = x >> (W == 128 ? 3 : 2);
-    const int swap = W == 128 ? ((x & 7) << 1) ^ (top * 9) : ((x & 3) << 1) ^ (top * 5);
-    return row * W + (((col >> 3) ^ swap) << 3) + (col & 7);
 }
 
 // A record's operand blocks of row tile m (see kT): its first, and its second or the first again.
