@@ -755,18 +755,291 @@ __global__ __launch_bounds__(512) void k_delta_chunks(const m27q_delta d, const 
     }
 }
 
-// Rows from which the chunks are faster.
-constexpr uint32_t kChunkRows = 17;
+// ------------------------------------------------------------------- few --
+//
+// The same products for 16 rows at a time in one launch: a wave holds 16 rows of the state,
+// lane n = lane % 16 the row n, g = lane / 16 its values 16 m + 4 g + 0 .. 3.  That is where
+// a matrix instruction leaves a 16x16 result, and two such tiles side by side are its right
+// operand over 32 of the contraction if the left one's columns are taken in the same order;
+// a result's 4 g + 0 .. 3 are the operand of the instructions over 16.  So state, right-hand
+// sides and U go from product to product in registers.  The four waves of a workgroup share
+// K and Q in LDS, as operand blocks [step][piece][64 lanes][8], a step of 32 columns a wave.
+
+template <int NA, int NB>
+__device__ __forceinline__ void mma16(const bf16x4 (&a)[NA], const bf16x4 (&b)[NB], f32x4 &c) {
+    typedef short s4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+    for (int o = 2; o >= 0; --o)
+#pragma unroll
+        for (int i = 0; i < NA; ++i)
+            if (o - i >= 0 && o - i < NB)
+                c = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s4, a[i]), __builtin_bit_cast(s4, b[o - i]),
+                                                              c, 0, 0, 0);
+}
+
+// Lane (n, g)'s 16 bytes of an operand block: for a transposing read (rows 4 g + 0 .. 3, every
+// g' of them) the rows of a g lie apart by banks.
+__device__ __forceinline__ int few_at(int n, int g) { return (16 * g + (n ^ (4 * g))) * 8; }
+
+constexpr int kFew = 16;
+
+template <int DK, typename T>
+__global__ __launch_bounds__(256, 3) void k_delta_few(const m27q_delta d) {
+    typedef typename Vec4<T>::t T4;
+    constexpr int N = In<T>::N, KS = DK / 32, M = DK / 16, LA = kFew + 4;
+    __shared__ __attribute__((aligned(16))) __bf16 kb[KS * N * 512], qb[KS * N * 512];
+    __shared__ f32x4 part[KS][2][64];
+    __shared__ __attribute__((aligned(16))) float At[4][kFew * LA];
+    __shared__ __attribute__((aligned(16))) double Gs[kFew];
+    __shared__ __attribute__((aligned(16))) float egs[kFew], ecs[kFew], bs[kFew];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    const int groups = ((int)d.v.dim + 63) / 64;
+    const int head = blockIdx.x / groups, v0 = 64 * (blockIdx.x - head * groups) + 16 * wave, s = blockIdx.y;
+    const int kh = d.head_map == M27Q_HEADS_CYCLED ? head % (int)d.k.heads : head / (int)(d.v.heads / d.k.heads);
+    const SeqRows sr = seq_rows(d.start, s, (int)d.tokens, (int)d.max_len);
+    const int slot = d.slots ? d.slots[s] : s;
+    const bool in = v0 < (int)d.v.dim, held = in && slot >= 0 && (uint32_t)slot < d.n_slots;
+    const int vc = min(v0, (int)d.v.dim - 16) + n;
+    const long long at = (((long long)slot * d.v.heads + head) * d.v.dim + vc) * DK + 4 * g;
+
+    f32x4 S[M];
+#pragma unroll
+    for (int m = 0; m < M; ++m) S[m] = f32x4{};
+    if (held && d.state_in) {
+#pragma unroll
+        for (int m = 0; m < M; ++m) S[m] = *(const f32x4 *)(d.state_in + at + 16 * m);
+    }
+    const T *kr = (const T *)d.k.ptr + (long long)sr.first * d.k.token_stride + (long long)kh * d.k.head_stride + 4 * g;
+    const T *qr = (const T *)d.q.ptr + (long long)sr.first * d.q.token_stride + (long long)kh * d.q.head_stride + 4 * g;
+    const T *vr = (const T *)d.v.ptr + (long long)sr.first * d.v.token_stride + (long long)head * d.v.head_stride + vc;
+    T *out = (T *)d.out.ptr + (long long)sr.first * d.out.token_stride + (long long)head * d.out.head_stride + vc;
+    const float *gs = d.g + (long long)sr.first * d.v.heads + head, *betas = d.beta + (long long)sr.first * d.v.heads + head;
+
+    // Past the end the last row again, with beta = 0.
+    T4 k[2], q[2];
+    T v[4];
+    float gf, beta;
+    const auto load = [&](int t0) {
+        const unsigned long long t = (uint32_t)min(t0 + n, sr.count - 1);
+        if (wave < KS) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                k[h] = *(const T4 *)(kr + t * (uint32_t)d.k.token_stride + 32 * wave + 16 * h);
+                q[h] = *(const T4 *)(qr + t * (uint32_t)d.q.token_stride + 32 * wave + 16 * h);
+            }
+        }
+        gf = gs[t * d.v.heads], beta = betas[t * d.v.heads];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            v[i] = vr[(unsigned long long)(uint32_t)min(t0 + 4 * g + i, sr.count - 1) * (uint32_t)d.v.token_stride];
+    };
+    if (sr.count > 0) load(0);
+    for (int t0 = 0; t0 < sr.count; t0 += kFew) {
+        if (wave < KS) {
+            bf16x8 a[N], b[2][N];
+            f32x4 kk[2] = {};  // of rows j = 4 g + 0 .. 3 and the row n: k_j.k_n and k_j.q_n
+            const f32x4 k0 = __builtin_convertvector(k[0], f32x4), k1 = __builtin_convertvector(k[1], f32x4);
+            const f32x4 q0 = __builtin_convertvector(q[0], f32x4), q1 = __builtin_convertvector(q[1], f32x4);
+            split<N>(__builtin_shufflevector(k0, k1, 0, 1, 2, 3, 4, 5, 6, 7), a);
+            split<N>(__builtin_shufflevector(q0, q1, 0, 1, 2, 3, 4, 5, 6, 7), b[1]);
+#pragma unroll
+            for (int u = 0; u < N; ++u) {
+                b[0][u] = a[u];
+                *(bf16x8 *)(kb + (wave * N + u) * 512 + few_at(n, g)) = a[u];
+                *(bf16x8 *)(qb + (wave * N + u) * 512 + few_at(n, g)) = b[1][u];
+            }
+            mma<2, N, N>(a, b, kk);
+            part[wave][0][lane] = kk[0];
+            part[wave][1][lane] = kk[1];
+        }
+        float last;  // sums of g in 64 bits: differences of them are taken
+        {
+            const bool row = t0 + n < sr.count;
+            const float gn = row ? gf : 0.0f, b = row ? beta : 0.0f;
+            double x = gn < -1e4f ? -1e4 : (double)gn;  // e^-10000 is 0 as e^-inf is, and no inf - inf
+#pragma unroll
+            for (int o = 1; o < kFew; o <<= 1) {
+                const double y = __shfl_up(x, o, kFew);
+                x += n >= o ? y : 0.0;
+            }
+            const double end = __shfl(x, kFew - 1, kFew);
+            last = expf((float)end);
+            if (wave == 0 && g == 0) {
+                Gs[n] = x;
+                egs[n] = expf((float)x);
+                ecs[n] = expf((float)(end - x));
+                bs[n] = b;
+            }
+        }
+        f32x4 vt;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) vt[i] = (float)v[i];
+        if (t0 + kFew < sr.count) load(t0 + kFew);
+        __syncthreads();
+
+        f32x4 xy[2] = {};  // K S^T and Q S^T
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+            bf16x8 a[2][N], b[3];
+            split<3>(__builtin_shufflevector(S[2 * i], S[2 * i + 1], 0, 1, 2, 3, 4, 5, 6, 7), b);
+#pragma unroll
+            for (int u = 0; u < N; ++u) {
+                a[0][u] = *(const bf16x8 *)(kb + (i * N + u) * 512 + few_at(n, g));
+                a[1][u] = *(const bf16x8 *)(qb + (i * N + u) * 512 + few_at(n, g));
+            }
+            mma<2, N, 3>(a, b, xy);
+        }
+        // Row n of A (into LDS, by columns) and of P, at 4 g + 0 .. 3
+        f32x4 kk = part[0][0][lane], P = part[0][1][lane];
+#pragma unroll
+        for (int i = 1; i < KS; ++i) kk += part[i][0][lane], P += part[i][1][lane];
+        const f32x4 eg = *(const f32x4 *)(egs + 4 * g), ec = *(const f32x4 *)(ecs + 4 * g), bt = *(const f32x4 *)(bs + 4 * g);
+        const double Gn = Gs[n];
+        const float bn = bs[n];
+        double Gj[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) Gj[i] = Gs[4 * g + i];
+        float *A = At[wave];
+        int row = n;
+        asm("" : "+v"(row));  // what is compared with it is not kept in registers over the loop
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int j = 4 * g + i;
+            const float e = expf((float)(Gn - Gj[i])), p = d.scale * e * P[i], a = bn * e * kk[i];
+            P[i] = j <= row ? p : 0.0f;
+            A[j * LA + n] = j < row ? a : 0.0f;
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        // Row n of (I + A)^-1 from its last value back: x_j = [j = n] - sum_(k > j) x_k A_kj
+        float x[kFew];
+#pragma unroll
+        for (int j = kFew - 1; j >= 0; --j) {
+            float y = j == row ? 1.0f : 0.0f;
+#pragma unroll
+            for (int o = (kFew - 1) / 4; o >= (j + 1) / 4; --o) {
+                const f32x4 a = *(const f32x4 *)(A + j * LA + 4 * o);
+#pragma unroll
+                for (int i = 3; i >= 0; --i)
+                    if (4 * o + i > j) y = __builtin_fmaf(-x[4 * o + i], a[i], y);
+            }
+            x[j] = y;
+            if (j % 4 == 0) asm volatile("" : "+v"(x[j]) : : "memory");  // not all of A at once in registers
+        }
+        f32x4 t, r, u = {};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float x0 = x[i], x1 = x[4 + i], x2 = x[8 + i], x3 = x[12 + i], lo = g & 1 ? x1 : x0, hi = g & 1 ? x3 : x2;
+            t[i] = (g & 2 ? hi : lo) * bt[i];
+            r[i] = vt[i] - eg[i] * xy[0][i];
+        }
+        bf16x4 tp[3], pp[3], rp[3], up[3], wp[3];
+        split<3>(t, tp);
+        split<3>(r, rp);
+        split<3>(P, pp);
+        mma16(tp, rp, u);
+        const f32x4 w = u * ec;
+        f32x4 y = xy[1] * (eg * d.scale);
+        split<3>(u, up);
+        split<3>(w, wp);
+        mma16(pp, up, y);
+        bool bad = !__builtin_isfinite(last);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            bad |= !(__builtin_isfinite(r[i]) && __builtin_isfinite(u[i]) && __builtin_isfinite(w[i]) && __builtin_isfinite(y[i]));
+        if (__builtin_expect(__any(bad), 0)) {
+            // Row by row: products would carry a value that is not finite, times zeros, to the rows before it.
+            for (int i = t0; i < min(t0 + kFew, sr.count); ++i) {
+                const float e = expf(gs[(unsigned long long)i * d.v.heads]), b = betas[(unsigned long long)i * d.v.heads];
+                const T *ki = kr + (unsigned long long)i * (uint32_t)d.k.token_stride;
+                const T *qi = qr + (unsigned long long)i * (uint32_t)d.q.token_stride;
+                const float vi = (float)vr[(unsigned long long)i * (uint32_t)d.v.token_stride];
+                float sk = 0, sq = 0;
+#pragma unroll
+                for (int m = 0; m < M; ++m) {
+                    __builtin_amdgcn_sched_barrier(0);  // few registers
+#pragma unroll
+                    for (int o = 0; o < 4; ++o) {
+                        S[m][o] *= e;
+                        sk += S[m][o] * (float)ki[16 * m + o];
+                    }
+                }
+                sk += __shfl_xor(sk, 16);
+                sk += __shfl_xor(sk, 32);
+                const float ui = b * (vi - sk);
+#pragma unroll
+                for (int m = 0; m < M; ++m) {
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int o = 0; o < 4; ++o) {
+                        S[m][o] += ui * (float)ki[16 * m + o];
+                        sq += S[m][o] * (float)qi[16 * m + o];
+                    }
+                }
+                sq += __shfl_xor(sq, 16);
+                sq += __shfl_xor(sq, 32);
+                if (in && g == 0) out[(unsigned long long)i * (uint32_t)d.out.token_stride] = (T)(d.scale * sq);
+            }
+        } else {
+#pragma unroll
+            for (int m = 0; m < M; ++m) {
+                typedef short s4 __attribute__((ext_vector_type(4)));
+                bf16x4 a[N];  // K^T: value 16 m + n of rows 4 g + 0 .. 3
+#pragma unroll
+                for (int j = 0; j < N; ++j)
+                    a[j] = __builtin_bit_cast(
+                        bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                    (LDS_AS s4 *)(kb + ((m >> 1) * N + j) * 512 + few_at(4 * g + (n >> 2), n & 3) + 4 * (m & 1))));
+                S[m] *= last;
+                mma16(a, wp, S[m]);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (in && t0 + 4 * g + i < sr.count)
+                    out[(unsigned long long)(uint32_t)(t0 + 4 * g + i) * (uint32_t)d.out.token_stride] = (T)y[i];
+        }
+        __syncthreads();
+    }
+    if (held && d.state_out) {
+#pragma unroll
+        for (int m = 0; m < M; ++m) *(f32x4 *)(d.state_out + at + 16 * m) = S[m];
+    }
+}
+
+// Which of the three.  A wave of 16 state rows takes 0.3 to 0.6 us a row, or 3.5 us for 16 and
+// at first 4 more; the chunks take 3.8 us for 64 with a quarter of the waves, after 15 us of
+// two launches and the rows' preparation.  48 heads of 128, fp32, us by rows, 16 rows and chunks:
+//   1 sequence   8 rows 7.6 and 8.5, 10 rows 9.0 and 8.7; 64 rows 22.8 and 23.3, 96 rows 31.7 and 26.7
+//   4 sequences  6 rows 12.4 and 12.8, 8 rows 14.6 and 12.9; 128 rows 53 and 58, 256 rows 97 and 88
+//   8 sequences  5 rows 17 and 17, 16 rows 35 and 18; 128 rows 72 and 107, 384 rows 194 and 211
+// (bf16: 1 sequence 6 rows 7.2 and 7.8, 8 rows 8.8 and 8.0; 4 sequences 5 rows 11.9 and 11.2;
+// 4 sequences of 128 rows 44 and 41.)
+constexpr uint32_t kMostFew = 64;
+// Waves of 16 state rows that have rows to the end, about: short sequences beside a long one do not keep the card busy.
+unsigned long long waves(const m27q_delta &d) {
+    return (unsigned long long)d.tokens * (d.v.heads * (d.v.dim / 16)) / (d.max_len ? d.max_len : 1);
+}
+bool by_chunks(uint32_t rows, unsigned long long waves) { return rows > kMostFew && rows > waves / 8; }
+bool by_rows(uint32_t rows, unsigned long long waves, bool wide) {
+    return rows < (waves <= 1024 ? 8u : wide ? 6u : 5u);
+}
 
 template <int DK, typename T>
 hipError_t launch_t(const m27q_delta &d, void *scratch, hipStream_t s) {
-    if (d.max_len < kChunkRows) {
+    const unsigned long long w = waves(d);
+    if (by_rows(d.max_len, w, sizeof(T) == 4)) {
         hipLaunchKernelGGL((k_delta_rows<DK, T>), dim3(d.v.heads * (d.v.dim / 16), d.n), dim3(64), 0, s, d);
         return hipGetLastError();
     }
+    if (!by_chunks(d.max_len, w)) {
+        hipLaunchKernelGGL((k_delta_few<DK, T>), dim3(d.v.heads * ((d.v.dim + 63) / 64), d.n), dim3(256), 0, s, d);
+        return hipGetLastError();
+    }
     const unsigned chunks = (d.max_len + kC - 1) / kC, per = d.v.heads / d.k.heads;
-    // a workgroup makes all value heads of a key head where that still leaves two for each CU
-    const unsigned parts = (unsigned long long)chunks * d.k.heads * d.n >= 512 ? 1 : per;
+    // A workgroup makes all value heads of a key head where that leaves enough of them: at 16 key
+    // heads of 3, fp32, 1024 rows 92 against 88 us (256 workgroups), 1500 rows 127 against 132.
+    const unsigned parts = (unsigned long long)chunks * d.k.heads * d.n >= 384 ? 1 : per;
     hipLaunchKernelGGL((k_delta_prepare<DK, T>), dim3(chunks, d.k.heads * parts, d.n), dim3(256), 0, s, d,
                        (float *)scratch, (int)parts);
     const unsigned slices = (d.v.dim + kSlice - 1) / kSlice;
@@ -778,7 +1051,7 @@ hipError_t launch_t(const m27q_delta &d, void *scratch, hipStream_t s) {
 }  // namespace
 
 size_t delta_scratch(uint32_t n, uint32_t tokens, uint32_t max_len, uint32_t heads, uint32_t dk, uint32_t dv) {
-    if (max_len < kChunkRows) return 16;
+    if (max_len <= kMostFew) return 16;  // not by the number of sequences: what does for many does for fewer
     return ((size_t)tokens / kC + n + 1) * heads * kRecord * sizeof(float);
 }
 

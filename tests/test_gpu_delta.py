@@ -274,3 +274,60 @@ def test_values_that_are_not_finite(m27q, dev, lens, row, where, what, t):
         tol = 8 * np.sqrt(max(n, 1) * 128) * 2.0 ** -24 * np.where(np.isfinite(sizes[s]), sizes[s], np.inf)[..., None]
         assert np.all((np.abs(state[s] - ends[s]) <= tol)[fine])
         at += n
+
+
+SIXTEENS = [
+    # lens, k heads, heads, dk, dv, type: 8 to 64 rows, and more of them where there are many sequences
+    ([8], 1, 1, 64, 16, "f32"), ([16], 16, 48, 128, 128, "bf16"), ([17, 1, 0, 31], 2, 6, 128, 80, "f32"),
+    ([33, 48], 1, 3, 64, 256, "f16"), ([64, 50, 63], 4, 4, 128, 128, "f32"), ([32], 2, 2, 64, 48, "bf16"),
+    ([20] * 7 + [130, 0, 75], 4, 8, 128, 256, "f32"), ([100] * 9, 8, 24, 64, 128, "f16"),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,Hk,H,dk,dv,t", SIXTEENS)
+def test_sixteen_rows_at_a_time(m27q, dev, lens, Hk, H, dk, dv, t):
+    say("delta sixteens", lens, Hk, H, dk, dv, t)
+    Problem(m27q, dev, lens, Hk, H, dk, dv, t).check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rate", [0.0, 20.0, 1000.0])
+@pytest.mark.parametrize("head_map", [0, 1])
+def test_sixteens_decays_slots_and_head_order(m27q, dev, rate, head_map):
+    say("delta sixteens", rate, head_map)
+    p = Problem(m27q, dev, [20, 9, 35], 2, 6, 128, 64, rate=rate, slots=[3, 0, -1], n_slots=5)
+    p.check(head_map=head_map)
+    p.check(head_map=head_map, state_out="same")
+    p.check(head_map=head_map, state=False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens", [[14, 49], [64]])
+def test_sixteens_alike_keys_and_cleared_states(m27q, dev, lens):
+    say("delta sixteens alike", lens)
+    p = Problem(m27q, dev, lens, 1, 2, 64, 32, rate=0.1)
+    p.k[:] = p.k[0]
+    p.beta[:] = 1.0
+    p.check()
+    for t in (0, 5, sum(lens) - 1):
+        p.g[t, 0] = -float("inf")
+    p.check()
+
+
+@pytest.mark.gpu
+def test_sixteens_past_what_the_products_hold(m27q, dev):
+    """Values near the largest fp32 one (whose 16-bit parts overflow) and growth that overflows on the way."""
+    say("delta sixteens, large")
+    p = Problem(m27q, dev, [40], 1, 2, 64, 32)
+    p.v[21, 1, 3] = 3.4e38
+    p.g[30, 0] = 60.0
+    p.g[33, 0] = 40.0
+    got, _ = p.run()
+    with np.errstate(all="ignore"):
+        want, _, _, _ = p.want()
+        want32 = np.abs(want) < 2.0 ** 127
+    tol = 8 * np.sqrt(40 * 128) * 2.0 ** -24 * 64 ** -0.5
+    for h, rows in ((0, slice(0, 30)), (1, slice(0, 21))):
+        assert np.all(np.abs(got[rows, h] - want[rows, h]) <= tol * 5)  # states of norm 5 at most before
+    assert np.all(np.isfinite(got[:33]) | ~want32[:33])
