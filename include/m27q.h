@@ -1,5 +1,6 @@
 /*
- * m27q.h -- C ABI of the MI355X (gfx950) quantized linear-algebra path.
+ * m27q.h -- C ABI of the MI355X (gfx950) quantized linear-algebra path and the
+ * token mixers beside it.
  *
  * Drop-in for the matvec launch layer of mono27b (eramax/mono-qwen27,
  * src/mono27b_executor.cu, "exec" below).  Every entry point names the
@@ -497,8 +498,9 @@ typedef struct m27q_delta {
 } m27q_delta;
 
 /* scratch (16-byte aligned) >= m27q_delta_scratch_bytes; what it holds is of no
- * matter.  Few rows go through the rule row by row, more in chunks of 64 as
- * triangular systems, with fp32-accurate products throughout. */
+ * matter.  Few rows go through the rule row by row, more 16 or 64 at a time as
+ * triangular systems, with fp32-accurate products throughout.  What is enough
+ * for some n, tokens, max_len and heads is enough for smaller ones. */
 M27Q_API size_t m27q_delta_scratch_bytes(uint32_t n, uint32_t tokens, uint32_t max_len, uint32_t heads, uint32_t dk,
                                          uint32_t dv);
 M27Q_API m27q_status m27q_delta_rule(const m27q_delta *d, void *scratch, size_t scratch_bytes, hipStream_t stream);

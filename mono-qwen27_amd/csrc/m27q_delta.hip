@@ -33,7 +33,10 @@ struct Vec4<__bf16> {
 // covers 64 contiguous bytes of a row and a row's sum is two DPP steps).  For a
 // single row the state's bytes bound it: it is read and written once.  The two
 // products of a row (S k, S q) are taken from the old state, with
-// S_new q = e^g S q + u (k.q): one pass, then the update.
+// S_new q = e^g S q + u (k.q): one pass, then the update.  64 sequences of 48 heads of 128 x
+// 128: 407 MB in 72 us, 5.6 TB/s (a copy runs at 4.97).  Of more rows the 160 fp32 operations
+// a lane and row bound it, 0.5 us where a SIMD has one wave; the next row's loads ahead of
+// them changed nothing (16 rows 12.3 and 12.1 us), and cost the single row registers.
 template <int DK, typename T>
 __global__ __launch_bounds__(64) void k_delta_rows(const m27q_delta d) {
     typedef typename Vec4<T>::t T4;
@@ -226,7 +229,10 @@ __device__ __forceinline__ int lds_at(int row, int col) {
 }
 
 // A chunk of a key head: K K^T and Q K^T once, then for its value heads (every `parts`-th
-// of them) the triangular inverse.
+// of them) the triangular inverse.  Chains of dependent steps bound it (vector and matrix
+// instructions fill 27 of 63 us), so it is made small, for four workgroups a CU: K lies in LDS
+// 64 columns at a time, P takes A's place there (4096 rows of 16 key heads of 3, fp32: 49 us;
+// with two workgroups a CU 63).  It writes 36 KB a chunk and head.
 template <int DK, typename T>
 __global__ __launch_bounds__(256, 4) void k_delta_prepare(const m27q_delta d, float *scratch, int parts) {
     constexpr int N = In<T>::N, LM = kC + 4;
@@ -488,6 +494,12 @@ __device__ __forceinline__ void row_by_row(const m27q_delta &d, const SeqRows &s
 //   3  S <- e^(G_C) S + K^T diag(..) U       | K's pieces to LDS, out = .. Q S^T + P U
 // Operands that come from memory are asked for again, for the next chunk, as soon as they have
 // been used, without branches (a load under one would keep later waits from telling it apart).
+// The chain of the three products bounds it: 4096 rows of 48 heads of 128 (192 workgroups),
+// fp32, 64 chunks of 3.8 us, 7000 to 9000 cycles of which the matrix units work 2900, LDS 3400;
+// Q S^T in pieces is the longest of part 2.  243 us after 49 of preparation; four BF16 sequences
+// of up to 1531 rows (768 workgroups, one a CU at a time: two would need 128 registers, which
+// spill, 296 against 258 us in all) 200 after 59.  Q cut into pieces in part 1 instead: 333
+// against 304; K's loads and pieces with the state's waves: 337.
 template <int DK, typename T>
 __global__ __launch_bounds__(512) void k_delta_chunks(const m27q_delta d, const float *scratch) {
     constexpr int N = In<T>::N, KS = DK / 32, MT = DK / 64;
@@ -764,6 +776,9 @@ __global__ __launch_bounds__(512) void k_delta_chunks(const m27q_delta d, const 
 // a result's 4 g + 0 .. 3 are the operand of the instructions over 16.  So state, right-hand
 // sides and U go from product to product in registers.  The four waves of a workgroup share
 // K and Q in LDS, as operand blocks [step][piece][64 lanes][8], a step of 32 columns a wave.
+// A wave's chain of products bounds it where a SIMD has one (16 more rows 4.2 us), the state's
+// bytes where it has several: 16 rows of 8 sequences, 48 heads of 128 x 128, 50 MB of states,
+// 17.6 us in fp32 and 15.1 in BF16 (row by row 35).
 
 template <int NA, int NB>
 __device__ __forceinline__ void mma16(const bf16x4 (&a)[NA], const bf16x4 (&b)[NB], f32x4 &c) {
