@@ -223,18 +223,22 @@ struct Rows {
         for (int i = 0; i < D / RW; ++i) o[i] = acc{};
     }
 
+    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+    struct Raw {
+        u4 v[D / KD];
+    };
     // token and head: a row of the call's, also for a lane that has none (and takes zeros)
-    __device__ __forceinline__ void load_q(const AttnParams &p, int token, int head, bool live) {
+    static __device__ __forceinline__ void load_q(const AttnParams &p, int token, int head, Raw &r) {
         const T *from =
             (const T *)p.q.ptr + (long long)token * p.q.token_stride + (long long)head * p.q.head_stride + 8 * part();
-        typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+        for (int i = 0; i < D / KD; ++i) r.v[i] = *(const u4 *)(from + KD * i);
+    }
+    __device__ __forceinline__ void set_q(const AttnParams &p, const Raw &r, bool live) {
         // a negative scale goes into q, exactly: scores are then compared before scaling
         const uint32_t flip = p.scale < 0 ? 0x80008000u : 0, keep = live ? ~0u : 0u;
-        u4 v[D / KD];
 #pragma unroll
-        for (int i = 0; i < D / KD; ++i) v[i] = *(const u4 *)(from + KD * i);
-#pragma unroll
-        for (int i = 0; i < D / KD; ++i) q[i] = __builtin_bit_cast(T8, (v[i] ^ flip) & keep);
+        for (int i = 0; i < D / KD; ++i) q[i] = __builtin_bit_cast(T8, (r.v[i] ^ flip) & keep);
     }
 
     // The tile in LDS.  MASK: some of its keys may be hidden from some row, or missing.
@@ -374,15 +378,15 @@ struct Rows {
     }
 };
 
-// Looks at every page of the keys once, for the whole workgroup: tiles trust them then.
-__device__ __forceinline__ bool any_gaps(const AttnParams &p, const Work &w) {
+// Looks at every page of the keys once, the threads of a workgroup in turn: tiles trust them then.
+__device__ __forceinline__ bool has_gaps(const AttnParams &p, const Work &w) {
     const int shift = __builtin_ctz(p.cache.page_size);
     const int32_t *table = p.seqs.table + (long long)w.s * p.seqs.table_stride;
     bool bad = false;
     if (w.lo < w.hi)
         for (int i = (w.lo >> shift) + (int)threadIdx.x; i <= (w.hi - 1) >> shift; i += kWaves * 64)
             bad |= (uint32_t)table[i] >= p.cache.pages;
-    return __syncthreads_or(bad);
+    return bad;
 }
 
 // Many rows: four waves of 32 rows a workgroup, K and V of a tile of 32 keys in LDS, the next
@@ -432,11 +436,13 @@ __global__ __launch_bounds__(kWaves * 64, 2) void k_attn(const AttnParams p) {
     R x;
     x.place = live ? place0 + row / group : -1;
     x.clear();
-    x.load_q(p, token, qh, live);
+    typename R::Raw q;
+    R::load_q(p, token, qh, q);
+    x.set_q(p, q, live);
     // (a scale of 0 would make NaN of a masked score's -inf)
     const float sc = fmaxf(fabsf(p.scale) * kLog2e, 1e-37f);
 
-    w.gaps = any_gaps(p, w);
+    w.gaps = __syncthreads_or(has_gaps(p, w));
     // tiles [ta, tb) are seen whole by every row of the workgroup: the next one is
     // on its way while one is worked on; the others, at the ends, go one by one
     const int tiles = max(0, w.hi - w.lo + kKeys - 1) / kKeys;
@@ -536,10 +542,12 @@ __global__ __launch_bounds__(kWaves * 64, 1) void k_attn_few(const AttnParams p)
     w.s = s;
     w.head = blockIdx.x - s * p.cache.heads;
     const SeqRows sr = seq_rows(p.seqs.start, s, (int)p.seqs.tokens, (int)p.seqs.max_q);
+    int len = p.seqs.kv_len[s];
+    asm("" : "+s"(len));  // asked for with the rows, not behind the branch
     w.rows = sr.count * group;
     if (w.rows == 0) return;
-    const int kv = min(max(p.seqs.kv_len[s], 0), (int)p.seqs.max_kv);
-    const int first = p.seqs.kv_len[s] - (sr.end - sr.first), last = first + sr.count - 1;
+    const int kv = min(max(len, 0), (int)p.seqs.max_kv);
+    const int first = len - (sr.end - sr.first), last = first + sr.count - 1;
     w.lo = p.window ? max(0, first - p.window + 1) & ~(kKeys - 1) : 0;
     w.hi = min(kv, last + 1);
     if (p.splits > 1) {
@@ -550,7 +558,13 @@ __global__ __launch_bounds__(kWaves * 64, 1) void k_attn_few(const AttnParams p)
     }
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const bool live = (lane & (RW - 1)) < w.rows;
-    const int row = min(lane & (RW - 1), w.rows - 1);
+    const int row = min(lane & (RW - 1), w.rows - 1), at = row / group;
+    const int token = sr.first + at, qh = w.head * group + row - at * group;
+    const long long part = ((long long)token * p.q.heads + qh) * p.splits + blockIdx.y;
+    // loads end in order: what is needed first is asked for first
+    typename R::Raw q;
+    R::load_q(p, token, qh, q);
+    const bool gaps = has_gaps(p, w);
     LDS_AS char *const kt = (LDS_AS char *)kts + wave * TB, *const vt = (LDS_AS char *)vts + wave * TB;
     const int32_t *table = p.seqs.table + (long long)s * p.seqs.table_stride;
     const int shift = __builtin_ctz(p.cache.page_size);
@@ -563,25 +577,26 @@ __global__ __launch_bounds__(kWaves * 64, 1) void k_attn_few(const AttnParams p)
     constexpr int RPI = 512 / D, CPR = D / 8;
     const int r0 = lane / CPR, pc = lane % CPR;
     const uint32_t ko = r0 * D * 2 + k_chunk<D>(r0, pc) * 16, vo = r0 * D * 2 + v_chunk<D>(r0, pc) * 16;
-    // K (or V) of the tile at k0; `checked` as in load_tile, otherwise a page that is none is
-    // read as the first (and what it gives is not used)
-    auto load = [&](const void *from, LDS_AS char *to, bool keys, int k0, const int (&pages)[2], bool checked,
-                    bool clear) {
+    // K (or V) of the tile at k0.  `checked`: of keys past `hi` or on a page that is not one,
+    // another row of the cache is read (their weights are 0); otherwise all 16 rows of each half
+    // are there, a page that is none is read as the first, and what it gives is not used.
+    auto load = [&](const void *from, LDS_AS char *to, bool keys, int k0, const int (&pages)[2], bool checked) {
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             const int id = __builtin_amdgcn_readfirstlane(pages[half]), key = k0 + 16 * half;
-            const bool ok = (uint32_t)id < p.cache.pages;
-            const int rows = checked ? (ok ? w.hi - key : 0) : 16;
-            const long long at = ((long long)(ok && rows > 0 ? id : 0) * p.cache.page_stride +
+            const bool ok = (uint32_t)id < p.cache.pages && (!checked || key < w.hi);
+            const int rows = checked ? (ok ? min(w.hi - key, 16) : 1) : 16;
+            const long long at = ((long long)(ok ? id : 0) * p.cache.page_stride +
                                   ((long long)w.head * p.cache.page_size + (key & (int)(p.cache.page_size - 1))) * D) * 2;
-            const __amdgpu_buffer_rsrc_t rs = buf_rsrc((const char *)from + at, 16 * D * 2);
+            const __amdgpu_buffer_rsrc_t rs = buf_rsrc((const char *)from + at, rows * D * 2);
 #pragma unroll
             for (int i = 0; i < 16 / RPI; ++i) {
                 LDS_AS char *d = to + (16 * half + i * RPI) * D * 2;
                 const uint32_t o = keys ? ko ^ (k_chunk<D>(i * RPI, 0) * 16) : vo ^ (v_chunk<D>(i * RPI, 0) * 16);
-                if (!checked || i * RPI + r0 < rows)
-                    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (LDS_AS void *)d, 16, o, i * 1024, 0, 0);
-                else if (clear) *(LDS_AS f32x4 *)(d + lane * 16) = f32x4{0, 0, 0, 0};
+                const uint32_t back = checked ? max(i * RPI + r0 - (rows - 1), 0) * D * 2 : 0;
+                const uint32_t oo = i * 1024 + o - back;
+                if (checked) __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (LDS_AS void *)d, 16, oo, 0, 0, 0);
+                else __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (LDS_AS void *)d, 16, o, i * 1024, 0, 0);
             }
         }
     };
@@ -596,8 +611,8 @@ __global__ __launch_bounds__(kWaves * 64, 1) void k_attn_few(const AttnParams p)
     if (t < tb) {
         ids[0] = page(w.lo + t * kKeys, 0);
         ids[1] = page(w.lo + t * kKeys, 1);
-        load(p.cache.k, kt, true, w.lo + t * kKeys, ids, false, false);
-        load(p.cache.v, vt, false, w.lo + t * kKeys, ids, false, false);
+        load(p.cache.k, kt, true, w.lo + t * kKeys, ids, false);
+        load(p.cache.v, vt, false, w.lo + t * kKeys, ids, false);
     }
     // a wave that has none of them asks for its first one of the others
     int there = -1;
@@ -606,16 +621,16 @@ __global__ __launch_bounds__(kWaves * 64, 1) void k_attn_few(const AttnParams p)
         if (there < tiles) {
             ids[0] = page(w.lo + there * kKeys, 0);
             ids[1] = page(w.lo + there * kKeys, 1);
-            load(p.cache.k, kt, true, w.lo + there * kKeys, ids, true, false);
-            load(p.cache.v, vt, false, w.lo + there * kKeys, ids, true, true);
+            load(p.cache.k, kt, true, w.lo + there * kKeys, ids, true);
+            load(p.cache.v, vt, false, w.lo + there * kKeys, ids, true);
         }
     }
     R x;
-    x.place = live ? first + row / group : -1;
+    x.place = live ? first + at : -1;
     x.clear();
-    x.load_q(p, sr.first + row / group, w.head * group + row % group, live);
+    x.set_q(p, q, live);
     const float sc = fmaxf(fabsf(p.scale) * kLog2e, 1e-37f);
-    w.gaps = any_gaps(p, w);
+    w.gaps = __syncthreads_or(gaps);
     if (w.gaps) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         ta = tb = 0;
@@ -631,20 +646,21 @@ __global__ __launch_bounds__(kWaves * 64, 1) void k_attn_few(const AttnParams p)
         x.scores(kt, sco);
         x.template weights<false>(p, w, sc, sco, k0, pcs);
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        if (t + kWaves < tb) load(p.cache.k, kt, true, k1, ids, false, false);
+        if (t + kWaves < tb) load(p.cache.k, kt, true, k1, ids, false);
         x.values(vt, pcs);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // V has been read
-        if (t + kWaves < tb) load(p.cache.v, vt, false, k1, ids, false, false);
+        if (t + kWaves < tb) load(p.cache.v, vt, false, k1, ids, false);
     }
+    // the others, which begin where none of those is
+    const auto other = [&](int t) { return t >= ta && t < tb ? t + ((tb - t + kWaves - 1) & ~(kWaves - 1)) : t; };
     bool odd = false;
-    for (int t = wave; t < tiles; t += kWaves) {
-        if (t >= ta && t < tb) continue;
+    for (int t = other(wave); t < tiles; t = other(t + kWaves)) {
         const int k0 = w.lo + t * kKeys;
         if (t != there) {
             ids[0] = page(k0, 0);
             ids[1] = page(k0, 1);
-            load(p.cache.k, kt, true, k0, ids, true, false);
-            load(p.cache.v, vt, false, k0, ids, true, true);
+            load(p.cache.k, kt, true, k0, ids, true);
+            load(p.cache.v, vt, false, k0, ids, true);
         }
         there = -1;
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
@@ -654,10 +670,9 @@ __global__ __launch_bounds__(kWaves * 64, 1) void k_attn_few(const AttnParams p)
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
     if (__builtin_expect(__any(odd), 0))
-        for (int t = wave; t < tiles; t += kWaves) {
-            if (t >= ta && t < tb) continue;
+        for (int t = other(wave); t < tiles; t = other(t + kWaves)) {
             const int k0 = w.lo + t * kKeys, ids[2] = {page(k0, 0), page(k0, 1)};
-            load(p.cache.v, vt, false, k0, ids, true, true);
+            load(p.cache.v, vt, false, k0, ids, true);
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
             x.add_odd(p, w, k0, vt);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -698,8 +713,6 @@ __global__ __launch_bounds__(kWaves * 64, 1) void k_attn_few(const AttnParams p)
         l += ls[i][col] * e;
     }
     if (!live) return;
-    const int token = sr.first + row / group, qh = w.head * group + row % group;
-    const long long part = ((long long)token * p.q.heads + qh) * p.splits + blockIdx.y;
     if (p.splits > 1 && threadIdx.x < RW) p.stat[part] = make_float2(m * sc, l);
     if (p.splits > 1 && l == 0) return;
     const long long to = (long long)token * p.out.token_stride + (long long)qh * p.out.head_stride;
@@ -709,9 +722,11 @@ __global__ __launch_bounds__(kWaves * 64, 1) void k_attn_few(const AttnParams p)
         const int quad = threadIdx.x / RW + u * (kWaves * 64 / RW);
         f32x4 o = {0, 0, 0, 0};
 #pragma unroll
-        for (int i = 0; i < kWaves; ++i)
-            if (fs[i] != 0)
-                o += *(const LDS_AS f32x4 *)((LDS_AS char *)(quad < HALF ? kts : vts - TB) + i * TB + (quad * RW + col) * 16);
+        for (int i = 0; i < kWaves; ++i) {  // all reads at once: what a wave without keys left is read and dropped
+            const f32x4 y = *(const LDS_AS f32x4 *)((LDS_AS char *)(quad < HALF ? kts : vts - TB) + i * TB + (quad * RW + col) * 16);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[j] += fs[i] != 0 ? y[j] : 0.0f;
+        }
         if (p.splits > 1) {
             *(f32x4 *)(p.part + part * D + 4 * quad) = o;
             continue;
