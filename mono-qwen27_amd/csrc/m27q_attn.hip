@@ -164,21 +164,30 @@ __device__ __forceinline__ void tile_barrier() {
 template <int D, bool BF, int ROWS>
 __device__ __forceinline__ bool clear_odd(LDS_AS char *at) {
     typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
     constexpr uint32_t E = BF ? 0x7f80u : 0x7c00u;
-    bool odd = false;
+    constexpr int N = ROWS * D / 512;
     at += (threadIdx.x & 63) * 16;
+    u4 v[N];
 #pragma unroll
-    for (int i = 0; i < ROWS * D / 512; ++i) {
-        u4 v = *(LDS_AS u4 *)(at + i * 1024);
-        bool here = false;
+    for (int i = 0; i < N; ++i) v[i] = *(LDS_AS u4 *)(at + i * 1024);
+    u16x2 top = {0, 0};  // the largest of the values without their signs
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const bool a = (v[j] & E) == E, b = ((v[j] >> 16) & E) == E;
-            v[j] &= (a ? 0xffff0000u : ~0u) & (b ? 0xffffu : ~0u);
-            here |= a || b;
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, v[i][j] & 0x7fff7fffu));
+    const bool odd = top[0] >= E || top[1] >= E;
+    if (__builtin_expect(odd, 0)) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const bool a = (v[i][j] & E) == E, b = ((v[i][j] >> 16) & E) == E;
+                v[i][j] &= (a ? 0xffff0000u : ~0u) & (b ? 0xffffu : ~0u);
+            }
+            *(LDS_AS u4 *)(at + i * 1024) = v[i];
         }
-        if (here) *(LDS_AS u4 *)(at + i * 1024) = v;
-        odd |= here;
     }
     return odd;
 }
@@ -241,17 +250,20 @@ struct Rows {
         for (int i = 0; i < D / KD; ++i) q[i] = __builtin_bit_cast(T8, (r.v[i] ^ flip) & keep);
     }
 
-    // The tile in LDS.  MASK: some of its keys may be hidden from some row, or missing.
-    template <bool MASK>
+    // The tile in LDS.  MASK: some of its keys may be hidden from some row, or missing.  AHEAD:
+    // all of a product's reads before its first instruction, for a wave that has its SIMD (and
+    // its registers) to itself; otherwise the compiler leaves each to wait for its own.
+    template <bool MASK, bool AHEAD>
     __device__ __forceinline__ void tile(const AttnParams &p, const Work &w, float sc, int k0, const LDS_AS char *kt,
                                          const LDS_AS char *vt) {
         float s[NS];
         T8 pc[NV][NP];
-        scores(kt, s);
+        scores<AHEAD>(kt, s);
         weights<MASK>(p, w, sc, s, k0, pc);
-        values(vt, pc);
+        values<AHEAD>(vt, pc);
     }
 
+    template <bool AHEAD>
     __device__ __forceinline__ void scores(const LDS_AS char *kt, float (&s)[NS]) const {
         const int r = threadIdx.x & (RW - 1);
         // chunk G i + part of key row r (and r + 16): k_chunk of it is (y ^ (G i & M)) + (G i & ~M),
@@ -263,10 +275,16 @@ struct Rows {
 #pragma unroll
         for (int b = 0; b < kKeys / RW; ++b) {
             acc c = {};
+            T8 a[D / KD];
 #pragma unroll
             for (int i = 0; i < D / KD; ++i) {
-                const T8 a = *(const LDS_AS T8 *)(kr + b * RW * D * 2 + (y ^ (G * i & M)) * 16 + (G * i & ~M) * 16);
-                c = N::mma(a, q[i], c);
+                a[i] = *(const LDS_AS T8 *)(kr + b * RW * D * 2 + (y ^ (G * i & M)) * 16 + (G * i & ~M) * 16);
+                if constexpr (!AHEAD) c = N::mma(a[i], q[i], c);
+            }
+            if constexpr (AHEAD) {
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int i = 0; i < D / KD; ++i) c = N::mma(a[i], q[i], c);
             }
 #pragma unroll
             for (int i = 0; i < NA; ++i) s[b * NA + i] = c[i];
@@ -322,20 +340,33 @@ struct Rows {
 
     // O += weights times values.  V^T: lane (value RW t + lane % RW, part g) takes the keys of its
     // weights, STEP (2 i + e) + 4 g + 0 .. 3.
+    template <bool AHEAD>
     __device__ __forceinline__ void values(const LDS_AS char *vt, const T8 (&pc)[NV][NP]) {
         const int lane = threadIdx.x & 63, x = 4 * part() + ((lane & 15) >> 2);  // the key this lane's 16 lanes read for
         const LDS_AS char *vr = vt + x * D * 2 + (lane & 3) * 8;
         constexpr int M = D >= 128 ? 7 : 3, U = RW / 16;
         const int y = v_swap<D>(x) ^ ((lane >> 4) & (U - 1));  // 32-byte unit U t + .. of a row, exchanged
+        T8 v[D / RW][NV];
 #pragma unroll
         for (int t = 0; t < D / RW; ++t)
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const LDS_AS char *at = vr + 2 * i * STEP * D * 2 + ((U * t & M) ^ y) * 32 + (U * t & ~M) * 32;
-                const T8 v = __builtin_shufflevector(tr4(at), tr4(at + STEP * D * 2), 0, 1, 2, 3, 4, 5, 6, 7);
+                v[t][i] = __builtin_shufflevector(tr4(at), tr4(at + STEP * D * 2), 0, 1, 2, 3, 4, 5, 6, 7);
+                if constexpr (!AHEAD) {
 #pragma unroll
-                for (int j = 0; j < NP; ++j) o[t] = N::mma(v, pc[i][j], o[t]);
+                    for (int j = 0; j < NP; ++j) o[t] = N::mma(v[t][i], pc[i][j], o[t]);
+                }
             }
+        if constexpr (AHEAD) {
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int j = 0; j < NP; ++j)
+#pragma unroll
+                    for (int t = 0; t < D / RW; ++t) o[t] = N::mma(v[t][i], pc[i][j], o[t]);
+        }
     }
 
     // Whether this lane's row sees a key.
@@ -465,14 +496,14 @@ __global__ __launch_bounds__(kWaves * 64, 2) void k_attn(const AttnParams p) {
             load_tile<D, false>(p, w, w.lo + (t + 1) * kKeys, id, kb, vb);
             id = tile_page(p, w, w.lo + (t + 2) * kKeys);
         }
-        if (any) x.template tile<false>(p, w, sc, w.lo + t * kKeys, ka, va);
+        if (any) x.template tile<false, false>(p, w, sc, w.lo + t * kKeys, ka, va);
         if (t + 1 >= tb) break;
         tile_barrier();
         if (t + 2 < tb) {
             load_tile<D, false>(p, w, w.lo + (t + 2) * kKeys, id, ka, va);
             id = tile_page(p, w, w.lo + (t + 3) * kKeys);
         }
-        if (any) x.template tile<false>(p, w, sc, w.lo + (t + 1) * kKeys, kb, vb);
+        if (any) x.template tile<false, false>(p, w, sc, w.lo + (t + 1) * kKeys, kb, vb);
     }
     bool odd = false;
     for (int i = 0; i < tiles - (tb - ta); ++i) {
@@ -482,7 +513,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void k_attn(const AttnParams p) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         odd |= clear_odd<D, BF, kKeys / kWaves>(va + wave * (kKeys / kWaves) * D * 2);
         __syncthreads();
-        if (any) x.template tile<true>(p, w, sc, k0, ka, va);
+        if (any) x.template tile<true, false>(p, w, sc, k0, ka, va);
     }
     if (__builtin_expect(__syncthreads_or(odd), 0))
         for (int i = 0; i < tiles - (tb - ta); ++i) {
@@ -530,7 +561,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void k_attn(const AttnParams p) {
 // copy runs at 4.97); 2 of up to 32768 keys and 5 rows each, 253 MB in 57 us and 6 of joining,
 // 4.1 TB/s: a wave has some 9 tiles between its start and the join.
 template <int D, bool BF, int NP, int RW>
-__global__ __launch_bounds__(kWaves * 64, 1) void k_attn_few(const AttnParams p) {
+__global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) void k_attn_few(const AttnParams p) {
     typedef Rows<D, BF, NP, RW> R;
     typedef typename R::T T;
     constexpr int TB = kKeys * D * 2;  // bytes of a tile
@@ -643,11 +674,11 @@ __global__ __launch_bounds__(kWaves * 64, 1) void k_attn_few(const AttnParams p)
         ids[1] = page(k1, 1);
         // K is there when no more than V's loads are on their way
         asm volatile("s_waitcnt vmcnt(%0)" ::"n"(32 / RPI) : "memory");
-        x.scores(kt, sco);
+        x.template scores<true>(kt, sco);
         x.template weights<false>(p, w, sc, sco, k0, pcs);
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         if (t + kWaves < tb) load(p.cache.k, kt, true, k1, ids, false);
-        x.values(vt, pcs);
+        x.template values<true>(vt, pcs);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // V has been read
         if (t + kWaves < tb) load(p.cache.v, vt, false, k1, ids, false);
     }
@@ -666,7 +697,7 @@ __global__ __launch_bounds__(kWaves * 64, 1) void k_attn_few(const AttnParams p)
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         odd |= clear_odd<D, BF, kKeys>(vt);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        x.template tile<true>(p, w, sc, k0, kt, vt);
+        x.template tile<true, true>(p, w, sc, k0, kt, vt);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
     if (__builtin_expect(__any(odd), 0))
