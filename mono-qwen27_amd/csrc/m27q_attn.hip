@@ -591,7 +591,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) void k_attn_few(cons
     const bool live = (lane & (RW - 1)) < w.rows;
     const int row = min(lane & (RW - 1), w.rows - 1), at = row / group;
     const int token = sr.first + at, qh = w.head * group + row - at * group;
-    const long long part = ((long long)token * p.q.heads + qh) * p.splits + blockIdx.y;
+    const unsigned long long part = (unsigned long long)((uint32_t)token * p.q.heads + qh) * (uint32_t)p.splits + blockIdx.y;
     // loads end in order: what is needed first is asked for first
     typename R::Raw q;
     R::load_q(p, token, qh, q);
@@ -744,27 +744,40 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) void k_attn_few(cons
         l += ls[i][col] * e;
     }
     if (!live) return;
-    if (p.splits > 1 && threadIdx.x < RW) p.stat[part] = make_float2(m * sc, l);
-    if (p.splits > 1 && l == 0) return;
+    constexpr int Q = D / 4 * RW / (kWaves * 64);  // quadruples of a thread
+    f32x4 y[Q][kWaves], o[Q];
+#pragma unroll
+    for (int u = 0; u < Q; ++u)  // all reads at once: what a wave without keys left is read and dropped
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) {
+            const int quad = threadIdx.x / RW + u * (kWaves * 64 / RW);
+            y[u][i] = *(const LDS_AS f32x4 *)((LDS_AS char *)(quad < HALF ? kts : vts - TB) + i * TB + (quad * RW + col) * 16);
+        }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < Q; ++u) {
+        o[u] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[u][j] += fs[i] != 0 ? y[u][i][j] : 0.0f;
+    }
+    if (p.splits > 1) {
+        if (threadIdx.x < RW) p.stat[part] = make_float2(m * sc, l);
+        if (l == 0) return;
+#pragma unroll
+        for (int u = 0; u < Q; ++u)
+            *(f32x4 *)(p.part + part * D + 4 * (threadIdx.x / RW + u * (kWaves * 64 / RW))) = o[u];
+        return;
+    }
     const long long to = (long long)token * p.out.token_stride + (long long)qh * p.out.head_stride;
     const float inv = l == 0 ? 0.0f : 1.0f / l;
 #pragma unroll
-    for (int u = 0; u < D / 4 * RW / (kWaves * 64); ++u) {
+    for (int u = 0; u < Q; ++u) {
         const int quad = threadIdx.x / RW + u * (kWaves * 64 / RW);
-        f32x4 o = {0, 0, 0, 0};
-#pragma unroll
-        for (int i = 0; i < kWaves; ++i) {  // all reads at once: what a wave without keys left is read and dropped
-            const f32x4 y = *(const LDS_AS f32x4 *)((LDS_AS char *)(quad < HALF ? kts : vts - TB) + i * TB + (quad * RW + col) * 16);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) o[j] += fs[i] != 0 ? y[j] : 0.0f;
-        }
-        if (p.splits > 1) {
-            *(f32x4 *)(p.part + part * D + 4 * quad) = o;
-            continue;
-        }
-        o = l == 0 ? f32x4{0, 0, 0, 0} : o * inv;
-        if (p.out.type == M27Q_TYPE_F32) *(f32x4 *)((float *)p.out.ptr + to + 4 * quad) = o;
-        else *(typename R::T4 *)((T *)p.out.ptr + to + 4 * quad) = __builtin_convertvector(o, typename R::T4);
+        const f32x4 x = l == 0 ? f32x4{0, 0, 0, 0} : o[u] * inv;
+        if (p.out.type == M27Q_TYPE_F32) *(f32x4 *)((float *)p.out.ptr + to + 4 * quad) = x;
+        else *(typename R::T4 *)((T *)p.out.ptr + to + 4 * quad) = __builtin_convertvector(x, typename R::T4);
     }
 }
 
