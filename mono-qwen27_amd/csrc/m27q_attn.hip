@@ -12,9 +12,9 @@
 // Two kernels.  Many rows (k_attn) share tiles of keys that a workgroup brings into LDS once:
 // the matrix units bound it.  Up to 32 rows of a sequence and cache head (k_attn_few) are one
 // wave's, so its waves take keys apart from each other, and the cache's bytes bound it.
-// Such rows through k_attn: one token over 1021 keys 24.5 us, by k_attn_few 15; 32 tokens over
-// up to 16381 keys 324 and 296; 2 x 5 rows over 32768 keys 99 and 74 (62 with the parts rule
-// below).
+// Such rows through k_attn: one token over 1021 keys 22.6 us, by k_attn_few 11.4; 32 tokens over
+// up to 16381 keys 312 and 288; 2 x 5 rows over 32768 keys 62.4 and 59.9; 64 tokens over 3000
+// keys 125 and 112.
 #include "m27q_device.h"
 #include "m27q_internal.h"
 #include "m27q_mix.h"
@@ -557,9 +557,11 @@ __global__ __launch_bounds__(kWaves * 64, 2) void k_attn(const AttnParams p) {
 // of a workgroup take tiles in turn, each for itself with K and V tiles of its own: K of
 // its next tile is on its way from the moment its scores are there, V from when its values
 // are added, and nothing waits for another wave.  At the end the four sums are joined.
-// 32 sequences of up to 16381 keys, 4 cache heads of 256, F16: 1.58 GB in 295 us, 5.4 TB/s (a
-// copy runs at 4.97); 2 of up to 32768 keys and 5 rows each, 253 MB in 57 us and 6 of joining,
-// 4.1 TB/s: a wave has some 9 tiles between its start and the join.
+// 32 sequences of up to 16381 keys, 4 cache heads of 256, F16: 1.58 GB in 288 us, 5.5 TB/s (a
+// copy runs at 4.97); 2 of up to 32768 keys and 5 rows each, 253 MB in 54 us and 6 of joining,
+// 4.2 TB/s: a wave has some 9 tiles between its start and the join.  One token over 1021 keys: a
+// tile a wave, and a chain of 16000 cycles (lengths 3500, page and loads 2700, their arrival
+// 2500, products and weights 2800, the waves' join 4300), then 3 us of the parts' join.
 template <int D, bool BF, int NP, int RW>
 __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) void k_attn_few(const AttnParams p) {
     typedef Rows<D, BF, NP, RW> R;
@@ -885,8 +887,9 @@ hipError_t launch_t(const AttnParams &p, const AttnPlan &plan, hipStream_t s) {
 // 256 keys at least.  Few rows: one workgroup on each CU (dim 256: its tiles take the LDS),
 // or two, and twice that from 64 pairs of sequence and head on, for ragged ones to even out,
 // unless the pairs fill the CUs; parts of 128 keys at least, a tile for each wave.  Measured
-// at one, two and four times the CUs: dim 256, 2 sequences of 32768 keys 63 / 74 / 75 us, 32
-// of 16381 301 / 294 / 297, 64 of 3000 117 / 123 / 129; dim 128, 2 of 16384 31 / 30 / 37.
+// at one, two and four times that: dim 256, 2 sequences of 32768 keys 60 / 71 / 70 us, 32 of
+// 16381 293 / 289 / 291, 64 of 3000 112 / 118 / 123; dim 128, 2 of 16384 30 / 35 / 35, 16 of
+// 8000 83 / 85 / 88; dim 64, 2 of 16384 20 / 23 / 23, 16 of 8000 49 / 48 / 49.
 AttnPlan attn_plan(const m27q_seqs &seqs, uint32_t q_heads, const m27q_cache &cache, int cus) {
     const bool few = (long long)seqs.max_q * (q_heads / cache.heads) <= kRows;
     const long long wgs = attn_groups(seqs, q_heads, cache), least = few ? 128 : 256;
