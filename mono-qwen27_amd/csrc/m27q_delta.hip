@@ -544,6 +544,16 @@ __global__ __launch_bounds__(512) void k_delta_chunks(const m27q_delta d, const 
         for (int u = 0; u < 3; ++u)
             b[u] = *(const bf16x8 *)(from + u * kSlice * kC + lds_at<kC>(16 * j + n, 32 * i + 8 * g));
     };
+    // Reads stay in front of the matrix instructions: left alone, the compiler puts each before
+    // its own, to wait for it.
+    auto reads_first = [] { __builtin_amdgcn_sched_barrier(0x476); };  // vector, scalar and memory instructions may pass
+    auto get_both = [&](const __bf16 *from, bf16x8(&b)[2][2][3]) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) get_rows(from, j, i, b[i][j]);
+        reads_first();
+    };
     auto get_state = [&](int i, bf16x8(&b)[2][3]) {
 #pragma unroll
         for (int j = 0; j < 2; ++j)
@@ -605,14 +615,21 @@ __global__ __launch_bounds__(512) void k_delta_chunks(const m27q_delta d, const 
         for (int t0 = 0; t0 < sr.count; t0 += kC) {
             rec += step;
             f32x4 x[2] = {};
+            {
+                bf16x8 a[2][N], b[2][2][3];
+                auto get = [&](int i) {
 #pragma unroll
-            for (int i = 0; i < KS; ++i) {
-                bf16x8 a[N], b[2][3];
+                    for (int u = 0; u < N; ++u)
+                        a[i & 1][u] = *(const bf16x8 *)(kp + u * kC * DK + lds_at<DK>(16 * mt + n, 32 * i + 8 * g));
+                    get_state(i, b[i & 1]);
+                };
+                get(0);
 #pragma unroll
-                for (int u = 0; u < N; ++u)
-                    a[u] = *(const bf16x8 *)(kp + u * kC * DK + lds_at<DK>(16 * mt + n, 32 * i + 8 * g));
-                get_state(i, b);
-                mma<2, N, 3>(a, b, x);
+                for (int i = 0; i < KS; ++i) {
+                    if (i + 1 < KS) get(i + 1);
+                    reads_first();
+                    mma<2, N, 3>(a[i & 1], b[i & 1], x);
+                }
             }
             bf16x8 kt[2][MT][N];  // K^T: dk = 16 (MT mt + m) + n, rows 32 i + 8 g + 0 .. 7
 #pragma unroll
@@ -649,14 +666,10 @@ __global__ __launch_bounds__(512) void k_delta_chunks(const m27q_delta d, const 
                 row_by_row<DK, T>(d, sr, kh, head, t0, v0, mt, S, (float *)ub, out);
             } else {
                 f32x4 u[2] = {};
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    if (i == 1 && mt < 2) break;  // above the diagonal
-                    bf16x8 b[2][3];
-                    get_rows(rb, 0, i, b[0]);
-                    get_rows(rb, 1, i, b[1]);
-                    mma<2, 3, 3>(t[i], b, u);
-                }
+                bf16x8 b[2][2][3];
+                get_both(rb, b);
+                mma<2, 3, 3>(t[0], b[0], u);
+                if (mt >= 2) mma<2, 3, 3>(t[1], b[1], u);  // otherwise above the diagonal
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     put_rows(ub, j, u[j]);
@@ -674,14 +687,12 @@ __global__ __launch_bounds__(512) void k_delta_chunks(const m27q_delta d, const 
                 for (int m = 0; m < MT; ++m)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) S[m][j] *= decay;
+                bf16x8 b[2][2][3];
+                get_both(wb, b);
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    bf16x8 b[2][3];
-                    get_rows(wb, 0, i, b[0]);
-                    get_rows(wb, 1, i, b[1]);
+                for (int i = 0; i < 2; ++i)
 #pragma unroll
-                    for (int m = 0; m < MT; ++m) mma<2, N, 3>(kt[i][m], b, S[m]);
-                }
+                    for (int m = 0; m < MT; ++m) mma<2, N, 3>(kt[i][m], b[i], S[m]);
             }
             put_state();
             __syncthreads();
@@ -726,12 +737,15 @@ __global__ __launch_bounds__(512) void k_delta_chunks(const m27q_delta d, const 
         if (__builtin_expect(slow, 0)) {
             for (int i = 0; i < 2 * min(kC, sr.count - t0); ++i) __syncthreads();  // those of row_by_row
         } else {
+            bf16x8 b[2][2][3];
+            get_state(0, b[0]);
 #pragma unroll
             for (int i = 0; i < KS; ++i) {
-                bf16x8 a[N], b[2][3];
+                bf16x8 a[N];
                 pieces<T>(q[i], a);
-                get_state(i, b);
-                mma<2, N, 3>(a, b, x);
+                if (i + 1 < KS) get_state(i + 1, b[(i + 1) & 1]);
+                reads_first();
+                mma<2, N, 3>(a, b[i & 1], x);
             }
         }
         load_rows<KS, T>(d.q, sr.first, kh, t0 + kC + 16 * mt, sr.count, 0, q);
@@ -741,14 +755,10 @@ __global__ __launch_bounds__(512) void k_delta_chunks(const m27q_delta d, const 
         __syncthreads();
         put_k();
         if (!slow) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                if (i == 1 && mt < 2) break;
-                bf16x8 b[2][3];
-                get_rows(ub, 0, i, b[0]);
-                get_rows(ub, 1, i, b[1]);
-                mma<2, 3, 3>(p[i], b, x);
-            }
+            bf16x8 b[2][2][3];
+            get_both(ub, b);
+            mma<2, 3, 3>(p[0], b[0], x);
+            if (mt >= 2) mma<2, 3, 3>(p[1], b[1], x);
         }
         load_blocks(rec + kP, mt, p);
         // last, behind all loads: a wait for one of those would be one for these too
