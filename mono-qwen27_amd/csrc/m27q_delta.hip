@@ -495,11 +495,12 @@ __device__ __forceinline__ void row_by_row(const m27q_delta &d, const SeqRows &s
 // Operands that come from memory are asked for again, for the next chunk, as soon as they have
 // been used, without branches (a load under one would keep later waits from telling it apart).
 // The chain of the three products bounds it: 4096 rows of 48 heads of 128 (192 workgroups),
-// fp32, 64 chunks of 3.8 us, 7000 to 9000 cycles of which the matrix units work 2900, LDS 3400;
-// Q S^T in pieces is the longest of part 2.  243 us after 49 of preparation; four BF16 sequences
-// of up to 1531 rows (768 workgroups, one a CU at a time: two would need 128 registers, which
-// spill, 296 against 258 us in all) 200 after 59.  Q cut into pieces in part 1 instead: 333
-// against 304; K's loads and pieces with the state's waves: 337.
+// fp32, 64 chunks of 3.7 us, 7000 to 8500 cycles of which the matrix units work 2900, LDS 3400;
+// Q S^T in pieces is the longest of part 2.  236 us after 49 of preparation; four BF16 sequences
+// of up to 1531 rows (768 workgroups, one a CU at a time) 198 after 59.  Measured before reads
+// stood in front of the products: Q cut into pieces in part 1 instead 333 us against 304 in all,
+// K's loads and pieces with the state's waves 337; BF16 in the 128 registers of two workgroups a
+// CU, which spill, 296 against 258.
 template <int DK, typename T>
 __global__ __launch_bounds__(512) void k_delta_chunks(const m27q_delta d, const float *scratch) {
     constexpr int N = In<T>::N, KS = DK / 32, MT = DK / 64;
@@ -1033,7 +1034,7 @@ __global__ __launch_bounds__(256, 3) void k_delta_few(const m27q_delta d) {
 }
 
 // Which of the three.  A wave of 16 state rows takes 0.3 to 0.6 us a row, or 3.5 us for 16 and
-// at first 4 more; the chunks take 3.8 us for 64 with a quarter of the waves, after 15 us of
+// at first 4 more; the chunks take 3.7 us for 64 with a quarter of the waves, after 15 us of
 // two launches and the rows' preparation.  48 heads of 128, fp32, us by rows, 16 rows and chunks:
 //   1 sequence   8 rows 7.6 and 8.5, 10 rows 9.0 and 8.7; 64 rows 22.8 and 23.3, 96 rows 31.7 and 26.7
 //   4 sequences  6 rows 12.4 and 12.8, 8 rows 14.6 and 12.9; 128 rows 53 and 58, 256 rows 97 and 88
