@@ -409,6 +409,26 @@ struct Rows {
     }
 };
 
+// The first key that a row at a place sees.  Rows before place 0 see none; a window may be as
+// long as its type holds, so nothing is taken off below 0.
+__device__ __forceinline__ int first_key(const AttnParams &p, int place) {
+    return p.window ? max(0, max(place, 0) - p.window + 1) : 0;
+}
+
+// The keys of a workgroup whose rows stand at first .. last (of len >= 0 cached tokens, so none
+// of these sums passes 32 bits), and its part of them: lo a multiple of a tile, hi >= lo, and
+// hi <= max_kv where there are any.
+__device__ __forceinline__ void set_keys(const AttnParams &p, Work &w, int len, int first, int last) {
+    w.lo = first_key(p, first) & ~(kKeys - 1);  // tiles lie whole within pages or the other way round
+    w.hi = max(w.lo, min(min(len, (int)p.seqs.max_kv), last + 1));
+    if (p.splits > 1) {
+        const int tiles = (w.hi - w.lo + kKeys - 1) / kKeys, each = (tiles + p.splits - 1) / p.splits;
+        const int end = w.hi;
+        w.lo += (int)blockIdx.y * each * kKeys;
+        w.hi = max(w.lo, min(end, w.lo + each * kKeys));
+    }
+}
+
 // Looks at every page of the keys once, the threads of a workgroup in turn: tiles trust them then.
 __device__ __forceinline__ bool has_gaps(const AttnParams &p, const Work &w) {
     const int shift = __builtin_ctz(p.cache.page_size);
@@ -444,20 +464,10 @@ __global__ __launch_bounds__(kWaves * 64, 2) void k_attn(const AttnParams p) {
     w.rows = sr.count * group;
     w.row0 = (int)(gridDim.x / pairs - 1 - fromlast) * kWaves * kRows;
     if (w.row0 >= w.rows) return;
-    const int kv = min(max(p.seqs.kv_len[s], 0), (int)p.seqs.max_kv);
-    const int place0 = p.seqs.kv_len[s] - (sr.end - sr.first);  // of the sequence's first row
+    const int len = max(p.seqs.kv_len[s], 0), place0 = len - (sr.end - sr.first);  // of the sequence's first row
     const int first = place0 + w.row0 / group;
     const int last = place0 + (min(w.row0 + kWaves * kRows, w.rows) - 1) / group;
-    int lo = p.window ? max(0, first - p.window + 1) & ~(kKeys - 1) : 0;  // tiles lie whole within pages or the other way round
-    int hi = min(kv, last + 1);
-    if (p.splits > 1) {
-        const int tiles = max(0, hi - lo + kKeys - 1) / kKeys;
-        const int each = (tiles + p.splits - 1) / p.splits;
-        lo += (int)blockIdx.y * each * kKeys;
-        hi = min(hi, lo + each * kKeys);
-    }
-    w.lo = lo;
-    w.hi = hi;
+    set_keys(p, w, len, first, last);
 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
     const int wrow = w.row0 + wave * kRows;  // this wave's first row
@@ -476,11 +486,11 @@ __global__ __launch_bounds__(kWaves * 64, 2) void k_attn(const AttnParams p) {
     w.gaps = __syncthreads_or(has_gaps(p, w));
     // tiles [ta, tb) are seen whole by every row of the workgroup: the next one is
     // on its way while one is worked on; the others, at the ends, go one by one
-    const int tiles = max(0, w.hi - w.lo + kKeys - 1) / kKeys;
+    const int tiles = (w.hi - w.lo + kKeys - 1) / kKeys;
     int ta = 0, tb = 0;
     if (!w.gaps) {
         tb = max(0, min(first + 1, w.hi) - w.lo) / kKeys;
-        ta = p.window ? min(tb, (max(0, last - p.window + 1 - w.lo) + kKeys - 1) / kKeys) : 0;
+        ta = p.window ? min(tb, (max(0, first_key(p, last) - w.lo) + kKeys - 1) / kKeys) : 0;
     }
     const bool any = wrow < w.rows;
     LDS_AS char *const ka = (LDS_AS char *)kt0, *const va = (LDS_AS char *)vt0;
@@ -579,16 +589,9 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) void k_attn_few(cons
     asm("" : "+s"(len));  // asked for with the rows, not behind the branch
     w.rows = sr.count * group;
     if (w.rows == 0) return;
-    const int kv = min(max(len, 0), (int)p.seqs.max_kv);
+    len = max(len, 0);
     const int first = len - (sr.end - sr.first), last = first + sr.count - 1;
-    w.lo = p.window ? max(0, first - p.window + 1) & ~(kKeys - 1) : 0;
-    w.hi = min(kv, last + 1);
-    if (p.splits > 1) {
-        const int tiles = max(0, w.hi - w.lo + kKeys - 1) / kKeys;
-        const int each = (tiles + p.splits - 1) / p.splits;
-        w.lo += (int)blockIdx.y * each * kKeys;
-        w.hi = min(w.hi, w.lo + each * kKeys);
-    }
+    set_keys(p, w, len, first, last);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const bool live = (lane & (RW - 1)) < w.rows;
     const int row = min(lane & (RW - 1), w.rows - 1), at = row / group;
@@ -636,9 +639,9 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) void k_attn_few(cons
 
     // tiles [ta, tb): seen whole by every row (if no page is missing, which is found out
     // while the first of them is on its way)
-    const int tiles = max(0, w.hi - w.lo + kKeys - 1) / kKeys;
+    const int tiles = (w.hi - w.lo + kKeys - 1) / kKeys;
     int tb = max(0, min(first + 1, w.hi) - w.lo) / kKeys;
-    int ta = p.window ? min(tb, (max(0, last - p.window + 1 - w.lo) + kKeys - 1) / kKeys) : 0;
+    int ta = p.window ? min(tb, (max(0, first_key(p, last) - w.lo) + kKeys - 1) / kKeys) : 0;
     int t = ta + ((wave - ta) & (kWaves - 1));  // this wave's first
     int ids[2];
     if (t < tb) {
