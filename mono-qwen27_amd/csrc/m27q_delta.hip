@@ -171,6 +171,10 @@ __device__ __forceinline__ void split(f32x4 x, bf16x4 (&p)[N]) {
     for (int j = 0; j < N; ++j) p[j] = __builtin_bit_cast(bf16x4, u2{a[j], b[j]});
 }
 
+// Whether the pieces of a value are finite: from the middle between the largest bf16 value and
+// the next that there would be, the first one is not.
+__device__ __forceinline__ bool fits(float x) { return fabsf(x) < 0x1.ffp127f; }
+
 // c[j] += a[j] b over 16x16 tiles and 32 of the contraction, the smallest parts first; the
 // tiles in turn, so that a product does not wait for the one before.
 template <int NC, int NA, int NB>
@@ -374,6 +378,7 @@ __global__ __launch_bounds__(256, 4) void k_delta_prepare(const m27q_delta d, fl
             for (int i = 0; i < 4; ++i) Xm[(r0 + 4 * g + i) * LM + c0 + n] = x[i];
         }
         __syncthreads();
+        bool bad = false;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {  // a wave's own rows: written and read without a barrier
             if (j > (wave | 1)) break;
@@ -385,15 +390,21 @@ __global__ __launch_bounds__(256, 4) void k_delta_prepare(const m27q_delta d, fl
             if (i == 1 && wave < 2) break;
             const int at = (r0 + n) * LM + 32 * i + 8 * g;
             __bf16 *to = (__bf16 *)(rec + kT) + block_of(wave, i) * kBlockHalves + lane * 8;
+            const f32x8 tt = *(const f32x8a *)(Xm + at) * *(const f32x8a *)(B + 32 * i + 8 * g);
+            const f32x8 pp = *(const f32x8a *)(Am + at);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) bad |= !fits(tt[u]) || !fits(pp[u]);
             bf16x8 x[3], y[3];
-            split<3>(*(const f32x8a *)(Xm + at) * *(const f32x8a *)(B + 32 * i + 8 * g), x);
-            split<3>(*(const f32x8a *)(Am + at), y);
+            split<3>(tt, x);
+            split<3>(pp, y);
 #pragma unroll
             for (int u = 0; u < 3; ++u) {
                 *(bf16x8 *)(to + u * 512) = x[u];
                 *(bf16x8 *)(to + 2 * (kP - kT) + u * 512) = y[u];
             }
         }
+        // T or P of products or factors that pass fp32, or of values that are not finite: the walk sees this
+        if (__builtin_expect(__any(bad), 0)) rec[kEg + lane] = __builtin_nanf("");
     }
 }
 
@@ -420,8 +431,8 @@ __device__ __forceinline__ void load_blocks(const float *from, int m, bf16x8 (&x
     }
 }
 
-// A chunk's rows one by one, for a chunk with a value that is not finite: its products would
-// carry it, times zeros, to the rows before it.  The four waves that hold the state (as in
+// A chunk's rows one by one, for a chunk with a value that is not finite, or whose products come
+// to one: they would carry it, times zeros, to the rows before it.  The four waves that hold the state (as in
 // k_delta_chunks) sum over their columns and, through `sums`, over each other's; two barriers
 // a row.
 template <int DK, typename T>
@@ -492,6 +503,8 @@ __device__ __forceinline__ void row_by_row(const m27q_delta &d, const SeqRows &s
 //   1  X = K S^T, R = V - diag(e^G) X        | K of the next chunk into pieces
 //   2  U = T R                               | Q S^T
 //   3  S <- e^(G_C) S + K^T diag(..) U       | K's pieces to LDS, out = .. Q S^T + P U
+// What in R, U or diag(..) U does not fit its pieces (T and P: by a NaN in e^G) is seen before the
+// third part, which then takes the chunk's rows one by one from the state that it started from.
 // Operands that come from memory are asked for again, for the next chunk, as soon as they have
 // been used, without branches (a load under one would keep later waits from telling it apart).
 // The chain of the three products bounds it: 4096 rows of 48 heads of 128 (192 workgroups),
@@ -509,7 +522,7 @@ __global__ __launch_bounds__(512) void k_delta_chunks(const m27q_delta d, const 
     __shared__ __attribute__((aligned(16))) __bf16 rb[3 * kSlice * kC];     // the right-hand sides' [3][dv][row]
     __shared__ __attribute__((aligned(16))) __bf16 ub[3 * kSlice * kC];     // U's
     __shared__ __attribute__((aligned(16))) __bf16 wb[3 * kSlice * kC];     // diag(e^(G_C - G)) U's
-    __shared__ int odd;                                                     // some right-hand side is not finite
+    __shared__ int odd[2];                                                  // this chunk's products hold: no, and the next one's
     // workgroups of one key head and sequence are gridDim.x apart, so that where that is a
     // multiple of the XCDs they share an L2
     const int kheads = (int)d.k.heads, per = (int)d.v.heads / kheads, slices = (int)(d.v.dim + kSlice - 1) / kSlice;
@@ -538,7 +551,7 @@ __global__ __launch_bounds__(512) void k_delta_chunks(const m27q_delta d, const 
                             d.state_in ? *(const f32x4 *)(d.state_in + at + 16 * j * DK + 16 * m) : f32x4{};
         return;
     }
-    if (threadIdx.x == 0) odd = 0;
+    if (threadIdx.x < 2) odd[threadIdx.x] = 0;
 
     auto get_rows = [&](const __bf16 *from, int j, int i, bf16x8(&b)[3]) {
 #pragma unroll
@@ -615,6 +628,7 @@ __global__ __launch_bounds__(512) void k_delta_chunks(const m27q_delta d, const 
         __syncthreads();
         for (int t0 = 0; t0 < sr.count; t0 += kC) {
             rec += step;
+            int *const mark = odd + (t0 / kC & 1);
             f32x4 x[2] = {};
             {
                 bf16x8 a[2][N], b[2][2][3];
@@ -654,18 +668,14 @@ __global__ __launch_bounds__(512) void k_delta_chunks(const m27q_delta d, const 
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     r[i] = (float)v[j][i] - eg[i] * x[j][i];
-                    bad |= !__builtin_isfinite(r[i]);
+                    bad |= !fits(r[i]);
                 }
                 put_rows(rb, j, r);
             }
-            if (bad) odd = 1;
             load_v(t0 + kC);
             eg = *(const f32x4 *)(rec + kEg + row);
             __syncthreads();
-            const bool slow = odd;
-            if (__builtin_expect(slow, 0)) {
-                row_by_row<DK, T>(d, sr, kh, head, t0, v0, mt, S, (float *)ub, out);
-            } else {
+            {
                 f32x4 u[2] = {};
                 bf16x8 b[2][2][3];
                 get_both(rb, b);
@@ -673,17 +683,23 @@ __global__ __launch_bounds__(512) void k_delta_chunks(const m27q_delta d, const 
                 if (mt >= 2) mma<2, 3, 3>(t[1], b[1], u);  // otherwise above the diagonal
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
+                    const f32x4 w = u[j] * ec;
                     put_rows(ub, j, u[j]);
-                    put_rows(wb, j, u[j] * ec);
+                    put_rows(wb, j, w);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) bad |= !fits(u[j][i]) || !fits(w[i]);
                 }
             }
+            if (bad) *mark = 1;
+            if (threadIdx.x == 0) odd[(t0 / kC & 1) ^ 1] = 0;  // the last chunk's: read before the barrier above
             load_blocks(rec + kT, mt, t);
             const float decay = last;
             ec = *(const f32x4 *)(rec + kEc + row);
             last = rec[kLast];
             __syncthreads();
-            if (threadIdx.x == 0) odd = 0;  // every wave has read it, and sets it behind the next barrier
-            if (!slow) {
+            if (__builtin_expect(*mark, 0)) {
+                row_by_row<DK, T>(d, sr, kh, head, t0, v0, mt, S, (float *)ub, out);
+            } else {
 #pragma unroll
                 for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -733,11 +749,8 @@ __global__ __launch_bounds__(512) void k_delta_chunks(const m27q_delta d, const 
         cut();
         load_rows<KS, T>(d.k, sr.first, kh, t0 + 2 * kC + 16 * mt, sr.count, 0, k);
         __syncthreads();
-        const bool slow = odd;
         f32x4 x[2] = {};
-        if (__builtin_expect(slow, 0)) {
-            for (int i = 0; i < 2 * min(kC, sr.count - t0); ++i) __syncthreads();  // those of row_by_row
-        } else {
+        {
             bf16x8 b[2][2][3];
             get_state(0, b[0]);
 #pragma unroll
@@ -754,8 +767,11 @@ __global__ __launch_bounds__(512) void k_delta_chunks(const m27q_delta d, const 
         for (int j = 0; j < 2; ++j) x[j] *= eg * d.scale;
         eg = *(const f32x4 *)(rec + kEg + row);
         __syncthreads();
+        const bool slow = odd[t0 / kC & 1];
         put_k();
-        if (!slow) {
+        if (__builtin_expect(slow, 0)) {
+            for (int i = 0; i < 2 * min(kC, sr.count - t0); ++i) __syncthreads();  // those of row_by_row
+        } else {
             bf16x8 b[2][2][3];
             get_both(ub, b);
             mma<2, 3, 3>(p[0], b[0], x);
