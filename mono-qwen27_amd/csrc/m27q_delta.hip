@@ -989,7 +989,7 @@ __global__ __launch_bounds__(256, 3) void k_delta_few(const m27q_delta d) {
         bool bad = !__builtin_isfinite(last);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            bad |= !(__builtin_isfinite(r[i]) && __builtin_isfinite(u[i]) && __builtin_isfinite(w[i]) && __builtin_isfinite(y[i]));
+            bad |= !(fits(r[i]) && fits(u[i]) && fits(w[i]) && __builtin_isfinite(y[i]));
         if (__builtin_expect(__any(bad), 0)) {
             // Row by row: products would carry a value that is not finite, times zeros, to the rows before it.
             for (int i = t0; i < min(t0 + kFew, sr.count); ++i) {

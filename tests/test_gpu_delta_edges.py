@@ -80,3 +80,16 @@ def test_decay_and_growth_that_undo_each_other(m27q, dev, lens, row):
     assert np.all(np.abs(got - want) <= tol), np.max(np.abs(got - want) / tol)
     for s in range(len(lens)):
         assert np.all(np.abs(state[s] - ends[s]) <= step * smalls[s][..., None])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,row", [([16], 10), ([150], 70)])
+def test_update_near_the_largest(m27q, dev, lens, row):
+    """u = 1e38 grown to 3.3985e38 within the rows that go together: finite, its nearest bf16 is not."""
+    say("delta update near the largest", lens, row)
+    p = Problem(m27q, dev, lens, 1, 2, 64, 32, rate=0.0)
+    p.v[row, 1, 3] = 1e38
+    p.beta[row, 1] = 1
+    p.beta[row + 1:, 1] = 0
+    p.g[row + 1, 1] = float(np.log(3.3985))
+    p.check()
