@@ -69,7 +69,8 @@ __global__ __launch_bounds__(64) void k_delta_rows(const m27q_delta d) {
             kk[i] = __builtin_convertvector(*(const T4 *)(k + 16 * i), f32x4);
             qq[i] = __builtin_convertvector(*(const T4 *)(q + 16 * i), f32x4);
         }
-        const float e = expf(*g), b = *beta, vv = (float)*v;
+        float e = expf(*g);
+        const float b = *beta, vv = (float)*v;
         f32x4 sk = {}, sq = {}, kq = {};
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -77,8 +78,27 @@ __global__ __launch_bounds__(64) void k_delta_rows(const m27q_delta d) {
             sq += S[i] * qq[i];
             kq += kk[i] * qq[i];
         }
-        const float u = b * (vv - e * quad_sum(sk[0] + sk[1] + sk[2] + sk[3]));
-        const float o = e * quad_sum(sq[0] + sq[1] + sq[2] + sq[3]) + u * quad_sum(kq[0] + kq[1] + kq[2] + kq[3]);
+        float u = b * (vv - e * quad_sum(sk[0] + sk[1] + sk[2] + sk[3]));
+        float o = e * quad_sum(sq[0] + sq[1] + sq[2] + sq[3]) + u * quad_sum(kq[0] + kq[1] + kq[2] + kq[3]);
+        if (__builtin_expect(__any(!__builtin_isfinite(u) || !__builtin_isfinite(o)), 0)) {
+            // in the rule's order: these products may pass fp32 where its own do not
+            sk = sq = f32x4{};
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                S[i] *= e;
+                sk += S[i] * kk[i];
+                __builtin_amdgcn_sched_barrier(0);  // few registers
+            }
+            u = b * (vv - quad_sum(sk[0] + sk[1] + sk[2] + sk[3]));
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                S[i] += kk[i] * u;
+                sq += S[i] * qq[i];
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            o = quad_sum(sq[0] + sq[1] + sq[2] + sq[3]);
+            e = 1, u = 0;
+        }
 #pragma unroll
         for (int i = 0; i < N; ++i) S[i] = S[i] * e + kk[i] * u;
         if ((lane & 3) == 0) *out = (T)(d.scale * o);

@@ -93,3 +93,26 @@ def test_update_near_the_largest(m27q, dev, lens, row):
     p.beta[row + 1:, 1] = 0
     p.g[row + 1, 1] = float(np.log(3.3985))
     p.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("g", [-float("inf"), -20.0])
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("lens", [[1], [3], [16], [150]])
+def test_large_states_that_decay(m27q, dev, lens, t, g):
+    """S k overflows before the decay, e^g S k does not; g = -inf clears any finite state."""
+    say("delta large states", lens, t, g)
+    p = Problem(m27q, dev, lens, 1, 2, 64, 32, t)
+    p.state[0, 1, 5] = 3e38
+    p.k[0], p.q[0] = 0.125, 0.125
+    p.g[0, 1] = g
+    got, state = p.run()
+    want, ends, _, _ = p.want()
+    flat = Problem(m27q, dev, lens, 1, 2, 64, 32, t)  # sizes behind the decay
+    flat.k[0], flat.q[0], flat.g[0, 1] = 0.125, 0.125, 0
+    flat.state[0, 1, 5] = float(3e38 * np.exp(g))
+    _, _, size, sizes = flat.want()
+    step = (8 * np.sqrt(max(lens) * 128) + 8) * 2.0 ** -24
+    tol = step * size * 64 ** -0.5 * 1.01 + {"f32": 2.0 ** -24, "bf16": 2.0 ** -8}[t] * np.abs(want)
+    assert np.all(np.abs(got - want) <= tol), np.max(np.abs(got - want) / tol)
+    assert np.all(np.abs(state[0] - ends[0]) <= step * sizes[0][..., None])
