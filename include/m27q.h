@@ -453,7 +453,8 @@ M27Q_API m27q_status m27q_rope_append(const m27q_rope_plan *rope, const int32_t 
  * is a multiple of cache.heads, at most 64 for each.  A row that sees no key
  * gives zeros; rows of no sequence are not written.  Keys whose table entry is
  * outside 0 .. pages - 1 are left out, as if masked; nothing of a masked key or
- * value is used, be it NaN.  Products are MFMA on the cache's type with fp32
+ * value is used, be it NaN, and an infinite value that is seen gives that
+ * infinity however small its weight (above 0 all the same).  Products are MFMA on the cache's type with fp32
  * sums; the weights p are rounded to it for the second product, for an F32
  * output as the sum of two (F16) or three (BF16) such values.
  * scratch (16-byte aligned) >= m27q_attn_scratch_bytes, whose bound holds for

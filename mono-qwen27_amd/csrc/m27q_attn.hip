@@ -385,6 +385,16 @@ struct Rows {
         return __builtin_bit_cast(T4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS s4 *)at));
     }
 
+    // Whether some sum of this lane is not finite.
+    __device__ __forceinline__ bool odd_sums() const {
+        float top = 0;
+#pragma unroll
+        for (int t = 0; t < D / RW; ++t)
+#pragma unroll
+            for (int j = 0; j < NA; ++j) top = __builtin_elementwise_maximum(top, fabsf(o[t][j]));
+        return !__builtin_isfinite(top);
+    }
+
     // O += the values of V that are not finite, where they are seen: the whole of
     // their effect, as a weight is positive.
     __device__ __forceinline__ void add_odd(const AttnParams &p, const Work &w, int k0, const LDS_AS char *vt) {
@@ -408,6 +418,10 @@ struct Rows {
         }
     }
 };
+
+// What a part's sums count beside the largest part's, never 0: an infinite sum stays what it is
+// (and 2^-126 of a finite one is nothing beside the largest part's weight of 2^6 and more).
+__device__ __forceinline__ float join_factor(float log2) { return fmaxf(__builtin_amdgcn_exp2f(log2), 0x1p-126f); }
 
 // The first key that a row at a place sees.  Rows before place 0 see none; a window may be as
 // long as its type holds, so nothing is taken off below 0.
@@ -525,7 +539,22 @@ __global__ __launch_bounds__(kWaves * 64, 2) void k_attn(const AttnParams p) {
         __syncthreads();
         if (any) x.template tile<true, false>(p, w, sc, k0, ka, va);
     }
-    if (__builtin_expect(__syncthreads_or(odd), 0))
+    // sums that are not finite: of values in the tiles seen whole, whose weights' pieces may be
+    // 0 or negative.  Once more then, all tiles as those at the ends.
+    const bool again = ta < tb && x.odd_sums();
+    if (__builtin_expect(__syncthreads_or(odd || again), 0)) {
+        if (__syncthreads_or(again)) {
+            x.clear();
+            ta = tb = 0;
+            for (int k0 = w.lo; k0 < w.hi; k0 += kKeys) {
+                __syncthreads();
+                load_tile<D, true>(p, w, k0, tile_page(p, w, k0), ka, va);
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                clear_odd<D, BF, kKeys / kWaves>(va + wave * (kKeys / kWaves) * D * 2);
+                __syncthreads();
+                if (any) x.template tile<true, false>(p, w, sc, k0, ka, va);
+            }
+        }
         for (int i = 0; i < tiles - (tb - ta); ++i) {
             const int k0 = w.lo + (i < ta ? i : i + tb - ta) * kKeys;
             __syncthreads();
@@ -533,6 +562,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void k_attn(const AttnParams p) {
             tile_barrier();
             if (any) x.add_odd(p, w, k0, va);
         }
+    }
 
     x.l = sum_row<kRows>(x.l);
     if (!live) return;
@@ -705,6 +735,21 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) void k_attn_few(cons
         x.template tile<true, true>(p, w, sc, k0, kt, vt);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
+    // as in k_attn: a value that is not finite in a tile seen whole
+    if (__builtin_expect(ta < tb && __any(x.odd_sums()), 0)) {
+        x.clear();
+        ta = tb = 0;
+        for (int t = wave; t < tiles; t += kWaves) {
+            const int k0 = w.lo + t * kKeys, ids[2] = {page(k0, 0), page(k0, 1)};
+            load(p.cache.k, kt, true, k0, ids, true);
+            load(p.cache.v, vt, false, k0, ids, true);
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            odd |= clear_odd<D, BF, kKeys>(vt);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            x.template tile<true, false>(p, w, sc, k0, kt, vt);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        }
+    }
     if (__builtin_expect(__any(odd), 0))
         for (int t = other(wave); t < tiles; t = other(t + kWaves)) {
             const int k0 = w.lo + t * kKeys, ids[2] = {page(k0, 0), page(k0, 1)};
@@ -728,7 +773,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) void k_attn_few(cons
     for (int i = 1; i < kWaves; ++i) m = fmaxf(m, ms[i][col]);
     constexpr int HALF = TB / (RW * 16);  // quadruples of a tile's room
     if (x.l != 0) {
-        const float f = __builtin_amdgcn_exp2f((x.m - m) * sc);
+        const float f = join_factor((x.m - m) * sc);
 #pragma unroll
         for (int t = 0; t < D / RW; ++t)
 #pragma unroll
@@ -745,7 +790,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) void k_attn_few(cons
 #pragma unroll
     for (int i = 0; i < kWaves; ++i) {
         fs[i] = ls[i][col];
-        const float e = ms[i][col] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((ms[i][col] - m) * sc);
+        const float e = ms[i][col] == -__builtin_inff() ? 0.0f : join_factor((ms[i][col] - m) * sc);
         l += ls[i][col] * e;
     }
     if (!live) return;
@@ -812,7 +857,7 @@ __global__ __launch_bounds__(256) void k_attn_join(const AttnParams p) {
         float m = st.y != 0 ? st.x : -__builtin_inff();
 #pragma unroll
         for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-        f[r] = st.y != 0 ? __builtin_amdgcn_exp2f(st.x - m) : 0.0f;
+        f[r] = st.y != 0 ? join_factor(st.x - m) : 0.0f;
         float l = st.y * f[r];
         f[r] = st.y != 0 ? f[r] : -1.0f;  // no key: its sums were not written
 #pragma unroll
