@@ -437,9 +437,9 @@ M27Q_API m27q_status m27q_rope(const m27q_rope_plan *rope, const int32_t *pos, i
 /* One launch in front of attention: q rotated into q_out, k rotated and v as it
  * is into their places in the cache (rounded to the cache's type).  q and q_out
  * as in m27q_rope; k and v have the cache's heads and dim, any type.  A row of no
- * sequence, or whose place is negative or past table_stride * page_size, or
- * whose table entry is outside 0 .. pages - 1, is not written to the cache (its
- * query is rotated all the same).  Replaces k_mrope_and_cache (exec:1180-1229),
+ * sequence or past its first max_q, or whose place is negative, from max_kv on or
+ * past table_stride * page_size, or whose table entry is outside 0 .. pages - 1,
+ * is not written to the cache (its query is rotated all the same).  Replaces k_mrope_and_cache (exec:1180-1229),
  * whose cache is one fp32 buffer per layer. */
 M27Q_API m27q_status m27q_rope_append(const m27q_rope_plan *rope, const int32_t *pos, const m27q_seqs *seqs,
                                       const m27q_cache *cache, const m27q_rows *q, const m27q_rows *q_out,
@@ -454,9 +454,10 @@ M27Q_API m27q_status m27q_rope_append(const m27q_rope_plan *rope, const int32_t 
  * gives zeros; rows of no sequence are not written.  Keys whose table entry is
  * outside 0 .. pages - 1 are left out, as if masked; nothing of a masked key or
  * value is used, be it NaN, and an infinite value that is seen gives that
- * infinity however small its weight (above 0 all the same).  Products are MFMA on the cache's type with fp32
- * sums; the weights p are rounded to it for the second product, for an F32
- * output as the sum of two (F16) or three (BF16) such values.
+ * infinity however small its weight (above 0 all the same).  Products are MFMA
+ * on the cache's type with fp32 sums; the weights p are rounded to it for the
+ * second product, for an F32 output as the sum of two (F16) or three (BF16) such
+ * values.
  * scratch (16-byte aligned) >= m27q_attn_scratch_bytes, whose bound holds for
  * any lengths within the seqs' bounds; what it holds is of no matter.
  * Replaces k_attn_decode_split_partial / _reduce (exec:1339-1484), one token

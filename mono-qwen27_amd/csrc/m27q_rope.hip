@@ -140,9 +140,10 @@ __global__ __launch_bounds__(kThreads) void k_rope(const RopeParams p, int parts
         const int s = seq_of(p.seqs.start, (int)p.seqs.n, t);
         if (s >= 0) {
             const long long at = (long long)p.seqs.kv_len[s] - (min(p.seqs.start[s + 1], p.tokens) - t);
-            const int shift = __builtin_ctz(p.cache.page_size);
+            const int shift = __builtin_ctz(p.cache.page_size), row = t - max(p.seqs.start[s], 0);
             const long long page = at >> shift;
-            if (at >= 0 && page < (long long)p.seqs.table_stride) {
+            if (at >= 0 && at < (long long)p.seqs.max_kv && page < (long long)p.seqs.table_stride &&
+                row < (int)p.seqs.max_q) {
                 const int32_t id = p.seqs.table[(long long)s * p.seqs.table_stride + page];
                 if (id >= 0 && (uint32_t)id < p.cache.pages)
                     place = (long long)id * p.cache.page_stride + (at & (p.cache.page_size - 1)) * p.cache.dim;
