@@ -3,18 +3,36 @@
 // A call costs the GPU as little as 4 us; reading shapes, strides and pointers of
 // up to ten tensors through Python costs the host as much again.  This module
 // reads them from the tensors themselves (0.4 us a call) and returns the
-// library's status; shapes that the records cannot express are M27Q_ERR_SHAPE.
+// library's status; shapes that the records cannot express are M27Q_ERR_SHAPE, and
+// a call with a tensor that the current GPU cannot read is kNotHere.
 #include <Python.h>
 
+#include <c10/core/impl/DeviceGuardImplInterface.h>
 #include <torch/csrc/autograd/python_variable.h>
+
+#include <cstring>
 
 #include "../../include/m27q.h"
 
 namespace {
 
 struct Bad {
-    m27q_status status;
+    int status;  // m27q_status, or kNotHere
 };
+constexpr int kNotHere = -1;
+
+// The GPU that a call's tensors lie on.  A kernel that follows a pointer to pageable host
+// memory or into another GPU faults, so such a call is refused.  The codes are those of the
+// binding's records: a GPU's number, kHost, or kPinned, which every GPU reads.
+constexpr int32_t kHost = -1, kPinned = -2;
+thread_local int32_t place;
+thread_local bool apart;
+
+void note(int32_t at) {
+    if (at == kPinned) return;
+    if (place == kPinned) place = at;
+    apart |= at == kHost || at != place;
+}
 
 const at::Tensor *tensor(PyObject *o, bool may_be_none = false) {
     if (may_be_none && o == Py_None) return nullptr;
@@ -31,7 +49,10 @@ uint32_t type_of(const at::Tensor &t) {
     }
 }
 
-void *data(const at::Tensor &t) { return t.mutable_data_ptr(); }
+void *data(const at::Tensor &t) {
+    note(t.is_cuda() ? t.get_device() : t.is_pinned() ? kPinned : kHost);
+    return t.mutable_data_ptr();
+}
 
 m27q_rows rows(PyObject *o, int64_t tokens) {
     const at::Tensor &t = *tensor(o);
@@ -55,10 +76,13 @@ float *floats(PyObject *o, int64_t n, bool may_be_none = false) {
     return (float *)data(*t);
 }
 
-// A record that the Python side packed when its object was made.
+// A record that the Python side packed when its object was made, and where its tensors lie.
 template <typename T>
 const T *record(PyObject *o) {
-    if (!PyBytes_Check(o) || PyBytes_GET_SIZE(o) != sizeof(T)) throw Bad{M27Q_ERR_NULL};
+    int32_t at;
+    if (!PyBytes_Check(o) || PyBytes_GET_SIZE(o) != sizeof(T) + sizeof at) throw Bad{M27Q_ERR_NULL};
+    memcpy(&at, PyBytes_AS_STRING(o) + sizeof(T), sizeof at);
+    note(at);
     return (const T *)PyBytes_AS_STRING(o);
 }
 
@@ -83,6 +107,8 @@ struct Args {
     }
     // Last, when all other arguments are known to fit.
     hipStream_t stream(int i) const {
+        if (apart || (place != kPinned && place != c10::impl::getDeviceGuardImpl(at::kCUDA)->getDevice().index()))
+            throw Bad{kNotHere};
         PyObject *h = stream_of ? PyObject_CallOneArg(stream_of, a[i]) : nullptr;
         const unsigned long long v = h ? PyLong_AsUnsignedLongLong(h) : 0;
         Py_XDECREF(h);
@@ -97,6 +123,8 @@ PyObject *call(PyObject *const *a, Py_ssize_t n, Py_ssize_t want, F f) {
         PyErr_SetString(PyExc_TypeError, "wrong number of arguments");
         return nullptr;
     }
+    place = kPinned;
+    apart = false;
     try {
         return PyLong_FromLong((long)f(Args{a}));
     } catch (const Bad &b) {

@@ -499,6 +499,25 @@ def _value_type(t) -> int:
     return {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}.get(t.dtype, 0xffffffff)
 
 
+# What the native calls say of a tensor that the current GPU cannot read.
+_NOT_HERE = -1
+
+
+def _mixer_check(status: int, what: str) -> None:
+    if status == _NOT_HERE:
+        raise M27QError(4, what + ": a tensor is not in the current GPU's memory")
+    check(status, what)
+
+
+def _packed(desc, *tensors) -> bytes:
+    """A record, and behind it the GPU that its tensors lie on: -1 for pageable host memory or more than one GPU,
+    -2 for pinned host memory alone."""
+    places = {t.get_device() if t.is_cuda else -2 if t.is_pinned() else -1 for t in tensors}
+    if len(places) > 1:
+        places.discard(-2)
+    return bytes(desc) + struct.pack("=i", places.pop() if len(places) == 1 else -1)
+
+
 def _int32(t, what: str):
     if t.dtype != _torch().int32 or not t.is_contiguous():
         raise M27QError(4, what)
@@ -519,7 +538,7 @@ class Rope:
         if turns.dtype != _torch().int64 or not turns.is_contiguous() or 2 * turns.numel() < rot:
             raise M27QError(4, "Rope")
         self.turns = turns
-        self.packed = bytes(RopePlan(turns.data_ptr(), rot, layout, mscale, 0))
+        self.packed = _packed(RopePlan(turns.data_ptr(), rot, layout, mscale, 0), turns)
 
     @staticmethod
     def make(rot: int, base: float, layout: int = ROPE_HALF, scaling: int = ROPE_PLAIN, factor: float = 1.0,
@@ -539,8 +558,8 @@ class KVCache:
         if k.stride()[1:] != (size * dim, dim, 1):
             raise M27QError(4, "KVCache")
         self.k, self.v, self.page_size = k, v, size
-        self.packed = bytes(CacheDesc(k.data_ptr(), v.data_ptr(), _value_type(k), pages, heads, size, dim, 0,
-                                      k.stride(0)))
+        self.packed = _packed(CacheDesc(k.data_ptr(), v.data_ptr(), _value_type(k), pages, heads, size, dim, 0,
+                                        k.stride(0)), k, v)
 
 
 class Seqs:
@@ -552,22 +571,22 @@ class Seqs:
         if start.numel() != n + 1 or kv_len.numel() != n:
             raise M27QError(2, "Seqs")
         self.start, self.kv_len, self.table, self.tokens = start, kv_len, table, tokens
-        self.packed = bytes(SeqsDesc(_int32(start, "Seqs"), _int32(kv_len, "Seqs"), _int32(table, "Seqs"), n, stride,
-                                     tokens, max_q, max_kv, 0))
+        self.packed = _packed(SeqsDesc(_int32(start, "Seqs"), _int32(kv_len, "Seqs"), _int32(table, "Seqs"), n, stride,
+                                       tokens, max_q, max_kv, 0), start, kv_len, table)
 
 
 def rope(rope: Rope, pos, x, out, stream=None) -> None:
     """out <- x rotated by pos; x and out [tokens, heads, dim]."""
     st = (_mixers_so or _mixers()).rope(rope.packed, pos, x, out, stream)
     if st:
-        check(st, "m27q_rope")
+        _mixer_check(st, "m27q_rope")
 
 
 def rope_append(rope: Rope, pos, seqs: Seqs, cache: KVCache, q, q_out, k, v, stream=None) -> None:
     """q_out <- q rotated; k rotated and v into the cache; q, k, v [tokens, heads, dim]."""
     st = (_mixers_so or _mixers()).rope_append(rope.packed, pos, seqs.packed, cache.packed, q, q_out, k, v, stream)
     if st:
-        check(st, "m27q_rope_append")
+        _mixer_check(st, "m27q_rope_append")
 
 
 def attn_scratch_bytes(seqs: Seqs, q_heads: int, cache: KVCache) -> int:
@@ -578,7 +597,7 @@ def attn_paged(seqs: Seqs, cache: KVCache, q, out, scratch, scale: float, window
     """out <- attention of the rows q [tokens, heads, dim] over their sequences' pages."""
     st = (_mixers_so or _mixers()).attn_paged(seqs.packed, cache.packed, q, out, scratch, scale, window, stream)
     if st:
-        check(st, "m27q_attn_paged")
+        _mixer_check(st, "m27q_attn_paged")
 
 
 def delta_scratch_bytes(n: int, tokens: int, max_len: int, heads: int, dk: int, dv: int) -> int:
@@ -592,4 +611,4 @@ def delta_rule(start, q, k, v, g, beta, state, state_out, out, scratch, scale: f
     st = (_mixers_so or _mixers()).delta_rule(start, q, k, v, g, beta, state, state_out, out, scratch, scale, max_len,
                                               slots, head_map, stream)
     if st:
-        check(st, "m27q_delta_rule")
+        _mixer_check(st, "m27q_delta_rule")
