@@ -12,9 +12,10 @@
 // Two kernels.  Many rows (k_attn) share tiles of keys that a workgroup brings into LDS once:
 // the matrix units bound it.  Up to 32 rows of a sequence and cache head (k_attn_few) are one
 // wave's, so its waves take keys apart from each other, and the cache's bytes bound it.
-// Such rows through k_attn: one token over 1021 keys 22.6 us, by k_attn_few 11.4; 32 tokens over
-// up to 16381 keys 312 and 288; 2 x 5 rows over 32768 keys 62.4 and 59.9; 64 tokens over 3000
-// keys 125 and 112.
+// Such rows through k_attn: one token over 1021 keys 22.6 us, by k_attn_few 11.2; 32 tokens over
+// up to 16381 keys 312 and 287; 2 x 5 rows over 32768 keys 62.4 and 59.8; 64 tokens over 3000
+// keys 125 and 112.  The longest sequence of a call chooses for all of them: 512 rows beside 31
+// single tokens over 13400 to 16384 keys take 1411 us, apart 44 and 340.
 #include "m27q_device.h"
 #include "m27q_internal.h"
 #include "m27q_mix.h"
@@ -457,8 +458,11 @@ __device__ __forceinline__ bool has_gaps(const AttnParams &p, const Work &w) {
 // Many rows: four waves of 32 rows a workgroup, K and V of a tile of 32 keys in LDS, the next
 // tile on its way while this one is worked on (two workgroups a CU: what one waits for, the
 // other works).  Tiles that every row sees whole are taken without masks, those at the ends of
-// the causal or window mask apart.  4096 rows over 8192 keys, 24 heads of 256, BF16: 630 us,
-// 980 TFLOP/s of the pairs that the mask lets through (a product of 8192^3 runs at 1208).
+// the causal or window mask apart.  4096 rows over 8192 keys, 24 heads of 256, BF16: 632 to 651
+// us from card to card, 950 to 980 TFLOP/s of the pairs that the mask lets through (a product of
+// 8192^3 runs at 1208), F16 676; to F32, with the second product once for each piece of a weight,
+// 1170 and 937.  A window shorter than a workgroup's tokens leaves no tile whole, so that nothing
+// is on its way while a tile is worked on: 2048 rows 114 us without a window, 73 with one of 128.
 template <int D, bool BF, int NP>
 __global__ __launch_bounds__(kWaves * 64, 2) void k_attn(const AttnParams p) {
     typedef Rows<D, BF, NP, kRows> R;
@@ -597,11 +601,12 @@ __global__ __launch_bounds__(kWaves * 64, 2) void k_attn(const AttnParams p) {
 // of a workgroup take tiles in turn, each for itself with K and V tiles of its own: K of
 // its next tile is on its way from the moment its scores are there, V from when its values
 // are added, and nothing waits for another wave.  At the end the four sums are joined.
-// 32 sequences of up to 16381 keys, 4 cache heads of 256, F16: 1.58 GB in 288 us, 5.5 TB/s (a
-// copy runs at 4.97); 2 of up to 32768 keys and 5 rows each, 253 MB in 54 us and 6 of joining,
-// 4.2 TB/s: a wave has some 9 tiles between its start and the join.  One token over 1021 keys: a
-// tile a wave, and a chain of 16000 cycles (lengths 3500, page and loads 2700, their arrival
-// 2500, products and weights 2800, the waves' join 4300), then 3 us of the parts' join.
+// 32 sequences of up to 16381 keys, 4 cache heads of 256, F16: 1.58 GB in 287 us, 5.5 TB/s (a
+// plain read of as much runs at 7.1); 2 of up to 32768 keys and 5 rows each, 253 MB in 54 us and
+// 6 of joining, 4.2 TB/s (a plain read: 6.8): a wave has some 9 tiles between its start and the
+// join.  One token over 1021 keys: a tile a wave, and a chain of 16000 cycles (lengths 3500, page
+// and loads 2700, their arrival 2500, products and weights 2800, the waves' join 4300), then 3 us
+// of the parts' join.
 template <int D, bool BF, int NP, int RW>
 __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) void k_attn_few(const AttnParams p) {
     typedef Rows<D, BF, NP, RW> R;

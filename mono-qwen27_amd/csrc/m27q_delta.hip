@@ -34,9 +34,10 @@ struct Vec4<__bf16> {
 // single row the state's bytes bound it: it is read and written once.  The two
 // products of a row (S k, S q) are taken from the old state, with
 // S_new q = e^g S q + u (k.q): one pass, then the update.  64 sequences of 48 heads of 128 x
-// 128: 407 MB in 72 us, 5.6 TB/s (a copy runs at 4.97).  Of more rows the 160 fp32 operations
-// a lane and row bound it, 0.5 us where a SIMD has one wave; the next row's loads ahead of
-// them changed nothing (16 rows 12.3 and 12.1 us), and cost the single row registers.
+// 128: 407 MB in 71 us, 5.7 TB/s (x / 2 from as many states into others runs at 6.1, in place at
+// 5.9).  Of more rows the 160 fp32 operations a lane and row bound it, 0.5 us where a SIMD has one
+// wave; the next row's loads ahead of them changed nothing (16 rows 12.3 and 12.1 us), and cost
+// the single row registers.
 template <int DK, typename T>
 __global__ __launch_bounds__(64) void k_delta_rows(const m27q_delta d) {
     typedef typename Vec4<T>::t T4;
@@ -529,8 +530,8 @@ __device__ __forceinline__ void row_by_row(const m27q_delta &d, const SeqRows &s
 // been used, without branches (a load under one would keep later waits from telling it apart).
 // The chain of the three products bounds it: 4096 rows of 48 heads of 128 (192 workgroups),
 // fp32, 64 chunks of 3.7 us, 7000 to 8500 cycles of which the matrix units work 2900, LDS 3400;
-// Q S^T in pieces is the longest of part 2.  236 us after 49 of preparation; four BF16 sequences
-// of up to 1531 rows (768 workgroups, one a CU at a time) 198 after 59.  Measured before reads
+// Q S^T in pieces is the longest of part 2.  237 us after 49 of preparation; four BF16 sequences
+// of up to 1531 rows (768 workgroups, one a CU at a time) 193 after 59.  Measured before reads
 // stood in front of the products: Q cut into pieces in part 1 instead 333 us against 304 in all,
 // K's loads and pieces with the state's waves 337; BF16 in the 128 registers of two workgroups a
 // CU, which spill, 296 against 258.
@@ -823,9 +824,11 @@ __global__ __launch_bounds__(512) void k_delta_chunks(const m27q_delta d, const 
 // a result's 4 g + 0 .. 3 are the operand of the instructions over 16.  So state, right-hand
 // sides and U go from product to product in registers.  The four waves of a workgroup share
 // K and Q in LDS, as operand blocks [step][piece][64 lanes][8], a step of 32 columns a wave.
-// A wave's chain of products bounds it where a SIMD has one (16 more rows 4.2 us), the state's
-// bytes where it has several: 16 rows of 8 sequences, 48 heads of 128 x 128, 50 MB of states,
-// 17.6 us in fp32 and 15.1 in BF16 (row by row 35).
+// A wave's chain of products bounds it where a SIMD has one (16 more rows 4.2 us).  With several
+// neither that nor the bytes do alone: 16 rows of 8 sequences, 48 heads of 128 x 128, take 17.1 us
+// in fp32 and 15.1 in BF16 (row by row 35) for 50 MB of states, 3 TB/s.  All waves are there at
+// once, so all load, then all compute, then all store; what needs no state (A and its inverse)
+// stands behind the products that wait for it.
 
 template <int NA, int NB>
 __device__ __forceinline__ void mma16(const bf16x4 (&a)[NA], const bf16x4 (&b)[NB], f32x4 &c) {
@@ -1076,7 +1079,8 @@ __global__ __launch_bounds__(256, 3) void k_delta_few(const m27q_delta d) {
 //   4 sequences  6 rows 12.4 and 12.8, 8 rows 14.6 and 12.9; 128 rows 53 and 58, 256 rows 97 and 88
 //   8 sequences  5 rows 17 and 17, 16 rows 35 and 18; 128 rows 72 and 107, 384 rows 194 and 211
 // (bf16: 1 sequence 6 rows 7.2 and 7.8, 8 rows 8.8 and 8.0; 4 sequences 5 rows 11.9 and 11.2;
-// 4 sequences of 128 rows 44 and 41.)
+// 4 sequences of 128 rows 44 and 41.)  The longest sequence of a call chooses for all of them: 2048
+// rows beside 63 single tokens take 1407 us by chunks, apart 151 and 70.
 constexpr uint32_t kMostFew = 64;
 // Waves of 16 state rows that have rows to the end, about: short sequences beside a long one do not keep the card busy.
 unsigned long long waves(const m27q_delta &d) {

@@ -12,9 +12,9 @@
 //
 // One token (24 query and 4 + 4 cache heads of 256) takes 3.6 us, 64 take 4.6: launch, one
 // round trip for the table entry, one for the store.  2999 and 2903 of them from fp32 into a
-// BF16 cache, 288 MB: 71 us, 4.05 TB/s (a copy of 2 GiB runs at 4.97).  Four units a thread
-// (fewer, longer workgroups) took 110 us, loads past the caches 77, a workgroup of queries
-// that leaves the table alone 71.
+// BF16 cache, 290 MB: 72 us, 4.0 TB/s (a plain conversion of as much takes 50, 5.8 TB/s).  Four
+// units a thread (fewer, longer workgroups) took 110 us, loads past the caches 77, a workgroup
+// of queries that leaves the table alone 71.
 #include "m27q_mix.h"
 
 namespace m27q {
