@@ -467,6 +467,36 @@ M27Q_API m27q_status m27q_attn_paged(const m27q_seqs *seqs, const m27q_cache *ca
                                      const m27q_rows *out, float scale, int window, void *scratch,
                                      size_t scratch_bytes, hipStream_t stream);
 
+/* Groups of sequences that share a prefix: group g is the sequences first[g] ..
+ * first[g + 1] - 1 of a call, whose places 0 .. len[g] - 1 hold the same tokens,
+ * in pages that all of them name.  first does not descend and stays within
+ * 0 .. n; a sequence before first[0] or from first[groups] on shares nothing.
+ * Bounds of the launch: a group has at most max_rows rows, from the first of its
+ * first sequence to the last of its last one (rows past them are not worked on), and
+ * at most max_len places of a len are taken as shared. */
+typedef struct m27q_prefixes {
+    const int32_t *first;   /* device, groups + 1 */
+    const int32_t *len;     /* device, groups */
+    uint32_t groups;        /* 1 .. n */
+    uint32_t max_rows;      /* 1 .. tokens */
+    uint32_t max_len;
+    uint32_t pad;
+} m27q_prefixes;
+
+/* m27q_attn_paged without a window, for a batch whose sequences share long
+ * prefixes: a prefix's keys and values are read once for all rows of its group,
+ * through the page table of the group's first sequence.  Only whole tiles of 32
+ * places are taken so; the rest of a sequence's places come from its own table.
+ * Where the tables of a group name the same pages, the results are those of
+ * m27q_attn_paged, to the order of sums; where they do not, the first sequence's
+ * count.  A len past a sequence's own tokens is fine: rows see what lies at or
+ * before their own place.  scratch as in m27q_attn_paged, by its own size. */
+M27Q_API size_t m27q_attn_shared_scratch_bytes(const m27q_seqs *seqs, const m27q_prefixes *prefix, uint32_t q_heads,
+                                               const m27q_cache *cache);
+M27Q_API m27q_status m27q_attn_shared(const m27q_seqs *seqs, const m27q_prefixes *prefix, const m27q_cache *cache,
+                                      const m27q_rows *q, const m27q_rows *out, float scale, void *scratch,
+                                      size_t scratch_bytes, hipStream_t stream);
+
 /* Which key head a value head of the delta rule goes with: h / (heads / k heads),
  * or h modulo k heads (the order of GGUF files). */
 enum { M27Q_HEADS_GROUPED = 0, M27Q_HEADS_CYCLED = 1 };
@@ -506,6 +536,61 @@ typedef struct m27q_delta {
 M27Q_API size_t m27q_delta_scratch_bytes(uint32_t n, uint32_t tokens, uint32_t max_len, uint32_t heads, uint32_t dk,
                                          uint32_t dv);
 M27Q_API m27q_status m27q_delta_rule(const m27q_delta *d, void *scratch, size_t scratch_bytes, hipStream_t stream);
+
+/* ------------------------------------------------------------------------
+ * What a batch's step needs beside products and mixers
+ * ---------------------------------------------------------------------- */
+
+/* Root-mean-square norm of each head's dim values, with a residual's addition:
+ *   h = x + add;  y = weight h / sqrt(mean(h^2) + eps)
+ * x, add, sum and out are rows of one shape (tokens of them), each of any type; add
+ * may be NULL (h = x), weight (device, dim fp32 values, for every head the same) may
+ * be NULL (ones); dim 1 .. 2^20, eps above 0.  Written are those that are not NULL,
+ * one at least, of sum (h), out (y) and xq: y's codes in the format of
+ * m27q_quant_act for tokens rows of K = heads * dim values, by its rule (dim % 32
+ * == 0, tokens up to 2^16, K up to 2^20).  Computed in fp32, the squares' sum
+ * too (a row whose squares pass fp32 gives zeros), and rounded once; y is of h
+ * before sum's rounding.  sum or out may be x or add (same type and strides), not
+ * each other.  Replaces k_rms_norm_mulw (exec:858-895), its batched forms
+ * (exec:698-760) and, with xq, the quantizer behind them. */
+M27Q_API m27q_status m27q_rms_norm(const m27q_rows *x, const m27q_rows *add, int tokens, const float *weight, float eps,
+                                   const m27q_rows *sum, const m27q_rows *out, void *xq, hipStream_t stream);
+
+/* A token for each row of logits, each by values of its own: the steps of
+ * m27q_sample, for a batch and without its 64 candidates.  A row's tokens are
+ * taken in the order of m27q_topk (value descending, index ascending, NaN last), with weights
+ * w_i = e^((l_i - max) / temperature); of these the first top_k; of these the ones with
+ * w_i >= min_p; of these the shortest prefix whose sum reaches top_p times the sum
+ * of the first top_k.  The first token is always kept.  token is the first whose
+ * running sum reaches u times the sum of what is kept, prob its share of that.
+ *
+ * All arrays are in device memory, a value a row; NULL: temperature 1, top_k all,
+ * top_p 1, min_p 0, prob not written.  temperature <= 0 (or NaN) takes the first
+ * token, prob 1, and so does a row whose largest logit is infinite or that holds
+ * NaN alone; top_k < 1 or past n is n; top_p >= 1 and min_p <= 0 cut nothing (nor
+ * does NaN); u is taken as within 0 .. 1 (NaN 0).  A banned token's logit is
+ * -infinity (weight 0 at any temperature).  Weights are computed in 64 bits (2^-36 of their size at most is
+ * rounded off) and summed as integers: the same row gives the same token in any
+ * batch.  rows up to 65535, n up to 2^24.
+ * scratch (16-byte aligned) >= m27q_sample_rows_scratch_bytes, what it holds is
+ * of no matter. */
+typedef struct m27q_sampling {
+    const void *logits;         /* [rows][n] */
+    const float *temperature;
+    const int32_t *top_k;
+    const float *top_p;
+    const float *min_p;
+    const float *u;
+    int32_t *token;
+    float *prob;
+    int64_t stride;             /* values from a row to the next, n at least */
+    uint32_t type;              /* M27Q_TYPE_F32, _F16 or _BF16 */
+    uint32_t rows;
+    uint32_t n;
+    uint32_t pad;
+} m27q_sampling;
+M27Q_API size_t m27q_sample_rows_scratch_bytes(uint32_t rows, uint32_t n);
+M27Q_API m27q_status m27q_sample_rows(const m27q_sampling *s, void *scratch, size_t scratch_bytes, hipStream_t stream);
 
 #ifdef __cplusplus
 }

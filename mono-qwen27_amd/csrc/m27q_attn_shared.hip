@@ -1,0 +1,79 @@
+// m27q_attn_shared.hip -- attention of sequences that share prefixes.
+#include "m27q_attn.h"
+
+namespace m27q {
+
+namespace {
+
+long long tiles_of(long long rows) { return (rows + kWaves * kRows - 1) / (kWaves * kRows); }
+
+template <int D, bool BF, int NP, Kind KIND>
+void launch_kind(const AttnParams &p, bool few, long long rows, unsigned units, int parts, hipStream_t s) {
+    if (few) {
+        const dim3 grid(units * p.cache.heads, parts);
+        if (rows <= 16) hipLaunchKernelGGL((k_attn_few<D, BF, NP, 16, KIND>), grid, dim3(kWaves * 64), 0, s, p);
+        else hipLaunchKernelGGL((k_attn_few<D, BF, NP, kRows, KIND>), grid, dim3(kWaves * 64), 0, s, p);
+    } else {
+        const dim3 grid((unsigned)(tiles_of(rows) * units * p.cache.heads), parts);
+        hipLaunchKernelGGL((k_attn<D, BF, NP, KIND>), grid, dim3(kWaves * 64), 0, s, p);
+    }
+}
+
+template <int D, bool BF>
+hipError_t launch_t(const AttnParams &p, const SharedPlan &plan, hipStream_t s) {
+    constexpr int NP = BF ? 3 : 2;
+    const int group = (int)(p.q.heads / p.cache.heads);
+    const long long pr = (long long)p.prefix.max_rows * group, orows = (long long)p.seqs.max_q * group;
+    if (p.out.type == M27Q_TYPE_F32) {
+        launch_kind<D, BF, NP, kPrefix>(p, plan.prefix.few, pr, p.prefix.groups, plan.prefix.splits, s);
+        launch_kind<D, BF, NP, kOwn>(p, plan.own.few, orows, p.seqs.n, plan.own.splits, s);
+    } else {
+        launch_kind<D, BF, 1, kPrefix>(p, plan.prefix.few, pr, p.prefix.groups, plan.prefix.splits, s);
+        launch_kind<D, BF, 1, kOwn>(p, plan.own.few, orows, p.seqs.n, plan.own.splits, s);
+    }
+    constexpr int RPB = 4 * 64 / (D / 4);
+    const dim3 g2((p.seqs.max_q * p.q.heads + RPB - 1) / RPB, p.seqs.n);
+    hipLaunchKernelGGL((k_attn_join<D, BF, kOwn>), g2, dim3(256), 0, s, p);
+    return hipGetLastError();
+}
+
+int parts_of(long long wgs, long long once, long long keys, long long least, int limit) {
+    const long long want = (once + wgs - 1) / wgs, most = (keys + least - 1) / least;
+    const long long parts = want < most ? want : most;
+    return parts < 1 ? 1 : parts > limit ? limit : (int)parts;
+}
+
+}  // namespace
+
+// Workgroups of a part of the keys, the larger of the prefixes' and the sequences'.
+long long shared_groups(const m27q_seqs &seqs, const m27q_prefixes &prefix, uint32_t q_heads, const m27q_cache &cache) {
+    const long long rows = (long long)prefix.max_rows * (q_heads / cache.heads);
+    const long long a = tiles_of(rows) * prefix.groups * cache.heads, b = attn_groups(seqs, q_heads, cache);
+    return a > b ? a : b;
+}
+
+// Parts as in attn_plan, the prefix's at most 48 of the join's 64 and the own ones the rest.
+SharedPlan shared_plan(const m27q_seqs &seqs, const m27q_prefixes &prefix, uint32_t q_heads, const m27q_cache &cache,
+                       int cus) {
+    const long long group = q_heads / cache.heads;
+    SharedPlan r{};
+    const long long rows = prefix.max_rows * group, wgs = tiles_of(rows) * prefix.groups * cache.heads;
+    r.prefix.few = rows <= kRows;
+    r.prefix.splits = parts_of(wgs, (r.prefix.few && cache.dim == 256 ? 1ll : 2ll) * cus, prefix.max_len,
+                               r.prefix.few ? 128 : 256, 48);
+    m27q_seqs own = seqs;
+    r.own = attn_plan(own, q_heads, cache, cus);
+    if (r.own.splits > kMaxSplits - r.prefix.splits) r.own.splits = kMaxSplits - r.prefix.splits;
+    return r;
+}
+
+hipError_t launch_shared(const AttnParams &p, const SharedPlan &plan, hipStream_t s) {
+    const bool bf = p.cache.type == M27Q_TYPE_BF16;
+    switch (p.cache.dim) {
+        case 64: return bf ? launch_t<64, true>(p, plan, s) : launch_t<64, false>(p, plan, s);
+        case 128: return bf ? launch_t<128, true>(p, plan, s) : launch_t<128, false>(p, plan, s);
+        default: return bf ? launch_t<256, true>(p, plan, s) : launch_t<256, false>(p, plan, s);
+    }
+}
+
+}  // namespace m27q

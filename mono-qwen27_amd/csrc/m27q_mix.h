@@ -1,5 +1,6 @@
 // m27q_mix.h -- launch interface and device helpers of the token mixers
-// (rotary positions, attention over pages, the gated delta rule).
+// (rotary positions, attention over pages, the gated delta rule) and of a
+// batch's steps beside them (norms, sampling).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -36,6 +37,9 @@ struct AttnParams {
     int splits;     // parts of each sequence's keys
     float *part;    // [tokens * heads][splits][dim] sums of the parts, where splits > 1
     float2 *stat;   // [tokens * heads][splits] their maximum (log2) and weight
+    // behind shared prefixes: parts 0 .. prefix_parts - 1 are of the prefix, the others of a sequence's own keys
+    m27q_prefixes prefix;
+    int prefix_parts;
 };
 struct AttnPlan {
     int few;        // the kernel for few rows
@@ -46,6 +50,31 @@ long long attn_groups(const m27q_seqs &seqs, uint32_t q_heads, const m27q_cache 
 AttnPlan attn_plan(const m27q_seqs &seqs, uint32_t q_heads, const m27q_cache &cache, int cus);
 size_t attn_scratch(const m27q_seqs &seqs, uint32_t q_heads, uint32_t dim, int splits);
 hipError_t launch_attn(const AttnParams &p, const AttnPlan &plan, hipStream_t s);
+
+// Attention behind shared prefixes: the prefixes' keys for the rows of a group, then each
+// sequence's own, as parts of one softmax.
+struct SharedPlan {
+    AttnPlan prefix, own;
+};
+long long shared_groups(const m27q_seqs &seqs, const m27q_prefixes &prefix, uint32_t q_heads, const m27q_cache &cache);
+SharedPlan shared_plan(const m27q_seqs &seqs, const m27q_prefixes &prefix, uint32_t q_heads, const m27q_cache &cache,
+                       int cus);
+hipError_t launch_shared(const AttnParams &p, const SharedPlan &plan, hipStream_t s);
+
+struct NormParams {
+    m27q_rows x, add, sum, out;  // of add, sum and out any may have no ptr
+    int tokens;
+    const float *weight;         // or NULL
+    float eps;
+    int8_t *q;                   // codes, or NULL; their scales and sums
+    float *d;
+    uint32_t *s;
+};
+bool norm_fits(const NormParams &p);
+hipError_t launch_norm(const NormParams &p, hipStream_t s);
+
+size_t sample_scratch(uint32_t rows, uint32_t n);
+hipError_t launch_sample_rows(const m27q_sampling &p, void *scratch, hipStream_t s);
 
 hipError_t launch_delta(const m27q_delta &d, void *scratch, hipStream_t s);
 size_t delta_scratch(uint32_t n, uint32_t tokens, uint32_t max_len, uint32_t heads, uint32_t dk, uint32_t dv);

@@ -1,4 +1,4 @@
-// m27q_torch.cpp -- the token mixers' calls for Python, straight from tensors.
+// m27q_torch.cpp -- the token mixers' calls, and those of a batch's steps beside them, for Python, straight from tensors.
 //
 // A call costs the GPU as little as 4 us; reading shapes, strides and pointers of
 // up to ten tensors through Python costs the host as much again.  This module
@@ -59,6 +59,16 @@ m27q_rows rows(PyObject *o, int64_t tokens) {
     if (t.dim() != 3 || t.size(0) != tokens || (t.stride(2) != 1 && t.size(2) != 1) || t.size(1) > 0xffff || t.size(2) > 0xffff)
         throw Bad{M27Q_ERR_SHAPE};
     return {data(t), type_of(t), (uint32_t)t.size(1), (uint32_t)t.size(2), 0, t.stride(0), t.stride(1)};
+}
+
+// [tokens][dim] or [tokens][heads][dim] of a norm, which may be missing (no ptr).
+m27q_rows norm_rows(PyObject *o, int64_t tokens) {
+    const at::Tensor *t = tensor(o, true);
+    if (!t) return {};
+    const int64_t d = t->dim(), dim = d < 2 ? 0 : t->size(d - 1), heads = d == 3 ? t->size(1) : 1;
+    if (d < 2 || d > 3 || t->size(0) != tokens || (t->stride(d - 1) != 1 && dim != 1) || heads > 0xffff || dim > 0x7fffffff)
+        throw Bad{M27Q_ERR_SHAPE};
+    return {data(*t), type_of(*t), (uint32_t)heads, (uint32_t)dim, 0, t->stride(0), d == 3 ? t->stride(1) : dim};
 }
 
 const int32_t *int32s(PyObject *o, int64_t n, bool may_be_none = false) {
@@ -172,6 +182,65 @@ PyObject *py_attn_paged(PyObject *, PyObject *const *a, Py_ssize_t n) {
     });
 }
 
+// seqs, prefixes, cache, q, out, scratch, scale, stream
+PyObject *py_attn_shared(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    return call(a, n, 8, [](Args c) {
+        const m27q_seqs *s = record<m27q_seqs>(c.a[0]);
+        const m27q_prefixes *x = record<m27q_prefixes>(c.a[1]);
+        const m27q_rows q = rows(c.a[3], s->tokens), out = rows(c.a[4], s->tokens);
+        const at::Tensor &scratch = *tensor(c.a[5]);
+        return m27q_attn_shared(s, x, record<m27q_cache>(c.a[2]), &q, &out, (float)c.real(6), data(scratch),
+                                scratch.numel() * scratch.element_size(), c.stream(7));
+    });
+}
+
+// x, add, weight, eps, sum, out, act's buffer, M, K, stream
+PyObject *py_rms_norm(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    return call(a, n, 10, [](Args c) {
+        const at::Tensor &t = *tensor(c.a[0]);
+        if (t.dim() < 2 || t.size(0) > 0x7fffffff) throw Bad{M27Q_ERR_SHAPE};
+        const int64_t tokens = t.size(0);
+        const m27q_rows x = norm_rows(c.a[0], tokens), add = norm_rows(c.a[1], tokens), sum = norm_rows(c.a[4], tokens),
+                        out = norm_rows(c.a[5], tokens);
+        const float *weight = floats(c.a[2], x.dim, true);
+        void *xq = nullptr;
+        if (const at::Tensor *act = tensor(c.a[6], true)) {
+            const long long M = c.whole(7), K = c.whole(8);
+            if (M != tokens || K != (long long)x.heads * x.dim || M > 0xffff + 1 || K > (1 << 20) ||
+                (size_t)(act->numel() * act->element_size()) < m27q_act_bytes((int)M, (int)K))
+                throw Bad{M27Q_ERR_SHAPE};
+            xq = data(*act);
+        }
+        return m27q_rms_norm(&x, add.ptr ? &add : nullptr, (int)tokens, weight, (float)c.real(3), sum.ptr ? &sum : nullptr,
+                             out.ptr ? &out : nullptr, xq, c.stream(9));
+    });
+}
+
+// logits, u, token, scratch, temperature, top_k, top_p, min_p, prob, stream
+PyObject *py_sample_rows(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    return call(a, n, 10, [](Args c) {
+        const at::Tensor &t = *tensor(c.a[0]);
+        if (t.dim() != 2 || t.size(0) > 0x7fffffff || t.size(1) > 0x7fffffff || (t.stride(1) != 1 && t.size(1) != 1))
+            throw Bad{M27Q_ERR_SHAPE};
+        const int64_t rows = t.size(0);
+        m27q_sampling s{};
+        s.logits = data(t);
+        s.type = type_of(t);
+        s.rows = (uint32_t)rows;
+        s.n = (uint32_t)t.size(1);
+        s.stride = rows == 1 ? t.size(1) : t.stride(0);
+        s.u = floats(c.a[1], rows);
+        s.token = const_cast<int32_t *>(int32s(c.a[2], rows));
+        s.temperature = floats(c.a[4], rows, true);
+        s.top_k = int32s(c.a[5], rows, true);
+        s.top_p = floats(c.a[6], rows, true);
+        s.min_p = floats(c.a[7], rows, true);
+        s.prob = floats(c.a[8], rows, true);
+        const at::Tensor &scratch = *tensor(c.a[3]);
+        return m27q_sample_rows(&s, data(scratch), scratch.numel() * scratch.element_size(), c.stream(9));
+    });
+}
+
 // start, q, k, v, g, beta, state, state_out, out, scratch, scale, max_len, slots, head_map, stream
 PyObject *py_delta_rule(PyObject *, PyObject *const *a, Py_ssize_t n) {
     return call(a, n, 15, [](Args c) {
@@ -218,7 +287,10 @@ PyObject *py_streams(PyObject *, PyObject *f) {
 PyMethodDef methods[] = {{"rope", FAST(py_rope), nullptr},
                          {"rope_append", FAST(py_rope_append), nullptr},
                          {"attn_paged", FAST(py_attn_paged), nullptr},
+                         {"attn_shared", FAST(py_attn_shared), nullptr},
                          {"delta_rule", FAST(py_delta_rule), nullptr},
+                         {"rms_norm", FAST(py_rms_norm), nullptr},
+                         {"sample_rows", FAST(py_sample_rows), nullptr},
                          {"streams", py_streams, METH_O, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "m27q_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -75,6 +75,19 @@ class SeqsDesc(C.Structure):
                 ("pad", C.c_uint32)]
 
 
+class PrefixesDesc(C.Structure):
+    """m27q_prefixes"""
+    _fields_ = [("first", C.c_void_p), ("len", C.c_void_p), ("groups", C.c_uint32), ("max_rows", C.c_uint32),
+                ("max_len", C.c_uint32), ("pad", C.c_uint32)]
+
+
+class SamplingDesc(C.Structure):
+    """m27q_sampling"""
+    _fields_ = [("logits", C.c_void_p), ("temperature", C.c_void_p), ("top_k", C.c_void_p), ("top_p", C.c_void_p),
+                ("min_p", C.c_void_p), ("u", C.c_void_p), ("token", C.c_void_p), ("prob", C.c_void_p),
+                ("stride", C.c_int64), ("type", C.c_uint32), ("rows", C.c_uint32), ("n", C.c_uint32), ("pad", C.c_uint32)]
+
+
 class DeltaDesc(C.Structure):
     """m27q_delta"""
     _fields_ = [("start", C.c_void_p), ("slots", C.c_void_p), ("g", C.c_void_p), ("beta", C.c_void_p),
@@ -121,11 +134,18 @@ _SIGS = {
     "m27q_attn_scratch_bytes": (_SZ, [C.POINTER(SeqsDesc), _U32, C.POINTER(CacheDesc)]),
     "m27q_attn_paged": (_I, [C.POINTER(SeqsDesc), C.POINTER(CacheDesc), C.POINTER(Rows), C.POINTER(Rows), C.c_float,
                              _I, _P, _SZ, _P]),
+    "m27q_attn_shared_scratch_bytes": (_SZ, [C.POINTER(SeqsDesc), C.POINTER(PrefixesDesc), _U32, C.POINTER(CacheDesc)]),
+    "m27q_attn_shared": (_I, [C.POINTER(SeqsDesc), C.POINTER(PrefixesDesc), C.POINTER(CacheDesc), C.POINTER(Rows),
+                              C.POINTER(Rows), C.c_float, _P, _SZ, _P]),
+    "m27q_rms_norm": (_I, [C.POINTER(Rows), C.POINTER(Rows), _I, _P, C.c_float, C.POINTER(Rows), C.POINTER(Rows), _P, _P]),
+    "m27q_sample_rows_scratch_bytes": (_SZ, [_U32, _U32]),
+    "m27q_sample_rows": (_I, [C.POINTER(SamplingDesc), _P, _SZ, _P]),
     "m27q_delta_scratch_bytes": (_SZ, [_U32] * 6),
     "m27q_delta_rule": (_I, [C.POINTER(DeltaDesc), _P, _SZ, _P]),
 }
 # What the wrappers pass as packed bytes.
-_PACKED = tuple(C.POINTER(t) for t in (WeightDesc, C.c_void_p, Rows, RopePlan, CacheDesc, SeqsDesc, DeltaDesc))
+_PACKED = tuple(C.POINTER(t) for t in (WeightDesc, C.c_void_p, Rows, RopePlan, CacheDesc, SeqsDesc, PrefixesDesc, SamplingDesc,
+                                           DeltaDesc))
 
 _lib = _fast = None
 
@@ -575,6 +595,19 @@ class Seqs:
                                        tokens, max_q, max_kv, 0), start, kv_len, table)
 
 
+class Prefixes:
+    """Groups of a call's sequences that share a prefix (m27q_prefixes): first [groups + 1], the sequence that each begins
+    with, and len [groups], int32 device tensors whose contents may change from call to call; the bounds max_rows (of a
+    group's rows) and max_len."""
+
+    def __init__(self, first, len, max_rows: int, max_len: int):  # noqa: A002 (the record's name)
+        if len.numel() < 1 or first.numel() != len.numel() + 1:
+            raise M27QError(2, "Prefixes")
+        self.first, self.len = first, len
+        self.packed = _packed(PrefixesDesc(_int32(first, "Prefixes"), _int32(len, "Prefixes"), len.numel(), max_rows,
+                                           max_len, 0), first, len)
+
+
 def rope(rope: Rope, pos, x, out, stream=None) -> None:
     """out <- x rotated by pos; x and out [tokens, heads, dim]."""
     st = (_mixers_so or _mixers()).rope(rope.packed, pos, x, out, stream)
@@ -600,6 +633,17 @@ def attn_paged(seqs: Seqs, cache: KVCache, q, out, scratch, scale: float, window
         _mixer_check(st, "m27q_attn_paged")
 
 
+def attn_shared_scratch_bytes(seqs: Seqs, prefixes: Prefixes, q_heads: int, cache: KVCache) -> int:
+    return (_fast or _calls()).m27q_attn_shared_scratch_bytes(seqs.packed, prefixes.packed, q_heads, cache.packed)
+
+
+def attn_shared(seqs: Seqs, prefixes: Prefixes, cache: KVCache, q, out, scratch, scale: float, stream=None) -> None:
+    """attn_paged for sequences that share prefixes, each prefix's pages read once for all rows of its group."""
+    st = (_mixers_so or _mixers()).attn_shared(seqs.packed, prefixes.packed, cache.packed, q, out, scratch, scale, stream)
+    if st:
+        _mixer_check(st, "m27q_attn_shared")
+
+
 def delta_scratch_bytes(n: int, tokens: int, max_len: int, heads: int, dk: int, dv: int) -> int:
     return lib().m27q_delta_scratch_bytes(n, tokens, max_len, heads, dk, dv)
 
@@ -612,3 +656,28 @@ def delta_rule(start, q, k, v, g, beta, state, state_out, out, scratch, scale: f
                                               slots, head_map, stream)
     if st:
         _mixer_check(st, "m27q_delta_rule")
+
+
+# ------------------------------------------------- beside products and mixers --
+
+def rms_norm(x, weight=None, eps: float = 1e-6, add=None, sum=None, out=None, act: Act | None = None,  # noqa: A002
+             stream=None) -> None:
+    """sum <- h = x + add; out <- y = weight h / sqrt(mean(h^2) + eps); act <- y quantized.  x, add, sum and out
+    [tokens, dim] or [tokens, heads, dim] (each head normed by itself), of any types; weight fp32 [dim] or None."""
+    buf, M, K = (None, 0, 0) if act is None else (act.buf, act.M, act.K)
+    st = (_mixers_so or _mixers()).rms_norm(x, add, weight, eps, sum, out, buf, M, K, stream)
+    if st:
+        _mixer_check(st, "m27q_rms_norm")
+
+
+def sample_rows_scratch_bytes(rows: int, n: int) -> int:
+    return lib().m27q_sample_rows_scratch_bytes(rows, n)
+
+
+def sample_rows(logits, u, token, scratch, temperature=None, top_k=None, top_p=None, min_p=None, prob=None,
+                stream=None) -> None:
+    """token[r] <- the token that row r of logits [rows, n] gives for u[r], by its own temperature, top_k (int32),
+    top_p and min_p; prob[r] <- its share of what was kept."""
+    st = (_mixers_so or _mixers()).sample_rows(logits, u, token, scratch, temperature, top_k, top_p, min_p, prob, stream)
+    if st:
+        _mixer_check(st, "m27q_sample_rows")
