@@ -15,7 +15,7 @@ namespace m27q {
 
 namespace {
 
-constexpr int kThreads = 1024;
+constexpr int kRowThreads = 1024;  // of a workgroup that works on one row
 
 // Descending order of keys: value, then the lower index; -0 as +0; NaN behind every number.
 __device__ __forceinline__ uint32_t order_bits(float v) {
@@ -29,6 +29,11 @@ __device__ __forceinline__ uint64_t order_key(float v, int i) {
 }
 constexpr int kKeyBits = 56;
 __device__ __forceinline__ int key_index(uint64_t key) { return (int)(0xffffffu - (uint32_t)(key & 0xffffffu)); }
+
+__device__ __forceinline__ float key_value(uint64_t key) {
+    const uint32_t b = (uint32_t)(key >> 24);
+    return __uint_as_float(b & 0x80000000u ? b ^ 0x80000000u : ~b);
+}
 
 // What a row is sampled with.
 struct Rule {
@@ -56,34 +61,24 @@ struct Found {
     uint64_t sum;    // of the weights down to it, itself included
 };
 
-// One workgroup a row: the token at which a count or a sum of weights in descending order
-// reaches its target, by 8 bits of the keys at a time, the row read once for each.
-__global__ __launch_bounds__(kThreads) void k_sample_row(const m27q_sampling p) {
-    __shared__ unsigned long long mass[256];
-    __shared__ uint32_t count[256];
-    __shared__ unsigned long long best_s, total_s;
-    __shared__ uint64_t found_key, found_sum;
-    __shared__ uint32_t found_count;
-    const int row = blockIdx.x, n = (int)p.n, tid = threadIdx.x;
+// What a workgroup that goes through a whole row keeps in LDS.
+struct WholeRow {
+    unsigned long long mass[256];
+    uint32_t count[256];
+    unsigned long long total;
+    uint64_t found_key, found_sum;
+    uint32_t found_count;
+};
+
+// A row whose borders lie among more tokens than a list holds (thousands of equal logits): the
+// token at which a count or a sum of weights in descending order reaches its target, by 8 bits of
+// the keys at a time, the row read once for each.
+__device__ void sample_whole_row(const m27q_sampling &p, int row, const Rule &r, uint64_t best, WholeRow &s) {
+    const int n = (int)p.n, tid = threadIdx.x;
     const long long base = (long long)row * p.stride;
     auto value = [&](int i) { return load1(p.logits, base + i, p.type); };
-    const Rule r = row_rule(p, row);
-
-    if (tid == 0) best_s = total_s = 0;
-    __syncthreads();
-    unsigned long long best = 0;
-    for (int i = tid; i < n; i += kThreads) best = max(best, (unsigned long long)order_key(value(i), i));
-    atomicMax(&best_s, best);
-    __syncthreads();
-    best = best_s;
     const float top = value(key_index(best));
-    if (r.greedy || !__builtin_isfinite(top)) {
-        if (tid == 0) {
-            p.token[row] = key_index(best);
-            if (p.prob) p.prob[row] = 1.0f;
-        }
-        return;
-    }
+    if (tid == 0) s.total = 0;
     const double one = (double)(1ull << (62 - (64 - __builtin_clzll((unsigned long long)n))));
     auto weight = [&](float v) {
         const double w = exp(((double)v - (double)top) * r.inv_t);
@@ -97,39 +92,39 @@ __global__ __launch_bounds__(kThreads) void k_sample_row(const m27q_sampling p) 
         uint32_t seen = 0;
         for (int shift = kKeyBits - 8; shift >= 0; shift -= 8) {
             __syncthreads();
-            if (tid < 256) mass[tid] = 0, count[tid] = 0;
+            if (tid < 256) s.mass[tid] = 0, s.count[tid] = 0;
             __syncthreads();
-            for (int i = tid; i < n; i += kThreads) {
+            for (int i = tid; i < n; i += kRowThreads) {
                 const float v = value(i);
                 const uint64_t key = order_key(v, i);
                 if ((key >> (shift + 8)) != prefix) continue;
                 const int digit = (int)(key >> shift) & 255;
-                atomicAdd(&count[digit], 1u);
-                atomicAdd(&mass[digit], fixed(weight(v)));
+                atomicAdd(&s.count[digit], 1u);
+                atomicAdd(&s.mass[digit], fixed(weight(v)));
             }
             __syncthreads();
             if (tid == 0) {
                 int digit = 255, last = -1;
                 for (; digit >= 0; --digit) {
-                    if (count[digit] == 0) continue;
+                    if (s.count[digit] == 0) continue;
                     last = digit;
-                    if (seen + count[digit] >= most || (double)(sum + mass[digit]) >= target) break;
-                    seen += count[digit];
-                    sum += mass[digit];
+                    if (seen + s.count[digit] >= most || (double)(sum + s.mass[digit]) >= target) break;
+                    seen += s.count[digit];
+                    sum += s.mass[digit];
                 }
                 if (digit < 0) {  // never reached: the last one
                     digit = last;
-                    seen -= count[digit];
-                    sum -= mass[digit];
+                    seen -= s.count[digit];
+                    sum -= s.mass[digit];
                 }
-                found_key = prefix << 8 | (uint64_t)digit;
-                found_sum = sum;
-                found_count = seen;
+                s.found_key = prefix << 8 | (uint64_t)digit;
+                s.found_sum = sum;
+                s.found_count = seen;
             }
             __syncthreads();
-            prefix = found_key;
-            sum = found_sum;
-            seen = found_count;
+            prefix = s.found_key;
+            sum = s.found_sum;
+            seen = s.found_count;
         }
         return Found{prefix, sum + fixed(weight(value(key_index(prefix))))};
     };
@@ -138,29 +133,532 @@ __global__ __launch_bounds__(kThreads) void k_sample_row(const m27q_sampling p) 
     uint64_t cut = all.key;
     if (r.top_p < 1.0) cut = max(cut, border(0xffffffffu, r.top_p * (double)all.sum).key);
     unsigned long long part = 0;
-    for (int i = tid; i < n; i += kThreads) {
+    for (int i = tid; i < n; i += kRowThreads) {
         const float v = value(i);
         const uint64_t key = order_key(v, i);
         const double w = weight(v);
         if (key == best || (key >= cut && w >= r.min_p)) part += fixed(w);
     }
-    atomicAdd(&total_s, part);
+    atomicAdd(&s.total, part);
     __syncthreads();
-    const Found pick = border(0xffffffffu, r.u * (double)total_s);
+    const Found pick = border(0xffffffffu, r.u * (double)s.total);
     if (tid == 0) {
         const int i = key_index(pick.key);
         p.token[row] = i;
-        if (p.prob) p.prob[row] = (float)(weight(value(i)) * one / (double)total_s);
+        if (p.prob) p.prob[row] = (float)(weight(value(i)) * one / (double)s.total);
     }
+}
+
+
+// ------------------------------------------------------------------ bins --
+//
+// Weights are told apart by y = 16 log2(e) l / T, a sixteenth of an octave a unit.  The tokens of a
+// row fall into bins by their distance from an anchor, the octave at or above the largest: 384
+// bins of a unit, 127 of an octave, and what lies below those 151 octaves counts for nothing.
+// Units are absolute (y rounded), anchors whole octaves: bins of parts of a row with anchors of
+// their own add up.  A bin holds how many tokens and the sum of their weights, in 2^-36 of
+// the weight at the bin's upper end.
+
+constexpr int kUnit = 16;               // units of an octave
+constexpr int kFine = 384, kCoarse = 127;
+constexpr int kBins = kFine + kCoarse;  // bin kBins: nothing
+constexpr int kMassBits = 36, kSumBits = 50;
+constexpr int kPart = 8192;             // tokens of a part at most: counts of 14 bits above sums of 50
+constexpr double kUnitsPerNat = 16 * 1.4426950408889634074;
+
+// 2^(z / 16): the Taylor polynomial of degree 6, whose next term is below 3e-13 for |z| <= 1.6.
+__device__ __forceinline__ double exp2_unit(double z) {
+    constexpr double a = 0.69314718055994530942 / 16;
+    double p = a * a * a * a * a * a / 720;
+    p = __builtin_fma(p, z, a * a * a * a * a / 120);
+    p = __builtin_fma(p, z, a * a * a * a / 24);
+    p = __builtin_fma(p, z, a * a * a / 6);
+    p = __builtin_fma(p, z, a * a / 2);
+    p = __builtin_fma(p, z, a);
+    return __builtin_fma(p, z, 1.0);
+}
+
+// The bin of a logit; z: its weight is 2^(z / 16) (a bin of an octave: 2^z) of that at the bin's upper end.
+// The product is taken with its remainder, so that z is right to 2^-50 wherever bins tell
+// weights apart at all.
+__device__ __forceinline__ int bin_of(float l, double c, double anchor, double &z) {
+    const double x = (double)l, hi = x * c, lo = __builtin_fma(x, c, -hi), b = __builtin_rint(hi);
+    const double r = fmin(fmax((hi - b) + lo, -0.5), 0.5), d = anchor - b;
+    if (!(d < kFine + kUnit * kCoarse)) return kBins;  // (-infinity and NaN too)
+    const int i = (int)d;
+    z = r;
+    if (i < kFine) return i;
+    const int o = (i - kFine) / kUnit;
+    z = (r - (double)((i - kFine) & (kUnit - 1))) * (1.0 / kUnit);
+    return kFine + o;
+}
+__device__ __forceinline__ unsigned long long bin_mass(int bin, double z) {
+    double p = exp2_unit(z);
+    if (bin >= kFine) {
+        p *= p;
+        p *= p;
+        p *= p;
+        p *= p;
+    }
+    return (unsigned long long)__builtin_rint(p * (double)(1ull << kMassBits));
+}
+// The weight at a bin's upper end, of that at the anchor.
+__device__ __forceinline__ double bin_scale(int bin) {
+    return exp2(-(bin < kFine ? bin : kFine + kUnit * (bin - kFine)) * (1.0 / kUnit));
+}
+
+// What is kept of a part of a row, and of a row.
+struct Part {
+    double anchor;        // -infinity: no token of any weight
+    uint64_t best;        // the largest key
+};
+constexpr int kList = 8192;
+struct RowPlan {
+    double anchor;
+    uint64_t best;
+    int state;            // 0: done; 1: the tokens of marked bins make a list; 2: the whole row is gone through
+    uint32_t listed;      // tokens on the list
+    unsigned long long min_p_sum;         // of the tokens that min_p leaves, where none of its border's bins cuts them
+    uint32_t marks[(kBins + 31) / 32];
+    uint32_t before[kBins + 1];           // tokens of the bins above
+    uint32_t at[kBins + 1];               // ... that are on the list
+    unsigned long long sum[kBins + 1];    // their weights, in 2^-s of the anchor's (s: row_scale)
+};
+struct Scratch {
+    Part *part;                 // [rows][parts]
+    unsigned long long *bins;   // [rows][parts][kBins + 1]
+    RowPlan *plan;              // [rows]
+    uint64_t *list;             // [rows][kList]
+    int parts, per;             // parts of a row and tokens of one
+};
+
+// Sums of a row's weights fit 62 bits.
+__device__ __forceinline__ double row_scale(uint32_t n) { return (double)(1ull << (62 - (32 - __builtin_clz(n)))); }
+
+constexpr int kPartThreads = 256;
+constexpr int kCopies = 4;  // of a part's bins: lanes that meet in a bin wait for each other
+
+// The i-th of a thread's tokens in a part.
+__device__ __forceinline__ int part_index(int i) { return i * kPartThreads + (int)threadIdx.x; }
+
+// A part's bins, and its largest token.
+template <int PER>
+__global__ __launch_bounds__(kPartThreads) void k_sample_parts(const m27q_sampling p, const Scratch sc) {
+    constexpr int N = PER / kPartThreads;
+    __shared__ unsigned long long bins[(kBins + 1) * kCopies];
+    __shared__ float top_s[kPartThreads / 64];
+    __shared__ int at_s[kPartThreads / 64];
+    const int row = blockIdx.y, first = (int)blockIdx.x * PER, count = min(PER, (int)p.n - first);
+    const long long base = (long long)row * p.stride + first;
+    float v[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = part_index(i) < count ? load1(p.logits, base + part_index(i), p.type) : __builtin_nanf("");
+    const Rule r = row_rule(p, row);
+    for (int i = threadIdx.x; i < (kBins + 1) * kCopies; i += kPartThreads) bins[i] = 0;
+    float top = -__builtin_inff();
+#pragma unroll
+    for (int i = 0; i < N; ++i) top = fmaxf(top, v[i]);
+#pragma unroll
+    for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    if (lane == 0) top_s[wave] = top;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kPartThreads / 64; ++i) top = fmaxf(top, top_s[i]);
+    int at = 0x7fffffff;
+#pragma unroll
+    for (int i = N - 1; i >= 0; --i) at = v[i] == top ? part_index(i) : at;
+#pragma unroll
+    for (int o = 32; o; o >>= 1) at = min(at, __shfl_xor(at, o));
+    if (lane == 0) at_s[wave] = at;
+
+    const double c = kUnitsPerNat * r.inv_t;
+    const double b = __builtin_rint((double)top * c);
+    const double anchor = __builtin_isfinite(top) ? ceil(b * (1.0 / kUnit)) * kUnit : -__builtin_inf();
+    if (!r.greedy && __builtin_isfinite(top)) {
+#pragma unroll 4
+        for (int i = 0; i < N; ++i) {
+            double z = 0;
+            const int bin = bin_of(v[i], c, anchor, z);
+            if (bin < kBins)
+                atomicAdd(&bins[bin * kCopies + (lane & (kCopies - 1))], bin_mass(bin, z) + (1ull << kSumBits));
+        }
+    }
+    __syncthreads();
+    const long long me = (long long)row * sc.parts + blockIdx.x;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kPartThreads / 64; ++i) at = min(at, at_s[i]);
+        const bool none = at == 0x7fffffff;  // NaN alone
+        sc.part[me] = {anchor, order_key(none ? __builtin_nanf("") : top, first + (none ? 0 : at))};
+    }
+    if (r.greedy) return;
+    for (int i = threadIdx.x; i <= kBins; i += kPartThreads) {
+        unsigned long long s = 0;
+#pragma unroll
+        for (int j = 0; j < kCopies; ++j) s += bins[i * kCopies + j];
+        sc.bins[me * (kBins + 1) + i] = s;
+    }
+}
+
+// The running sums of a workgroup's values, one a thread: before this thread's, and all of them.
+template <typename T>
+__device__ __forceinline__ T scan_group(T v, T *lds, T &all) {
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, waves = (int)blockDim.x >> 6;
+    T run = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const T x = __shfl_up(run, o);
+        run += lane >= o ? x : T(0);
+    }
+    if (lane == 63) lds[wave] = run;
+    __syncthreads();
+    T before = 0;
+    all = 0;
+    for (int i = 0; i < waves; ++i) {
+        before += i < wave ? lds[i] : T(0);
+        all += lds[i];
+    }
+    __syncthreads();
+    return before + run - v;
+}
+
+constexpr int kPlanThreads = 512;
+static_assert(kBins + 1 == kPlanThreads, "a thread a bin");
+
+// A row's bins from those of its parts, and the bins in which its borders can lie: of the top_k-th
+// token, of top_p, of min_p and of the pick.  What is not known before another border is found
+// leaves a range of bins.
+__global__ __launch_bounds__(kPlanThreads) void k_sample_plan(const m27q_sampling p, const Scratch sc) {
+    __shared__ unsigned long long lds[kPlanThreads / 64], best_s;
+    __shared__ uint32_t lds32[kPlanThreads / 64];
+    __shared__ double anchors[kPlanThreads / 64], octave[kUnit];
+    __shared__ int found[8];
+    __shared__ unsigned long long sum[kBins + 2];
+    const int row = blockIdx.x, J = threadIdx.x;
+    const Part *part = sc.part + (long long)row * sc.parts;
+    const Rule r = row_rule(p, row);
+    RowPlan &out = sc.plan[row];
+    if (J == 0) best_s = 0;
+    if (J < 8) found[J] = kBins;
+    if (J < kUnit) octave[J] = exp2(-J * (1.0 / kUnit));
+    double anchor = -__builtin_inf();
+    unsigned long long best = 0;
+    for (int i = J; i < sc.parts; i += kPlanThreads) {
+        anchor = fmax(anchor, part[i].anchor);
+        best = max(best, (unsigned long long)part[i].best);
+    }
+#pragma unroll
+    for (int o = 32; o; o >>= 1) {
+        anchor = fmax(anchor, __shfl_xor(anchor, o));
+        best = max(best, (unsigned long long)__shfl_xor(best, o));
+    }
+    if ((J & 63) == 0) anchors[J >> 6] = anchor;
+    __syncthreads();
+    if ((J & 63) == 0) atomicMax(&best_s, best);
+    for (int i = 0; i < kPlanThreads / 64; ++i) anchor = fmax(anchor, anchors[i]);
+    __syncthreads();
+    best = best_s;
+    const float top = key_value(best);
+    if (r.greedy || !__builtin_isfinite(top)) {
+        if (J == 0) {
+            p.token[row] = key_index(best);
+            if (p.prob) p.prob[row] = 1.0f;
+            out.state = 0;
+        }
+        return;
+    }
+
+    // this thread's bin: whole numbers of weights where the parts' bins are of the same kind
+    unsigned long long mass = 0;
+    uint32_t count = 0;
+    double more = 0;
+    const unsigned long long *bins = sc.bins + (long long)row * sc.parts * (kBins + 1);
+    constexpr unsigned long long kMask = (1ull << kSumBits) - 1;
+    for (int i = 0; i < sc.parts; ++i, bins += kBins + 1) {
+        const double off_d = anchor - part[i].anchor;
+        if (!(off_d < kFine + kUnit * kCoarse)) continue;
+        const int off = (int)off_d;
+        int from = J - off;  // the part's bin, as far as it is one
+        if (J >= kFine) {
+            const int d = kFine + kUnit * (J - kFine) - off;  // the octave's distance there
+            if (d < kFine) {
+                for (int k = 0; k < kUnit && d >= 0 && J < kBins; ++k) {
+                    const unsigned long long x = bins[d + k];
+                    count += (uint32_t)(x >> kSumBits);
+                    more += (double)(x & kMask) * octave[k];
+                }
+                continue;
+            }
+            from = kFine + (d - kFine) / kUnit;
+        }
+        if (from < 0 || J >= kBins) continue;
+        const unsigned long long x = bins[from];
+        count += (uint32_t)(x >> kSumBits);
+        mass += x & kMask;
+    }
+    const double unit = row_scale(p.n) / (double)(1ull << kMassBits);
+    mass = (unsigned long long)__builtin_rint(((double)mass + more) * unit * bin_scale(J));
+    unsigned long long total;
+    uint32_t tokens;
+    const unsigned long long above = scan_group(mass, lds, total);
+    const uint32_t before = scan_group(count, lds32, tokens);
+    sum[J] = above;
+    if (J == kBins) sum[kBins + 1] = total;
+    __syncthreads();
+
+    // the bin in which the running sum reaches a target, the last one that holds a token if none does
+    auto bin_at = [&](int slot, double target) {
+        if (count && (double)(above + mass) >= target && (before == 0 || (double)above < target)) found[slot] = J;
+        __syncthreads();
+        return found[slot];
+    };
+    if (count && before + count == tokens) found[7] = J;
+    if (count && before < (uint32_t)r.k && before + count >= (uint32_t)r.k && (uint32_t)r.k < tokens) found[0] = J;
+    __syncthreads();
+    const int last = found[7], kb = found[0];
+    const bool k_cuts = kb < kBins;
+    // the sum of the first top_k
+    const double s_lo = (double)(k_cuts ? sum[kb] : total), s_hi = (double)(k_cuts ? sum[kb + 1] : total);
+    double t_lo = s_lo, t_hi = s_hi;  // the sum of what is kept
+    int p0 = kBins, p1 = -1, mb = kBins;
+    if (r.top_p < 1.0) {
+        p0 = min(bin_at(1, r.top_p * s_lo), last);
+        p1 = min(bin_at(2, r.top_p * s_hi), last);
+        t_lo = fmin(t_lo, (double)sum[p0]);
+        t_hi = fmin(t_hi, (double)sum[p1 + 1]);
+    }
+    if (r.min_p > 0.0) {
+        const double c = kUnitsPerNat * r.inv_t;
+        // the bin of the weight min_p, and its neighbours for what rounding does
+        const double y = (double)top * c + kUnit * log2(r.min_p), d = anchor - __builtin_rint(y);
+        mb = !(d < kFine + kUnit * kCoarse) ? kBins : d < 0 ? 0 : d < kFine ? (int)d : kFine + ((int)d - kFine) / kUnit;
+        t_lo = fmin(t_lo, (double)sum[max(mb - 1, 0)]);
+        t_hi = fmin(t_hi, (double)sum[min(mb + 2, kBins + 1)]);
+    }
+    // the first token alone is always kept
+    const int q0 = min(bin_at(3, r.u * t_lo), last), q1 = min(bin_at(4, r.u * t_hi), last);
+    const bool mark = count && (J == kb || (J >= p0 && J <= p1) || (mb < kBins && J >= mb - 1 && J <= mb + 1) ||
+                                (J >= q0 && J <= q1) || before == 0);
+    uint32_t listed;
+    const uint32_t at = scan_group(mark ? count : 0u, lds32, listed);
+    out.sum[J] = above;
+    out.before[J] = before;
+    out.at[J] = at;
+    const unsigned long long m = __ballot(mark);
+    if ((J & 31) == 0) out.marks[J / 32] = (uint32_t)(m >> (J & 32));
+    if (J == 0) {
+        out.anchor = anchor;
+        out.best = best;
+        out.min_p_sum = mb < kBins ? sum[min(mb + 2, kBins)] : total;
+        out.state = listed <= (uint32_t)kList ? 1 : 2;
+        out.listed = 0;  // counted by the next launch
+    }
+}
+
+// The tokens of marked bins, in no order.
+template <int PER>
+__global__ __launch_bounds__(kPartThreads) void k_sample_list(const m27q_sampling p, const Scratch sc) {
+    constexpr int N = PER / kPartThreads;
+    constexpr uint32_t M = 2048;  // (a part's tokens past them go by themselves)
+    __shared__ uint64_t keys[M];
+    __shared__ uint32_t count_s, to_s;
+    const int row = blockIdx.y, first = (int)blockIdx.x * PER, count = min(PER, (int)p.n - first);
+    RowPlan &plan = sc.plan[row];
+    if (plan.state != 1) return;
+    const long long base = (long long)row * p.stride + first;
+    float v[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = part_index(i) < count ? load1(p.logits, base + part_index(i), p.type) : __builtin_nanf("");
+    if (threadIdx.x == 0) count_s = 0;
+    __syncthreads();
+    uint64_t *const list = sc.list + (long long)row * kList;
+    const double c = kUnitsPerNat * row_rule(p, row).inv_t, anchor = plan.anchor;
+#pragma unroll 4
+    for (int i = 0; i < N; ++i) {
+        double z;
+        const int bin = bin_of(v[i], c, anchor, z);
+        if (bin < kBins && (plan.marks[bin / 32] >> (bin & 31) & 1)) {
+            const uint64_t key = order_key(v[i], first + part_index(i));
+            const uint32_t at = atomicAdd(&count_s, 1u);
+            if (at < M) {
+                keys[at] = key;
+            } else {
+                const uint32_t to = atomicAdd(&plan.listed, 1u);
+                if (to < (uint32_t)kList) list[to] = key;
+            }
+        }
+    }
+    __syncthreads();
+    const uint32_t m = min(count_s, M);
+    if (m == 0) return;
+    if (threadIdx.x == 0) to_s = atomicAdd(&plan.listed, m);
+    __syncthreads();
+    const uint32_t to = to_s;
+    for (uint32_t i = threadIdx.x; i < m; i += kPartThreads)
+        if (to + i < (uint32_t)kList) list[to + i] = keys[i];
+}
+
+// A row's list in order, the running sums of its tokens, and the borders among them.
+__global__ __launch_bounds__(kRowThreads) void k_sample_pick(const m27q_sampling p, const Scratch sc) {
+    __shared__ uint64_t keys[kList];
+    __shared__ union {
+        unsigned long long scan[kRowThreads / 64];
+        WholeRow whole;
+    } s;
+    __shared__ unsigned long long start[kBins + 1];  // the list's running sum in front of a bin
+    // sums down to the first token, the top_k-th, the one that reaches top_p and the last one that min_p leaves
+    __shared__ unsigned long long first_s, among_s, top_p_s, min_p_s;
+    __shared__ int pick_s;
+    const int row = blockIdx.x, tid = threadIdx.x;
+    const RowPlan &plan = sc.plan[row];
+    const int state = plan.state;
+    if (state == 0) return;
+    const Rule r = row_rule(p, row);
+    if (state == 2) {
+        sample_whole_row(p, row, r, plan.best, s.whole);
+        return;
+    }
+    const int n = (int)min(plan.listed, (uint32_t)kList);
+    int size = 64;
+    while (size < n) size *= 2;
+    for (int i = tid; i < size; i += kRowThreads) keys[i] = i < n ? sc.list[(long long)row * kList + i] : 0;
+    if (tid == 0) {
+        first_s = 0;
+        among_s = plan.sum[kBins];  // unless the top_k-th is on the list
+        top_p_s = ~0ull;
+        min_p_s = plan.min_p_sum;
+        pick_s = 0x7fffffff;
+    }
+    __syncthreads();
+    for (int k = 2; k <= size; k *= 2)
+        for (int j = k / 2; j > 0; j /= 2) {
+            for (int t = tid; t < size / 2; t += kRowThreads) {
+                const int i = 2 * t - (t & (j - 1)), l = i + j;
+                const uint64_t a = keys[i], b = keys[l];
+                if ((a < b) == ((i & k) == 0)) {
+                    keys[i] = b;
+                    keys[l] = a;
+                }
+            }
+            __syncthreads();
+        }
+
+    // each thread a run of the list: the sums of the row down to each of its tokens.  In front of a
+    // bin, and at its end, they are the plan's.
+    constexpr int E = kList / kRowThreads;
+    const int each = (n + kRowThreads - 1) / kRowThreads, i0 = min(tid * each, n), i1 = min(i0 + each, n);
+    const double c = kUnitsPerNat * r.inv_t, anchor = plan.anchor;
+    const double unit = row_scale(p.n) / (double)(1ull << kMassBits);
+    unsigned long long own[E], sum = 0;
+    int bin[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        own[e] = 0;
+        bin[e] = 0;
+        if (i0 + e < i1) {
+            double z = 0;
+            bin[e] = bin_of(key_value(keys[i0 + e]), c, anchor, z);
+            own[e] = bin_mass(bin[e], z);
+        }
+        sum += own[e];
+    }
+    unsigned long long all, run = scan_group(sum, s.scan, all);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        if (i0 + e < i1 && (uint32_t)(i0 + e) == plan.at[bin[e]]) start[bin[e]] = run;
+        run += own[e];
+    }
+    run -= sum;
+    __syncthreads();
+    unsigned long long below[E], down[E];  // without and with the token
+    int rank[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const uint32_t i = (uint32_t)(i0 + e), at = plan.at[bin[e]];
+        const unsigned long long lo = plan.sum[bin[e]], hi = plan.sum[bin[e] + 1], in = run - start[bin[e]];
+        const double f = unit * bin_scale(bin[e]);
+        below[e] = min(lo + (unsigned long long)__builtin_rint((double)in * f), hi);
+        down[e] = i + 1 == plan.at[bin[e] + 1] ? hi : min(lo + (unsigned long long)__builtin_rint((double)(in + own[e]) * f), hi);
+        rank[e] = (int)(plan.before[bin[e]] + i - at);
+        run += own[e];
+    }
+    const float top = key_value(plan.best);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        if (i0 + e >= i1) continue;
+        if (rank[e] == 0) first_s = down[e];
+        if (rank[e] == r.k - 1) among_s = down[e];
+        if (r.min_p > 0.0 && exp(((double)key_value(keys[i0 + e]) - (double)top) * r.inv_t) < r.min_p) atomicMin(&min_p_s, below[e]);
+    }
+    __syncthreads();
+    const unsigned long long among = among_s;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+        if (i0 + e < i1 && r.top_p < 1.0 && (double)down[e] >= r.top_p * (double)among) atomicMin(&top_p_s, down[e]);
+    __syncthreads();
+    const unsigned long long total = max(first_s, min(among, min(top_p_s, min_p_s)));
+    const double target = r.u * (double)total;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+        if (i0 + e < i1 && (double)down[e] >= target) atomicMin(&pick_s, rank[e]);
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+        if (i0 + e < i1 && rank[e] == pick_s) {
+            p.token[row] = key_index(keys[i0 + e]);
+            if (p.prob) p.prob[row] = (float)((double)own[e] * unit * bin_scale(bin[e]) / (double)total);
+        }
 }
 
 }  // namespace
 
-size_t sample_scratch(uint32_t, uint32_t) { return 16; }
+namespace {
 
-hipError_t launch_sample_rows(const m27q_sampling &p, void *, hipStream_t s) {
-    hipLaunchKernelGGL(k_sample_row, dim3(p.rows), dim3(kThreads), 0, s, p);
+// Tokens of a part: enough parts to fill the card, and no more than it takes.
+int part_tokens(uint32_t rows, uint32_t n) {
+    int per = 2048;
+    while (per < kPart && (long long)rows * ((n + per - 1) / per) > 1024) per *= 2;
+    return per;
+}
+
+struct Sizes {
+    int per, parts;
+    size_t part, bins, plan, list;
+    Sizes(uint32_t rows, uint32_t n)
+        : per(part_tokens(rows, n)), parts((int)((n + per - 1) / per)), part(align((size_t)rows * parts * sizeof(Part))),
+          bins((size_t)rows * parts * (kBins + 1) * 8), plan(align((size_t)rows * sizeof(RowPlan))), list((size_t)rows * kList * 8) {}
+    static size_t align(size_t v) { return (v + 255) & ~(size_t)255; }
+};
+
+template <int PER>
+hipError_t launch_t(const m27q_sampling &p, const Scratch &sc, hipStream_t s) {
+    const dim3 parts(sc.parts, p.rows);
+    hipLaunchKernelGGL((k_sample_parts<PER>), parts, dim3(kPartThreads), 0, s, p, sc);
+    hipLaunchKernelGGL(k_sample_plan, dim3(p.rows), dim3(kPlanThreads), 0, s, p, sc);
+    hipLaunchKernelGGL((k_sample_list<PER>), parts, dim3(kPartThreads), 0, s, p, sc);
+    hipLaunchKernelGGL(k_sample_pick, dim3(p.rows), dim3(kRowThreads), 0, s, p, sc);
     return hipGetLastError();
+}
+
+}  // namespace
+
+size_t sample_scratch(uint32_t rows, uint32_t n) {
+    const Sizes z(rows, n);
+    return z.part + z.bins + z.plan + z.list;
+}
+
+hipError_t launch_sample_rows(const m27q_sampling &p, void *scratch, hipStream_t s) {
+    const Sizes z(p.rows, p.n);
+    Scratch sc;
+    char *at = (char *)scratch;
+    sc.part = (Part *)at;
+    sc.bins = (unsigned long long *)(at += z.part);
+    sc.plan = (RowPlan *)(at += z.bins);
+    sc.list = (uint64_t *)(at + z.plan);
+    sc.parts = z.parts;
+    sc.per = z.per;
+    if (z.per == 2048) return launch_t<2048>(p, sc, s);
+    return z.per == 4096 ? launch_t<4096>(p, sc, s) : launch_t<kPart>(p, sc, s);
 }
 
 }  // namespace m27q
