@@ -63,12 +63,141 @@ __global__ __launch_bounds__(kThreads) void k_norm_any(const NormParams p) {
     }
 }
 
+// Eight of a row's values: h, with the residual's loads beside x's.
+struct Unit8 {
+    f32x8 x, a;
+};
+__device__ __forceinline__ void load_unit(const NormParams &p, long long xr, long long ar, int i, Unit8 &u) {
+    u.x = load8(p.x.ptr, xr + 8 * i, p.x.type);
+    if (p.add.ptr) u.a = load8(p.add.ptr, ar + 8 * i, p.add.type);
+}
+__device__ __forceinline__ f32x8 unit_h(const NormParams &p, const Unit8 &u) { return p.add.ptr ? u.x + u.a : u.x; }
+__device__ __forceinline__ float unit_squares(f32x8 h, float s) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s = __builtin_fmaf(h[j], h[j], s);
+    return s;
+}
+__device__ __forceinline__ void store_unit(const NormParams &p, long long sr, long long yr, long long base, int i, f32x8 h, f32x8 w,
+                                           float r) {
+    f32x8 y = h * r;
+    if (p.weight) y *= w;
+    if (p.sum.ptr) store8(p.sum.ptr, sr + 8 * i, p.sum.type, h);
+    if (p.out.ptr) store8(p.out.ptr, yr + 8 * i, p.out.type, y);
+    if (p.q) {  // four lanes have a group of 32
+        float d;
+        uint32_t s;
+        const uint2 q = quant32x8(make_float4(y[0], y[1], y[2], y[3]), make_float4(y[4], y[5], y[6], y[7]), &d, &s);
+        const long long at = base + 8 * i;
+        *(uint2 *)(p.q + at) = q;
+        if ((i & 3) == 0) {
+            p.d[at / 32] = d;
+            p.s[at / 32] = s;
+        }
+    }
+}
+
+// Long rows: a workgroup a row, U units of 8 values a thread, in registers between the two passes.
+template <int U, int THREADS>
+__global__ __launch_bounds__(THREADS) void k_norm_row(const NormParams p, int threads) {
+    __shared__ float lds[THREADS / 64];
+    const int t = blockIdx.x / p.x.heads, head = blockIdx.x - t * p.x.heads, units = (int)p.x.dim / 8;
+    const long long xr = (long long)t * p.x.token_stride + (long long)head * p.x.head_stride;
+    const long long ar = (long long)t * p.add.token_stride + (long long)head * p.add.head_stride;
+    Unit8 u[U];
+    f32x8 w[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+        const int i = (int)threadIdx.x + k * threads;
+        if (i < units) load_unit(p, xr, ar, i, u[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+        const int i = (int)threadIdx.x + k * threads;
+        if (i < units && p.weight) w[k] = *(const f32x8a *)(p.weight + 8 * i);
+    }
+    float ss = 0;
+    f32x8 h[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+        if ((int)threadIdx.x + k * threads < units) {
+            h[k] = unit_h(p, u[k]);
+            ss = unit_squares(h[k], ss);
+        }
+    const float r = 1.0f / __builtin_sqrtf(sum_group(ss, lds, threads / 64) / (float)(int)p.x.dim + p.eps);
+    const long long sr = (long long)t * p.sum.token_stride + (long long)head * p.sum.head_stride;
+    const long long yr = (long long)t * p.out.token_stride + (long long)head * p.out.head_stride;
+    const long long base = ((long long)t * p.x.heads + head) * p.x.dim;
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+        const int i = (int)threadIdx.x + k * threads;
+        if (i < units) store_unit(p, sr, yr, base, i, h[k], w[k], r);
+    }
+}
+
+// Short rows (a head's): L lanes a row.
+template <int L>
+__global__ __launch_bounds__(kThreads) void k_norm_heads(const NormParams p, long long rows) {
+    const long long row = (long long)blockIdx.x * (kThreads / L) + threadIdx.x / L;
+    const int i = threadIdx.x & (L - 1), units = (int)p.x.dim / 8;
+    if (row >= rows) return;
+    const int t = (int)(row / p.x.heads), head = (int)(row - (long long)t * p.x.heads);
+    const bool live = i < units;
+    Unit8 u;
+    f32x8 w, h = {};
+    if (live) {
+        load_unit(p, (long long)t * p.x.token_stride + (long long)head * p.x.head_stride,
+                  (long long)t * p.add.token_stride + (long long)head * p.add.head_stride, i, u);
+        if (p.weight) w = *(const f32x8a *)(p.weight + 8 * i);
+        h = unit_h(p, u);
+    }
+    float ss = unit_squares(h, 0);
+#pragma unroll
+    for (int o = L / 2; o; o >>= 1) ss += __shfl_xor(ss, o);
+    const float r = 1.0f / __builtin_sqrtf(ss / (float)(int)p.x.dim + p.eps);
+    if (live)
+        store_unit(p, (long long)t * p.sum.token_stride + (long long)head * p.sum.head_stride,
+                   (long long)t * p.out.token_stride + (long long)head * p.out.head_stride, row * p.x.dim, i, h, w, r);
+}
+
+bool rows16(const m27q_rows &r) {
+    const int b = type_bytes(r.type);
+    return !r.ptr || ((uintptr_t)r.ptr % 16 == 0 && r.token_stride * b % 16 == 0 && r.head_stride * b % 16 == 0);
+}
+
 }  // namespace
 
-bool norm_fits(const NormParams &p) { return (long long)p.tokens * p.x.heads * kThreads < (1ll << 32); }
+// Units of 8 values need whole units in a head and 16-byte aligned rows.
+static bool norm_vectorizes(const NormParams &p) {
+    return p.x.dim % 8 == 0 && p.x.dim <= 4 * 8 * 1024 && rows16(p.x) && rows16(p.add) && rows16(p.sum) && rows16(p.out) &&
+           (uintptr_t)p.weight % 16 == 0;
+}
+
+bool norm_fits(const NormParams &p) { return (long long)p.tokens * p.x.heads * 1024 < (1ll << 32) || (p.x.dim <= 512 && (long long)p.tokens * p.x.heads * kThreads < (1ll << 32)); }
 
 hipError_t launch_norm(const NormParams &p, hipStream_t s) {
-    hipLaunchKernelGGL(k_norm_any, dim3((unsigned)(p.tokens * p.x.heads)), dim3(kThreads), 0, s, p);
+    const long long rows = (long long)p.tokens * p.x.heads;
+    const int units = (int)p.x.dim / 8;
+    if (!norm_vectorizes(p)) {
+        hipLaunchKernelGGL(k_norm_any, dim3((unsigned)rows), dim3(kThreads), 0, s, p);
+    } else if (units <= 64) {
+        int L = 4;
+        while (L < units) L *= 2;
+        const dim3 grid((unsigned)((rows * L + kThreads - 1) / kThreads));
+        switch (L) {
+            case 4: hipLaunchKernelGGL((k_norm_heads<4>), grid, dim3(kThreads), 0, s, p, rows); break;
+            case 8: hipLaunchKernelGGL((k_norm_heads<8>), grid, dim3(kThreads), 0, s, p, rows); break;
+            case 16: hipLaunchKernelGGL((k_norm_heads<16>), grid, dim3(kThreads), 0, s, p, rows); break;
+            case 32: hipLaunchKernelGGL((k_norm_heads<32>), grid, dim3(kThreads), 0, s, p, rows); break;
+            default: hipLaunchKernelGGL((k_norm_heads<64>), grid, dim3(kThreads), 0, s, p, rows);
+        }
+    } else if (units <= 1024) {
+        const int threads = (units + 63) / 64 * 64;
+        hipLaunchKernelGGL((k_norm_row<1, 1024>), dim3((unsigned)rows), dim3(threads), 0, s, p, threads);
+    } else if (units <= 2048) {
+        hipLaunchKernelGGL((k_norm_row<2, 1024>), dim3((unsigned)rows), dim3(1024), 0, s, p, 1024);
+    } else {
+        hipLaunchKernelGGL((k_norm_row<4, 1024>), dim3((unsigned)rows), dim3(1024), 0, s, p, 1024);
+    }
     return hipGetLastError();
 }
 

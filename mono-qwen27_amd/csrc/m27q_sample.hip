@@ -162,8 +162,10 @@ __device__ void sample_whole_row(const m27q_sampling &p, int row, const Rule &r,
 constexpr int kUnit = 16;               // units of an octave
 constexpr int kFine = 384, kCoarse = 127;
 constexpr int kBins = kFine + kCoarse;  // bin kBins: nothing
+constexpr int kOctaves = kFine / kUnit; // of the fine bins, whose sums a part has too
+constexpr int kStored = kBins + 1 + kOctaves;
 constexpr int kMassBits = 36, kSumBits = 50;
-constexpr int kPart = 8192;             // tokens of a part at most: counts of 14 bits above sums of 50
+constexpr int kPart = 8192;             // tokens of a part: counts of 14 bits above sums of 50
 constexpr double kUnitsPerNat = 16 * 1.4426950408889634074;
 
 // 2^(z / 16): the Taylor polynomial of degree 6, whose next term is below 3e-13 for |z| <= 1.6.
@@ -178,20 +180,33 @@ __device__ __forceinline__ double exp2_unit(double z) {
     return __builtin_fma(p, z, 1.0);
 }
 
-// The bin of a logit; z: its weight is 2^(z / 16) (a bin of an octave: 2^z) of that at the bin's upper end.
-// The product is taken with its remainder, so that z is right to 2^-50 wherever bins tell
-// weights apart at all.
-__device__ __forceinline__ int bin_of(float l, double c, double anchor, double &z) {
-    const double x = (double)l, hi = x * c, lo = __builtin_fma(x, c, -hi), b = __builtin_rint(hi);
-    const double r = fmin(fmax((hi - b) + lo, -0.5), 0.5), d = anchor - b;
+// What a row's logits are placed by.
+struct Scale {
+    double c;       // units of a logit
+    double anchor;
+    bool wide;      // y passes 2^18: its product is taken with its remainder
+    double near;    // 1; 0 where a step of a logit is thousands of octaves and only equal ones have a weight
+};
+__device__ __forceinline__ Scale row_scale(const Rule &r, double anchor) {
+    const double far = fabs(anchor) + kFine + kUnit * kCoarse;
+    return {kUnitsPerNat * r.inv_t, anchor, far > 0x1p18, far > 0x1p40 ? 0.0 : 1.0};
+}
+
+// The bin of a logit; z: its weight is 2^(z / 16) (a bin of an octave: 2^z) of that at the bin's upper
+// end.  The error of z is below 2^-35.
+__device__ __forceinline__ int bin_of(float l, const Scale &s, double &z) {
+    const double x = (double)l, hi = x * s.c, b = __builtin_rint(hi), d = s.anchor - b;
+    double r = hi - b;
+    if (s.wide) r += __builtin_fma(x, s.c, -hi);
     if (!(d < kFine + kUnit * kCoarse)) return kBins;  // (-infinity and NaN too)
+    z = r * s.near;
     const int i = (int)d;
-    z = r;
     if (i < kFine) return i;
     const int o = (i - kFine) / kUnit;
-    z = (r - (double)((i - kFine) & (kUnit - 1))) * (1.0 / kUnit);
+    z = (z - (double)((i - kFine) & (kUnit - 1))) * (1.0 / kUnit);
     return kFine + o;
 }
+// In 2^-36, rounded by an addition that leaves the whole number in the low bits.
 __device__ __forceinline__ unsigned long long bin_mass(int bin, double z) {
     double p = exp2_unit(z);
     if (bin >= kFine) {
@@ -200,12 +215,11 @@ __device__ __forceinline__ unsigned long long bin_mass(int bin, double z) {
         p *= p;
         p *= p;
     }
-    return (unsigned long long)__builtin_rint(p * (double)(1ull << kMassBits));
+    return __builtin_bit_cast(unsigned long long, __builtin_fma(p, (double)(1ull << kMassBits), 0x1p52)) & ((1ull << kSumBits) - 1);
 }
 // The weight at a bin's upper end, of that at the anchor.
-__device__ __forceinline__ double bin_scale(int bin) {
-    return exp2(-(bin < kFine ? bin : kFine + kUnit * (bin - kFine)) * (1.0 / kUnit));
-}
+__device__ __forceinline__ int bin_distance(int bin) { return bin < kFine ? bin : kFine + kUnit * (bin - kFine); }
+__device__ __forceinline__ double bin_scale(int bin) { return exp2(-bin_distance(bin) * (1.0 / kUnit)); }
 
 // What is kept of a part of a row, and of a row.
 struct Part {
@@ -213,73 +227,91 @@ struct Part {
     uint64_t best;        // the largest key
 };
 constexpr int kList = 8192;
+constexpr int kRanges = 4;
 struct RowPlan {
     double anchor;
     uint64_t best;
     int state;            // 0: done; 1: the tokens of marked bins make a list; 2: the whole row is gone through
     uint32_t listed;      // tokens on the list
     unsigned long long min_p_sum;         // of the tokens that min_p leaves, where none of its border's bins cuts them
+    float lo[kRanges], hi[kRanges];       // logits of marked bins lie within these
     uint32_t marks[(kBins + 31) / 32];
     uint32_t before[kBins + 1];           // tokens of the bins above
     uint32_t at[kBins + 1];               // ... that are on the list
-    unsigned long long sum[kBins + 1];    // their weights, in 2^-s of the anchor's (s: row_scale)
+    unsigned long long sum[kBins + 1];    // their weights, in units of sum_unit
 };
 struct Scratch {
     Part *part;                 // [rows][parts]
-    unsigned long long *bins;   // [rows][parts][kBins + 1]
+    unsigned long long *bins;   // [rows][parts][kStored]
     RowPlan *plan;              // [rows]
     uint64_t *list;             // [rows][kList]
-    int parts, per;             // parts of a row and tokens of one
+    int parts;                  // of a row
 };
 
-// Sums of a row's weights fit 62 bits.
-__device__ __forceinline__ double row_scale(uint32_t n) { return (double)(1ull << (62 - (32 - __builtin_clz(n)))); }
+// 1 / 2^-36 of the anchor's weight in a row's sums, which fit 62 bits.
+__device__ __forceinline__ double sum_unit(uint32_t n) { return (double)(1ull << (62 - (32 - __builtin_clz(n)))) / (double)(1ull << kMassBits); }
 
-constexpr int kPartThreads = 256;
+template <typename T>
+__device__ __forceinline__ float logit(const void *p, long long at) { return (float)((const T *)p)[at]; }
+
+constexpr int kPartThreads = 512;
+constexpr int kEach = kPart / kPartThreads;
 constexpr int kCopies = 4;  // of a part's bins: lanes that meet in a bin wait for each other
 
 // The i-th of a thread's tokens in a part.
 __device__ __forceinline__ int part_index(int i) { return i * kPartThreads + (int)threadIdx.x; }
 
-// A part's bins, and its largest token.
-template <int PER>
-__global__ __launch_bounds__(kPartThreads) void k_sample_parts(const m27q_sampling p, const Scratch sc) {
-    constexpr int N = PER / kPartThreads;
-    __shared__ unsigned long long bins[(kBins + 1) * kCopies];
-    __shared__ float top_s[kPartThreads / 64];
-    __shared__ int at_s[kPartThreads / 64];
-    const int row = blockIdx.y, first = (int)blockIdx.x * PER, count = min(PER, (int)p.n - first);
+// A part's logits, all on their way at once; NaN behind the end.
+template <typename T>
+__device__ __forceinline__ void load_part(const m27q_sampling &p, int row, int first, float (&v)[kEach]) {
+    const int count = min(kPart, (int)p.n - first);
     const long long base = (long long)row * p.stride + first;
-    float v[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = part_index(i) < count ? load1(p.logits, base + part_index(i), p.type) : __builtin_nanf("");
+    for (int i = 0; i < kEach; ++i) v[i] = logit<T>(p.logits, base + min(part_index(i), count - 1));
+    if (count < kPart)
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) v[i] = part_index(i) < count ? v[i] : __builtin_nanf("");
+}
+
+// A part's bins, and its largest token.
+template <typename T>
+__global__ __launch_bounds__(kPartThreads) void k_sample_parts(const m27q_sampling p, const Scratch sc) {
+    static_assert(kPartThreads == kBins + 1, "a thread a bin");
+    constexpr int W = kPartThreads / 64;
+    __shared__ unsigned long long bins[(kBins + 1) * kCopies];
+    __shared__ float top_s[W];
+    __shared__ int at_s[W];
+    const int row = blockIdx.y, first = (int)blockIdx.x * kPart;
+    float v[kEach];
+    load_part<T>(p, row, first, v);
     const Rule r = row_rule(p, row);
-    for (int i = threadIdx.x; i < (kBins + 1) * kCopies; i += kPartThreads) bins[i] = 0;
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) bins[i * (kBins + 1) + threadIdx.x] = 0;
     float top = -__builtin_inff();
 #pragma unroll
-    for (int i = 0; i < N; ++i) top = fmaxf(top, v[i]);
+    for (int i = 0; i < kEach; ++i) top = fmaxf(top, v[i]);
 #pragma unroll
     for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     if (lane == 0) top_s[wave] = top;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kPartThreads / 64; ++i) top = fmaxf(top, top_s[i]);
+    for (int i = 0; i < W; ++i) top = fmaxf(top, top_s[i]);
     int at = 0x7fffffff;
 #pragma unroll
-    for (int i = N - 1; i >= 0; --i) at = v[i] == top ? part_index(i) : at;
+    for (int i = kEach - 1; i >= 0; --i) at = v[i] == top ? part_index(i) : at;
 #pragma unroll
     for (int o = 32; o; o >>= 1) at = min(at, __shfl_xor(at, o));
     if (lane == 0) at_s[wave] = at;
 
-    const double c = kUnitsPerNat * r.inv_t;
-    const double b = __builtin_rint((double)top * c);
-    const double anchor = __builtin_isfinite(top) ? ceil(b * (1.0 / kUnit)) * kUnit : -__builtin_inf();
-    if (!r.greedy && __builtin_isfinite(top)) {
+    const bool any = !r.greedy && __builtin_isfinite(top);
+    const double b = __builtin_rint((double)top * (kUnitsPerNat * r.inv_t));
+    const Scale s = row_scale(r, any ? ceil(b * (1.0 / kUnit)) * kUnit : -__builtin_inf());
+    if (any) {
 #pragma unroll 4
-        for (int i = 0; i < N; ++i) {
-            double z = 0;
-            const int bin = bin_of(v[i], c, anchor, z);
+        for (int i = 0; i < kEach; ++i) {
+            double z;
+            const int bin = bin_of(v[i], s, z);
             if (bin < kBins)
                 atomicAdd(&bins[bin * kCopies + (lane & (kCopies - 1))], bin_mass(bin, z) + (1ull << kSumBits));
         }
@@ -287,16 +319,27 @@ __global__ __launch_bounds__(kPartThreads) void k_sample_parts(const m27q_sampli
     __syncthreads();
     const long long me = (long long)row * sc.parts + blockIdx.x;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < kPartThreads / 64; ++i) at = min(at, at_s[i]);
+        for (int i = 0; i < W; ++i) at = min(at, at_s[i]);
         const bool none = at == 0x7fffffff;  // NaN alone
-        sc.part[me] = {anchor, order_key(none ? __builtin_nanf("") : top, first + (none ? 0 : at))};
+        sc.part[me] = {s.anchor, order_key(none ? __builtin_nanf("") : top, first + (none ? 0 : at))};
     }
-    if (r.greedy) return;
-    for (int i = threadIdx.x; i <= kBins; i += kPartThreads) {
-        unsigned long long s = 0;
+    if (!any) return;  // its anchor says so
+    unsigned long long sum = 0;
 #pragma unroll
-        for (int j = 0; j < kCopies; ++j) s += bins[i * kCopies + j];
-        sc.bins[me * (kBins + 1) + i] = s;
+    for (int j = 0; j < kCopies; ++j) sum += bins[threadIdx.x * kCopies + j];
+    sc.bins[me * kStored + threadIdx.x] = sum;
+    // the octaves of the fine bins, 16 lanes each, for a row whose anchor lies so far above that they are one bin there
+    if (threadIdx.x < kFine) {
+        double mass = (double)(sum & ((1ull << kSumBits) - 1)) * bin_scale(threadIdx.x & (kUnit - 1));
+        uint32_t count = (uint32_t)(sum >> kSumBits);
+#pragma unroll
+        for (int o = kUnit / 2; o; o >>= 1) {
+            mass += __shfl_xor(mass, o);
+            count += __shfl_xor(count, o);
+        }
+        if ((threadIdx.x & (kUnit - 1)) == 0)
+            sc.bins[me * kStored + kBins + 1 + threadIdx.x / kUnit] =
+                (unsigned long long)__builtin_rint(mass) | (unsigned long long)count << kSumBits;
     }
 }
 
@@ -331,8 +374,8 @@ static_assert(kBins + 1 == kPlanThreads, "a thread a bin");
 __global__ __launch_bounds__(kPlanThreads) void k_sample_plan(const m27q_sampling p, const Scratch sc) {
     __shared__ unsigned long long lds[kPlanThreads / 64], best_s;
     __shared__ uint32_t lds32[kPlanThreads / 64];
-    __shared__ double anchors[kPlanThreads / 64], octave[kUnit];
-    __shared__ int found[8];
+    __shared__ double anchors[kPlanThreads / 64];
+    __shared__ int found[8], off_s[kPlanThreads];
     __shared__ unsigned long long sum[kBins + 2];
     const int row = blockIdx.x, J = threadIdx.x;
     const Part *part = sc.part + (long long)row * sc.parts;
@@ -340,7 +383,6 @@ __global__ __launch_bounds__(kPlanThreads) void k_sample_plan(const m27q_samplin
     RowPlan &out = sc.plan[row];
     if (J == 0) best_s = 0;
     if (J < 8) found[J] = kBins;
-    if (J < kUnit) octave[J] = exp2(-J * (1.0 / kUnit));
     double anchor = -__builtin_inf();
     unsigned long long best = 0;
     for (int i = J; i < sc.parts; i += kPlanThreads) {
@@ -368,43 +410,48 @@ __global__ __launch_bounds__(kPlanThreads) void k_sample_plan(const m27q_samplin
         return;
     }
 
-    // this thread's bin: whole numbers of weights where the parts' bins are of the same kind
+    // this thread's bin, from one stored sum of each part: the same bin there, or, where an octave here lies
+    // among the part's fine bins, their octave
     unsigned long long mass = 0;
     uint32_t count = 0;
-    double more = 0;
-    const unsigned long long *bins = sc.bins + (long long)row * sc.parts * (kBins + 1);
     constexpr unsigned long long kMask = (1ull << kSumBits) - 1;
-    for (int i = 0; i < sc.parts; ++i, bins += kBins + 1) {
-        const double off_d = anchor - part[i].anchor;
-        if (!(off_d < kFine + kUnit * kCoarse)) continue;
-        const int off = (int)off_d;
-        int from = J - off;  // the part's bin, as far as it is one
-        if (J >= kFine) {
-            const int d = kFine + kUnit * (J - kFine) - off;  // the octave's distance there
-            if (d < kFine) {
-                for (int k = 0; k < kUnit && d >= 0 && J < kBins; ++k) {
-                    const unsigned long long x = bins[d + k];
-                    count += (uint32_t)(x >> kSumBits);
-                    more += (double)(x & kMask) * octave[k];
-                }
-                continue;
-            }
-            from = kFine + (d - kFine) / kUnit;
+    constexpr int kSkip = 1 << 20;
+    for (int i0 = 0; i0 < sc.parts; i0 += kPlanThreads) {
+        const int parts = min(sc.parts - i0, kPlanThreads);
+        if (J < parts) {
+            const double off = anchor - part[i0 + J].anchor;
+            off_s[J] = off < kFine + kUnit * kCoarse ? (int)off : kSkip;
         }
-        if (from < 0 || J >= kBins) continue;
-        const unsigned long long x = bins[from];
-        count += (uint32_t)(x >> kSumBits);
-        mass += x & kMask;
+        __syncthreads();
+        const unsigned long long *bins = sc.bins + ((long long)row * sc.parts + i0) * kStored;
+        constexpr int AT = 16;  // on their way at a time
+        for (int i = 0; i < parts; i += AT) {
+            unsigned long long x[AT];
+            bool ok[AT];
+#pragma unroll
+            for (int k = 0; k < AT; ++k) {
+                const int j = min(i + k, parts - 1), off = off_s[j];
+                const int oct = kOctaves + J - kFine - off / kUnit;  // of a bin of an octave
+                const int from = J < kFine ? J - off : oct >= kOctaves ? kFine + oct - kOctaves : oct >= 0 ? kBins + 1 + oct : -1;
+                ok[k] = i + k < parts && off != kSkip && from >= 0 && J < kBins;
+                x[k] = bins[(long long)(ok[k] ? j : 0) * kStored + (ok[k] ? from : 0)];
+            }
+#pragma unroll
+            for (int k = 0; k < AT; ++k) {
+                count += ok[k] ? (uint32_t)(x[k] >> kSumBits) : 0u;
+                mass += ok[k] ? x[k] & kMask : 0ull;
+            }
+        }
+        __syncthreads();
     }
-    const double unit = row_scale(p.n) / (double)(1ull << kMassBits);
-    mass = (unsigned long long)__builtin_rint(((double)mass + more) * unit * bin_scale(J));
+    const double unit = sum_unit(p.n);
+    mass = (unsigned long long)__builtin_rint((double)mass * unit * bin_scale(J));
     unsigned long long total;
     uint32_t tokens;
     const unsigned long long above = scan_group(mass, lds, total);
     const uint32_t before = scan_group(count, lds32, tokens);
     sum[J] = above;
     if (J == kBins) sum[kBins + 1] = total;
-    __syncthreads();
 
     // the bin in which the running sum reaches a target, the last one that holds a token if none does
     auto bin_at = [&](int slot, double target) {
@@ -420,7 +467,8 @@ __global__ __launch_bounds__(kPlanThreads) void k_sample_plan(const m27q_samplin
     // the sum of the first top_k
     const double s_lo = (double)(k_cuts ? sum[kb] : total), s_hi = (double)(k_cuts ? sum[kb + 1] : total);
     double t_lo = s_lo, t_hi = s_hi;  // the sum of what is kept
-    int p0 = kBins, p1 = -1, mb = kBins;
+    int p0 = kBins, p1 = -1, m0 = kBins, m1 = -1;
+    unsigned long long min_p_sum = total;
     if (r.top_p < 1.0) {
         p0 = min(bin_at(1, r.top_p * s_lo), last);
         p1 = min(bin_at(2, r.top_p * s_hi), last);
@@ -428,17 +476,19 @@ __global__ __launch_bounds__(kPlanThreads) void k_sample_plan(const m27q_samplin
         t_hi = fmin(t_hi, (double)sum[p1 + 1]);
     }
     if (r.min_p > 0.0) {
-        const double c = kUnitsPerNat * r.inv_t;
         // the bin of the weight min_p, and its neighbours for what rounding does
-        const double y = (double)top * c + kUnit * log2(r.min_p), d = anchor - __builtin_rint(y);
-        mb = !(d < kFine + kUnit * kCoarse) ? kBins : d < 0 ? 0 : d < kFine ? (int)d : kFine + ((int)d - kFine) / kUnit;
-        t_lo = fmin(t_lo, (double)sum[max(mb - 1, 0)]);
-        t_hi = fmin(t_hi, (double)sum[min(mb + 2, kBins + 1)]);
+        const double y = (double)top * (kUnitsPerNat * r.inv_t) + kUnit * log2(r.min_p), d = anchor - __builtin_rint(y);
+        if (d < kFine + kUnit * kCoarse) {
+            const int m = d < 0 ? 0 : d < kFine ? (int)d : kFine + ((int)d - kFine) / kUnit;
+            m0 = max(m - 1, 0);
+            m1 = min(m + 1, kBins - 1);
+            min_p_sum = sum[m1 + 1];
+            t_lo = fmin(t_lo, (double)sum[m0]);
+            t_hi = fmin(t_hi, (double)min_p_sum);
+        }
     }
-    // the first token alone is always kept
     const int q0 = min(bin_at(3, r.u * t_lo), last), q1 = min(bin_at(4, r.u * t_hi), last);
-    const bool mark = count && (J == kb || (J >= p0 && J <= p1) || (mb < kBins && J >= mb - 1 && J <= mb + 1) ||
-                                (J >= q0 && J <= q1) || before == 0);
+    const bool mark = count && (J == kb || (J >= p0 && J <= p1) || (J >= m0 && J <= m1) || (J >= q0 && J <= q1));
     uint32_t listed;
     const uint32_t at = scan_group(mark ? count : 0u, lds32, listed);
     out.sum[J] = above;
@@ -446,38 +496,56 @@ __global__ __launch_bounds__(kPlanThreads) void k_sample_plan(const m27q_samplin
     out.at[J] = at;
     const unsigned long long m = __ballot(mark);
     if ((J & 31) == 0) out.marks[J / 32] = (uint32_t)(m >> (J & 32));
+    if (J < kRanges) {
+        // logits of bins b0 .. b1, and a little more than those
+        const int b0 = J == 0 ? kb : J == 1 ? p0 : J == 2 ? m0 : q0, b1 = J == 0 ? (k_cuts ? kb : -1) : J == 1 ? p1 : J == 2 ? m1 : q1;
+        const double c = kUnitsPerNat * r.inv_t, up = anchor - bin_distance(b0) + 1;
+        const double down = anchor - bin_distance(b1) - (b1 < kFine ? 1 : kUnit);
+        const bool none = b1 < b0, all = !(c > 1e-30);
+        const double eps = 0x1p-20;
+        out.lo[J] = none ? __builtin_inff() : all ? -__builtin_inff() : (float)(down / c - fabs(down / c) * eps);
+        out.hi[J] = none ? -__builtin_inff() : all ? __builtin_inff() : (float)(up / c + fabs(up / c) * eps);
+    }
     if (J == 0) {
         out.anchor = anchor;
         out.best = best;
-        out.min_p_sum = mb < kBins ? sum[min(mb + 2, kBins)] : total;
+        out.min_p_sum = min_p_sum;
         out.state = listed <= (uint32_t)kList ? 1 : 2;
         out.listed = 0;  // counted by the next launch
     }
 }
 
 // The tokens of marked bins, in no order.
-template <int PER>
+template <typename T>
 __global__ __launch_bounds__(kPartThreads) void k_sample_list(const m27q_sampling p, const Scratch sc) {
-    constexpr int N = PER / kPartThreads;
     constexpr uint32_t M = 2048;  // (a part's tokens past them go by themselves)
     __shared__ uint64_t keys[M];
-    __shared__ uint32_t count_s, to_s;
-    const int row = blockIdx.y, first = (int)blockIdx.x * PER, count = min(PER, (int)p.n - first);
+    __shared__ uint32_t count_s, to_s, marks[(kBins + 31) / 32];
+    const int row = blockIdx.y, first = (int)blockIdx.x * kPart;
     RowPlan &plan = sc.plan[row];
+    float v[kEach];
+    load_part<T>(p, row, first, v);
     if (plan.state != 1) return;
-    const long long base = (long long)row * p.stride + first;
-    float v[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = part_index(i) < count ? load1(p.logits, base + part_index(i), p.type) : __builtin_nanf("");
     if (threadIdx.x == 0) count_s = 0;
+    if (threadIdx.x < (kBins + 31) / 32) marks[threadIdx.x] = plan.marks[threadIdx.x];
     __syncthreads();
     uint64_t *const list = sc.list + (long long)row * kList;
-    const double c = kUnitsPerNat * row_rule(p, row).inv_t, anchor = plan.anchor;
-#pragma unroll 4
-    for (int i = 0; i < N; ++i) {
+    const Scale s = row_scale(row_rule(p, row), plan.anchor);
+    float lo[kRanges], hi[kRanges];
+#pragma unroll
+    for (int j = 0; j < kRanges; ++j) {
+        lo[j] = plan.lo[j];
+        hi[j] = plan.hi[j];
+    }
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        bool near = false;
+#pragma unroll
+        for (int j = 0; j < kRanges; ++j) near |= v[i] >= lo[j] && v[i] <= hi[j];
+        if (!near) continue;
         double z;
-        const int bin = bin_of(v[i], c, anchor, z);
-        if (bin < kBins && (plan.marks[bin / 32] >> (bin & 31) & 1)) {
+        const int bin = bin_of(v[i], s, z);
+        if (bin < kBins && (marks[bin / 32] >> (bin & 31) & 1)) {
             const uint64_t key = order_key(v[i], first + part_index(i));
             const uint32_t at = atomicAdd(&count_s, 1u);
             if (at < M) {
@@ -498,18 +566,143 @@ __global__ __launch_bounds__(kPartThreads) void k_sample_list(const m27q_samplin
         if (to + i < (uint32_t)kList) list[to + i] = keys[i];
 }
 
-// A row's list in order, the running sums of its tokens, and the borders among them.
-__global__ __launch_bounds__(kRowThreads) void k_sample_pick(const m27q_sampling p, const Scratch sc) {
-    __shared__ uint64_t keys[kList];
-    __shared__ union {
-        unsigned long long scan[kRowThreads / 64];
+// Keys in descending order, E of each thread side by side: a bitonic network whose steps stay in a
+// thread's registers, or in a wave, as long as they can.
+template <int E>
+__device__ __forceinline__ void sort_keys(uint64_t (&x)[E], uint64_t *lds) {
+    const int tid = threadIdx.x;
+    for (int k = 2; k <= E * kRowThreads; k *= 2)
+        for (int j = k / 2; j > 0; j /= 2) {
+            if (j < E) {
+#pragma unroll
+                for (int m = E / 2; m > 0; m /= 2) {
+                    if (j != m) continue;
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        if (e & m) continue;
+                        const bool down = ((tid * E + e) & k) == 0;
+                        const uint64_t a = x[e], b = x[e + m];
+                        const bool swap = (a < b) == down;
+                        x[e] = swap ? b : a;
+                        x[e + m] = swap ? a : b;
+                    }
+                }
+                continue;
+            }
+            const int t = j / E;  // the other thread's distance
+            const bool take_max = ((tid & t) == 0) == ((tid * E & k) == 0);
+            uint64_t y[E];
+            if (t < 64) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) y[e] = (uint64_t)__shfl_xor((unsigned long long)x[e], t);
+            } else {
+                __syncthreads();
+#pragma unroll
+                for (int e = 0; e < E; ++e) lds[e * kRowThreads + tid] = x[e];
+                __syncthreads();
+#pragma unroll
+                for (int e = 0; e < E; ++e) y[e] = lds[e * kRowThreads + (tid ^ t)];
+            }
+#pragma unroll
+            for (int e = 0; e < E; ++e) x[e] = (x[e] > y[e]) == take_max ? x[e] : y[e];
+        }
+}
+
+struct PickShared {
+    union {
+        uint64_t keys[kList];
         WholeRow whole;
-    } s;
-    __shared__ unsigned long long start[kBins + 1];  // the list's running sum in front of a bin
+    };
+    unsigned long long scan[kRowThreads / 64];
+    unsigned long long start[kBins + 1];  // the list's running sum in front of a bin
     // sums down to the first token, the top_k-th, the one that reaches top_p and the last one that min_p leaves
-    __shared__ unsigned long long first_s, among_s, top_p_s, min_p_s;
-    __shared__ int pick_s;
-    const int row = blockIdx.x, tid = threadIdx.x;
+    unsigned long long among, top_p, min_p;
+    int pick;
+};
+
+// A row's list in order, the running sums of its tokens, and the borders among them.
+template <int E>
+__device__ __forceinline__ void pick_from_list(const m27q_sampling &p, const Scratch &sc, const RowPlan &plan, const Rule &r, int n,
+                                               PickShared &s) {
+    const int row = blockIdx.x, tid = threadIdx.x, i0 = tid * E;
+    uint64_t key[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const int i = e * kRowThreads + tid;
+        key[e] = i < n ? sc.list[(long long)row * kList + i] : 0;
+    }
+    sort_keys<E>(key, s.keys);
+
+    // the sums of the row down to each token of the list.  In front of a bin, and at its end, they are the plan's.
+    const Scale scale = row_scale(r, plan.anchor);
+    const double unit = sum_unit(p.n);
+    unsigned long long own[E], sum = 0;
+    int bin[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        own[e] = 0;
+        bin[e] = 0;
+        if (i0 + e < n) {
+            double z = 0;
+            bin[e] = bin_of(key_value(key[e]), scale, z);
+            own[e] = bin_mass(bin[e], z);
+        }
+        sum += own[e];
+    }
+    uint32_t at[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) at[e] = plan.at[bin[e]];
+    unsigned long long all, run = scan_group(sum, s.scan, all);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        if (i0 + e < n && (uint32_t)(i0 + e) == at[e]) s.start[bin[e]] = run;
+        run += own[e];
+    }
+    run -= sum;
+    __syncthreads();
+    const float top = key_value(plan.best);
+    unsigned long long down[E];
+    int rank[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const uint32_t i = (uint32_t)(i0 + e);
+        const unsigned long long lo = plan.sum[bin[e]], hi = plan.sum[bin[e] + 1], in = run - s.start[bin[e]];
+        const double f = unit * bin_scale(bin[e]);
+        const auto to = [&](unsigned long long x) { return min(lo + (unsigned long long)__builtin_rint((double)x * f), hi); };
+        down[e] = i + 1 == plan.at[bin[e] + 1] ? hi : to(in + own[e]);
+        rank[e] = i < (uint32_t)n ? (int)(plan.before[bin[e]] + i - at[e]) : 0x7fffffff;
+        run += own[e];
+        if (rank[e] == r.k - 1) s.among = down[e];
+        if (r.min_p > 0.0 && i < (uint32_t)n && exp(((double)key_value(key[e]) - (double)top) * r.inv_t) < r.min_p)
+            atomicMin(&s.min_p, to(in));
+    }
+    __syncthreads();
+    const double reach = r.top_p * (double)s.among;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+        if (r.top_p < 1.0 && i0 + e < n && (double)down[e] >= reach) atomicMin(&s.top_p, down[e]);
+    __syncthreads();
+    // the first token is kept whatever the rest says
+    double z = 0;
+    const int b0 = bin_of(top, scale, z);
+    const unsigned long long first = min((unsigned long long)__builtin_rint((double)bin_mass(b0, z) * unit * bin_scale(b0)), plan.sum[b0 + 1]);
+    const unsigned long long total = max(first, min(s.among, min(s.top_p, s.min_p)));
+    const double target = r.u * (double)total;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+        if (i0 + e < n && (double)down[e] >= target) atomicMin(&s.pick, rank[e]);
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+        if (i0 + e < n && rank[e] == s.pick) {
+            p.token[row] = key_index(key[e]);
+            if (p.prob) p.prob[row] = (float)((double)own[e] * unit * bin_scale(bin[e]) / (double)total);
+        }
+}
+
+__global__ __launch_bounds__(kRowThreads) void k_sample_pick(const m27q_sampling p, const Scratch sc) {
+    __shared__ PickShared s;
+    const int row = blockIdx.x;
     const RowPlan &plan = sc.plan[row];
     const int state = plan.state;
     if (state == 0) return;
@@ -518,124 +711,35 @@ __global__ __launch_bounds__(kRowThreads) void k_sample_pick(const m27q_sampling
         sample_whole_row(p, row, r, plan.best, s.whole);
         return;
     }
+    if (threadIdx.x == 0) {
+        s.among = plan.sum[kBins];  // unless the top_k-th is on the list
+        s.top_p = ~0ull;
+        s.min_p = plan.min_p_sum;
+        s.pick = 0x7fffffff;
+    }
     const int n = (int)min(plan.listed, (uint32_t)kList);
-    int size = 64;
-    while (size < n) size *= 2;
-    for (int i = tid; i < size; i += kRowThreads) keys[i] = i < n ? sc.list[(long long)row * kList + i] : 0;
-    if (tid == 0) {
-        first_s = 0;
-        among_s = plan.sum[kBins];  // unless the top_k-th is on the list
-        top_p_s = ~0ull;
-        min_p_s = plan.min_p_sum;
-        pick_s = 0x7fffffff;
-    }
     __syncthreads();
-    for (int k = 2; k <= size; k *= 2)
-        for (int j = k / 2; j > 0; j /= 2) {
-            for (int t = tid; t < size / 2; t += kRowThreads) {
-                const int i = 2 * t - (t & (j - 1)), l = i + j;
-                const uint64_t a = keys[i], b = keys[l];
-                if ((a < b) == ((i & k) == 0)) {
-                    keys[i] = b;
-                    keys[l] = a;
-                }
-            }
-            __syncthreads();
-        }
-
-    // each thread a run of the list: the sums of the row down to each of its tokens.  In front of a
-    // bin, and at its end, they are the plan's.
-    constexpr int E = kList / kRowThreads;
-    const int each = (n + kRowThreads - 1) / kRowThreads, i0 = min(tid * each, n), i1 = min(i0 + each, n);
-    const double c = kUnitsPerNat * r.inv_t, anchor = plan.anchor;
-    const double unit = row_scale(p.n) / (double)(1ull << kMassBits);
-    unsigned long long own[E], sum = 0;
-    int bin[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        own[e] = 0;
-        bin[e] = 0;
-        if (i0 + e < i1) {
-            double z = 0;
-            bin[e] = bin_of(key_value(keys[i0 + e]), c, anchor, z);
-            own[e] = bin_mass(bin[e], z);
-        }
-        sum += own[e];
-    }
-    unsigned long long all, run = scan_group(sum, s.scan, all);
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        if (i0 + e < i1 && (uint32_t)(i0 + e) == plan.at[bin[e]]) start[bin[e]] = run;
-        run += own[e];
-    }
-    run -= sum;
-    __syncthreads();
-    unsigned long long below[E], down[E];  // without and with the token
-    int rank[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const uint32_t i = (uint32_t)(i0 + e), at = plan.at[bin[e]];
-        const unsigned long long lo = plan.sum[bin[e]], hi = plan.sum[bin[e] + 1], in = run - start[bin[e]];
-        const double f = unit * bin_scale(bin[e]);
-        below[e] = min(lo + (unsigned long long)__builtin_rint((double)in * f), hi);
-        down[e] = i + 1 == plan.at[bin[e] + 1] ? hi : min(lo + (unsigned long long)__builtin_rint((double)(in + own[e]) * f), hi);
-        rank[e] = (int)(plan.before[bin[e]] + i - at);
-        run += own[e];
-    }
-    const float top = key_value(plan.best);
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        if (i0 + e >= i1) continue;
-        if (rank[e] == 0) first_s = down[e];
-        if (rank[e] == r.k - 1) among_s = down[e];
-        if (r.min_p > 0.0 && exp(((double)key_value(keys[i0 + e]) - (double)top) * r.inv_t) < r.min_p) atomicMin(&min_p_s, below[e]);
-    }
-    __syncthreads();
-    const unsigned long long among = among_s;
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-        if (i0 + e < i1 && r.top_p < 1.0 && (double)down[e] >= r.top_p * (double)among) atomicMin(&top_p_s, down[e]);
-    __syncthreads();
-    const unsigned long long total = max(first_s, min(among, min(top_p_s, min_p_s)));
-    const double target = r.u * (double)total;
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-        if (i0 + e < i1 && (double)down[e] >= target) atomicMin(&pick_s, rank[e]);
-    __syncthreads();
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-        if (i0 + e < i1 && rank[e] == pick_s) {
-            p.token[row] = key_index(keys[i0 + e]);
-            if (p.prob) p.prob[row] = (float)((double)own[e] * unit * bin_scale(bin[e]) / (double)total);
-        }
-}
-
-}  // namespace
-
-namespace {
-
-// Tokens of a part: enough parts to fill the card, and no more than it takes.
-int part_tokens(uint32_t rows, uint32_t n) {
-    int per = 2048;
-    while (per < kPart && (long long)rows * ((n + per - 1) / per) > 1024) per *= 2;
-    return per;
+    if (n <= kRowThreads) pick_from_list<1>(p, sc, plan, r, n, s);
+    else if (n <= 2 * kRowThreads) pick_from_list<2>(p, sc, plan, r, n, s);
+    else if (n <= 4 * kRowThreads) pick_from_list<4>(p, sc, plan, r, n, s);
+    else pick_from_list<8>(p, sc, plan, r, n, s);
 }
 
 struct Sizes {
-    int per, parts;
+    int parts;
     size_t part, bins, plan, list;
     Sizes(uint32_t rows, uint32_t n)
-        : per(part_tokens(rows, n)), parts((int)((n + per - 1) / per)), part(align((size_t)rows * parts * sizeof(Part))),
-          bins((size_t)rows * parts * (kBins + 1) * 8), plan(align((size_t)rows * sizeof(RowPlan))), list((size_t)rows * kList * 8) {}
+        : parts((int)((n + kPart - 1) / kPart)), part(align((size_t)rows * parts * sizeof(Part))),
+          bins((size_t)rows * parts * kStored * 8), plan(align((size_t)rows * sizeof(RowPlan))), list((size_t)rows * kList * 8) {}
     static size_t align(size_t v) { return (v + 255) & ~(size_t)255; }
 };
 
-template <int PER>
+template <typename T>
 hipError_t launch_t(const m27q_sampling &p, const Scratch &sc, hipStream_t s) {
     const dim3 parts(sc.parts, p.rows);
-    hipLaunchKernelGGL((k_sample_parts<PER>), parts, dim3(kPartThreads), 0, s, p, sc);
+    hipLaunchKernelGGL((k_sample_parts<T>), parts, dim3(kPartThreads), 0, s, p, sc);
     hipLaunchKernelGGL(k_sample_plan, dim3(p.rows), dim3(kPlanThreads), 0, s, p, sc);
-    hipLaunchKernelGGL((k_sample_list<PER>), parts, dim3(kPartThreads), 0, s, p, sc);
+    hipLaunchKernelGGL((k_sample_list<T>), parts, dim3(kPartThreads), 0, s, p, sc);
     hipLaunchKernelGGL(k_sample_pick, dim3(p.rows), dim3(kRowThreads), 0, s, p, sc);
     return hipGetLastError();
 }
@@ -656,9 +760,8 @@ hipError_t launch_sample_rows(const m27q_sampling &p, void *scratch, hipStream_t
     sc.plan = (RowPlan *)(at += z.bins);
     sc.list = (uint64_t *)(at + z.plan);
     sc.parts = z.parts;
-    sc.per = z.per;
-    if (z.per == 2048) return launch_t<2048>(p, sc, s);
-    return z.per == 4096 ? launch_t<4096>(p, sc, s) : launch_t<kPart>(p, sc, s);
+    if (p.type == M27Q_TYPE_F32) return launch_t<float>(p, sc, s);
+    return p.type == M27Q_TYPE_F16 ? launch_t<_Float16>(p, sc, s) : launch_t<__bf16>(p, sc, s);
 }
 
 }  // namespace m27q
