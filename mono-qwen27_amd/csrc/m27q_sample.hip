@@ -168,54 +168,64 @@ constexpr int kMassBits = 36, kSumBits = 50;
 constexpr int kPart = 8192;             // tokens of a part: counts of 14 bits above sums of 50
 constexpr double kUnitsPerNat = 16 * 1.4426950408889634074;
 
-// 2^(z / 16): the Taylor polynomial of degree 6, whose next term is below 3e-13 for |z| <= 1.6.
-__device__ __forceinline__ double exp2_unit(double z) {
-    constexpr double a = 0.69314718055994530942 / 16;
-    double p = a * a * a * a * a * a / 720;
-    p = __builtin_fma(p, z, a * a * a * a * a / 120);
-    p = __builtin_fma(p, z, a * a * a * a / 24);
-    p = __builtin_fma(p, z, a * a * a / 6);
-    p = __builtin_fma(p, z, a * a / 2);
-    p = __builtin_fma(p, z, a);
-    return __builtin_fma(p, z, 1.0);
-}
+// Weights of places within a bin: 2^(z / 16) by its Taylor polynomial (degree 5 for |z| <= 1 / 2: the next
+// term is below 2^-42), times 2^36 and, in a bin of an octave, 2^(-k / 16) for a place k units down it.
+// The constants are kept in registers: scalar ones, but for what a product's or sum's second
+// constant has to be.
+struct Exp2Unit {
+    double c[6], add;
+    const double *octave;  // 2^(36 - k / 16), in LDS
+    __device__ __forceinline__ Exp2Unit(const double *octave) : octave(octave) {
+        constexpr double a = 0.69314718055994530942 / 16;
+        c[0] = 1.0;
+        c[1] = a;
+        c[2] = a * a / 2;
+        c[3] = a * a * a / 6;
+        c[4] = a * a * a * a / 24;
+        c[5] = a * a * a * a * a / 120;
+        add = 0x1p52;
+        asm("" : "+s"(c[1]), "+s"(c[2]), "+s"(c[3]), "+v"(c[4]), "+s"(c[5]), "+v"(add));
+    }
+    // threads 0 .. 15
+    static __device__ __forceinline__ double factor(int k) { return exp2(kMassBits - k * (1.0 / kUnit)); }
+    // `count` above the bits of a sum.  Rounded by an addition that leaves the whole number in the low
+    // bits; 2^52's exponent off and the count on in one subtraction.
+    __device__ __forceinline__ unsigned long long mass(double z, int k, unsigned count) const {
+        double p = c[5];
+#pragma unroll
+        for (int i = 4; i >= 0; --i) p = __builtin_fma(p, z, c[i]);
+        const unsigned long long m = __builtin_bit_cast(unsigned long long, __builtin_fma(p, octave[k], add));
+        return (unsigned long long)((uint32_t)(m >> 32) - (0x43300000u - (count << (kSumBits - 32)))) << 32 | (uint32_t)m;
+    }
+};
 
 // What a row's logits are placed by.
 struct Scale {
     double c;       // units of a logit
     double anchor;
-    bool wide;      // y passes 2^18: its product is taken with its remainder
+    int wide;       // distances from the anchor pass 32 bits, or T is infinite
     double near;    // 1; 0 where a step of a logit is thousands of octaves and only equal ones have a weight
 };
 __device__ __forceinline__ Scale row_scale(const Rule &r, double anchor) {
     const double far = fabs(anchor) + kFine + kUnit * kCoarse;
-    return {kUnitsPerNat * r.inv_t, anchor, far > 0x1p18, far > 0x1p40 ? 0.0 : 1.0};
+    const double c = kUnitsPerNat * r.inv_t;
+    return {c, anchor, __builtin_amdgcn_readfirstlane(far > 0x1p30 || !(c > 0.0)), far > 0x1p40 ? 0.0 : 1.0};
 }
 
-// The bin of a logit; z: its weight is 2^(z / 16) (a bin of an octave: 2^z) of that at the bin's upper
-// end.  The error of z is below 2^-35.
-__device__ __forceinline__ int bin_of(float l, const Scale &s, double &z) {
-    const double x = (double)l, hi = x * s.c, b = __builtin_rint(hi), d = s.anchor - b;
-    double r = hi - b;
-    if (s.wide) r += __builtin_fma(x, s.c, -hi);
-    if (!(d < kFine + kUnit * kCoarse)) return kBins;  // (-infinity and NaN too)
-    z = r * s.near;
+// The bin of a logit, and its place in it: k units down a bin of an octave (0 otherwise), z from there (up is
+// positive), from the product's remainder behind the whole units, which loses nothing to their number.
+struct Place {
+    int bin, k;
+    double z;
+};
+__device__ __forceinline__ Place place_of(float l, const Scale &s) {
+    const double x = (double)l, b = __builtin_rint(x * s.c), d = s.anchor - b;
+    Place p{kBins, 0, __builtin_fma(x, s.c, -b) * s.near};
+    if (!(d < kFine + kUnit * kCoarse)) return p;  // (-infinity and NaN too)
     const int i = (int)d;
-    if (i < kFine) return i;
-    const int o = (i - kFine) / kUnit;
-    z = (z - (double)((i - kFine) & (kUnit - 1))) * (1.0 / kUnit);
-    return kFine + o;
-}
-// In 2^-36, rounded by an addition that leaves the whole number in the low bits.
-__device__ __forceinline__ unsigned long long bin_mass(int bin, double z) {
-    double p = exp2_unit(z);
-    if (bin >= kFine) {
-        p *= p;
-        p *= p;
-        p *= p;
-        p *= p;
-    }
-    return __builtin_bit_cast(unsigned long long, __builtin_fma(p, (double)(1ull << kMassBits), 0x1p52)) & ((1ull << kSumBits) - 1);
+    p.bin = i < kFine ? i : kFine + (i - kFine) / kUnit;
+    p.k = i < kFine ? 0 : i & (kUnit - 1);
+    return p;
 }
 // The weight at a bin's upper end, of that at the anchor.
 __device__ __forceinline__ int bin_distance(int bin) { return bin < kFine ? bin : kFine + kUnit * (bin - kFine); }
@@ -239,6 +249,7 @@ struct RowPlan {
     uint32_t before[kBins + 1];           // tokens of the bins above
     uint32_t at[kBins + 1];               // ... that are on the list
     unsigned long long sum[kBins + 1];    // their weights, in units of sum_unit
+    double unit[kBins + 1];               // those units in 2^-36 of the weight at the bin's upper end
 };
 struct Scratch {
     Part *part;                 // [rows][parts]
@@ -261,7 +272,7 @@ constexpr int kCopies = 4;  // of a part's bins: lanes that meet in a bin wait f
 // The i-th of a thread's tokens in a part.
 __device__ __forceinline__ int part_index(int i) { return i * kPartThreads + (int)threadIdx.x; }
 
-// A part's logits, all on their way at once; NaN behind the end.
+// A part's logits, all on their way at once; -infinity behind the end.
 template <typename T>
 __device__ __forceinline__ void load_part(const m27q_sampling &p, int row, int first, float (&v)[kEach]) {
     const int count = min(kPart, (int)p.n - first);
@@ -270,7 +281,7 @@ __device__ __forceinline__ void load_part(const m27q_sampling &p, int row, int f
     for (int i = 0; i < kEach; ++i) v[i] = logit<T>(p.logits, base + min(part_index(i), count - 1));
     if (count < kPart)
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) v[i] = part_index(i) < count ? v[i] : __builtin_nanf("");
+        for (int i = 0; i < kEach; ++i) v[i] = part_index(i) < count ? v[i] : -__builtin_inff();
 }
 
 // A part's bins, and its largest token.
@@ -279,6 +290,7 @@ __global__ __launch_bounds__(kPartThreads) void k_sample_parts(const m27q_sampli
     static_assert(kPartThreads == kBins + 1, "a thread a bin");
     constexpr int W = kPartThreads / 64;
     __shared__ unsigned long long bins[(kBins + 1) * kCopies];
+    __shared__ double octave[kUnit];
     __shared__ float top_s[W];
     __shared__ int at_s[W];
     const int row = blockIdx.y, first = (int)blockIdx.x * kPart;
@@ -287,6 +299,7 @@ __global__ __launch_bounds__(kPartThreads) void k_sample_parts(const m27q_sampli
     const Rule r = row_rule(p, row);
 #pragma unroll
     for (int i = 0; i < kCopies; ++i) bins[i * (kBins + 1) + threadIdx.x] = 0;
+    if (threadIdx.x < kUnit) octave[threadIdx.x] = Exp2Unit::factor(threadIdx.x);
     float top = -__builtin_inff();
 #pragma unroll
     for (int i = 0; i < kEach; ++i) top = fmaxf(top, v[i]);
@@ -308,19 +321,45 @@ __global__ __launch_bounds__(kPartThreads) void k_sample_parts(const m27q_sampli
     const double b = __builtin_rint((double)top * (kUnitsPerNat * r.inv_t));
     const Scale s = row_scale(r, any ? ceil(b * (1.0 / kUnit)) * kUnit : -__builtin_inf());
     if (any) {
-#pragma unroll 4
-        for (int i = 0; i < kEach; ++i) {
-            double z;
-            const int bin = bin_of(v[i], s, z);
-            if (bin < kBins)
-                atomicAdd(&bins[bin * kCopies + (lane & (kCopies - 1))], bin_mass(bin, z) + (1ull << kSumBits));
+        const Exp2Unit x(octave);
+        const int copy = lane & (kCopies - 1);
+        bool odd = false;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) odd |= v[i] != v[i];
+        if (s.wide || __any(odd)) {
+#pragma unroll 1
+            for (int i = 0; i < kEach; ++i) {
+                const Place a = place_of(v[i], s);
+                if (a.bin < kBins) atomicAdd(&bins[a.bin * kCopies + copy], x.mass(a.z, a.k, 1));
+            }
+        } else {  // the same, in whole numbers of 32 bits and several tokens' chains beside each other
+            const int anchor = (int)s.anchor;
+            constexpr int AT = 4;
+#pragma unroll
+            for (int i0 = 0; i0 < kEach; i0 += AT) {
+                unsigned long long m[AT];
+                uint32_t d[AT], bin[AT];
+#pragma unroll
+                for (int j = 0; j < AT; ++j) {
+                    const double l = (double)v[i0 + j], b = __builtin_rint(l * s.c);
+                    d[j] = (uint32_t)(anchor - (int)b);  // (what is too far below saturates, or wraps above all bins)
+                    const bool fine = d[j] < (uint32_t)kFine;
+                    bin[j] = fine ? d[j] : (d[j] >> 4) + (kFine - kFine / kUnit);
+                    m[j] = x.mass(__builtin_fma(l, s.c, -b), fine ? 0 : d[j] & (kUnit - 1), 1);
+                }
+#pragma unroll
+                for (int j = 0; j < AT; ++j) asm volatile("" : "+v"(m[j]), "+v"(bin[j]));  // computed by now, for all lanes
+#pragma unroll
+                for (int j = 0; j < AT; ++j)
+                    if (d[j] < (uint32_t)(kFine + kUnit * kCoarse)) atomicAdd(&bins[bin[j] * kCopies + copy], m[j]);
+            }
         }
     }
     __syncthreads();
     const long long me = (long long)row * sc.parts + blockIdx.x;
     if (threadIdx.x == 0) {
         for (int i = 0; i < W; ++i) at = min(at, at_s[i]);
-        const bool none = at == 0x7fffffff;  // NaN alone
+        const bool none = at >= (int)p.n - first;  // NaN alone
         sc.part[me] = {s.anchor, order_key(none ? __builtin_nanf("") : top, first + (none ? 0 : at))};
     }
     if (!any) return;  // its anchor says so
@@ -343,25 +382,45 @@ __global__ __launch_bounds__(kPartThreads) void k_sample_parts(const m27q_sampli
     }
 }
 
-// The running sums of a workgroup's values, one a thread: before this thread's, and all of them.
+// Lanes' values moved up by DPP within a wave, 0 where there is none.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t moved(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ unsigned long long moved(unsigned long long v) {
+    return (unsigned long long)moved<CTRL, ROWS>((uint32_t)(v >> 32)) << 32 | moved<CTRL, ROWS>((uint32_t)v);
+}
+// The running sum over a wave's lanes, the lane's own included: 1, 2, 4, 8 lanes up within rows of 16,
+// then a row's last to the next row, and the lower half's last to the upper half.
 template <typename T>
+__device__ __forceinline__ T scan_wave(T v) {
+    v += moved<0x111, 0xf>(v);
+    v += moved<0x112, 0xf>(v);
+    v += moved<0x114, 0xf>(v);
+    v += moved<0x118, 0xf>(v);
+    v += moved<0x142, 0xa>(v);
+    v += moved<0x143, 0xc>(v);
+    return v;
+}
+
+// The running sums of a workgroup's values, one a thread: before this thread's, and all of them.
+// `lds` is used once between barriers of the caller's.
+template <int THREADS, typename T>
 __device__ __forceinline__ T scan_group(T v, T *lds, T &all) {
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, waves = (int)blockDim.x >> 6;
-    T run = v;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const T x = __shfl_up(run, o);
-        run += lane >= o ? x : T(0);
-    }
-    if (lane == 63) lds[wave] = run;
+    constexpr int W = THREADS / 64;
+    const int wave = threadIdx.x >> 6;
+    const T run = scan_wave(v);
+    if ((threadIdx.x & 63) == 63) lds[wave] = run;
     __syncthreads();
     T before = 0;
     all = 0;
-    for (int i = 0; i < waves; ++i) {
-        before += i < wave ? lds[i] : T(0);
-        all += lds[i];
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+        const T x = lds[i];
+        before += i < wave ? x : T(0);
+        all += x;
     }
-    __syncthreads();
     return before + run - v;
 }
 
@@ -373,7 +432,7 @@ static_assert(kBins + 1 == kPlanThreads, "a thread a bin");
 // leaves a range of bins.
 __global__ __launch_bounds__(kPlanThreads) void k_sample_plan(const m27q_sampling p, const Scratch sc) {
     __shared__ unsigned long long lds[kPlanThreads / 64], best_s;
-    __shared__ uint32_t lds32[kPlanThreads / 64];
+    __shared__ uint32_t lds32[kPlanThreads / 64], lds_at[kPlanThreads / 64];
     __shared__ double anchors[kPlanThreads / 64];
     __shared__ int found[8], off_s[kPlanThreads];
     __shared__ unsigned long long sum[kBins + 2];
@@ -424,7 +483,7 @@ __global__ __launch_bounds__(kPlanThreads) void k_sample_plan(const m27q_samplin
         }
         __syncthreads();
         const unsigned long long *bins = sc.bins + ((long long)row * sc.parts + i0) * kStored;
-        constexpr int AT = 16;  // on their way at a time
+        constexpr int AT = 32;  // on their way at a time
         for (int i = 0; i < parts; i += AT) {
             unsigned long long x[AT];
             bool ok[AT];
@@ -444,12 +503,12 @@ __global__ __launch_bounds__(kPlanThreads) void k_sample_plan(const m27q_samplin
         }
         __syncthreads();
     }
-    const double unit = sum_unit(p.n);
-    mass = (unsigned long long)__builtin_rint((double)mass * unit * bin_scale(J));
+    const double unit = sum_unit(p.n) * bin_scale(J);
+    mass = (unsigned long long)__builtin_rint((double)mass * unit);
     unsigned long long total;
     uint32_t tokens;
-    const unsigned long long above = scan_group(mass, lds, total);
-    const uint32_t before = scan_group(count, lds32, tokens);
+    const unsigned long long above = scan_group<kPlanThreads>(mass, lds, total);
+    const uint32_t before = scan_group<kPlanThreads>(count, lds32, tokens);
     sum[J] = above;
     if (J == kBins) sum[kBins + 1] = total;
 
@@ -490,8 +549,9 @@ __global__ __launch_bounds__(kPlanThreads) void k_sample_plan(const m27q_samplin
     const int q0 = min(bin_at(3, r.u * t_lo), last), q1 = min(bin_at(4, r.u * t_hi), last);
     const bool mark = count && (J == kb || (J >= p0 && J <= p1) || (J >= m0 && J <= m1) || (J >= q0 && J <= q1));
     uint32_t listed;
-    const uint32_t at = scan_group(mark ? count : 0u, lds32, listed);
+    const uint32_t at = scan_group<kPlanThreads>(mark ? count : 0u, lds_at, listed);
     out.sum[J] = above;
+    out.unit[J] = unit;
     out.before[J] = before;
     out.at[J] = at;
     const unsigned long long m = __ballot(mark);
@@ -515,127 +575,164 @@ __global__ __launch_bounds__(kPlanThreads) void k_sample_plan(const m27q_samplin
     }
 }
 
-// The tokens of marked bins, in no order.
+// The tokens of marked bins, in no order.  Those within the marked bins' range of logits are
+// gathered first, with a few more, and then told apart side by side.
 template <typename T>
 __global__ __launch_bounds__(kPartThreads) void k_sample_list(const m27q_sampling p, const Scratch sc) {
-    constexpr uint32_t M = 2048;  // (a part's tokens past them go by themselves)
-    __shared__ uint64_t keys[M];
-    __shared__ uint32_t count_s, to_s, marks[(kBins + 31) / 32];
-    const int row = blockIdx.y, first = (int)blockIdx.x * kPart;
+    __shared__ uint16_t near_at[kPart];
+    __shared__ uint32_t near_s, marks[(kBins + 31) / 32];
+    const int row = blockIdx.y, first = (int)blockIdx.x * kPart, lane = threadIdx.x & 63;
     RowPlan &plan = sc.plan[row];
     float v[kEach];
     load_part<T>(p, row, first, v);
     if (plan.state != 1) return;
-    if (threadIdx.x == 0) count_s = 0;
+    if (threadIdx.x == 0) near_s = 0;
     if (threadIdx.x < (kBins + 31) / 32) marks[threadIdx.x] = plan.marks[threadIdx.x];
-    __syncthreads();
-    uint64_t *const list = sc.list + (long long)row * kList;
-    const Scale s = row_scale(row_rule(p, row), plan.anchor);
-    float lo[kRanges], hi[kRanges];
+    unsigned long long near[kEach];  // a bit a lane
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) near[i] = 0;
 #pragma unroll
     for (int j = 0; j < kRanges; ++j) {
-        lo[j] = plan.lo[j];
-        hi[j] = plan.hi[j];
+        const float lo = plan.lo[j], hi = plan.hi[j];
+        if (!__builtin_amdgcn_readfirstlane(lo <= hi)) continue;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) near[i] |= __ballot(v[i] >= lo) & __ballot(v[i] <= hi);
     }
+    __syncthreads();
+    int up = 0;
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-        bool near = false;
+    for (int i = 0; i < kEach; ++i) up += __popcll(near[i]);
+    if (up) {
+        uint32_t to = 0;
+        if (lane == 0) to = atomicAdd(&near_s, (uint32_t)up);
+        to = __builtin_amdgcn_readfirstlane(to);
 #pragma unroll
-        for (int j = 0; j < kRanges; ++j) near |= v[i] >= lo[j] && v[i] <= hi[j];
-        if (!near) continue;
-        double z;
-        const int bin = bin_of(v[i], s, z);
-        if (bin < kBins && (marks[bin / 32] >> (bin & 31) & 1)) {
-            const uint64_t key = order_key(v[i], first + part_index(i));
-            const uint32_t at = atomicAdd(&count_s, 1u);
-            if (at < M) {
-                keys[at] = key;
-            } else {
-                const uint32_t to = atomicAdd(&plan.listed, 1u);
-                if (to < (uint32_t)kList) list[to] = key;
-            }
+        for (int i = 0; i < kEach; ++i) {
+            if (near[i] >> lane & 1) near_at[to + __popcll(near[i] & ((1ull << lane) - 1))] = (uint16_t)part_index(i);
+            to += (uint32_t)__popcll(near[i]);
         }
     }
     __syncthreads();
-    const uint32_t m = min(count_s, M);
+    const int m = (int)near_s;
     if (m == 0) return;
-    if (threadIdx.x == 0) to_s = atomicAdd(&plan.listed, m);
-    __syncthreads();
-    const uint32_t to = to_s;
-    for (uint32_t i = threadIdx.x; i < m; i += kPartThreads)
-        if (to + i < (uint32_t)kList) list[to + i] = keys[i];
+    const Scale s = row_scale(row_rule(p, row), plan.anchor);
+    const long long base = (long long)row * p.stride + first;
+    uint64_t *const list = sc.list + (long long)row * kList;
+    for (int i0 = 0; i0 < m; i0 += kPartThreads) {
+        const int i = i0 + (int)threadIdx.x, at = near_at[min(i, m - 1)];
+        const float l = logit<T>(p.logits, base + at);
+        const int bin = place_of(l, s).bin;
+        const bool ok = i < m && bin < kBins && (marks[min(bin, kBins) / 32] >> (bin & 31) & 1);
+        const unsigned long long all = __ballot(ok);
+        if (all == 0) continue;
+        uint32_t to = 0;
+        if (lane == 0) to = atomicAdd(&plan.listed, (uint32_t)__popcll(all));
+        to = __builtin_amdgcn_readfirstlane(to) + (uint32_t)__popcll(all & ((1ull << lane) - 1));
+        if (ok && to < (uint32_t)kList) list[to] = order_key(l, first + at);
+    }
 }
 
-// Keys in descending order, E of each thread side by side: a bitonic network whose steps stay in a
-// thread's registers, or in a wave, as long as they can.
-template <int E>
-__device__ __forceinline__ void sort_keys(uint64_t (&x)[E], uint64_t *lds) {
-    const int tid = threadIdx.x;
-    for (int k = 2; k <= E * kRowThreads; k *= 2)
-        for (int j = k / 2; j > 0; j /= 2) {
-            if (j < E) {
-#pragma unroll
-                for (int m = E / 2; m > 0; m /= 2) {
-                    if (j != m) continue;
-#pragma unroll
-                    for (int e = 0; e < E; ++e) {
-                        if (e & m) continue;
-                        const bool down = ((tid * E + e) & k) == 0;
-                        const uint64_t a = x[e], b = x[e + m];
-                        const bool swap = (a < b) == down;
-                        x[e] = swap ? b : a;
-                        x[e + m] = swap ? a : b;
-                    }
-                }
-                continue;
-            }
-            const int t = j / E;  // the other thread's distance
-            const bool take_max = ((tid & t) == 0) == ((tid * E & k) == 0);
-            uint64_t y[E];
-            if (t < 64) {
-#pragma unroll
-                for (int e = 0; e < E; ++e) y[e] = (uint64_t)__shfl_xor((unsigned long long)x[e], t);
-            } else {
-                __syncthreads();
-#pragma unroll
-                for (int e = 0; e < E; ++e) lds[e * kRowThreads + tid] = x[e];
-                __syncthreads();
-#pragma unroll
-                for (int e = 0; e < E; ++e) y[e] = lds[e * kRowThreads + (tid ^ t)];
-            }
-#pragma unroll
-            for (int e = 0; e < E; ++e) x[e] = (x[e] > y[e]) == take_max ? x[e] : y[e];
-        }
-}
-
+constexpr int kCrowd = 1024;
 struct PickShared {
     union {
-        uint64_t keys[kList];
+        struct {
+            uint64_t keys[kList];
+            uint32_t count[kList];  // of the tokens in a bucket, then of those before it
+        };
         WholeRow whole;
     };
+    uint32_t scan32[kRowThreads / 64];
     unsigned long long scan[kRowThreads / 64];
+    // the plan's
+    uint32_t before[kBins + 1], at[kBins + 1];
+    unsigned long long sum[kBins + 1];
+    double unit[kBins + 1];
     unsigned long long start[kBins + 1];  // the list's running sum in front of a bin
-    // sums down to the first token, the top_k-th, the one that reaches top_p and the last one that min_p leaves
+    // sums down to the top_k-th token, the one that reaches top_p and the last one that min_p leaves
     unsigned long long among, top_p, min_p;
     int pick;
+    uint32_t most;
+    double octave[kUnit];
 };
 
-// A row's list in order, the running sums of its tokens, and the borders among them.
+// The smallest of a workgroup's values that do not descend from thread to thread, but for the largest of
+// their type, which stands for none: that of each wave's first.
+template <typename T>
+__device__ __forceinline__ void min_of_first(T v, T &to) {
+    const T none = sizeof(T) == 8 ? (T)~0ull : (T)0x7fffffff;
+    const unsigned long long m = __ballot(v != none);
+    if (m && (int)(threadIdx.x & 63) == __builtin_ctzll(m)) atomicMin(&to, v);
+}
+
+// A row's list in order, the running sums of its tokens, and the borders among them.  E tokens a thread.
+// In order: a bin's tokens have as many buckets as they are, by z, so that few share one; a
+// token's place in its bucket is how many of it are larger.  False: some bucket holds so many
+// (equal logits) that this would take long.
 template <int E>
-__device__ __forceinline__ void pick_from_list(const m27q_sampling &p, const Scratch &sc, const RowPlan &plan, const Rule &r, int n,
+__device__ __forceinline__ bool pick_from_list(const m27q_sampling &p, const Scratch &sc, const RowPlan &plan, const Rule &r, int n,
                                                PickShared &s) {
     const int row = blockIdx.x, tid = threadIdx.x, i0 = tid * E;
+    const Scale scale = row_scale(r, plan.anchor);
+    const Exp2Unit x(s.octave);
     uint64_t key[E];
+    uint32_t bucket[E], slot[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) {
         const int i = e * kRowThreads + tid;
         key[e] = i < n ? sc.list[(long long)row * kList + i] : 0;
+        if (e * kRowThreads < kList) s.count[i] = 0;
     }
-    sort_keys<E>(key, s.keys);
+    __syncthreads();  // the plan's arrays are there too
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        bucket[e] = slot[e] = 0;
+        if (e * kRowThreads + tid >= n) continue;
+        const Place a = place_of(key_value(key[e]), scale);
+        const uint32_t at = s.at[a.bin], count = s.at[a.bin + 1] - at;
+        const float part = ((float)a.k + 0.5f - (float)a.z) * (a.bin < kFine ? 1.0f : 1.0f / kUnit);
+        bucket[e] = at + min((uint32_t)fmaxf(part * (float)count, 0.0f), count - 1);
+        slot[e] = atomicAdd(&s.count[bucket[e]], 1u);
+    }
+    __syncthreads();
+    uint32_t c[E], sum32 = 0, most = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        c[e] = s.count[i0 + e];
+        sum32 += c[e];
+        most = max(most, c[e]);
+    }
+    if (most > (uint32_t)kCrowd) s.most = most;
+    uint32_t all32, run32 = scan_group<kRowThreads>(sum32, s.scan32, all32);
+    if (s.most) return false;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        s.count[i0 + e] = run32;
+        run32 += c[e];
+    }
+    __syncthreads();
+    uint32_t first[E], held[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        first[e] = held[e] = 0;
+        if (e * kRowThreads + tid >= n) continue;
+        first[e] = s.count[bucket[e]];
+        held[e] = (bucket[e] + 1 < (uint32_t)(E * kRowThreads) ? s.count[bucket[e] + 1] : (uint32_t)n) - first[e];
+        s.keys[first[e] + slot[e]] = key[e];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        uint32_t larger = 0;
+        for (uint32_t j = 0; j < held[e]; ++j) larger += s.keys[first[e] + j] > key[e];
+        slot[e] = first[e] + larger;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+        if (e * kRowThreads + tid < n) s.keys[slot[e]] = key[e];
+    __syncthreads();
 
     // the sums of the row down to each token of the list.  In front of a bin, and at its end, they are the plan's.
-    const Scale scale = row_scale(r, plan.anchor);
-    const double unit = sum_unit(p.n);
     unsigned long long own[E], sum = 0;
     int bin[E];
 #pragma unroll
@@ -643,61 +740,66 @@ __device__ __forceinline__ void pick_from_list(const m27q_sampling &p, const Scr
         own[e] = 0;
         bin[e] = 0;
         if (i0 + e < n) {
-            double z = 0;
-            bin[e] = bin_of(key_value(key[e]), scale, z);
-            own[e] = bin_mass(bin[e], z);
+            key[e] = s.keys[i0 + e];
+            const Place a = place_of(key_value(key[e]), scale);
+            bin[e] = a.bin;
+            own[e] = x.mass(a.z, a.k, 0);
         }
         sum += own[e];
     }
-    uint32_t at[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) at[e] = plan.at[bin[e]];
-    unsigned long long all, run = scan_group(sum, s.scan, all);
+    unsigned long long all, run = scan_group<kRowThreads>(sum, s.scan, all);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-        if (i0 + e < n && (uint32_t)(i0 + e) == at[e]) s.start[bin[e]] = run;
+        if (i0 + e < n && (uint32_t)(i0 + e) == s.at[bin[e]]) s.start[bin[e]] = run;
         run += own[e];
     }
     run -= sum;
     __syncthreads();
     const float top = key_value(plan.best);
-    unsigned long long down[E];
+    unsigned long long down[E], dropped = ~0ull;
     int rank[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) {
         const uint32_t i = (uint32_t)(i0 + e);
-        const unsigned long long lo = plan.sum[bin[e]], hi = plan.sum[bin[e] + 1], in = run - s.start[bin[e]];
-        const double f = unit * bin_scale(bin[e]);
-        const auto to = [&](unsigned long long x) { return min(lo + (unsigned long long)__builtin_rint((double)x * f), hi); };
-        down[e] = i + 1 == plan.at[bin[e] + 1] ? hi : to(in + own[e]);
-        rank[e] = i < (uint32_t)n ? (int)(plan.before[bin[e]] + i - at[e]) : 0x7fffffff;
+        const unsigned long long lo = s.sum[bin[e]], hi = s.sum[bin[e] + 1], in = run - s.start[bin[e]];
+        const auto to = [&](unsigned long long x) { return min(lo + (unsigned long long)__builtin_rint((double)x * s.unit[bin[e]]), hi); };
+        down[e] = i + 1 == s.at[bin[e] + 1] ? hi : to(in + own[e]);
+        rank[e] = i < (uint32_t)n ? (int)(s.before[bin[e]] + i - s.at[bin[e]]) : 0x7fffffff;
         run += own[e];
         if (rank[e] == r.k - 1) s.among = down[e];
-        if (r.min_p > 0.0 && i < (uint32_t)n && exp(((double)key_value(key[e]) - (double)top) * r.inv_t) < r.min_p)
-            atomicMin(&s.min_p, to(in));
+        if (r.min_p > 0.0 && i < (uint32_t)n && dropped == ~0ull &&
+            exp(((double)key_value(key[e]) - (double)top) * r.inv_t) < r.min_p)
+            dropped = to(in);
     }
+    if (r.min_p > 0.0) min_of_first(dropped, s.min_p);
     __syncthreads();
-    const double reach = r.top_p * (double)s.among;
+    if (r.top_p < 1.0) {
+        const double reach = r.top_p * (double)s.among;
+        unsigned long long at = ~0ull;
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-        if (r.top_p < 1.0 && i0 + e < n && (double)down[e] >= reach) atomicMin(&s.top_p, down[e]);
-    __syncthreads();
+        for (int e = E - 1; e >= 0; --e)
+            if (i0 + e < n && (double)down[e] >= reach) at = down[e];
+        min_of_first(at, s.top_p);
+        __syncthreads();
+    }
     // the first token is kept whatever the rest says
-    double z = 0;
-    const int b0 = bin_of(top, scale, z);
-    const unsigned long long first = min((unsigned long long)__builtin_rint((double)bin_mass(b0, z) * unit * bin_scale(b0)), plan.sum[b0 + 1]);
-    const unsigned long long total = max(first, min(s.among, min(s.top_p, s.min_p)));
+    const Place f = place_of(top, scale);
+    const unsigned long long one = min((unsigned long long)__builtin_rint((double)x.mass(f.z, f.k, 0) * s.unit[f.bin]), s.sum[f.bin + 1]);
+    const unsigned long long total = max(one, min(s.among, min(s.top_p, s.min_p)));
     const double target = r.u * (double)total;
+    int at = 0x7fffffff;
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-        if (i0 + e < n && (double)down[e] >= target) atomicMin(&s.pick, rank[e]);
+    for (int e = E - 1; e >= 0; --e)
+        if (i0 + e < n && (double)down[e] >= target) at = rank[e];
+    min_of_first(at, s.pick);
     __syncthreads();
 #pragma unroll
     for (int e = 0; e < E; ++e)
         if (i0 + e < n && rank[e] == s.pick) {
             p.token[row] = key_index(key[e]);
-            if (p.prob) p.prob[row] = (float)((double)own[e] * unit * bin_scale(bin[e]) / (double)total);
+            if (p.prob) p.prob[row] = (float)((double)own[e] * s.unit[bin[e]] / (double)total);
         }
+    return true;
 }
 
 __global__ __launch_bounds__(kRowThreads) void k_sample_pick(const m27q_sampling p, const Scratch sc) {
@@ -707,22 +809,30 @@ __global__ __launch_bounds__(kRowThreads) void k_sample_pick(const m27q_sampling
     const int state = plan.state;
     if (state == 0) return;
     const Rule r = row_rule(p, row);
-    if (state == 2) {
-        sample_whole_row(p, row, r, plan.best, s.whole);
-        return;
+    bool done = false;
+    if (state == 1) {
+        if (threadIdx.x <= kBins) {
+            s.before[threadIdx.x] = plan.before[threadIdx.x];
+            s.at[threadIdx.x] = plan.at[threadIdx.x];
+            s.sum[threadIdx.x] = plan.sum[threadIdx.x];
+            s.unit[threadIdx.x] = plan.unit[threadIdx.x];
+        }
+        if (threadIdx.x == 0) {
+            s.among = plan.sum[kBins];  // unless the top_k-th is on the list
+            s.top_p = ~0ull;
+            s.min_p = plan.min_p_sum;
+            s.pick = 0x7fffffff;
+            s.most = 0;
+        }
+        if (threadIdx.x < kUnit) s.octave[threadIdx.x] = Exp2Unit::factor(threadIdx.x);
+        const int n = (int)min(plan.listed, (uint32_t)kList);
+        if (n <= kRowThreads) done = pick_from_list<1>(p, sc, plan, r, n, s);
+        else if (n <= 2 * kRowThreads) done = pick_from_list<2>(p, sc, plan, r, n, s);
+        else if (n <= 4 * kRowThreads) done = pick_from_list<4>(p, sc, plan, r, n, s);
+        else done = pick_from_list<8>(p, sc, plan, r, n, s);
+        if (!done) __syncthreads();
     }
-    if (threadIdx.x == 0) {
-        s.among = plan.sum[kBins];  // unless the top_k-th is on the list
-        s.top_p = ~0ull;
-        s.min_p = plan.min_p_sum;
-        s.pick = 0x7fffffff;
-    }
-    const int n = (int)min(plan.listed, (uint32_t)kList);
-    __syncthreads();
-    if (n <= kRowThreads) pick_from_list<1>(p, sc, plan, r, n, s);
-    else if (n <= 2 * kRowThreads) pick_from_list<2>(p, sc, plan, r, n, s);
-    else if (n <= 4 * kRowThreads) pick_from_list<4>(p, sc, plan, r, n, s);
-    else pick_from_list<8>(p, sc, plan, r, n, s);
+    if (!done) sample_whole_row(p, row, r, plan.best, s.whole);
 }
 
 struct Sizes {
