@@ -157,7 +157,7 @@ __device__ void sample_whole_row(const m27q_sampling &p, int row, const Rule &r,
 // bins of a unit, 127 of an octave, and what lies below those 151 octaves counts for nothing.
 // Units are absolute (y rounded), anchors whole octaves: bins of parts of a row with anchors of
 // their own add up.  A bin holds how many tokens and the sum of their weights, in 2^-36 of
-// the weight at the bin's upper end.
+// the weight at its octave's upper end.
 
 constexpr int kUnit = 16;               // units of an octave
 constexpr int kFine = 384, kCoarse = 127;
@@ -168,15 +168,14 @@ constexpr int kMassBits = 36, kSumBits = 50;
 constexpr int kPart = 8192;             // tokens of a part: counts of 14 bits above sums of 50
 constexpr double kUnitsPerNat = 16 * 1.4426950408889634074;
 
-// Weights of places within a bin: 2^(z / 16) by its Taylor polynomial (degree 5 for |z| <= 1 / 2: the next
-// term is below 2^-42), times 2^36 and, in a bin of an octave, 2^(-k / 16) for a place k units down it.
-// The constants are kept in registers: scalar ones, but for what a product's or sum's second
-// constant has to be.
-struct Exp2Unit {
+// Weights of places within an octave, k units and z down it: 2^(-(k + z) / 16), from a table for k and the
+// Taylor polynomial for |z| <= 1 / 2 (degree 5: the next term is below 2^-42), in 2^-36.  The
+// constants are kept in registers: scalar ones, but for what a product's or sum's second one has to be.
+struct Weights {
     double c[6], add;
     const double *octave;  // 2^(36 - k / 16), in LDS
-    __device__ __forceinline__ Exp2Unit(const double *octave) : octave(octave) {
-        constexpr double a = 0.69314718055994530942 / 16;
+    __device__ __forceinline__ Weights(const double *octave) : octave(octave) {
+        constexpr double a = -0.69314718055994530942 / kUnit;
         c[0] = 1.0;
         c[1] = a;
         c[2] = a * a / 2;
@@ -200,36 +199,53 @@ struct Exp2Unit {
 };
 
 // What a row's logits are placed by.
+constexpr int kReach = kFine + kUnit * kCoarse;  // units down to where weights end
 struct Scale {
     double c;       // units of a logit
     double anchor;
-    int wide;       // distances from the anchor pass 32 bits, or T is infinite
+    int wide;       // distances from the anchor are not whole numbers of 2^26 at most, or T is infinite
     double near;    // 1; 0 where a step of a logit is thousands of octaves and only equal ones have a weight
 };
 __device__ __forceinline__ Scale row_scale(const Rule &r, double anchor) {
-    const double far = fabs(anchor) + kFine + kUnit * kCoarse;
+    const double far = fabs(anchor) + kReach;
     const double c = kUnitsPerNat * r.inv_t;
-    return {c, anchor, __builtin_amdgcn_readfirstlane(far > 0x1p30 || !(c > 0.0)), far > 0x1p40 ? 0.0 : 1.0};
+    return {c, anchor, __builtin_amdgcn_readfirstlane(!(far < 0x1p26) || !(c > 0.0)), far > 0x1p40 ? 0.0 : 1.0};
 }
 
-// The bin of a logit, and its place in it: k units down a bin of an octave (0 otherwise), z from there (up is
-// positive), from the product's remainder behind the whole units, which loses nothing to their number.
+// The distance of a logit from the anchor in whole units, and what is left over: both of the exact
+// product, as an addition that leaves the whole number in the low bits rounds it once, and alike for any anchor.
+__device__ __forceinline__ uint32_t units_down(double l, double c, double low, double anchor, double &z) {
+    const double t = __builtin_fma(l, -c, low);  // low = anchor + 1.5 2^52
+    z = __builtin_fma(l, -c, anchor - (t - 0x1.8p52));
+    return (uint32_t)__builtin_bit_cast(unsigned long long, t);
+}
+
+// The bin of a logit, and its place in its octave.
 struct Place {
     int bin, k;
     double z;
 };
+__device__ __forceinline__ int bin_of(uint32_t d) { return (int)min(d, (d >> 4) + (kFine - kFine / kUnit)); }
 __device__ __forceinline__ Place place_of(float l, const Scale &s) {
-    const double x = (double)l, b = __builtin_rint(x * s.c), d = s.anchor - b;
-    Place p{kBins, 0, __builtin_fma(x, s.c, -b) * s.near};
-    if (!(d < kFine + kUnit * kCoarse)) return p;  // (-infinity and NaN too)
-    const int i = (int)d;
-    p.bin = i < kFine ? i : kFine + (i - kFine) / kUnit;
-    p.k = i < kFine ? 0 : i & (kUnit - 1);
+    Place p{kBins, 0, 0};
+    uint32_t d;
+    if (s.wide) {
+        const double b = __builtin_rint((double)l * s.c), far = s.anchor - b;
+        if (!(far < kReach)) return p;  // (-infinity and NaN too)
+        d = (uint32_t)far;
+        p.z = -__builtin_fma((double)l, s.c, -b) * s.near;
+    } else {
+        if (!((double)l * s.c > s.anchor - (kReach + kUnit))) return p;
+        d = units_down((double)l, s.c, s.anchor + 0x1.8p52, s.anchor, p.z);
+        if (d >= (uint32_t)kReach) return p;
+    }
+    p.bin = bin_of(d);
+    p.k = (int)(d & (kUnit - 1));
     return p;
 }
-// The weight at a bin's upper end, of that at the anchor.
+// The weight at the upper end of a bin's octave, of that at the anchor.
 __device__ __forceinline__ int bin_distance(int bin) { return bin < kFine ? bin : kFine + kUnit * (bin - kFine); }
-__device__ __forceinline__ double bin_scale(int bin) { return exp2(-bin_distance(bin) * (1.0 / kUnit)); }
+__device__ __forceinline__ double bin_scale(int bin) { return __builtin_ldexp(1.0, -(bin_distance(bin) / kUnit)); }
 
 // What is kept of a part of a row, and of a row.
 struct Part {
@@ -244,8 +260,9 @@ struct RowPlan {
     int state;            // 0: done; 1: the tokens of marked bins make a list; 2: the whole row is gone through
     uint32_t listed;      // tokens on the list
     unsigned long long min_p_sum;         // of the tokens that min_p leaves, where none of its border's bins cuts them
-    float lo[kRanges], hi[kRanges];       // logits of marked bins lie within these
-    uint32_t marks[(kBins + 31) / 32];
+    int first[kRanges], last[kRanges];    // the marked bins
+    float lo[kRanges], hi[kRanges];       // their logits lie within these
+    float least;                          // and above this
     uint32_t before[kBins + 1];           // tokens of the bins above
     uint32_t at[kBins + 1];               // ... that are on the list
     unsigned long long sum[kBins + 1];    // their weights, in units of sum_unit
@@ -299,59 +316,61 @@ __global__ __launch_bounds__(kPartThreads) void k_sample_parts(const m27q_sampli
     const Rule r = row_rule(p, row);
 #pragma unroll
     for (int i = 0; i < kCopies; ++i) bins[i * (kBins + 1) + threadIdx.x] = 0;
-    if (threadIdx.x < kUnit) octave[threadIdx.x] = Exp2Unit::factor(threadIdx.x);
+    if (threadIdx.x < kUnit) octave[threadIdx.x] = Weights::factor(threadIdx.x);
     float top = -__builtin_inff();
 #pragma unroll
     for (int i = 0; i < kEach; ++i) top = fmaxf(top, v[i]);
 #pragma unroll
     for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const float mine = top;
     if (lane == 0) top_s[wave] = top;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < W; ++i) top = fmaxf(top, top_s[i]);
     int at = 0x7fffffff;
+    if (__builtin_amdgcn_readfirstlane(mine == top)) {
 #pragma unroll
-    for (int i = kEach - 1; i >= 0; --i) at = v[i] == top ? part_index(i) : at;
+        for (int i = kEach - 1; i >= 0; --i) at = v[i] == top ? part_index(i) : at;
 #pragma unroll
-    for (int o = 32; o; o >>= 1) at = min(at, __shfl_xor(at, o));
+        for (int o = 32; o; o >>= 1) at = min(at, __shfl_xor(at, o));
+    }
     if (lane == 0) at_s[wave] = at;
 
     const bool any = !r.greedy && __builtin_isfinite(top);
     const double b = __builtin_rint((double)top * (kUnitsPerNat * r.inv_t));
     const Scale s = row_scale(r, any ? ceil(b * (1.0 / kUnit)) * kUnit : -__builtin_inf());
     if (any) {
-        const Exp2Unit x(octave);
+        const Weights w(octave);
         const int copy = lane & (kCopies - 1);
-        bool odd = false;
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) odd |= v[i] != v[i];
-        if (s.wide || __any(odd)) {
+        if (s.wide) {
 #pragma unroll 1
             for (int i = 0; i < kEach; ++i) {
                 const Place a = place_of(v[i], s);
-                if (a.bin < kBins) atomicAdd(&bins[a.bin * kCopies + copy], x.mass(a.z, a.k, 1));
+                if (a.bin < kBins) atomicAdd(&bins[a.bin * kCopies + copy], w.mass(a.z, a.k, 1));
             }
-        } else {  // the same, in whole numbers of 32 bits and several tokens' chains beside each other
-            const int anchor = (int)s.anchor;
+        } else {
+            // the same without branches, several tokens' chains beside each other.  A logit above this one is
+            // less than 16 units past the last bin: what is further down, -infinity and NaN are left out by it.
+            const float least = fmaxf((float)((s.anchor - (kReach + kUnit / 2)) / s.c), -0x1.fffffep+127f);
+            const double low = s.anchor + 0x1.8p52;
             constexpr int AT = 4;
 #pragma unroll
             for (int i0 = 0; i0 < kEach; i0 += AT) {
                 unsigned long long m[AT];
-                uint32_t d[AT], bin[AT];
+                int bin[AT];
 #pragma unroll
                 for (int j = 0; j < AT; ++j) {
-                    const double l = (double)v[i0 + j], b = __builtin_rint(l * s.c);
-                    d[j] = (uint32_t)(anchor - (int)b);  // (what is too far below saturates, or wraps above all bins)
-                    const bool fine = d[j] < (uint32_t)kFine;
-                    bin[j] = fine ? d[j] : (d[j] >> 4) + (kFine - kFine / kUnit);
-                    m[j] = x.mass(__builtin_fma(l, s.c, -b), fine ? 0 : d[j] & (kUnit - 1), 1);
+                    double z;
+                    const uint32_t d = units_down((double)v[i0 + j], s.c, low, s.anchor, z);
+                    bin[j] = bin_of(d);
+                    m[j] = w.mass(z, (int)(d & (kUnit - 1)), 1);
                 }
 #pragma unroll
                 for (int j = 0; j < AT; ++j) asm volatile("" : "+v"(m[j]), "+v"(bin[j]));  // computed by now, for all lanes
 #pragma unroll
                 for (int j = 0; j < AT; ++j)
-                    if (d[j] < (uint32_t)(kFine + kUnit * kCoarse)) atomicAdd(&bins[bin[j] * kCopies + copy], m[j]);
+                    if (v[i0 + j] >= least) atomicAdd(&bins[bin[j] * kCopies + copy], m[j]);
             }
         }
     }
@@ -369,16 +388,9 @@ __global__ __launch_bounds__(kPartThreads) void k_sample_parts(const m27q_sampli
     sc.bins[me * kStored + threadIdx.x] = sum;
     // the octaves of the fine bins, 16 lanes each, for a row whose anchor lies so far above that they are one bin there
     if (threadIdx.x < kFine) {
-        double mass = (double)(sum & ((1ull << kSumBits) - 1)) * bin_scale(threadIdx.x & (kUnit - 1));
-        uint32_t count = (uint32_t)(sum >> kSumBits);
 #pragma unroll
-        for (int o = kUnit / 2; o; o >>= 1) {
-            mass += __shfl_xor(mass, o);
-            count += __shfl_xor(count, o);
-        }
-        if ((threadIdx.x & (kUnit - 1)) == 0)
-            sc.bins[me * kStored + kBins + 1 + threadIdx.x / kUnit] =
-                (unsigned long long)__builtin_rint(mass) | (unsigned long long)count << kSumBits;
+        for (int o = kUnit / 2; o; o >>= 1) sum += __shfl_xor(sum, o);
+        if ((threadIdx.x & (kUnit - 1)) == 0) sc.bins[me * kStored + kBins + 1 + threadIdx.x / kUnit] = sum;
     }
 }
 
@@ -422,6 +434,13 @@ __device__ __forceinline__ T scan_group(T v, T *lds, T &all) {
         all += x;
     }
     return before + run - v;
+}
+
+// Where a part whose anchor lies `off` units (whole octaves) below the row's has the sum for the row's bin J: the same
+// bin's, or, where an octave of the row lies among the part's fine bins, their octave's.  -1: it has none.
+__device__ __forceinline__ int part_bin(int J, int off) {
+    const int oct = kOctaves + J - kFine - off / kUnit;
+    return J >= kBins ? -1 : J < kFine ? max(J - off, -1) : oct >= kOctaves ? kFine + oct - kOctaves : oct >= 0 ? kBins + 1 + oct : -1;
 }
 
 constexpr int kPlanThreads = 512;
@@ -479,7 +498,7 @@ __global__ __launch_bounds__(kPlanThreads) void k_sample_plan(const m27q_samplin
         const int parts = min(sc.parts - i0, kPlanThreads);
         if (J < parts) {
             const double off = anchor - part[i0 + J].anchor;
-            off_s[J] = off < kFine + kUnit * kCoarse ? (int)off : kSkip;
+            off_s[J] = off < kReach ? (int)off : kSkip;
         }
         __syncthreads();
         const unsigned long long *bins = sc.bins + ((long long)row * sc.parts + i0) * kStored;
@@ -489,10 +508,8 @@ __global__ __launch_bounds__(kPlanThreads) void k_sample_plan(const m27q_samplin
             bool ok[AT];
 #pragma unroll
             for (int k = 0; k < AT; ++k) {
-                const int j = min(i + k, parts - 1), off = off_s[j];
-                const int oct = kOctaves + J - kFine - off / kUnit;  // of a bin of an octave
-                const int from = J < kFine ? J - off : oct >= kOctaves ? kFine + oct - kOctaves : oct >= 0 ? kBins + 1 + oct : -1;
-                ok[k] = i + k < parts && off != kSkip && from >= 0 && J < kBins;
+                const int j = min(i + k, parts - 1), off = off_s[j], from = part_bin(J, off);
+                ok[k] = i + k < parts && off != kSkip && from >= 0;
                 x[k] = bins[(long long)(ok[k] ? j : 0) * kStored + (ok[k] ? from : 0)];
             }
 #pragma unroll
@@ -537,7 +554,7 @@ __global__ __launch_bounds__(kPlanThreads) void k_sample_plan(const m27q_samplin
     if (r.min_p > 0.0) {
         // the bin of the weight min_p, and its neighbours for what rounding does
         const double y = (double)top * (kUnitsPerNat * r.inv_t) + kUnit * log2(r.min_p), d = anchor - __builtin_rint(y);
-        if (d < kFine + kUnit * kCoarse) {
+        if (d < kReach) {
             const int m = d < 0 ? 0 : d < kFine ? (int)d : kFine + ((int)d - kFine) / kUnit;
             m0 = max(m - 1, 0);
             m1 = min(m + 1, kBins - 1);
@@ -554,16 +571,19 @@ __global__ __launch_bounds__(kPlanThreads) void k_sample_plan(const m27q_samplin
     out.unit[J] = unit;
     out.before[J] = before;
     out.at[J] = at;
-    const unsigned long long m = __ballot(mark);
-    if ((J & 31) == 0) out.marks[J / 32] = (uint32_t)(m >> (J & 32));
     if (J < kRanges) {
         // logits of bins b0 .. b1, and a little more than those
         const int b0 = J == 0 ? kb : J == 1 ? p0 : J == 2 ? m0 : q0, b1 = J == 0 ? (k_cuts ? kb : -1) : J == 1 ? p1 : J == 2 ? m1 : q1;
-        const double c = kUnitsPerNat * r.inv_t, up = anchor - bin_distance(b0) + 1;
-        const double down = anchor - bin_distance(b1) - (b1 < kFine ? 1 : kUnit);
+        const double c = kUnitsPerNat * r.inv_t, up = anchor - bin_distance(b0) + 0.5;
+        const double down = anchor - bin_distance(b1) - (b1 < kFine ? 0.5 : kUnit - 0.5);
         const bool none = b1 < b0, all = !(c > 1e-30);
         const double eps = 0x1p-20;
-        out.lo[J] = none ? __builtin_inff() : all ? -__builtin_inff() : (float)(down / c - fabs(down / c) * eps);
+        out.first[J] = b0;
+        out.last[J] = b1;
+        const float lo = none ? __builtin_inff() : all ? -__builtin_inff() : (float)(down / c - fabs(down / c) * eps);
+        const float least = fminf(fminf(__shfl(lo, 0), __shfl(lo, 1)), fminf(__shfl(lo, 2), __shfl(lo, 3)));
+        if (J == 0) out.least = least;
+        out.lo[J] = lo;
         out.hi[J] = none ? -__builtin_inff() : all ? __builtin_inff() : (float)(up / c + fabs(up / c) * eps);
     }
     if (J == 0) {
@@ -575,33 +595,36 @@ __global__ __launch_bounds__(kPlanThreads) void k_sample_plan(const m27q_samplin
     }
 }
 
-// The tokens of marked bins, in no order.  Those within the marked bins' range of logits are
-// gathered first, with a few more, and then told apart side by side.
+// The tokens of marked bins, in no order.  Those within the bins' ranges of logits, hardly more, are
+// gathered first and told apart side by side: in their places, a few lanes of most waves would work.  One
+// atomic a workgroup: those of a row meet at one address, one after another.
 template <typename T>
 __global__ __launch_bounds__(kPartThreads) void k_sample_list(const m27q_sampling p, const Scratch sc) {
     __shared__ uint16_t near_at[kPart];
-    __shared__ uint32_t near_s, marks[(kBins + 31) / 32];
+    __shared__ uint32_t near_s, count_s, to_s;
     const int row = blockIdx.y, first = (int)blockIdx.x * kPart, lane = threadIdx.x & 63;
     RowPlan &plan = sc.plan[row];
+    // a part whose largest token lies below all of them has none
+    if (plan.state != 1 || key_value(sc.part[(long long)row * sc.parts + blockIdx.x].best) < plan.least) return;
     float v[kEach];
     load_part<T>(p, row, first, v);
-    if (plan.state != 1) return;
-    if (threadIdx.x == 0) near_s = 0;
-    if (threadIdx.x < (kBins + 31) / 32) marks[threadIdx.x] = plan.marks[threadIdx.x];
+    if (threadIdx.x == 0) near_s = count_s = 0;
     unsigned long long near[kEach];  // a bit a lane
+    int b0[kRanges], b1[kRanges], up = 0;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) near[i] = 0;
 #pragma unroll
     for (int j = 0; j < kRanges; ++j) {
+        b0[j] = plan.first[j];
+        b1[j] = plan.last[j];
         const float lo = plan.lo[j], hi = plan.hi[j];
-        if (!__builtin_amdgcn_readfirstlane(lo <= hi)) continue;
+        if (b1[j] < b0[j]) continue;
 #pragma unroll
         for (int i = 0; i < kEach; ++i) near[i] |= __ballot(v[i] >= lo) & __ballot(v[i] <= hi);
     }
-    __syncthreads();
-    int up = 0;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) up += __popcll(near[i]);
+    __syncthreads();
     if (up) {
         uint32_t to = 0;
         if (lane == 0) to = atomicAdd(&near_s, (uint32_t)up);
@@ -622,12 +645,20 @@ __global__ __launch_bounds__(kPartThreads) void k_sample_list(const m27q_samplin
         const int i = i0 + (int)threadIdx.x, at = near_at[min(i, m - 1)];
         const float l = logit<T>(p.logits, base + at);
         const int bin = place_of(l, s).bin;
-        const bool ok = i < m && bin < kBins && (marks[min(bin, kBins) / 32] >> (bin & 31) & 1);
-        const unsigned long long all = __ballot(ok);
-        if (all == 0) continue;
+        bool ok = false;
+#pragma unroll
+        for (int j = 0; j < kRanges; ++j) ok |= bin >= b0[j] && bin <= b1[j];
+        ok &= i < m && bin < kBins;
+        const unsigned long long mine = __ballot(ok);
         uint32_t to = 0;
-        if (lane == 0) to = atomicAdd(&plan.listed, (uint32_t)__popcll(all));
-        to = __builtin_amdgcn_readfirstlane(to) + (uint32_t)__popcll(all & ((1ull << lane) - 1));
+        if (lane == 0 && mine) to = atomicAdd(&count_s, (uint32_t)__popcll(mine));
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            to_s = atomicAdd(&plan.listed, count_s);
+            count_s = 0;
+        }
+        __syncthreads();
+        to = __builtin_amdgcn_readfirstlane(to) + to_s + (uint32_t)__popcll(mine & ((1ull << lane) - 1));
         if (ok && to < (uint32_t)kList) list[to] = order_key(l, first + at);
     }
 }
@@ -673,7 +704,7 @@ __device__ __forceinline__ bool pick_from_list(const m27q_sampling &p, const Scr
                                                PickShared &s) {
     const int row = blockIdx.x, tid = threadIdx.x, i0 = tid * E;
     const Scale scale = row_scale(r, plan.anchor);
-    const Exp2Unit x(s.octave);
+    const Weights x(s.octave);
     uint64_t key[E];
     uint32_t bucket[E], slot[E];
 #pragma unroll
@@ -689,7 +720,7 @@ __device__ __forceinline__ bool pick_from_list(const m27q_sampling &p, const Scr
         if (e * kRowThreads + tid >= n) continue;
         const Place a = place_of(key_value(key[e]), scale);
         const uint32_t at = s.at[a.bin], count = s.at[a.bin + 1] - at;
-        const float part = ((float)a.k + 0.5f - (float)a.z) * (a.bin < kFine ? 1.0f : 1.0f / kUnit);
+        const float part = a.bin < kFine ? (float)a.z + 0.5f : ((float)a.k + (float)a.z + 0.5f) * (1.0f / kUnit);
         bucket[e] = at + min((uint32_t)fmaxf(part * (float)count, 0.0f), count - 1);
         slot[e] = atomicAdd(&s.count[bucket[e]], 1u);
     }
@@ -824,7 +855,7 @@ __global__ __launch_bounds__(kRowThreads) void k_sample_pick(const m27q_sampling
             s.pick = 0x7fffffff;
             s.most = 0;
         }
-        if (threadIdx.x < kUnit) s.octave[threadIdx.x] = Exp2Unit::factor(threadIdx.x);
+        if (threadIdx.x < kUnit) s.octave[threadIdx.x] = Weights::factor(threadIdx.x);
         const int n = (int)min(plan.listed, (uint32_t)kList);
         if (n <= kRowThreads) done = pick_from_list<1>(p, sc, plan, r, n, s);
         else if (n <= 2 * kRowThreads) done = pick_from_list<2>(p, sc, plan, r, n, s);
