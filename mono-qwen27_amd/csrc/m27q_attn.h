@@ -190,7 +190,7 @@ __device__ __forceinline__ int2 group_places(const AttnParams &p, const Unit &x,
         lo = min(lo, lds[2 * i]);
         hi = max(hi, lds[2 * i + 1]);
     }
-    return make_int2(lo, hi);
+    return make_int2(__builtin_amdgcn_readfirstlane(lo), __builtin_amdgcn_readfirstlane(hi));
 }
 // The place of one of a group's rows.
 __device__ __forceinline__ int place_of(const AttnParams &p, const Unit &x, int token) {
@@ -543,7 +543,7 @@ __device__ __forceinline__ int first_key(const AttnParams &p, int place) {
 // of these sums passes 32 bits), and its part of them: lo a multiple of a tile, hi >= lo, and
 // hi <= max_kv where there are any.
 template <Kind KIND>
-__device__ __forceinline__ void set_keys(const AttnParams &p, Work &w, int len, int shared, int first, int last) {
+__device__ __forceinline__ void set_keys(const AttnParams &p, Work &w, int len, int shared, int first, int last, int part) {
     // tiles lie whole within pages or the other way round
     w.lo = KIND == kOwn ? max(shared, 0) : KIND == kPrefix ? 0 : first_key(p, first) & ~(kKeys - 1);
     w.hi = max(w.lo, min(min(len, (int)p.seqs.max_kv), last + 1));
@@ -551,7 +551,7 @@ __device__ __forceinline__ void set_keys(const AttnParams &p, Work &w, int len, 
     if (parts > 1) {
         const int tiles = (w.hi - w.lo + kKeys - 1) / kKeys, each = (tiles + parts - 1) / parts;
         const int end = w.hi;
-        w.lo += (int)blockIdx.y * each * kKeys;
+        w.lo += part * each * kKeys;
         w.hi = max(w.lo, min(end, w.lo + each * kKeys));
     }
 }
@@ -586,7 +586,17 @@ __global__ __launch_bounds__(kWaves * 64, 2) void k_attn(const AttnParams p) {
     // where that is a multiple of the XCDs they share an L2; the last rows see the most keys
     // and go first
     const unsigned pairs = (KIND == kPrefix ? p.prefix.groups : p.seqs.n) * p.cache.heads;
-    const unsigned fromlast = blockIdx.x / pairs, pair = blockIdx.x - fromlast * pairs;
+    unsigned bx = blockIdx.x, part_id = blockIdx.y;
+    if constexpr (KIND == kPrefix) {
+        // the row tiles of a part of a prefix read the same keys: an XCD (each takes every eighth workgroup) gets
+        // a run of parts, tile by tile
+        const unsigned tiles = gridDim.x / pairs, all = gridDim.x * gridDim.y;
+        const unsigned id = blockIdx.y * gridDim.x + blockIdx.x, xcd = id & 7;
+        const unsigned item = xcd * (all >> 3) + min(xcd, all & 7) + (id >> 3), unit = item / tiles;
+        bx = (item - unit * tiles) * pairs + unit % pairs;
+        part_id = unit / pairs;
+    }
+    const unsigned fromlast = bx / pairs, pair = bx - fromlast * pairs;
     const int s = pair / p.cache.heads;
     Work w;
     w.head = pair - s * p.cache.heads;
@@ -604,16 +614,21 @@ __global__ __launch_bounds__(kWaves * 64, 2) void k_attn(const AttnParams p) {
         last = at.y;
         __syncthreads();
     }
-    set_keys<KIND>(p, w, len, sr.shared, first, last);
+    set_keys<KIND>(p, w, len, sr.shared, first, last, (int)part_id);
 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
     const int wrow = w.row0 + wave * kRows;  // this wave's first row
     const bool live = wrow + (lane & 31) < w.rows;
     const int row = min(wrow + (lane & 31), w.rows - 1);
-    const int token = sr.first + row / group, qh = w.head * group + row % group;
+    int token = sr.first + row / group, qh = w.head * group + row % group;
     R x;
-    x.place = live ? place0 + row / group : -1;
-    if constexpr (KIND == kPrefix) x.place = !live ? -1 : first >= w.hi ? first : place_of(p, sr, token);
+    // (of a group's rows: in LDS while tiles are seen whole, which leaves registers none to spare)
+    __shared__ int places[KIND == kPrefix ? kWaves * kRows : 1];
+    if constexpr (KIND == kPrefix) {
+        if (h == 0) places[wave * kRows + lane] = !live ? -1 : first >= w.hi ? first : place_of(p, sr, token);
+    } else {
+        x.place = live ? place0 + row / group : -1;
+    }
     x.clear();
     typename R::Raw q;
     R::load_q(p, token, qh, q);
@@ -653,6 +668,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void k_attn(const AttnParams p) {
         }
         if (any) x.template tile<false, false>(p, w, sc, w.lo + (t + 1) * kKeys, kb, vb);
     }
+    if constexpr (KIND == kPrefix) x.place = places[wave * kRows + (lane & 31)];
     bool odd = false;
     for (int i = 0; i < tiles - (tb - ta); ++i) {
         const int k0 = w.lo + (i < ta ? i : i + tb - ta) * kKeys;
@@ -690,11 +706,18 @@ __global__ __launch_bounds__(kWaves * 64, 2) void k_attn(const AttnParams p) {
 
     x.l = sum_row<kRows>(x.l);
     if (!live) return;
+    if constexpr (KIND == kPrefix) {  // once more, not kept
+        int r = w.row0;
+        asm volatile("" : "+s"(r));
+        r = min(r + wave * kRows + (lane & 31), w.rows - 1);
+        token = sr.first + r / group;
+        qh = w.head * group + r % group;
+    }
     if (KIND != kAll || p.splits > 1) {
         const long long row0 = ((long long)token * p.q.heads + qh) * p.splits;
-        const long long at = row0 + (KIND == kOwn ? p.prefix_parts : 0) + blockIdx.y;
+        const long long at = row0 + (KIND == kOwn ? p.prefix_parts : 0) + part_id;
         if (h == 0) p.stat[at] = make_float2(x.m * sc, x.l);
-        if (KIND == kOwn && sr.shared < 0 && blockIdx.y == 0 && h == 0)  // no prefix
+        if (KIND == kOwn && sr.shared < 0 && part_id == 0 && h == 0)  // no prefix
             for (int i = 0; i < p.prefix_parts; ++i) p.stat[row0 + i] = make_float2(0, 0);
         if (x.l == 0) return;
         float *o = p.part + at * D;
@@ -753,7 +776,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) void k_attn_few(cons
         last = at.y;
         __syncthreads();
     }
-    set_keys<KIND>(p, w, len, sr.shared, first, last);
+    set_keys<KIND>(p, w, len, sr.shared, first, last, (int)blockIdx.y);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const bool live = (lane & (RW - 1)) < w.rows;
     const int row = min(lane & (RW - 1), w.rows - 1), at = row / group;

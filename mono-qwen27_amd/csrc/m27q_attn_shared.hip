@@ -1,4 +1,6 @@
 // m27q_attn_shared.hip -- attention of sequences that share prefixes.
+#include <algorithm>
+
 #include "m27q_attn.h"
 
 namespace m27q {
@@ -37,10 +39,19 @@ hipError_t launch_t(const AttnParams &p, const SharedPlan &plan, hipStream_t s) 
     return hipGetLastError();
 }
 
-int parts_of(long long wgs, long long once, long long keys, long long least, int limit) {
-    const long long want = (once + wgs - 1) / wgs, most = (keys + least - 1) / least;
-    const long long parts = want < most ? want : most;
-    return parts < 1 ? 1 : parts > limit ? limit : (int)parts;
+// Parts of `keys` keys for `wgs` workgroups a part, of which `slots` run at once: the number whose rounds
+// of workgroups, each as long as a part, take least, a part costing as much as `cost` keys more (its
+// sums written and joined).
+int parts_of(long long wgs, long long slots, long long keys, long long least, long long cost, int limit) {
+    long long best = 1, time = -1;
+    for (long long n = 1; n <= limit && (n == 1 || (keys + n - 1) / n >= least); ++n) {
+        const long long t = (wgs * n + slots - 1) / slots * ((keys + n - 1) / n + cost);
+        if (time < 0 || t < time) {
+            time = t;
+            best = n;
+        }
+    }
+    return (int)best;
 }
 
 }  // namespace
@@ -52,18 +63,22 @@ long long shared_groups(const m27q_seqs &seqs, const m27q_prefixes &prefix, uint
     return a > b ? a : b;
 }
 
-// Parts as in attn_plan, the prefix's at most 48 of the join's 64 and the own ones the rest.
+// The prefix's parts, at most 48 of the join's 64, and those of a sequence's own keys.
 SharedPlan shared_plan(const m27q_seqs &seqs, const m27q_prefixes &prefix, uint32_t q_heads, const m27q_cache &cache,
                        int cus) {
     const long long group = q_heads / cache.heads;
     SharedPlan r{};
     const long long rows = prefix.max_rows * group, wgs = tiles_of(rows) * prefix.groups * cache.heads;
+    const long long shared = prefix.max_len < seqs.max_kv ? prefix.max_len : seqs.max_kv;
     r.prefix.few = rows <= kRows;
-    r.prefix.splits = parts_of(wgs, (r.prefix.few && cache.dim == 256 ? 1ll : 2ll) * cus, prefix.max_len,
-                               r.prefix.few ? 128 : 256, 48);
-    m27q_seqs own = seqs;
-    r.own = attn_plan(own, q_heads, cache, cus);
-    if (r.own.splits > kMaxSplits - r.prefix.splits) r.own.splits = kMaxSplits - r.prefix.splits;
+    r.prefix.splits = parts_of(wgs, (r.prefix.few && cache.dim == 256 ? 1ll : 2ll) * cus, shared, r.prefix.few ? 128 : 256,
+                               r.prefix.few ? 128 : 384, 48);
+    // own keys: as many as the longest sequence has behind the longest prefix; ragged lengths even out over
+    // four rounds of workgroups
+    const long long own = (long long)seqs.max_kv - shared, owgs = attn_groups(seqs, q_heads, cache);
+    r.own.few = (long long)seqs.max_q * group <= kRows;
+    const long long want = (r.own.few ? 4ll : 2ll) * cus / owgs, most = own / 256, limit = kMaxSplits - r.prefix.splits;
+    r.own.splits = (int)std::max(1ll, std::min({want, most, limit}));
     return r;
 }
 
