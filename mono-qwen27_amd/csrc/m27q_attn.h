@@ -557,12 +557,13 @@ __device__ __forceinline__ void set_keys(const AttnParams &p, Work &w, int len, 
 }
 
 // Looks at every page of the keys once, the threads of a workgroup in turn: tiles trust them then.
+template <int NW = kWaves>
 __device__ __forceinline__ bool has_gaps(const AttnParams &p, const Work &w) {
     const int shift = __builtin_ctz(p.cache.page_size);
     const int32_t *table = p.seqs.table + (long long)w.s * p.seqs.table_stride;
     bool bad = false;
     if (w.lo < w.hi)
-        for (int i = (w.lo >> shift) + (int)threadIdx.x; i <= (w.hi - 1) >> shift; i += kWaves * 64)
+        for (int i = (w.lo >> shift) + (int)threadIdx.x; i <= (w.hi - 1) >> shift; i += NW * 64)
             bad |= (uint32_t)table[i] >= p.cache.pages;
     return bad;
 }
@@ -753,13 +754,13 @@ __global__ __launch_bounds__(kWaves * 64, 2) void k_attn(const AttnParams p) {
 // join.  One token over 1021 keys: a tile a wave, and a chain of 16000 cycles (lengths 3500, page
 // and loads 2700, their arrival 2500, products and weights 2800, the waves' join 4300), then 3 us
 // of the parts' join.
-template <int D, bool BF, int NP, int RW, Kind KIND = kAll>
-__global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) void k_attn_few(const AttnParams p) {
+template <int D, bool BF, int NP, int RW, Kind KIND = kAll, int NW = kWaves>
+__global__ __launch_bounds__(NW * 64, D == 256 ? 1 : 2) void k_attn_few(const AttnParams p) {
     typedef Rows<D, BF, NP, RW> R;
     typedef typename R::T T;
     constexpr int TB = kKeys * D * 2;  // bytes of a tile
-    __shared__ __attribute__((aligned(1024))) char kts[kWaves * TB], vts[kWaves * TB];
-    __shared__ float ms[kWaves][RW], ls[kWaves][RW];
+    __shared__ __attribute__((aligned(1024))) char kts[NW * TB], vts[NW * TB];
+    __shared__ float ms[NW][RW], ls[NW][RW];
     const int group = (int)(p.q.heads / p.cache.heads);
     const int s = blockIdx.x / p.cache.heads;
     Work w;
@@ -786,7 +787,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) void k_attn_few(cons
     // loads end in order: what is needed first is asked for first
     typename R::Raw q;
     R::load_q(p, token, qh, q);
-    const bool gaps = has_gaps(p, w);
+    const bool gaps = has_gaps<NW>(p, w);
     LDS_AS char *const kt = (LDS_AS char *)kts + wave * TB, *const vt = (LDS_AS char *)vts + wave * TB;
     const int32_t *table = p.seqs.table + (long long)w.s * p.seqs.table_stride;
     const int shift = __builtin_ctz(p.cache.page_size);
@@ -828,7 +829,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) void k_attn_few(cons
     const int tiles = (w.hi - w.lo + kKeys - 1) / kKeys;
     int tb = max(0, min(first + 1, w.hi) - w.lo) / kKeys;
     int ta = p.window ? min(tb, (max(0, first_key(p, last) - w.lo) + kKeys - 1) / kKeys) : 0;
-    int t = ta + ((wave - ta) & (kWaves - 1));  // this wave's first
+    int t = ta + ((wave - ta) & (NW - 1));  // this wave's first
     int ids[2];
     if (t < tb) {
         ids[0] = page(w.lo + t * kKeys, 0);
@@ -839,7 +840,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) void k_attn_few(cons
     // a wave that has none of them asks for its first one of the others
     int there = -1;
     if (t >= tb) {
-        for (there = wave; there >= ta && there < tb;) there += kWaves;
+        for (there = wave; there >= ta && there < tb;) there += NW;
         if (there < tiles) {
             ids[0] = page(w.lo + there * kKeys, 0);
             ids[1] = page(w.lo + there * kKeys, 1);
@@ -860,8 +861,8 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) void k_attn_few(cons
     }
     typename R::T8 pcs[R::NV][NP];
     float sco[R::NS];
-    for (; t < tb; t += kWaves) {
-        const int k0 = w.lo + t * kKeys, k1 = k0 + kWaves * kKeys;
+    for (; t < tb; t += NW) {
+        const int k0 = w.lo + t * kKeys, k1 = k0 + NW * kKeys;
         ids[0] = page(k1, 0);
         ids[1] = page(k1, 1);
         // K is there when no more than V's loads are on their way
@@ -869,15 +870,15 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) void k_attn_few(cons
         x.template scores<true>(kt, sco);
         x.template weights<false>(p, w, sc, sco, k0, pcs);
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        if (t + kWaves < tb) load(p.cache.k, kt, true, k1, ids, false);
+        if (t + NW < tb) load(p.cache.k, kt, true, k1, ids, false);
         x.template values<true>(vt, pcs);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // V has been read
-        if (t + kWaves < tb) load(p.cache.v, vt, false, k1, ids, false);
+        if (t + NW < tb) load(p.cache.v, vt, false, k1, ids, false);
     }
     // the others, which begin where none of those is
-    const auto other = [&](int t) { return t >= ta && t < tb ? t + ((tb - t + kWaves - 1) & ~(kWaves - 1)) : t; };
+    const auto other = [&](int t) { return t >= ta && t < tb ? t + ((tb - t + NW - 1) & ~(NW - 1)) : t; };
     bool odd = false;
-    for (int t = other(wave); t < tiles; t = other(t + kWaves)) {
+    for (int t = other(wave); t < tiles; t = other(t + NW)) {
         const int k0 = w.lo + t * kKeys;
         if (t != there) {
             ids[0] = page(k0, 0);
@@ -896,7 +897,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) void k_attn_few(cons
     if (__builtin_expect(ta < tb && __any(x.odd_sums()), 0)) {
         x.clear();
         ta = tb = 0;
-        for (int t = wave; t < tiles; t += kWaves) {
+        for (int t = wave; t < tiles; t += NW) {
             const int k0 = w.lo + t * kKeys, ids[2] = {page(k0, 0), page(k0, 1)};
             load(p.cache.k, kt, true, k0, ids, true);
             load(p.cache.v, vt, false, k0, ids, true);
@@ -908,7 +909,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) void k_attn_few(cons
         }
     }
     if (__builtin_expect(__any(odd), 0))
-        for (int t = other(wave); t < tiles; t = other(t + kWaves)) {
+        for (int t = other(wave); t < tiles; t = other(t + NW)) {
             const int k0 = w.lo + t * kKeys, ids[2] = {page(k0, 0), page(k0, 1)};
             load(p.cache.v, vt, false, k0, ids, true);
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
@@ -927,7 +928,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) void k_attn_few(cons
     __syncthreads();
     float m = ms[0][col];
 #pragma unroll
-    for (int i = 1; i < kWaves; ++i) m = fmaxf(m, ms[i][col]);
+    for (int i = 1; i < NW; ++i) m = fmaxf(m, ms[i][col]);
     constexpr int HALF = TB / (RW * 16);  // quadruples of a tile's room
     if (x.l != 0) {
         const float f = join_factor((x.m - m) * sc);
@@ -943,21 +944,21 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) void k_attn_few(cons
             }
     }
     __syncthreads();
-    float fs[kWaves], l = 0;
+    float fs[NW], l = 0;
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
+    for (int i = 0; i < NW; ++i) {
         fs[i] = ls[i][col];
         const float e = ms[i][col] == -__builtin_inff() ? 0.0f : join_factor((ms[i][col] - m) * sc);
         l += ls[i][col] * e;
     }
     if (!live) return;
-    constexpr int Q = D / 4 * RW / (kWaves * 64);  // quadruples of a thread
-    f32x4 y[Q][kWaves], o[Q];
+    constexpr int Q = D / 4 * RW / (NW * 64);  // quadruples of a thread
+    f32x4 y[Q][NW], o[Q];
 #pragma unroll
     for (int u = 0; u < Q; ++u)  // all reads at once: what a wave without keys left is read and dropped
 #pragma unroll
-        for (int i = 0; i < kWaves; ++i) {
-            const int quad = threadIdx.x / RW + u * (kWaves * 64 / RW);
+        for (int i = 0; i < NW; ++i) {
+            const int quad = threadIdx.x / RW + u * (NW * 64 / RW);
             y[u][i] = *(const LDS_AS f32x4 *)((LDS_AS char *)(quad < HALF ? kts : vts - TB) + i * TB + (quad * RW + col) * 16);
         }
     __builtin_amdgcn_sched_barrier(0);
@@ -965,7 +966,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) void k_attn_few(cons
     for (int u = 0; u < Q; ++u) {
         o[u] = f32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int i = 0; i < kWaves; ++i)
+        for (int i = 0; i < NW; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) o[u][j] += fs[i] != 0 ? y[u][i][j] : 0.0f;
     }
@@ -976,14 +977,14 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) void k_attn_few(cons
         if (l == 0) return;
 #pragma unroll
         for (int u = 0; u < Q; ++u)
-            *(f32x4 *)(p.part + part * D + 4 * (threadIdx.x / RW + u * (kWaves * 64 / RW))) = o[u];
+            *(f32x4 *)(p.part + part * D + 4 * (threadIdx.x / RW + u * (NW * 64 / RW))) = o[u];
         return;
     }
     const long long to = (long long)token * p.out.token_stride + (long long)qh * p.out.head_stride;
     const float inv = l == 0 ? 0.0f : 1.0f / l;
 #pragma unroll
     for (int u = 0; u < Q; ++u) {
-        const int quad = threadIdx.x / RW + u * (kWaves * 64 / RW);
+        const int quad = threadIdx.x / RW + u * (NW * 64 / RW);
         const f32x4 x = l == 0 ? f32x4{0, 0, 0, 0} : o[u] * inv;
         if (p.out.type == M27Q_TYPE_F32) *(f32x4 *)((float *)p.out.ptr + to + 4 * quad) = x;
         else *(typename R::T4 *)((T *)p.out.ptr + to + 4 * quad) = __builtin_convertvector(x, typename R::T4);

@@ -13,8 +13,9 @@ template <int D, bool BF, int NP, Kind KIND>
 void launch_kind(const AttnParams &p, bool few, long long rows, unsigned units, int parts, hipStream_t s) {
     if (few) {
         const dim3 grid(units * p.cache.heads, parts);
-        if (rows <= 16) hipLaunchKernelGGL((k_attn_few<D, BF, NP, 16, KIND>), grid, dim3(kWaves * 64), 0, s, p);
-        else hipLaunchKernelGGL((k_attn_few<D, BF, NP, kRows, KIND>), grid, dim3(kWaves * 64), 0, s, p);
+        constexpr int NW = KIND == kOwn && D == 256 ? 2 : kWaves;
+        if (rows <= 16) hipLaunchKernelGGL((k_attn_few<D, BF, NP, 16, KIND, NW>), grid, dim3(NW * 64), 0, s, p);
+        else hipLaunchKernelGGL((k_attn_few<D, BF, NP, kRows, KIND, NW>), grid, dim3(NW * 64), 0, s, p);
     } else {
         const dim3 grid((unsigned)(tiles_of(rows) * units * p.cache.heads), parts);
         hipLaunchKernelGGL((k_attn<D, BF, NP, KIND>), grid, dim3(kWaves * 64), 0, s, p);
@@ -39,19 +40,10 @@ hipError_t launch_t(const AttnParams &p, const SharedPlan &plan, hipStream_t s) 
     return hipGetLastError();
 }
 
-// Parts of `keys` keys for `wgs` workgroups a part, of which `slots` run at once: the number whose rounds
-// of workgroups, each as long as a part, take least, a part costing as much as `cost` keys more (its
-// sums written and joined).
-int parts_of(long long wgs, long long slots, long long keys, long long least, long long cost, int limit) {
-    long long best = 1, time = -1;
-    for (long long n = 1; n <= limit && (n == 1 || (keys + n - 1) / n >= least); ++n) {
-        const long long t = (wgs * n + slots - 1) / slots * ((keys + n - 1) / n + cost);
-        if (time < 0 || t < time) {
-            time = t;
-            best = n;
-        }
-    }
-    return (int)best;
+// Parts of `keys` keys, as many as run at once: two workgroups on each CU, or one of few rows of 256 (its tiles
+// take the LDS).
+int parts_of(long long wgs, long long slots, long long keys, long long least, long long limit) {
+    return (int)std::max(1ll, std::min({slots / wgs, (keys + least - 1) / least, limit}));
 }
 
 }  // namespace
@@ -63,22 +55,23 @@ long long shared_groups(const m27q_seqs &seqs, const m27q_prefixes &prefix, uint
     return a > b ? a : b;
 }
 
-// The prefix's parts, at most 48 of the join's 64, and those of a sequence's own keys.
+// The prefix's parts, at most 48 of the join's 64, and those of a sequence's own keys, of which there are as
+// many as the longest sequence has behind the longest prefix: parts of 64, a tile for each of two waves, at least.
+// Measured, with other numbers of parts: 64 tokens behind 32768 places 150 us with 42 of the prefix, 151 with 21, 32
+// and 40; 3 groups of 8 x 5 tokens behind 12000 places 80 with 21, 83 with 16, 98 with 10; 8 prompts of 301
+// behind 8192 places 473 with 1, 507, 543 and 472 with 2, 3 and 4.  Own keys: 64 sequences 150 with 2, 156, 154 and 157
+// with 1, 3 and 6; 4 sequences 23.1 with 5, 27.8, 25.5 and 24.0 with 1, 2 and 10.
 SharedPlan shared_plan(const m27q_seqs &seqs, const m27q_prefixes &prefix, uint32_t q_heads, const m27q_cache &cache,
                        int cus) {
-    const long long group = q_heads / cache.heads;
-    SharedPlan r{};
+    const long long group = q_heads / cache.heads, slots = 2ll * cus;
     const long long rows = prefix.max_rows * group, wgs = tiles_of(rows) * prefix.groups * cache.heads;
     const long long shared = prefix.max_len < seqs.max_kv ? prefix.max_len : seqs.max_kv;
+    SharedPlan r{};
     r.prefix.few = rows <= kRows;
-    r.prefix.splits = parts_of(wgs, (r.prefix.few && cache.dim == 256 ? 1ll : 2ll) * cus, shared, r.prefix.few ? 128 : 256,
-                               r.prefix.few ? 128 : 384, 48);
-    // own keys: as many as the longest sequence has behind the longest prefix; ragged lengths even out over
-    // four rounds of workgroups
-    const long long own = (long long)seqs.max_kv - shared, owgs = attn_groups(seqs, q_heads, cache);
+    r.prefix.splits = parts_of(wgs, r.prefix.few && cache.dim == 256 ? cus : slots, shared, r.prefix.few ? 128 : 256, 48);
     r.own.few = (long long)seqs.max_q * group <= kRows;
-    const long long want = (r.own.few ? 4ll : 2ll) * cus / owgs, most = own / 256, limit = kMaxSplits - r.prefix.splits;
-    r.own.splits = (int)std::max(1ll, std::min({want, most, limit}));
+    r.own.splits = parts_of(attn_groups(seqs, q_heads, cache), slots, (long long)seqs.max_kv - shared, r.own.few ? 64 : 256,
+                            kMaxSplits - r.prefix.splits);
     return r;
 }
 
