@@ -446,38 +446,55 @@ __device__ __forceinline__ int part_bin(int J, int off) {
 constexpr int kPlanThreads = 512;
 static_assert(kBins + 1 == kPlanThreads, "a thread a bin");
 
+// The largest of a wave's values, all above 0, for every lane.
+__device__ __forceinline__ unsigned long long max_wave(unsigned long long v) {
+    v = max(v, moved<0x111, 0xf>(v));
+    v = max(v, moved<0x112, 0xf>(v));
+    v = max(v, moved<0x114, 0xf>(v));
+    v = max(v, moved<0x118, 0xf>(v));
+    v = max(v, moved<0x142, 0xa>(v));
+    v = max(v, moved<0x143, 0xc>(v));
+    return (unsigned long long)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), 63) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+// Numbers in their order as bits, and back.
+__device__ __forceinline__ unsigned long long ordered(double v) {
+    const long long b = __builtin_bit_cast(long long, v);
+    return (unsigned long long)(b ^ (b >> 63 | (long long)(1ull << 63)));
+}
+__device__ __forceinline__ double unordered(unsigned long long u) {
+    return __builtin_bit_cast(double, u >> 63 ? u ^ 1ull << 63 : ~u);
+}
+
+// The first of `n` <= 512 values that do not descend which reaches a target (n: none does), by a wave: of every
+// eighth, then of eight.
+template <typename T, typename F>
+__device__ __forceinline__ int first_of(const T *v, int n, F reaches) {
+    const int lane = threadIdx.x & 63;
+    const unsigned long long far = __ballot(8 * lane < n && reaches(v[min(8 * lane + 7, n - 1)]));
+    if (!far) return n;
+    const int i = 8 * __builtin_ctzll(far), j = min(i + (lane & 7), n - 1);
+    return i + __builtin_ctzll(__ballot(reaches(v[j])));
+}
+
 // A row's bins from those of its parts, and the bins in which its borders can lie: of the top_k-th
 // token, of top_p, of min_p and of the pick.  What is not known before another border is found
-// leaves a range of bins.
+// leaves a range of bins.  A chain of steps that wait for each other bounds it: each wave does
+// for itself what is not a bin's (it took 11.4 us with the workgroup's threads looking for each border).
 __global__ __launch_bounds__(kPlanThreads) void k_sample_plan(const m27q_sampling p, const Scratch sc) {
-    __shared__ unsigned long long lds[kPlanThreads / 64], best_s;
-    __shared__ uint32_t lds32[kPlanThreads / 64], lds_at[kPlanThreads / 64];
-    __shared__ double anchors[kPlanThreads / 64];
-    __shared__ int found[8], off_s[kPlanThreads];
-    __shared__ unsigned long long sum[kBins + 2];
-    const int row = blockIdx.x, J = threadIdx.x;
+    constexpr int W = kPlanThreads / 64;
+    __shared__ unsigned long long mass_s[W], sum[kBins + 2];
+    __shared__ uint32_t count_s[W], tokens_s[kBins + 2];  // down to a bin, without it
+    const int row = blockIdx.x, J = threadIdx.x, lane = J & 63, wave = J >> 6;
     const Part *part = sc.part + (long long)row * sc.parts;
     const Rule r = row_rule(p, row);
     RowPlan &out = sc.plan[row];
-    if (J == 0) best_s = 0;
-    if (J < 8) found[J] = kBins;
-    double anchor = -__builtin_inf();
-    unsigned long long best = 0;
-    for (int i = J; i < sc.parts; i += kPlanThreads) {
-        anchor = fmax(anchor, part[i].anchor);
+    unsigned long long best = 0, high = 0;
+    for (int i = lane; i < sc.parts; i += 64) {
+        high = max(high, ordered(part[i].anchor));
         best = max(best, (unsigned long long)part[i].best);
     }
-#pragma unroll
-    for (int o = 32; o; o >>= 1) {
-        anchor = fmax(anchor, __shfl_xor(anchor, o));
-        best = max(best, (unsigned long long)__shfl_xor(best, o));
-    }
-    if ((J & 63) == 0) anchors[J >> 6] = anchor;
-    __syncthreads();
-    if ((J & 63) == 0) atomicMax(&best_s, best);
-    for (int i = 0; i < kPlanThreads / 64; ++i) anchor = fmax(anchor, anchors[i]);
-    __syncthreads();
-    best = best_s;
+    best = max_wave(best);
+    const double anchor = unordered(max_wave(high));
     const float top = key_value(best);
     if (r.greedy || !__builtin_isfinite(top)) {
         if (J == 0) {
@@ -488,66 +505,69 @@ __global__ __launch_bounds__(kPlanThreads) void k_sample_plan(const m27q_samplin
         return;
     }
 
-    // this thread's bin, from one stored sum of each part: the same bin there, or, where an octave here lies
-    // among the part's fine bins, their octave
+    // this thread's bin, from one stored sum of each part
     unsigned long long mass = 0;
     uint32_t count = 0;
     constexpr unsigned long long kMask = (1ull << kSumBits) - 1;
-    constexpr int kSkip = 1 << 20;
-    for (int i0 = 0; i0 < sc.parts; i0 += kPlanThreads) {
-        const int parts = min(sc.parts - i0, kPlanThreads);
-        if (J < parts) {
-            const double off = anchor - part[i0 + J].anchor;
-            off_s[J] = off < kReach ? (int)off : kSkip;
-        }
-        __syncthreads();
+    constexpr int kSkip = 1 << 20, AT = 32;  // parts on their way at a time
+    for (int i0 = 0; i0 < sc.parts; i0 += AT) {
+        const double down = anchor - part[min(i0 + (lane & (AT - 1)), sc.parts - 1)].anchor;
+        const int offs = i0 + (lane & (AT - 1)) < sc.parts && down < kReach ? (int)down : kSkip;
         const unsigned long long *bins = sc.bins + ((long long)row * sc.parts + i0) * kStored;
-        constexpr int AT = 32;  // on their way at a time
-        for (int i = 0; i < parts; i += AT) {
-            unsigned long long x[AT];
-            bool ok[AT];
+        unsigned long long x[AT];
+        bool ok[AT];
 #pragma unroll
-            for (int k = 0; k < AT; ++k) {
-                const int j = min(i + k, parts - 1), off = off_s[j], from = part_bin(J, off);
-                ok[k] = i + k < parts && off != kSkip && from >= 0;
-                x[k] = bins[(long long)(ok[k] ? j : 0) * kStored + (ok[k] ? from : 0)];
-            }
-#pragma unroll
-            for (int k = 0; k < AT; ++k) {
-                count += ok[k] ? (uint32_t)(x[k] >> kSumBits) : 0u;
-                mass += ok[k] ? x[k] & kMask : 0ull;
-            }
+        for (int k = 0; k < AT; ++k) {
+            const int off = __builtin_amdgcn_readlane(offs, k), from = part_bin(J, off);
+            ok[k] = off != kSkip && from >= 0;
+            x[k] = bins[(off != kSkip ? k * kStored : 0) + (ok[k] ? from : 0)];
         }
-        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < AT; ++k) {
+            count += ok[k] ? (uint32_t)(x[k] >> kSumBits) : 0u;
+            mass += ok[k] ? x[k] & kMask : 0ull;
+        }
     }
     const double unit = sum_unit(p.n) * bin_scale(J);
     mass = (unsigned long long)__builtin_rint((double)mass * unit);
-    unsigned long long total;
-    uint32_t tokens;
-    const unsigned long long above = scan_group<kPlanThreads>(mass, lds, total);
-    const uint32_t before = scan_group<kPlanThreads>(count, lds32, tokens);
-    sum[J] = above;
-    if (J == kBins) sum[kBins + 1] = total;
-
-    // the bin in which the running sum reaches a target, the last one that holds a token if none does
-    auto bin_at = [&](int slot, double target) {
-        if (count && (double)(above + mass) >= target && (before == 0 || (double)above < target)) found[slot] = J;
-        __syncthreads();
-        return found[slot];
-    };
-    if (count && before + count == tokens) found[7] = J;
-    if (count && before < (uint32_t)r.k && before + count >= (uint32_t)r.k && (uint32_t)r.k < tokens) found[0] = J;
+    unsigned long long above = scan_wave(mass);
+    uint32_t before = scan_wave(count);
+    if (lane == 63) {
+        mass_s[wave] = above;
+        count_s[wave] = before;
+    }
     __syncthreads();
-    const int last = found[7], kb = found[0];
-    const bool k_cuts = kb < kBins;
+    above -= mass;
+    before -= count;
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+        above += i < wave ? mass_s[i] : 0ull;
+        before += i < wave ? count_s[i] : 0u;
+    }
+    sum[J] = above;
+    tokens_s[J] = before;
+    if (J == kBins) {
+        sum[kBins + 1] = above + mass;
+        tokens_s[kBins + 1] = before + count;
+    }
+    __syncthreads();
+
+    const unsigned long long total = sum[kBins];
+    const uint32_t tokens = tokens_s[kBins];
+    const auto bin_at = [&](double target) {  // the bin in which the running sum reaches it, the last one that holds a token if none does
+        const double t = fmax(target, 1.0);   // (the first token's own bin holds far more)
+        return first_of(sum + 1, kBins, [&](unsigned long long v) { return (double)v >= t || v == total; });
+    };
+    const bool k_cuts = (uint32_t)r.k < tokens;
+    const int kb = k_cuts ? first_of(tokens_s + 1, kBins, [&](uint32_t v) { return v >= (uint32_t)r.k; }) : kBins;
     // the sum of the first top_k
     const double s_lo = (double)(k_cuts ? sum[kb] : total), s_hi = (double)(k_cuts ? sum[kb + 1] : total);
     double t_lo = s_lo, t_hi = s_hi;  // the sum of what is kept
     int p0 = kBins, p1 = -1, m0 = kBins, m1 = -1;
     unsigned long long min_p_sum = total;
     if (r.top_p < 1.0) {
-        p0 = min(bin_at(1, r.top_p * s_lo), last);
-        p1 = min(bin_at(2, r.top_p * s_hi), last);
+        p0 = bin_at(r.top_p * s_lo);
+        p1 = bin_at(r.top_p * s_hi);
         t_lo = fmin(t_lo, (double)sum[p0]);
         t_hi = fmin(t_hi, (double)sum[p1 + 1]);
     }
@@ -563,30 +583,52 @@ __global__ __launch_bounds__(kPlanThreads) void k_sample_plan(const m27q_samplin
             t_hi = fmin(t_hi, (double)min_p_sum);
         }
     }
-    const int q0 = min(bin_at(3, r.u * t_lo), last), q1 = min(bin_at(4, r.u * t_hi), last);
-    const bool mark = count && (J == kb || (J >= p0 && J <= p1) || (J >= m0 && J <= m1) || (J >= q0 && J <= q1));
-    uint32_t listed;
-    const uint32_t at = scan_group<kPlanThreads>(mark ? count : 0u, lds_at, listed);
+    const int q0 = bin_at(r.u * t_lo), q1 = bin_at(r.u * t_hi);
+    // the marked ranges in order, without what an earlier one has
+    int b0[kRanges] = {k_cuts ? kb : kBins, p0, m0, q0}, b1[kRanges] = {k_cuts ? kb : -1, p1, m1, q1};
+#pragma unroll
+    for (int i = 1; i < kRanges; ++i)
+#pragma unroll
+        for (int j = kRanges - 1; j >= i; --j)
+            if (b0[j] < b0[j - 1]) {
+                const int x = b0[j], y = b1[j];
+                b0[j] = b0[j - 1];
+                b1[j] = b1[j - 1];
+                b0[j - 1] = x;
+                b1[j - 1] = y;
+            }
+    uint32_t at = 0, listed = 0;
+    int end = -1;
+#pragma unroll
+    for (int j = 0; j < kRanges; ++j) {
+        b0[j] = max(b0[j], end + 1);
+        end = max(end, b1[j]);
+        if (b1[j] < b0[j]) continue;
+        const uint32_t from = tokens_s[b0[j]];
+        at += tokens_s[min(max(J, b0[j]), b1[j] + 1)] - from;
+        listed += tokens_s[b1[j] + 1] - from;
+    }
     out.sum[J] = above;
     out.unit[J] = unit;
     out.before[J] = before;
     out.at[J] = at;
-    if (J < kRanges) {
-        // logits of bins b0 .. b1, and a little more than those
-        const int b0 = J == 0 ? kb : J == 1 ? p0 : J == 2 ? m0 : q0, b1 = J == 0 ? (k_cuts ? kb : -1) : J == 1 ? p1 : J == 2 ? m1 : q1;
-        const double c = kUnitsPerNat * r.inv_t, up = anchor - bin_distance(b0) + 0.5;
-        const double down = anchor - bin_distance(b1) - (b1 < kFine ? 0.5 : kUnit - 0.5);
-        const bool none = b1 < b0, all = !(c > 1e-30);
-        const double eps = 0x1p-20;
-        out.first[J] = b0;
-        out.last[J] = b1;
-        const float lo = none ? __builtin_inff() : all ? -__builtin_inff() : (float)(down / c - fabs(down / c) * eps);
-        const float least = fminf(fminf(__shfl(lo, 0), __shfl(lo, 1)), fminf(__shfl(lo, 2), __shfl(lo, 3)));
-        if (J == 0) out.least = least;
-        out.lo[J] = lo;
-        out.hi[J] = none ? -__builtin_inff() : all ? __builtin_inff() : (float)(up / c + fabs(up / c) * eps);
-    }
     if (J == 0) {
+        const double c = kUnitsPerNat * r.inv_t;
+        float least = __builtin_inff();
+#pragma unroll
+        for (int j = 0; j < kRanges; ++j) {
+            // logits of the bins, and a little more than those
+            const double up = (anchor - bin_distance(b0[j]) + 0.5) / c;
+            const double down = (anchor - bin_distance(b1[j]) - (b1[j] < kFine ? 0.5 : kUnit - 0.5)) / c;
+            const bool none = b1[j] < b0[j], all = !(c > 1e-30);
+            const float lo = none ? __builtin_inff() : all ? -__builtin_inff() : (float)(down - fabs(down) * 0x1p-20);
+            out.first[j] = b0[j];
+            out.last[j] = b1[j];
+            out.lo[j] = lo;
+            out.hi[j] = none ? -__builtin_inff() : all ? __builtin_inff() : (float)(up + fabs(up) * 0x1p-20);
+            least = fminf(least, lo);
+        }
+        out.least = least;
         out.anchor = anchor;
         out.best = best;
         out.min_p_sum = min_p_sum;
