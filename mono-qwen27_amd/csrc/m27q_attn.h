@@ -568,6 +568,14 @@ __device__ __forceinline__ bool has_gaps(const AttnParams &p, const Work &w) {
     return bad;
 }
 
+// The four tiles in LDS of a workgroup of many rows, apart for the compiler: what is on its way into one does not
+// keep reads of another waiting.
+template <int D, int I>
+__device__ __forceinline__ LDS_AS char *tile_lds() {
+    __shared__ __attribute__((aligned(1024))) char tile[kKeys * D * 2];
+    return (LDS_AS char *)tile;
+}
+
 // Many rows: four waves of 32 rows a workgroup, K and V of a tile of 32 keys in LDS, the next
 // tile on its way while this one is worked on (two workgroups a CU: what one waits for, the
 // other works).  Tiles that every row sees whole are taken without masks, those at the ends of
@@ -576,23 +584,24 @@ __device__ __forceinline__ bool has_gaps(const AttnParams &p, const Work &w) {
 // 8192^3 runs at 1208), F16 676; to F32, with the second product once for each piece of a weight,
 // 1170 and 937.  A window shorter than a workgroup's tokens leaves no tile whole, so that nothing
 // is on its way while a tile is worked on: 2048 rows 114 us without a window, 73 with one of 128.
-template <int D, bool BF, int NP, Kind KIND = kAll>
-__global__ __launch_bounds__(kWaves * 64, 2) void k_attn(const AttnParams p) {
+// Workgroup (bx, by) of (nx, ny).
+template <int D, bool BF, int NP, Kind KIND>
+__device__ __forceinline__ void attn_many(const AttnParams &p, unsigned bx, unsigned by, unsigned nx, unsigned ny) {
     typedef Rows<D, BF, NP, kRows> R;
     typedef typename R::T T;
-    __shared__ __attribute__((aligned(1024))) char kt0[kKeys * D * 2], vt0[kKeys * D * 2];
-    __shared__ __attribute__((aligned(1024))) char kt1[kKeys * D * 2], vt1[kKeys * D * 2];
+    LDS_AS char *const ka = tile_lds<D, 0>(), *const va = tile_lds<D, 1>();
+    LDS_AS char *const kb = tile_lds<D, 2>(), *const vb = tile_lds<D, 3>();
     const int group = (int)(p.q.heads / p.cache.heads);
     // workgroups of one (sequence, head) are seqs * heads apart in dispatch order, so that
     // where that is a multiple of the XCDs they share an L2; the last rows see the most keys
     // and go first
     const unsigned pairs = (KIND == kPrefix ? p.prefix.groups : p.seqs.n) * p.cache.heads;
-    unsigned bx = blockIdx.x, part_id = blockIdx.y;
+    unsigned part_id = by;
     if constexpr (KIND == kPrefix) {
         // the row tiles of a part of a prefix read the same keys: an XCD (each takes every eighth workgroup) gets
         // a run of parts, tile by tile
-        const unsigned tiles = gridDim.x / pairs, all = gridDim.x * gridDim.y;
-        const unsigned id = blockIdx.y * gridDim.x + blockIdx.x, xcd = id & 7;
+        const unsigned tiles = nx / pairs, all = nx * ny;
+        const unsigned id = by * nx + bx, xcd = id & 7;
         const unsigned item = xcd * (all >> 3) + min(xcd, all & 7) + (id >> 3), unit = item / tiles;
         bx = (item - unit * tiles) * pairs + unit % pairs;
         part_id = unit / pairs;
@@ -604,13 +613,13 @@ __global__ __launch_bounds__(kWaves * 64, 2) void k_attn(const AttnParams p) {
     const Unit sr = unit_rows<KIND>(p, s);
     w.s = sr.s;
     w.rows = sr.count * group;
-    w.row0 = (int)(gridDim.x / pairs - 1 - fromlast) * kWaves * kRows;
+    w.row0 = (int)(nx / pairs - 1 - fromlast) * kWaves * kRows;
     if (w.row0 >= w.rows) return;
     const int len = max(sr.len, 0), place0 = len - (sr.end - sr.first);  // of the sequence's first row
     int first = place0 + w.row0 / group;
     int last = place0 + (min(w.row0 + kWaves * kRows, w.rows) - 1) / group;
     if constexpr (KIND == kPrefix) {
-        const int2 at = group_places(p, sr, (int *)kt0);
+        const int2 at = group_places(p, sr, (int *)(char *)ka);
         first = at.x;
         last = at.y;
         __syncthreads();
@@ -647,8 +656,6 @@ __global__ __launch_bounds__(kWaves * 64, 2) void k_attn(const AttnParams p) {
         ta = p.window ? min(tb, (max(0, first_key(p, last) - w.lo) + kKeys - 1) / kKeys) : 0;
     }
     const bool any = wrow < w.rows;
-    LDS_AS char *const ka = (LDS_AS char *)kt0, *const va = (LDS_AS char *)vt0;
-    LDS_AS char *const kb = (LDS_AS char *)kt1, *const vb = (LDS_AS char *)vt1;
     int id = ta < tb ? tile_page(p, w, w.lo + ta * kKeys) : 0;
     if (ta < tb) {
         load_tile<D, false>(p, w, w.lo + ta * kKeys, id, ka, va);
@@ -742,6 +749,11 @@ __global__ __launch_bounds__(kWaves * 64, 2) void k_attn(const AttnParams p) {
             if (p.out.type == M27Q_TYPE_F32) *(f32x4 *)((float *)p.out.ptr + at) = v;
             else *(typename R::T4 *)((T *)p.out.ptr + at) = __builtin_convertvector(v, typename R::T4);
         }
+}
+
+template <int D, bool BF, int NP>
+__global__ __launch_bounds__(kWaves * 64, 2) void k_attn(const AttnParams p) {
+    attn_many<D, BF, NP, kAll>(p, blockIdx.x, blockIdx.y, gridDim.x, gridDim.y);
 }
 
 // Few rows (up to 32 of a sequence and cache head): the cache's bytes bound it.  The waves

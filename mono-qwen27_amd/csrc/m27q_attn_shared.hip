@@ -9,31 +9,42 @@ namespace {
 
 long long tiles_of(long long rows) { return (rows + kWaves * kRows - 1) / (kWaves * kRows); }
 
-template <int D, bool BF, int NP, Kind KIND>
-void launch_kind(const AttnParams &p, bool few, long long rows, unsigned units, int parts, hipStream_t s) {
-    if (few) {
-        const dim3 grid(units * p.cache.heads, parts);
-        constexpr int NW = KIND == kOwn && D == 256 ? 2 : kWaves;
-        if (rows <= 16) hipLaunchKernelGGL((k_attn_few<D, BF, NP, 16, KIND, NW>), grid, dim3(NW * 64), 0, s, p);
-        else hipLaunchKernelGGL((k_attn_few<D, BF, NP, kRows, KIND, NW>), grid, dim3(NW * 64), 0, s, p);
+// A prefix of many rows and all sequences' own keys in one launch: the prefix's workgroups, bound by the matrix units,
+// come first, one on each CU, and beside them those of the own keys, bound by memory.
+template <int D, bool BF, int NP>
+__global__ __launch_bounds__(kWaves * 64, 2) void k_attn_both(const AttnParams p, unsigned px, unsigned prefix, unsigned ox) {
+    if (blockIdx.x < prefix) {
+        const unsigned by = blockIdx.x / px;
+        attn_many<D, BF, NP, kPrefix>(p, blockIdx.x - by * px, by, px, (unsigned)p.prefix_parts);
     } else {
-        const dim3 grid((unsigned)(tiles_of(rows) * units * p.cache.heads), parts);
-        hipLaunchKernelGGL((k_attn<D, BF, NP, KIND>), grid, dim3(kWaves * 64), 0, s, p);
+        const unsigned id = blockIdx.x - prefix, by = id / ox;
+        attn_many<D, BF, NP, kOwn>(p, id - by * ox, by, ox, (unsigned)(p.splits - p.prefix_parts));
     }
+}
+
+template <int D, bool BF, int NP>
+void launch_parts(const AttnParams &p, const SharedPlan &plan, hipStream_t s) {
+    const int group = (int)(p.q.heads / p.cache.heads);
+    const long long pr = (long long)p.prefix.max_rows * group, orows = (long long)p.seqs.max_q * group;
+    if (!plan.prefix.few) {
+        const unsigned px = (unsigned)(tiles_of(pr) * p.prefix.groups * p.cache.heads), prefix = px * plan.prefix.splits;
+        const unsigned ox = (unsigned)(tiles_of(orows) * p.seqs.n * p.cache.heads);
+        hipLaunchKernelGGL((k_attn_both<D, BF, NP>), dim3(prefix + ox * plan.own), dim3(kWaves * 64), 0, s, p, px, prefix, ox);
+        return;
+    }
+    const dim3 g1(p.prefix.groups * p.cache.heads, plan.prefix.splits), g2(p.seqs.n * p.cache.heads, plan.own);
+    constexpr int NW = D == 256 ? 2 : kWaves;
+    if (pr <= 16) hipLaunchKernelGGL((k_attn_few<D, BF, NP, 16, kPrefix>), g1, dim3(kWaves * 64), 0, s, p);
+    else hipLaunchKernelGGL((k_attn_few<D, BF, NP, kRows, kPrefix>), g1, dim3(kWaves * 64), 0, s, p);
+    if (orows <= 16) hipLaunchKernelGGL((k_attn_few<D, BF, NP, 16, kOwn, NW>), g2, dim3(NW * 64), 0, s, p);
+    else hipLaunchKernelGGL((k_attn_few<D, BF, NP, kRows, kOwn, NW>), g2, dim3(NW * 64), 0, s, p);
 }
 
 template <int D, bool BF>
 hipError_t launch_t(const AttnParams &p, const SharedPlan &plan, hipStream_t s) {
     constexpr int NP = BF ? 3 : 2;
-    const int group = (int)(p.q.heads / p.cache.heads);
-    const long long pr = (long long)p.prefix.max_rows * group, orows = (long long)p.seqs.max_q * group;
-    if (p.out.type == M27Q_TYPE_F32) {
-        launch_kind<D, BF, NP, kPrefix>(p, plan.prefix.few, pr, p.prefix.groups, plan.prefix.splits, s);
-        launch_kind<D, BF, NP, kOwn>(p, plan.own.few, orows, p.seqs.n, plan.own.splits, s);
-    } else {
-        launch_kind<D, BF, 1, kPrefix>(p, plan.prefix.few, pr, p.prefix.groups, plan.prefix.splits, s);
-        launch_kind<D, BF, 1, kOwn>(p, plan.own.few, orows, p.seqs.n, plan.own.splits, s);
-    }
+    if (p.out.type == M27Q_TYPE_F32) launch_parts<D, BF, NP>(p, plan, s);
+    else launch_parts<D, BF, 1>(p, plan, s);
     constexpr int RPB = 4 * 64 / (D / 4);
     const dim3 g2((p.seqs.max_q * p.q.heads + RPB - 1) / RPB, p.seqs.n);
     hipLaunchKernelGGL((k_attn_join<D, BF, kOwn>), g2, dim3(256), 0, s, p);
@@ -56,22 +67,24 @@ long long shared_groups(const m27q_seqs &seqs, const m27q_prefixes &prefix, uint
 }
 
 // The prefix's parts, at most 48 of the join's 64, and those of a sequence's own keys, of which there are as
-// many as the longest sequence has behind the longest prefix: parts of 64, a tile for each of two waves, at least.
-// Measured, with other numbers of parts: 64 tokens behind 32768 places 150 us with 42 of the prefix, 151 with 21, 32
-// and 40; 3 groups of 8 x 5 tokens behind 12000 places 80 with 21, 83 with 16, 98 with 10; 8 prompts of 301
-// behind 8192 places 473 with 1, 507, 543 and 472 with 2, 3 and 4.  Own keys: 64 sequences 150 with 2, 156, 154 and 157
-// with 1, 3 and 6; 4 sequences 23.1 with 5, 27.8, 25.5 and 24.0 with 1, 2 and 10.
+// many as the longest sequence has behind the longest prefix.  Few rows of a prefix: in two launches, own keys by
+// parts of 64, a tile for each of two waves, at least.  Many: in one launch, a place on a CU for the own keys of
+// each sequence and head, up to one of its two, and the others for the prefix.  Measured, with other numbers of
+// parts: 64 tokens behind 32768 places 130 us with 21 of the prefix, 161, 141, 138 and 150 with 14, 17, 32 and 42; 3
+// groups of 8 x 5 tokens behind 12000 places 66 with 17, 62, 64, 75 and 72 with 16, 18, 10 and 21; 8 prompts of 301
+// behind 8192 places 438 with 1, 474, 500 and 433 with 2, 3 and 4.  4 sequences of 300 own keys 23.1 with 5 parts of
+// those, 27.8, 25.5 and 24.0 with 1, 2 and 10.  (Each kind in a launch of its own: 150, 80 and 473 us.)
 SharedPlan shared_plan(const m27q_seqs &seqs, const m27q_prefixes &prefix, uint32_t q_heads, const m27q_cache &cache,
                        int cus) {
     const long long group = q_heads / cache.heads, slots = 2ll * cus;
     const long long rows = prefix.max_rows * group, wgs = tiles_of(rows) * prefix.groups * cache.heads;
+    const long long own = attn_groups(seqs, q_heads, cache);
     const long long shared = prefix.max_len < seqs.max_kv ? prefix.max_len : seqs.max_kv;
     SharedPlan r{};
     r.prefix.few = rows <= kRows;
-    r.prefix.splits = parts_of(wgs, r.prefix.few && cache.dim == 256 ? cus : slots, shared, r.prefix.few ? 128 : 256, 48);
-    r.own.few = (long long)seqs.max_q * group <= kRows;
-    r.own.splits = parts_of(attn_groups(seqs, q_heads, cache), slots, (long long)seqs.max_kv - shared, r.own.few ? 64 : 256,
-                            kMaxSplits - r.prefix.splits);
+    if (r.prefix.few) r.prefix.splits = parts_of(wgs, cache.dim == 256 ? cus : slots, shared, 128, 48);
+    else r.prefix.splits = parts_of(wgs, slots - std::min<long long>(own, cus), shared, 256, 48);
+    r.own = parts_of(own, slots, (long long)seqs.max_kv - shared, r.prefix.few ? 64 : 256, kMaxSplits - r.prefix.splits);
     return r;
 }
 

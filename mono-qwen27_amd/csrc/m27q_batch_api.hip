@@ -77,7 +77,7 @@ M27Q_API size_t m27q_attn_shared_scratch_bytes(const m27q_seqs *seqs, const m27q
     if (!shared_shape(seqs, prefix, q_heads, cache)) return 0;
     const m27q_seqs s = bounded(*seqs, *cache);
     const SharedPlan plan = shared_plan(s, *prefix, q_heads, *cache, cu_count());
-    return attn_scratch(s, q_heads, cache->dim, plan.prefix.splits + plan.own.splits);
+    return attn_scratch(s, q_heads, cache->dim, plan.prefix.splits + plan.own);
 }
 
 M27Q_API m27q_status m27q_attn_shared(const m27q_seqs *seqs, const m27q_prefixes *prefix, const m27q_cache *cache,
@@ -98,7 +98,7 @@ M27Q_API m27q_status m27q_attn_shared(const m27q_seqs *seqs, const m27q_prefixes
     p.prefix = *prefix;
     const SharedPlan plan = shared_plan(p.seqs, *prefix, q->heads, *cache, cu_count());
     p.prefix_parts = plan.prefix.splits;
-    p.splits = plan.prefix.splits + plan.own.splits;
+    p.splits = plan.prefix.splits + plan.own;
     if (scratch_bytes < attn_scratch(p.seqs, q->heads, cache->dim, p.splits)) return M27Q_ERR_SCRATCH;
     p.part = (float *)scratch;
     p.stat = (float2 *)(p.part + (size_t)p.seqs.tokens * q->heads * p.splits * cache->dim);
