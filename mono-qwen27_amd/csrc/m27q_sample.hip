@@ -203,17 +203,27 @@ constexpr int kReach = kFine + kUnit * kCoarse;  // units down to where weights 
 struct Scale {
     double c;       // units of a logit
     double anchor;
-    int wide;       // distances from the anchor are not whole numbers of 2^26 at most, or T is infinite
-    double near;    // 1; 0 where a step of a logit is thousands of octaves and only equal ones have a weight
+    bool wide;      // distances from the anchor are not whole numbers of 2^26 at most, or T is infinite
 };
 __device__ __forceinline__ Scale row_scale(const Rule &r, double anchor) {
     const double far = fabs(anchor) + kReach;
     const double c = kUnitsPerNat * r.inv_t;
-    return {c, anchor, __builtin_amdgcn_readfirstlane(!(far < 0x1p26) || !(c > 0.0)), far > 0x1p40 ? 0.0 : 1.0};
+    return {c, anchor, __builtin_amdgcn_readfirstlane(!(far < 0x1p26) || !(c > 0.0)) != 0};
 }
 
-// The distance of a logit from the anchor in whole units, and what is left over: both of the exact
-// product, as an addition that leaves the whole number in the low bits rounds it once, and alike for any anchor.
+// A logit in whole units, and what is left over: of the exact product, rounded once, whatever anchor it is
+// measured from, so that parts of a row and the row count a token in the same bin.  From 2^50 units on a
+// step of a logit is thousands of octaves and only equal ones have a weight: there the rounded product does.
+__device__ __forceinline__ double units_of(double l, double c, double &z) {
+    const double y = l * c;
+    const bool near = fabs(y) < 0x1p50;
+    const double b = near ? __builtin_fma(l, c, 0x1.8p52) - 0x1.8p52 : __builtin_rint(y);
+    z = near ? __builtin_fma(l, -c, b) : 0.0;
+    return b;
+}
+
+// The same for logits less than 2^26 units from the anchor: how far down from it, the whole number in the low bits of an
+// addition.
 __device__ __forceinline__ uint32_t units_down(double l, double c, double low, double anchor, double &z) {
     const double t = __builtin_fma(l, -c, low);  // low = anchor + 1.5 2^52
     z = __builtin_fma(l, -c, anchor - (t - 0x1.8p52));
@@ -228,17 +238,9 @@ struct Place {
 __device__ __forceinline__ int bin_of(uint32_t d) { return (int)min(d, (d >> 4) + (kFine - kFine / kUnit)); }
 __device__ __forceinline__ Place place_of(float l, const Scale &s) {
     Place p{kBins, 0, 0};
-    uint32_t d;
-    if (s.wide) {
-        const double b = __builtin_rint((double)l * s.c), far = s.anchor - b;
-        if (!(far < kReach)) return p;  // (-infinity and NaN too)
-        d = (uint32_t)far;
-        p.z = -__builtin_fma((double)l, s.c, -b) * s.near;
-    } else {
-        if (!((double)l * s.c > s.anchor - (kReach + kUnit))) return p;
-        d = units_down((double)l, s.c, s.anchor + 0x1.8p52, s.anchor, p.z);
-        if (d >= (uint32_t)kReach) return p;
-    }
+    const double far = s.anchor - units_of((double)l, s.c, p.z);
+    if (!(far < kReach)) return p;  // (-infinity and NaN too)
+    const uint32_t d = (uint32_t)far;
     p.bin = bin_of(d);
     p.k = (int)(d & (kUnit - 1));
     return p;
@@ -338,7 +340,8 @@ __global__ __launch_bounds__(kPartThreads) void k_sample_parts(const m27q_sampli
     if (lane == 0) at_s[wave] = at;
 
     const bool any = !r.greedy && __builtin_isfinite(top);
-    const double b = __builtin_rint((double)top * (kUnitsPerNat * r.inv_t));
+    double z;
+    const double b = units_of((double)top, kUnitsPerNat * r.inv_t, z);
     const Scale s = row_scale(r, any ? ceil(b * (1.0 / kUnit)) * kUnit : -__builtin_inf());
     if (any) {
         const Weights w(octave);
@@ -763,7 +766,8 @@ __device__ __forceinline__ bool pick_from_list(const m27q_sampling &p, const Scr
         const Place a = place_of(key_value(key[e]), scale);
         const uint32_t at = s.at[a.bin], count = s.at[a.bin + 1] - at;
         const float part = a.bin < kFine ? (float)a.z + 0.5f : ((float)a.k + (float)a.z + 0.5f) * (1.0f / kUnit);
-        bucket[e] = at + min((uint32_t)fmaxf(part * (float)count, 0.0f), count - 1);
+        // (below n even if somebody writes to the logits meanwhile)
+        bucket[e] = min(at + min((uint32_t)fmaxf(part * (float)count, 0.0f), count - 1), (uint32_t)n - 1);
         slot[e] = atomicAdd(&s.count[bucket[e]], 1u);
     }
     __syncthreads();

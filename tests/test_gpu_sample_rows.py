@@ -191,6 +191,24 @@ def test_values_at_the_ends(m27q, dev, n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T", [1e-3, 1e-5, 8e-6, 3e-6, 1e-6, 1e-9, 1e-11, 1e-13])
+def test_temperatures_near_0(m27q, dev, T):
+    """Steps between logits from a few octaves to more than numbers of 32 and of 52 bits hold: several sizes of logits, rows with
+    two parts of a row far apart, and equal largest ones."""
+    say("sample cold", T)
+    rng = np.random.default_rng(6)
+    x = logits(rng, 6, 20000, "ties") + np.float32(7)
+    x[1] *= 1000
+    x[2, 8192:] -= 200
+    x[3] = np.nextafter(np.float32(10), np.float32(20) * (rng.integers(0, 2, 20000) * 2 - 1)).astype(np.float32)
+    x[4, :8192] += 3e6
+    x[5] = -x[5] * 1e4
+    for top_k, top_p, min_p in ((0, 1.0, 0.0), (50, 0.9, 0.0), (0, 0.6, 0.3)):
+        for u in (0.0, 0.4, 0.99):
+            check(m27q, dev, x, T, top_k, top_p, min_p, u)
+
+
+@pytest.mark.gpu
 def test_agrees_with_sampling_of_candidates(m27q, ora, dev):
     """m27q_topk and m27q_sample give the same tokens where u is not beside a border (they sum in 32 bits)."""
     import torch
