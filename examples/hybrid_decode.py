@@ -2,9 +2,10 @@
 
 One gated-delta layer and one attention layer with random Q8_0 weights.  Sequences of different lengths share each step:
 their rows lie one after the other, `start` says where each begins.  A step has at most 64 rows (what a quantized product
-takes), so prompts go in by chunks, and short ones decode beside a long one that is still being read.
+takes), so prompts go in by chunks, and short ones decode beside a long one that is still being read.  Prompts that begin
+alike can share that beginning: it is read once, its pages lie in each sequence's table, and attention reads them once for all.
 
-    python examples/hybrid_decode.py [--new 16] [--lengths 5,90,33]
+    python examples/hybrid_decode.py [--new 16] [--lengths 5,90,33] [--prefix 0] [--temperature 0] [--top-k 0] [--top-p 1]
 """
 import argparse
 import importlib
@@ -52,11 +53,8 @@ class Model:
         self.free_pages = list(range(max_seqs * pages))
         self.free_slots = list(range(max_seqs))
 
-    def products(self, weights, x):
-        rows = x.shape[0]
-        act = self.m.Act(rows, x.shape[1], self.device)
-        ys = [self.torch.empty(rows, w.rc, device=self.device) for w in weights]
-        self.m.quant_act(x, act)
+    def products(self, weights, act):
+        ys = [self.torch.empty(act.M, w.rc, device=self.device) for w in weights]
         self.m.matmul_q8_multi(weights, act, ys)
         return ys
 
@@ -69,10 +67,24 @@ class Model:
         return y
 
     def norm(self, x):
-        return x * (x.square().mean(-1, keepdim=True) + 1e-6).rsqrt()
+        """The normed rows, quantized for the products that read them."""
+        act = self.m.Act(x.shape[0], x.shape[1], self.device)
+        self.m.rms_norm(x, act=act)
+        return act
 
-    def step(self, work):
-        """work: (sequence, its next token ids) pairs of at most 64 ids together; the logits after each one's last."""
+    def pick(self, logits, u, temperature, top_k, top_p):
+        """A token for each row of logits."""
+        rows, n = logits.shape
+        each = lambda v, t: self.torch.full((rows,), v, dtype=t, device=self.device)  # noqa: E731
+        token = each(0, self.torch.int32)
+        scratch = self.torch.empty(self.m.sample_rows_scratch_bytes(rows, n), dtype=self.torch.uint8, device=self.device)
+        self.m.sample_rows(logits, u, token, scratch, each(temperature, self.torch.float32), each(top_k, self.torch.int32),
+                           each(top_p, self.torch.float32))
+        return token.tolist()
+
+    def step(self, work, shared=0):
+        """work: (sequence, its next token ids) pairs of at most 64 ids together; the logits after each one's last.  The first
+        `shared` cached tokens of all of them lie in the same pages."""
         m, torch, F = self.m, self.torch, self.torch.nn.functional
         lens = [len(ids) for _, ids in work]
         rows = sum(lens)
@@ -108,8 +120,13 @@ class Model:
         q, k, v = q.view(rows, Q_HEADS, DIM), k.view(rows, KV_HEADS, DIM), v.view(rows, KV_HEADS, DIM)
         turned, out = torch.empty(rows, Q_HEADS, DIM, dtype=torch.bfloat16, device=self.device), torch.empty_like(q)
         m.rope_append(self.rope, pos, seqs, self.cache, q, turned, k, v)
-        scratch = torch.empty(m.attn_scratch_bytes(seqs, Q_HEADS, self.cache), dtype=torch.uint8, device=self.device)
-        m.attn_paged(seqs, self.cache, turned, out, scratch, DIM ** -0.5)
+        if shared and len(work) > 1:
+            prefixes = m.Prefixes(ints([0, len(work)]), ints([shared]), rows, shared)
+            scratch = torch.empty(m.attn_shared_scratch_bytes(seqs, prefixes, Q_HEADS, self.cache), dtype=torch.uint8, device=self.device)
+            m.attn_shared(seqs, prefixes, self.cache, turned, out, scratch, DIM ** -0.5)
+        else:
+            scratch = torch.empty(m.attn_scratch_bytes(seqs, Q_HEADS, self.cache), dtype=torch.uint8, device=self.device)
+            m.attn_paged(seqs, self.cache, turned, out, scratch, DIM ** -0.5)
         x = self.add(out.view(rows, -1), self.attn_out, x)
 
         last = torch.tensor(np.cumsum(lens) - 1, device=self.device)
@@ -117,10 +134,16 @@ class Model:
 
 
 class Sequence:
-    def __init__(self, model, prompt):
+    def __init__(self, model, prompt, behind=None):
+        """behind: a sequence whose tokens, whole pages of them, were all read: this one goes on from there."""
         self.ids, self.read, self.length = list(prompt), 0, 0  # tokens, how many of them were given to a step, and cached
-        self.pages, self.slot = [], model.free_slots.pop()
-        model.states[self.slot].zero_()
+        self.pages, self.borrowed, self.slot = [], 0, model.free_slots.pop()
+        if behind is None:
+            model.states[self.slot].zero_()
+            return
+        self.ids, self.read, self.length = behind.ids + self.ids, behind.length, behind.length
+        self.pages, self.borrowed = list(behind.pages), len(behind.pages)
+        model.states[self.slot].copy_(model.states[behind.slot])
 
     def grow(self, model, n):
         self.length += n
@@ -130,14 +153,23 @@ class Sequence:
             self.pages.append(model.free_pages.pop())
 
     def done(self, model):
-        model.free_pages += self.pages
+        model.free_pages += self.pages[self.borrowed:]
         model.free_slots.append(self.slot)
 
 
-def generate(model, prompts, new, rows=ROWS):
-    """Greedy continuations of `new` tokens, and each sequence's logits after its prompt and after every new token but the last."""
-    seqs = [Sequence(model, p) for p in prompts]
-    ends = [len(p) + new for p in prompts]
+def generate(model, prompts, new, rows=ROWS, prefix=(), temperature=0.0, top_k=0, top_p=1.0, seed=0):
+    """Continuations of `new` tokens, and each sequence's logits after its prompt and after every new token but the last.  All
+    prompts follow `prefix`, whole pages of tokens."""
+    g = model.torch.Generator(device=model.device).manual_seed(seed)
+    head, prefix = None, list(prefix)
+    if len(prefix) % PAGE:
+        raise ValueError("a prefix of %d tokens: whole pages of %d are shared" % (len(prefix), PAGE))
+    if prefix:
+        head = Sequence(model, prefix)
+        for i in range(0, len(prefix), rows):
+            model.step([(head, prefix[i: i + rows])])
+    seqs = [Sequence(model, p, head) for p in prompts]
+    ends = [len(s.ids) + new for s in seqs]
     logits = [[] for _ in seqs]
     while True:
         work, left = [], rows
@@ -149,14 +181,14 @@ def generate(model, prompts, new, rows=ROWS):
                 left -= n
         if not work:
             break
-        y = model.step([(seqs[i], ids) for i, ids in work])
-        best = y.argmax(-1).tolist()
-        for (i, ids), row, token in zip(work, y, best):
+        y = model.step([(seqs[i], ids) for i, ids in work], len(prefix))
+        tokens = model.pick(y, model.torch.rand(len(work), generator=g, device=model.device), temperature, top_k, top_p)
+        for (i, ids), row, token in zip(work, y, tokens):
             seqs[i].read += len(ids)
             if seqs[i].read == len(seqs[i].ids):
                 logits[i].append(row)
                 seqs[i].ids.append(token)
-    for s in seqs:
+    for s in seqs + ([head] if head else []):
         s.done(model)
     return [s.ids for s in seqs], logits
 
@@ -165,13 +197,19 @@ def main():
     p = argparse.ArgumentParser(description=__doc__.split("\n")[0])
     p.add_argument("--new", type=int, default=16)
     p.add_argument("--lengths", default="5,90,33")
+    p.add_argument("--prefix", type=int, default=0, help="tokens that all prompts begin with (whole pages of %d)" % PAGE)
+    p.add_argument("--temperature", type=float, default=0.0)
+    p.add_argument("--top-k", type=int, default=0)
+    p.add_argument("--top-p", type=float, default=1.0)
     a = p.parse_args()
     m = importlib.import_module("mono-qwen27_amd").m27q
     rng = np.random.default_rng(1)
+    prefix = rng.integers(0, VOCAB, a.prefix).tolist()
     prompts = [rng.integers(0, VOCAB, int(n)).tolist() for n in a.lengths.split(",")]
-    ids, _ = generate(Model(m, len(prompts), max(map(len, prompts)) + a.new), prompts, a.new)
+    model = Model(m, len(prompts) + 1, a.prefix + max(map(len, prompts)) + a.new)
+    ids, _ = generate(model, prompts, a.new, prefix=prefix, temperature=a.temperature, top_k=a.top_k, top_p=a.top_p)
     for prompt, s in zip(prompts, ids):
-        print("%3d tokens -> %s" % (len(prompt), s[len(prompt):]))
+        print("%3d tokens -> %s" % (a.prefix + len(prompt), s[a.prefix + len(prompt):]))
 
 
 if __name__ == "__main__":
