@@ -557,13 +557,12 @@ __device__ __forceinline__ void set_keys(const AttnParams &p, Work &w, int len, 
 }
 
 // Looks at every page of the keys once, the threads of a workgroup in turn: tiles trust them then.
-template <int NW = kWaves>
 __device__ __forceinline__ bool has_gaps(const AttnParams &p, const Work &w) {
     const int shift = __builtin_ctz(p.cache.page_size);
     const int32_t *table = p.seqs.table + (long long)w.s * p.seqs.table_stride;
     bool bad = false;
     if (w.lo < w.hi)
-        for (int i = (w.lo >> shift) + (int)threadIdx.x; i <= (w.hi - 1) >> shift; i += NW * 64)
+        for (int i = (w.lo >> shift) + (int)threadIdx.x; i <= (w.hi - 1) >> shift; i += kWaves * 64)
             bad |= (uint32_t)table[i] >= p.cache.pages;
     return bad;
 }
@@ -756,6 +755,18 @@ __global__ __launch_bounds__(kWaves * 64, 2) void k_attn(const AttnParams p) {
     attn_many<D, BF, NP, kAll>(p, blockIdx.x, blockIdx.y, gridDim.x, gridDim.y);
 }
 
+// What a workgroup of few rows keeps in LDS, for all that one launch does.
+template <int D, int I>
+__device__ __forceinline__ char *few_lds() {
+    __shared__ __attribute__((aligned(1024))) char tiles[kWaves * kKeys * D * 2];
+    return tiles;
+}
+template <int I>
+__device__ __forceinline__ float (*few_stats())[kRows] {
+    __shared__ float stats[kWaves][kRows];
+    return stats;
+}
+
 // Few rows (up to 32 of a sequence and cache head): the cache's bytes bound it.  The waves
 // of a workgroup take tiles in turn, each for itself with K and V tiles of its own: K of
 // its next tile is on its way from the moment its scores are there, V from when its values
@@ -766,17 +777,18 @@ __global__ __launch_bounds__(kWaves * 64, 2) void k_attn(const AttnParams p) {
 // join.  One token over 1021 keys: a tile a wave, and a chain of 16000 cycles (lengths 3500, page
 // and loads 2700, their arrival 2500, products and weights 2800, the waves' join 4300), then 3 us
 // of the parts' join.
-template <int D, bool BF, int NP, int RW, Kind KIND = kAll, int NW = kWaves>
-__global__ __launch_bounds__(NW * 64, D == 256 ? 1 : 2) void k_attn_few(const AttnParams p) {
+// Workgroup (bx, by).
+template <int D, bool BF, int NP, int RW, Kind KIND>
+__device__ __forceinline__ void attn_few(const AttnParams &p, unsigned bx, unsigned by) {
     typedef Rows<D, BF, NP, RW> R;
     typedef typename R::T T;
-    constexpr int TB = kKeys * D * 2;  // bytes of a tile
-    __shared__ __attribute__((aligned(1024))) char kts[NW * TB], vts[NW * TB];
-    __shared__ float ms[NW][RW], ls[NW][RW];
+    constexpr int TB = kKeys * D * 2, NW = kWaves;  // bytes of a tile
+    char *const kts = few_lds<D, 0>(), *const vts = few_lds<D, 1>();
+    float(*const ms)[kRows] = few_stats<0>(), (*const ls)[kRows] = few_stats<1>();
     const int group = (int)(p.q.heads / p.cache.heads);
-    const int s = blockIdx.x / p.cache.heads;
+    const int s = bx / p.cache.heads;
     Work w;
-    w.head = blockIdx.x - s * p.cache.heads;
+    w.head = bx - s * p.cache.heads;
     const Unit sr = unit_rows<KIND>(p, s);
     w.s = sr.s;
     w.rows = sr.count * group;
@@ -789,17 +801,17 @@ __global__ __launch_bounds__(NW * 64, D == 256 ? 1 : 2) void k_attn_few(const At
         last = at.y;
         __syncthreads();
     }
-    set_keys<KIND>(p, w, len, sr.shared, first, last, (int)blockIdx.y);
+    set_keys<KIND>(p, w, len, sr.shared, first, last, (int)by);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const bool live = (lane & (RW - 1)) < w.rows;
     const int row = min(lane & (RW - 1), w.rows - 1), at = row / group;
     const int token = sr.first + at, qh = w.head * group + row - at * group;
     const unsigned long long part0 = (unsigned long long)((uint32_t)token * p.q.heads + qh) * (uint32_t)p.splits;
-    const unsigned long long part = part0 + (KIND == kOwn ? p.prefix_parts : 0) + blockIdx.y;
+    const unsigned long long part = part0 + (KIND == kOwn ? p.prefix_parts : 0) + by;
     // loads end in order: what is needed first is asked for first
     typename R::Raw q;
     R::load_q(p, token, qh, q);
-    const bool gaps = has_gaps<NW>(p, w);
+    const bool gaps = has_gaps(p, w);
     LDS_AS char *const kt = (LDS_AS char *)kts + wave * TB, *const vt = (LDS_AS char *)vts + wave * TB;
     const int32_t *table = p.seqs.table + (long long)w.s * p.seqs.table_stride;
     const int shift = __builtin_ctz(p.cache.page_size);
@@ -984,7 +996,7 @@ __global__ __launch_bounds__(NW * 64, D == 256 ? 1 : 2) void k_attn_few(const At
     }
     if (KIND != kAll || p.splits > 1) {
         if (threadIdx.x < RW) p.stat[part] = make_float2(m * sc, l);
-        if (KIND == kOwn && sr.shared < 0 && blockIdx.y == 0 && threadIdx.x < RW)  // no prefix
+        if (KIND == kOwn && sr.shared < 0 && by == 0 && threadIdx.x < RW)  // no prefix
             for (int i = 0; i < p.prefix_parts; ++i) p.stat[part0 + i] = make_float2(0, 0);
         if (l == 0) return;
 #pragma unroll
@@ -1001,6 +1013,11 @@ __global__ __launch_bounds__(NW * 64, D == 256 ? 1 : 2) void k_attn_few(const At
         if (p.out.type == M27Q_TYPE_F32) *(f32x4 *)((float *)p.out.ptr + to + 4 * quad) = x;
         else *(typename R::T4 *)((T *)p.out.ptr + to + 4 * quad) = __builtin_convertvector(x, typename R::T4);
     }
+}
+
+template <int D, bool BF, int NP, int RW>
+__global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) void k_attn_few(const AttnParams p) {
+    attn_few<D, BF, NP, RW, kAll>(p, blockIdx.x, blockIdx.y);
 }
 
 // Joins the parts of each row, in order of the parts: a wave a row (two for D = 128, four

@@ -22,22 +22,30 @@ __global__ __launch_bounds__(kWaves * 64, 2) void k_attn_both(const AttnParams p
     }
 }
 
+// The same of few rows.
+template <int D, bool BF, int NP, int PREFIX_ROWS, int OWN_ROWS>
+__global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) void k_attn_few_both(const AttnParams p, unsigned px, unsigned prefix,
+                                                                                  unsigned ox) {
+    if (blockIdx.x < prefix) {
+        const unsigned by = blockIdx.x / px;
+        attn_few<D, BF, NP, PREFIX_ROWS, kPrefix>(p, blockIdx.x - by * px, by);
+    } else {
+        const unsigned id = blockIdx.x - prefix, by = id / ox;
+        attn_few<D, BF, NP, OWN_ROWS, kOwn>(p, id - by * ox, by);
+    }
+}
+
 template <int D, bool BF, int NP>
 void launch_parts(const AttnParams &p, const SharedPlan &plan, hipStream_t s) {
     const int group = (int)(p.q.heads / p.cache.heads);
     const long long pr = (long long)p.prefix.max_rows * group, orows = (long long)p.seqs.max_q * group;
-    if (!plan.prefix.few) {
-        const unsigned px = (unsigned)(tiles_of(pr) * p.prefix.groups * p.cache.heads), prefix = px * plan.prefix.splits;
-        const unsigned ox = (unsigned)(tiles_of(orows) * p.seqs.n * p.cache.heads);
-        hipLaunchKernelGGL((k_attn_both<D, BF, NP>), dim3(prefix + ox * plan.own), dim3(kWaves * 64), 0, s, p, px, prefix, ox);
-        return;
-    }
-    const dim3 g1(p.prefix.groups * p.cache.heads, plan.prefix.splits), g2(p.seqs.n * p.cache.heads, plan.own);
-    constexpr int NW = D == 256 ? 2 : kWaves;
-    if (pr <= 16) hipLaunchKernelGGL((k_attn_few<D, BF, NP, 16, kPrefix>), g1, dim3(kWaves * 64), 0, s, p);
-    else hipLaunchKernelGGL((k_attn_few<D, BF, NP, kRows, kPrefix>), g1, dim3(kWaves * 64), 0, s, p);
-    if (orows <= 16) hipLaunchKernelGGL((k_attn_few<D, BF, NP, 16, kOwn, NW>), g2, dim3(NW * 64), 0, s, p);
-    else hipLaunchKernelGGL((k_attn_few<D, BF, NP, kRows, kOwn, NW>), g2, dim3(NW * 64), 0, s, p);
+    const unsigned tp = plan.prefix.few ? 1 : (unsigned)tiles_of(pr), to = plan.prefix.few ? 1 : (unsigned)tiles_of(orows);
+    const unsigned px = tp * p.prefix.groups * p.cache.heads, ox = to * p.seqs.n * p.cache.heads, prefix = px * plan.prefix.splits;
+    const dim3 grid(prefix + ox * plan.own), block(kWaves * 64);
+    if (!plan.prefix.few) hipLaunchKernelGGL((k_attn_both<D, BF, NP>), grid, block, 0, s, p, px, prefix, ox);
+    else if (std::max(pr, orows) <= 16) hipLaunchKernelGGL((k_attn_few_both<D, BF, NP, 16, 16>), grid, block, 0, s, p, px, prefix, ox);
+    else if (orows <= 16) hipLaunchKernelGGL((k_attn_few_both<D, BF, NP, kRows, 16>), grid, block, 0, s, p, px, prefix, ox);
+    else hipLaunchKernelGGL((k_attn_few_both<D, BF, NP, kRows, kRows>), grid, block, 0, s, p, px, prefix, ox);
 }
 
 template <int D, bool BF>
@@ -59,11 +67,11 @@ int parts_of(long long wgs, long long slots, long long keys, long long least, lo
 
 }  // namespace
 
-// Workgroups of a part of the keys, the larger of the prefixes' and the sequences'.
+// Workgroups of a part of the keys, the prefixes' and the sequences'.
 long long shared_groups(const m27q_seqs &seqs, const m27q_prefixes &prefix, uint32_t q_heads, const m27q_cache &cache) {
     const long long rows = (long long)prefix.max_rows * (q_heads / cache.heads);
     const long long a = tiles_of(rows) * prefix.groups * cache.heads, b = attn_groups(seqs, q_heads, cache);
-    return a > b ? a : b;
+    return a + b;
 }
 
 // The prefix's parts, at most 48 of the join's 64, and those of a sequence's own keys, of which there are as
@@ -81,10 +89,11 @@ SharedPlan shared_plan(const m27q_seqs &seqs, const m27q_prefixes &prefix, uint3
     const long long own = attn_groups(seqs, q_heads, cache);
     const long long shared = prefix.max_len < seqs.max_kv ? prefix.max_len : seqs.max_kv;
     SharedPlan r{};
-    r.prefix.few = rows <= kRows;
-    if (r.prefix.few) r.prefix.splits = parts_of(wgs, cache.dim == 256 ? cus : slots, shared, 128, 48);
-    else r.prefix.splits = parts_of(wgs, slots - std::min<long long>(own, cus), shared, 256, 48);
-    r.own = parts_of(own, slots, (long long)seqs.max_kv - shared, r.prefix.few ? 64 : 256, kMaxSplits - r.prefix.splits);
+    r.prefix.few = rows <= kRows && seqs.max_q * group <= kRows;
+    const int least = r.prefix.few ? 128 : 256;
+    const long long places = r.prefix.few && cache.dim == 256 ? cus : slots;
+    r.prefix.splits = parts_of(wgs, places - std::min(own, places / 2), shared, least, 48);
+    r.own = parts_of(own, r.prefix.few ? places - wgs * r.prefix.splits : slots, (long long)seqs.max_kv - shared, least, kMaxSplits - r.prefix.splits);
     return r;
 }
 

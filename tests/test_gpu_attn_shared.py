@@ -71,6 +71,15 @@ CASES = [
     ([(1, 2100), (1, 2050)], [(0, 2, 2048)], 64, 1, 128, 256, "bf16", "f32"),
     ([(1, 64)] * 5, [(0, 5, 64)], 3, 1, 64, 16, "f16", "f32"),                                  # nothing but the prefix
     ([(1, 31), (1, 20)], [(0, 2, 16)], 2, 1, 64, 16, "f16", "f32"),                             # below a tile
+    ([(1, 300), (1, 290), (40, 100), (9, 700)], [(0, 2, 256)], 6, 2, 128, 16, "bf16", "f32"),   # few rows share, more do not
+    ([(1, 300), (1, 290), (12, 700)], [(0, 2, 256)], 4, 2, 256, 64, "f16", "f16"),              # 16 rows share, 32 do not
+    ([(2, 90), (9, 100), (5, 77)], [(0, 3, 64)], 2, 1, 64, 16, "f16", "f32"),                   # 32 rows
+    ([(2, 90), (9, 100), (6, 77)], [(0, 3, 64)], 2, 1, 256, 16, "f16", "f32"),                  # 34
+    ([(1, 3300)] * 16, [(0, 16, 3200)], 8, 1, 64, 128, "f16", "f32"),                           # 128: one workgroup's
+    ([(1, 3300)] * 16 + [(2, 3250)], [(0, 17, 3200)], 8, 1, 64, 128, "bf16", "bf16"),           # 144
+    ([(1, 40 + i) for i in range(150)], [(2 * i, 2, 32) for i in range(75)], 2, 1, 64, 16, "f16", "f32"),  # groups past 64
+    ([(1, 9000)] * 3, [(0, 3, 64)], 4, 2, 128, 64, "f16", "f32"),                               # mostly their own
+    ([(1, 12100), (3, 12050)], [(0, 2, 12032)], 2, 2, 64, 64, "bf16", "f32"),                   # mostly shared
 ]
 
 

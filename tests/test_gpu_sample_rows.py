@@ -111,6 +111,18 @@ def test_rows_of_every_rule(m27q, dev, n, kind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n", [8191, 8192, 8193, 32 * 8192, 32 * 8192 + 1, 64 * 8192 + 1, 1000003, 1 << 24])
+def test_lengths_around_parts(m27q, dev, n):
+    """Parts of 8192 tokens, 32 or 64 of them at a time, up to the longest row."""
+    say("sample parts", n)
+    rng = np.random.default_rng(n)
+    x = logits(rng, 2, n, "peaks")
+    x[1, -1] = x[1].max()  # a tie with the last token
+    for T, k, top_p, min_p in ((1.0, 0, 0.97, 0.0), (0.8, 40, 1.0, 0.02))[: 1 if n > 1 << 20 else 2]:
+        check(m27q, dev, x, T, k, top_p, min_p, (0.3, 1.0))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("n", [5, 2000, 50000, 248320])
 def test_all_the_same(m27q, dev, n):
     """Equal logits: ties go by index, and every cut falls inside them."""
