@@ -10,7 +10,9 @@ namespace {
 long long tiles_of(long long rows) { return (rows + kWaves * kRows - 1) / (kWaves * kRows); }
 
 // A prefix of many rows and all sequences' own keys in one launch: the prefix's workgroups, bound by the matrix units,
-// come first, one on each CU, and beside them those of the own keys, bound by memory.
+// come first, one on each CU, and beside them those of the own keys, bound by memory.  64 tokens behind 32768
+// places and up to 1021 own ones, 24 heads of 256 on 4, F16 to F32: 123 us and 6 of joining, of 45 for the bytes (300 MB) and
+// 67 for the products; 8 prompts of 301 tokens behind 8192, BF16: 444 us, 1.0 PFLOP/s of the pairs that count.
 template <int D, bool BF, int NP>
 __global__ __launch_bounds__(kWaves * 64, 2) void k_attn_both(const AttnParams p, unsigned px, unsigned prefix, unsigned ox) {
     if (blockIdx.x < prefix) {
@@ -22,7 +24,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void k_attn_both(const AttnParams p
     }
 }
 
-// The same of few rows.
+// The same of few rows, bound by the latency of a part's steps: 4 tokens behind 2048 places and up to 300 own ones, 10 MB,
+// 11 us and 5.5 of joining.
 template <int D, bool BF, int NP, int PREFIX_ROWS, int OWN_ROWS>
 __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) void k_attn_few_both(const AttnParams p, unsigned px, unsigned prefix,
                                                                                   unsigned ox) {
@@ -75,13 +78,15 @@ long long shared_groups(const m27q_seqs &seqs, const m27q_prefixes &prefix, uint
 }
 
 // The prefix's parts, at most 48 of the join's 64, and those of a sequence's own keys, of which there are as
-// many as the longest sequence has behind the longest prefix.  Few rows of a prefix: in two launches, own keys by
-// parts of 64, a tile for each of two waves, at least.  Many: in one launch, a place on a CU for the own keys of
-// each sequence and head, up to one of its two, and the others for the prefix.  Measured, with other numbers of
-// parts: 64 tokens behind 32768 places 130 us with 21 of the prefix, 161, 141, 138 and 150 with 14, 17, 32 and 42; 3
-// groups of 8 x 5 tokens behind 12000 places 66 with 17, 62, 64, 75 and 72 with 16, 18, 10 and 21; 8 prompts of 301
-// behind 8192 places 438 with 1, 474, 500 and 433 with 2, 3 and 4.  4 sequences of 300 own keys 23.1 with 5 parts of
-// those, 27.8, 25.5 and 24.0 with 1, 2 and 10.  (Each kind in a launch of its own: 150, 80 and 473 us.)
+// many as the longest sequence has behind the longest prefix: what runs at once, in one launch.  Many rows: a
+// place on a CU for the own keys of each sequence and head, up to one of its two, and the others for the
+// prefix.  Few: up to half of the places for the own keys, in parts of 128, a tile a wave, at least.  Measured, with
+// other numbers of parts: 64 tokens behind 32768 places 130 us with 21 of the prefix, 161, 141, 138 and 150 with 14,
+// 17, 32 and 42; 3 groups of 8 x 5 tokens behind 12000 places 66 with 17, 62, 64, 75 and 72 with 16, 18, 10 and 21; 8
+// prompts of 301 behind 8192 places 438 with 1, 474, 500 and 433 with 2, 3 and 4.  (Each kind in a launch of its own:
+// 150, 80 and 473 us.)  Few rows: 4 tokens behind 2048 places 16.5 with 16, 17.2, 17.1 and 17.8 with 11, 22 and 32 (two
+// launches: 23.1); behind 32768 places 38.9 with 48, 40.6, 37.7 and 38.4 with 24, 32 and 40; 8 tokens, 8 cache heads of 128,
+// 4096 places and up to 1500 own ones 21.2, 18.5 with half as many parts of the own ones.
 SharedPlan shared_plan(const m27q_seqs &seqs, const m27q_prefixes &prefix, uint32_t q_heads, const m27q_cache &cache,
                        int cus) {
     const long long group = q_heads / cache.heads, slots = 2ll * cus;
@@ -93,7 +98,8 @@ SharedPlan shared_plan(const m27q_seqs &seqs, const m27q_prefixes &prefix, uint3
     const int least = r.prefix.few ? 128 : 256;
     const long long places = r.prefix.few && cache.dim == 256 ? cus : slots;
     r.prefix.splits = parts_of(wgs, places - std::min(own, places / 2), shared, least, 48);
-    r.own = parts_of(own, r.prefix.few ? places - wgs * r.prefix.splits : slots, (long long)seqs.max_kv - shared, least, kMaxSplits - r.prefix.splits);
+    const long long left = r.prefix.few ? places - wgs * r.prefix.splits : slots;
+    r.own = parts_of(own, left, (long long)seqs.max_kv - shared, least, kMaxSplits - r.prefix.splits);
     return r;
 }
 
