@@ -6,6 +6,11 @@
 // of each head's dim values; h and y as rows of any type, y's per-32 codes as
 // m27q_quant_act makes them.  h is fp32 until the end: y is of h before the
 // rounding to the sum's type.
+//
+// Memory bounds it: a row is read once, kept in registers between the sum of its squares and the
+// outputs (k_norm_row, k_norm_heads), and the codes are made where y is, which saves the
+// quantizer's launch and 8 bytes a value.  4096 rows of 5120, residual, sum and codes (278 MB): 49 us, 5.7 TB/s;
+// 1531 x 24 heads of 256, BF16 (38 MB): 10; a row of 5120: 3.6, a launch.
 #include "m27q_device.h"
 #include "m27q_mix.h"
 
@@ -26,7 +31,8 @@ __device__ __forceinline__ float sum_group(float v, float *lds, int waves) {
     return s;
 }
 
-// Any dim and alignment, a value a thread at a time: a workgroup a row, which it reads twice.
+// Any dim and alignment, a value a thread at a time: a workgroup a row, which it reads twice.  4096 rows of 5120,
+// F32 with sum and y: 92 us, 63 by units of 8; BF16 92 and 31; 98304 heads of 256 168 and 33.
 __global__ __launch_bounds__(kThreads) void k_norm_any(const NormParams p) {
     __shared__ float lds[kThreads / 64];
     const int t = blockIdx.x / p.x.heads, head = blockIdx.x - t * p.x.heads, dim = (int)p.x.dim;
@@ -172,8 +178,16 @@ static bool norm_vectorizes(const NormParams &p) {
            (uintptr_t)p.weight % 16 == 0;
 }
 
-bool norm_fits(const NormParams &p) { return (long long)p.tokens * p.x.heads * 1024 < (1ll << 32) || (p.x.dim <= 512 && (long long)p.tokens * p.x.heads * kThreads < (1ll << 32)); }
+// Work-items of a grid's x are less than 2^32: workgroups of at most 1024 a row, of 256 for short rows.
+bool norm_fits(const NormParams &p) {
+    const long long rows = (long long)p.tokens * p.x.heads;
+    return rows * (p.x.dim <= 512 ? kThreads : 1024) < (1ll << 32);
+}
 
+// A head's lanes for up to 512 values: 98304 heads of 96 15.8 us, a workgroup each 35.5; of 256 32.6 and 36.9 (65536 of
+// 512: 43.1 and 41.4).  Longer rows: a unit a thread, two of 16 bits (BF16, 4096 rows of 5120: two 30.5 us, one
+// 32.9, four 34.3; of 2048 12.9, 14.5 and 13.1; of 8192 46.4, 49.5 and 49.7.  F32: 63.9, 62.6 and 66.0, a
+// single row 3.7, 3.4 and 4.2).  Not by the number of rows: the squares are summed in one order in any batch.
 hipError_t launch_norm(const NormParams &p, hipStream_t s) {
     const long long rows = (long long)p.tokens * p.x.heads;
     const int units = (int)p.x.dim / 8;
@@ -190,6 +204,9 @@ hipError_t launch_norm(const NormParams &p, hipStream_t s) {
             case 32: hipLaunchKernelGGL((k_norm_heads<32>), grid, dim3(kThreads), 0, s, p, rows); break;
             default: hipLaunchKernelGGL((k_norm_heads<64>), grid, dim3(kThreads), 0, s, p, rows);
         }
+    } else if (units > 128 && units <= 2048 && p.x.type != M27Q_TYPE_F32) {
+        const int threads = (units + 127) / 128 * 64;
+        hipLaunchKernelGGL((k_norm_row<2, 1024>), dim3((unsigned)rows), dim3(threads), 0, s, p, threads);
     } else if (units <= 1024) {
         const int threads = (units + 63) / 64 * 64;
         hipLaunchKernelGGL((k_norm_row<1, 1024>), dim3((unsigned)rows), dim3(threads), 0, s, p, threads);

@@ -81,11 +81,25 @@ def test_dims(m27q, dev, dim):
 @pytest.mark.gpu
 @pytest.mark.parametrize("types", [("f32", None, None, "f32"), ("f16", "f16", "f16", "f16"), ("bf16", "bf16", "bf16", "bf16"),
                                    ("f32", "bf16", "bf16", None), ("f16", "f32", None, "bf16"), ("bf16", None, "f32", "f16")])
-@pytest.mark.parametrize("tokens,heads,dim", [(3, 1, 5120), (7, 24, 256), (65, 4, 64), (2, 3, 96), (9, 16, 128), (4, 2, 800)])
+@pytest.mark.parametrize("tokens,heads,dim", [(3, 1, 5120), (7, 24, 256), (65, 4, 64), (2, 3, 96), (9, 16, 128), (4, 2, 800), (2, 1, 1056), (2, 1, 8224), (3, 1, 16384)])
 def test_types_and_heads(m27q, dev, types, tokens, heads, dim):
     say("norm types", types, tokens, heads, dim)
     check(m27q, dev, tokens, heads, dim, types, codes=True)
     check(m27q, dev, tokens, heads, dim, types, codes=False, weighted=False, eps=0.5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("tokens,heads,dim", [(1500, 1, 1056), (1100, 1, 5120), (700, 3, 256), (1030, 1, 100)])
+def test_rows_alone_and_in_a_batch(m27q, dev, t, tokens, heads, dim):
+    import torch
+    say("norm batch", t, tokens, heads, dim)
+    x = torch.randn(tokens, heads, dim, device=dev, generator=torch.Generator(dev).manual_seed(dim)).to(torch.float32 if t == "f32" else torch.bfloat16)
+    y, one = torch.empty_like(x), torch.empty_like(x[:1])
+    m27q.rms_norm(x, out=y)
+    for i in (0, tokens // 2, tokens - 1):
+        m27q.rms_norm(x[i:i + 1], out=one)
+        assert torch.equal(one[0], y[i])
 
 
 @pytest.mark.gpu
