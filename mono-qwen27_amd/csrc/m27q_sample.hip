@@ -755,10 +755,25 @@ __device__ __forceinline__ void min_of_first(T v, T &to) {
     if (m && (int)(threadIdx.x & 63) == __builtin_ctzll(m)) atomicMin(&to, v);
 }
 
+// How far down in its bin a logit lies, of 1: by what it is off a whole unit.
+__device__ __forceinline__ float part_of(const Place &a) {
+    return a.bin < kFine ? (float)a.z + 0.5f : ((float)a.k + (float)a.z + 0.5f) * (1.0f / kUnit);
+}
+// The same for logits of 16 bits (`low` bits of theirs as floats are 0), of which hundreds are equal: by how many
+// 16-bit numbers lie between it and the bin's upper end, equal ones by index.  Whole numbers, so that what is
+// before another in the row's order is never behind it here.  24 rows of 248320, BF16, top-p: 35 us, by z 64.
+__device__ __forceinline__ float part_of(uint64_t key, int bin, const Scale &s, int low, uint32_t n) {
+    const double d = s.anchor - bin_distance(bin);
+    const int up = (int)(order_bits((float)((d + 0.5) / s.c)) >> low) + 1;  // (rounding, of less than one number)
+    const int down = (int)(order_bits((float)((d - (bin < kFine ? 0.5 : kUnit - 0.5)) / s.c)) >> low);
+    const int at = up - (int)((uint32_t)(key >> 24) >> low);
+    return ((float)at + (float)key_index(key) / (float)n) / (float)(up - down + 1);
+}
+
 // A row's list in order, the running sums of its tokens, and the borders among them.  E tokens a thread.
-// In order: a bin's tokens have as many buckets as they are, by z, so that few share one; a
+// In order: a bin's tokens have as many buckets as they are, by their place in it, so that few share one; a
 // token's place in its bucket is how many of it are larger.  False: some bucket holds so many
-// (equal logits) that this would take long.
+// (equal logits of 32 bits) that this would take long.
 template <int E>
 __device__ __forceinline__ bool pick_from_list(const m27q_sampling &p, const Scratch &sc, const RowPlan &plan, const Rule &r, int n,
                                                PickShared &s) {
@@ -780,7 +795,7 @@ __device__ __forceinline__ bool pick_from_list(const m27q_sampling &p, const Scr
         if (e * kRowThreads + tid >= n) continue;
         const Place a = place_of(key_value(key[e]), scale);
         const uint32_t at = s.at[a.bin], count = s.at[a.bin + 1] - at;
-        const float part = a.bin < kFine ? (float)a.z + 0.5f : ((float)a.k + (float)a.z + 0.5f) * (1.0f / kUnit);
+        const float part = p.type == M27Q_TYPE_F32 ? part_of(a) : part_of(key[e], a.bin, scale, p.type == M27Q_TYPE_BF16 ? 16 : 13, p.n);
         // (below n even if somebody writes to the logits meanwhile)
         bucket[e] = min(at + min((uint32_t)fmaxf(part * (float)count, 0.0f), count - 1), (uint32_t)n - 1);
         slot[e] = atomicAdd(&s.count[bucket[e]], 1u);

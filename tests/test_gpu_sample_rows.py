@@ -145,6 +145,22 @@ def test_types_and_strides(m27q, dev, t, n, stride):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("kind", ["bulk", "flat", "far", "ties"])
+def test_many_equal_logits(m27q, dev, t, kind):
+    """16 bits: hundreds of tokens share a value, and several values, or one, a bin."""
+    say("sample equal", t, kind)
+    rng = np.random.default_rng(len(kind))
+    x = logits(rng, 8, 120000, kind)
+    if kind == "flat":
+        x += np.float32(3)
+    for T in (1.0, 0.2, 4.0, 1e-3, float("inf")):
+        T = np.full(8, T, np.float32)
+        check(m27q, dev, x, T, [0, 0, 0, 700, 30000, 50, 0, 0], [0.9, 0.5, 0.999, 1.0, 1.0, 0.9, 1.0, 1.0],
+              [0.0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.1, 0.0], rng.random(8), t=t)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows", [1, 2, 17, 130, 300])
 def test_batches(m27q, dev, rows):
     """A row gives in a batch what it gives alone."""
