@@ -239,9 +239,9 @@ __device__ __forceinline__ double units_of(double l, double c, double &z) {
 
 // The same for logits less than 2^26 units from the anchor: how far down from it, the whole number in the low bits of an
 // addition.
-__device__ __forceinline__ uint32_t units_down(double l, double c, double low, double anchor, double &z) {
+__device__ __forceinline__ uint32_t units_down(double l, double c, double low, double &z) {
     const double t = __builtin_fma(l, -c, low);  // low = anchor + 1.5 2^52
-    z = __builtin_fma(l, -c, anchor - (t - 0x1.8p52));
+    z = __builtin_fma(l, -c, low - t);           // (the difference is a whole number below 2^27)
     return (uint32_t)__builtin_bit_cast(unsigned long long, t);
 }
 
@@ -380,7 +380,7 @@ __global__ __launch_bounds__(kPartThreads) void k_sample_parts(const m27q_sampli
 #pragma unroll
                 for (int j = 0; j < AT; ++j) {
                     double z;
-                    const uint32_t d = units_down((double)v[i0 + j], s.c, low, s.anchor, z);
+                    const uint32_t d = units_down((double)v[i0 + j], s.c, low, z);
                     bin[j] = bin_of(d);
                     m[j] = w.mass(z, (int)(d & (kUnit - 1)), 1);
                 }
