@@ -472,8 +472,8 @@ M27Q_API m27q_status m27q_attn_paged(const m27q_seqs *seqs, const m27q_cache *ca
  * in pages that all of them name.  first does not descend and stays within
  * 0 .. n; a sequence before first[0] or from first[groups] on shares nothing.
  * Bounds of the launch: a group has at most max_rows rows, from the first of its
- * first sequence to the last of its last one (rows past them are not worked on), and
- * at most max_len places of a len are taken as shared. */
+ * first sequence to the last of its last one (rows past them may be left as they are),
+ * and at most max_len places of a len are taken as shared. */
 typedef struct m27q_prefixes {
     const int32_t *first;   /* device, groups + 1 */
     const int32_t *len;     /* device, groups */
@@ -487,9 +487,10 @@ typedef struct m27q_prefixes {
  * prefixes: a prefix's keys and values are read once for all rows of its group,
  * through the page table of the group's first sequence.  Only whole tiles of 32
  * places are taken so; the rest of a sequence's places come from its own table.
- * Where the tables of a group name the same pages, the results are those of
- * m27q_attn_paged, to the order of sums; where they do not, the first sequence's
- * count.  A len past a sequence's own tokens is fine: rows see what lies at or
+ * Where that saves nothing (by the bounds and the numbers of sequences and heads), all
+ * places do.  The tables of a group name the same pages for its prefix: the results
+ * are those of m27q_attn_paged, to the order of sums.  (Where they do not, which one is
+ * read is not said.)  A len past a sequence's own tokens is fine: rows see what lies at or
  * before their own place.  scratch as in m27q_attn_paged, by its own size. */
 M27Q_API size_t m27q_attn_shared_scratch_bytes(const m27q_seqs *seqs, const m27q_prefixes *prefix, uint32_t q_heads,
                                                const m27q_cache *cache);

@@ -24,8 +24,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void k_attn_both(const AttnParams p
     }
 }
 
-// The same of few rows, bound by the latency of a part's steps: 4 tokens behind 2048 places and up to 300 own ones, 10 MB,
-// 11 us and 5.5 of joining.
+// The same of few rows, bound by the latency of a part's steps: 4 tokens behind 32768 places and up to 300 own ones, 137
+// MB, 38.5 us with the join, 3.6 TB/s.
 template <int D, bool BF, int NP, int PREFIX_ROWS, int OWN_ROWS>
 __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) void k_attn_few_both(const AttnParams p, unsigned px, unsigned prefix,
                                                                                   unsigned ox) {
@@ -68,6 +68,25 @@ int parts_of(long long wgs, long long slots, long long keys, long long least, lo
     return (int)std::max(1ll, std::min({slots / wgs, (keys + least - 1) / least, limit}));
 }
 
+// Whether a prefix is read once for its group, or by each sequence as the rest of its keys (from the caches then, which hold
+// it after the first): what is saved against what a pass of its own costs, from the bounds, as if all sequences
+// shared.  In tiles of 32 places of 256 values, by times measured with 4 cache heads of 256 (24 query heads, F16 to F32):
+// 656 tiles a us of up to 16 rows and 496 of 32 by themselves, 160 of 128 rows of a group.  A few rows (of a group 32):
+// what is saved has to be 1200 tiles, for lengths, groups and places are looked up one after another; 4 tokens behind
+// 2048, 8192, 16384 and 32768 places 16.6, 24.3, 29.0 and 38.5 us, by themselves 13.0, 22.7, 31.1 and 48.3; 9 behind
+// 1560 (8 heads) 15.0 and 19.9.  More: 6 us, and 1 for 400 tiles of own keys, which have a wave of a workgroup here; 64 tokens and up
+// to 600 own places behind 1024, 2048, 8192 and 32768 41.7, 44.1, 66 and 117 and 35.0, 46.4, 117 and 403; 8 x 5 tokens behind 8192,
+// 16384 and 32768 37.9, 53.9 and 78.7 and 34.5, 50.5 and 83.4; 3 x 8 x 5 behind 12000 66 and 96.  Prompts save
+// what is left over of tiles of 128 rows: 4 of 200 tokens behind 512, 1024 and 4096 49, 61 and 147 and 48, 74 and 165.
+bool worth_sharing(const m27q_seqs &seqs, const m27q_prefixes &prefix, long long group, const m27q_cache &cache, long long shared) {
+    const double n = seqs.n, groups = prefix.groups, tile = (double)cache.heads * cache.dim / (256 * kKeys), tiles = shared * tile;
+    const long long rows = seqs.max_q * group, together = prefix.max_rows * group;
+    const double others = groups * tiles * tiles_of(together) / 160;
+    if (rows > kRows) return n * tiles * tiles_of(rows) / 160 - others >= 1.5;
+    if (together <= kRows) return (n - groups) * tiles >= 1200;
+    return n * tiles / (rows <= 16 ? 656 : 496) - others >= 6 + n * (seqs.max_kv - shared) * tile / 400;
+}
+
 }  // namespace
 
 // Workgroups of a part of the keys, the prefixes' and the sequences'.
@@ -94,6 +113,10 @@ SharedPlan shared_plan(const m27q_seqs &seqs, const m27q_prefixes &prefix, uint3
     const long long own = attn_groups(seqs, q_heads, cache);
     const long long shared = prefix.max_len < seqs.max_kv ? prefix.max_len : seqs.max_kv;
     SharedPlan r{};
+    if (!worth_sharing(seqs, prefix, group, cache, shared)) {
+        const AttnPlan each = attn_plan(seqs, q_heads, cache, cus);
+        return {{each.few, 0}, each.splits};
+    }
     r.prefix.few = rows <= kRows && seqs.max_q * group <= kRows;
     const int least = r.prefix.few ? 128 : 256;
     const long long places = r.prefix.few && cache.dim == 256 ? cus : slots;
@@ -104,6 +127,7 @@ SharedPlan shared_plan(const m27q_seqs &seqs, const m27q_prefixes &prefix, uint3
 }
 
 hipError_t launch_shared(const AttnParams &p, const SharedPlan &plan, hipStream_t s) {
+    if (plan.prefix.splits == 0) return launch_attn(p, {plan.prefix.few, plan.own}, s);
     const bool bf = p.cache.type == M27Q_TYPE_BF16;
     switch (p.cache.dim) {
         case 64: return bf ? launch_t<64, true>(p, plan, s) : launch_t<64, false>(p, plan, s);

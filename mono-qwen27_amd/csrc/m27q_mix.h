@@ -54,8 +54,8 @@ hipError_t launch_attn(const AttnParams &p, const AttnPlan &plan, hipStream_t s)
 // Attention behind shared prefixes: the prefixes' keys for the rows of a group, then each
 // sequence's own, as parts of one softmax.
 struct SharedPlan {
-    AttnPlan prefix;
-    int own;        // parts of a sequence's own keys
+    AttnPlan prefix;  // no parts: not worth a pass of its own, every sequence reads all of its keys
+    int own;          // parts of a sequence's own keys
 };
 long long shared_groups(const m27q_seqs &seqs, const m27q_prefixes &prefix, uint32_t q_heads, const m27q_cache &cache);
 SharedPlan shared_plan(const m27q_seqs &seqs, const m27q_prefixes &prefix, uint32_t q_heads, const m27q_cache &cache,

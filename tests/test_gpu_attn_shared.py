@@ -27,10 +27,32 @@ class Shared(Problem):
         for s in range(len(lens)):
             self.put(s)
 
-    def run(self, out_t, scale, stream=None, fill=0.0, max_q=None, max_kv=None, max_rows=None, max_len=None, first=None, length=None):
+    def run(self, out_t, scale, stream=None, fill=0.0, max_q=None, max_kv=None, max_rows=None, max_len=None, first=None, length=None,
+            times=None):
+        """With every head `times` over, so that the prefix is worth a pass of its own (None: as many as that takes, or
+        once where that is more than there can be); all copies give the same."""
         import torch
         d, m = self.dev, self.m
-        cache = m.KVCache(self.kc.to(d), self.vc.to(d))
+        if times is None:
+            times = next((f for f in (1, 4, 16, 64, 256) if self.Hk * f <= 512 and self.H * f <= 1024 and self.pair(
+                f, max_q, max_kv, max_rows, max_len, first, length)[3]), 1)
+        seqs, x, cache, self.apart = self.pair(times, max_q, max_kv, max_rows, max_len, first, length)
+        H = self.H * times
+        scratch = torch.full((m.attn_shared_scratch_bytes(seqs, x, H, cache),), 255, dtype=torch.uint8, device=d)
+        out = torch.full((self.T, H, self.D), fill, dtype=dtype(out_t), device=d)
+        q = self.q.to(d).repeat(1, times, 1)[..., : self.D]
+        torch.cuda.synchronize()
+        m.attn_shared(seqs, x, cache, q, out, scratch, scale, stream=stream)
+        torch.cuda.synchronize()
+        out = out.view(self.T, times, self.H, self.D)
+        assert times == 1 or torch.equal(out.view(torch.uint8), out[:, :1].expand_as(out).contiguous().view(torch.uint8))
+        return out[:, 0].double().cpu().numpy()
+
+    def pair(self, times, max_q, max_kv, max_rows, max_len, first, length):
+        """The call's records, and whether its prefix is taken by itself (its scratch tells)."""
+        import torch
+        d, m = self.dev, self.m
+        cache = m.KVCache(self.kc.to(d).repeat(1, times, 1, 1), self.vc.to(d).repeat(1, times, 1, 1))
         seqs = m.Seqs(self.start.to(d), self.kv.to(d), self.table.to(d), self.T, max_q or self.max_q, max_kv or self.max_kv)
         edge = first or [g[0] for g in self.groups] + [self.groups[-1][0] + self.groups[-1][1]]
         length = length or [g[2] for g in self.groups]
@@ -39,20 +61,16 @@ class Shared(Problem):
                                           for a, b in zip(edge, edge[1:])))
         x = m.Prefixes(torch.tensor(edge, dtype=torch.int32, device=d), torch.tensor(length, dtype=torch.int32, device=d), rows,
                        max_len or max(1, max(length)))
-        scratch = torch.full((m.attn_shared_scratch_bytes(seqs, x, self.H, cache),), 255, dtype=torch.uint8, device=d)
-        out = torch.full((self.T, self.H, self.D), fill, dtype=dtype(out_t), device=d)
-        q = self.q.to(d)[..., : self.D]
-        torch.cuda.synchronize()
-        m.attn_shared(seqs, x, cache, q, out, scratch, scale, stream=stream)
-        torch.cuda.synchronize()
-        return out.double().cpu().numpy()
+        H = self.H * times
+        return seqs, x, cache, m.attn_shared_scratch_bytes(seqs, x, H, cache) != m.attn_scratch_bytes(seqs, H, cache)
 
     def check(self, out_t, scale, gone=(), **how):
-        got = self.run(out_t, scale, **how)
         want, A, es, small = self.want(scale, 0, gone)
         tol = (WEIGHT[self.t, out_t] + es) * A + small + OUT[out_t] * np.abs(want) + 2.0 ** -25 * (out_t == "f16")
-        assert np.isfinite(got).all()
-        assert np.all(np.abs(got - want) <= tol), np.max(np.abs(got - want) / tol)
+        for times in (1, None):
+            got = self.run(out_t, scale, times=times, **how)
+            assert np.isfinite(got).all()
+            assert np.all(np.abs(got - want) <= tol), np.max(np.abs(got - want) / tol)
 
 
 CASES = [
@@ -88,6 +106,26 @@ CASES = [
 def test_shared_attention_against_definition(m27q, dev, lens, groups, H, Hk, D, page, t, out):
     say("shared", lens[:4], groups, H, Hk, D, page, t, out)
     Shared(m27q, dev, lens, groups, H, Hk, D, page, t).check(out, D ** -0.5)
+
+
+@pytest.mark.gpu
+def test_which_prefixes_are_taken_by_themselves(m27q, dev):
+    """Most of the cases above, some of them with their heads as they are: both ways are tested."""
+    import torch
+    apart = []
+    for lens, groups, H, Hk, D, page, t, _ in CASES:
+        p = Shared(m27q, dev, lens, groups, H, Hk, D, page, t)
+        p.run("f32", 0.1)
+        apart.append(p.apart)
+    assert sum(apart) >= len(CASES) // 2, apart
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
+    one = lambda n, places, heads: (m27q.Seqs(i32(*range(n + 1)), i32(*[places + 300] * n), torch.zeros(  # noqa: E731
+        n, 1024, dtype=torch.int32, device=dev), n, 1, places + 300), m27q.Prefixes(i32(0, n), i32(places), n, places), heads)
+    pages = torch.zeros(1, 4, 64, 256, dtype=torch.float16, device=dev)
+    cache = m27q.KVCache(pages, pages)
+    for (seqs, x, heads), apart in ((one(4, 2048, 24), False), (one(4, 32768, 24), True), (one(64, 512, 24), False), (one(64, 32768, 24), True),
+                                    (one(1, 32768, 24), False)):
+        assert (m27q.attn_shared_scratch_bytes(seqs, x, heads, cache) != m27q.attn_scratch_bytes(seqs, heads, cache)) == apart
 
 
 @pytest.mark.gpu
@@ -163,7 +201,8 @@ def test_untouched_rows_and_same_results(m27q, dev):
     part = p.run("f32", 0.125, fill=9.0, max_q=6)
     assert (part[11] == 9).all() and np.allclose(np.delete(part, 11, 0), np.delete(full, 11, 0), rtol=0, atol=1e-5)
     part = p.run("f32", 0.125, fill=9.0, max_rows=8)
-    assert (part[8:12] == 9).all() and np.allclose(part[:8], full[:8], rtol=0, atol=1e-5)
+    assert not p.apart or (part[8:12] == 9).all()
+    assert np.allclose(part[:8], full[:8], rtol=0, atol=1e-5)
     assert np.allclose(part[12:], full[12:], rtol=0, atol=1e-5)
     assert np.allclose(Problem.run(p, "f32", 0.125, fill=9.0), full, rtol=0, atol=1e-5)
 
@@ -173,7 +212,7 @@ def test_graph_replays_with_new_groups(m27q, dev):
     """Captured once; each replay finds new lengths, groups, shared places and rows in the same buffers."""
     import torch
     say("shared graph")
-    H, Hk, D, page, n = 6, 1, 128, 16, 5
+    H, Hk, D, page, n = 336, 56, 128, 16, 5
     g = torch.Generator(device=dev).manual_seed(4)
     kc, vc = (torch.randn(200, Hk, page, D, generator=g, device=dev).half() for _ in range(2))
     cache = m27q.KVCache(kc, vc)
@@ -221,22 +260,24 @@ def test_pages_past_32_bits(m27q, dev):
     """Pages 2^31 values apart."""
     import torch
     say("shared far pages")
-    D, page = 64, 32
-    pool = torch.empty((3 << 31) + 2 * page * D, dtype=torch.float16, device=dev)
-    kc = pool.as_strided((3, 1, page, D), (1 << 31, page * D, D, 1))
-    vc = pool[page * D:].as_strided((3, 1, page, D), (1 << 31, page * D, D, 1))
+    D, page, H = 256, 1024, 40
+    size = H * page * D
+    pool = torch.empty((2 << 31) + 2 * size, dtype=torch.float16, device=dev)
+    kc = pool.as_strided((3, H, page, D), (1 << 31, page * D, D, 1))
+    vc = pool[size:].as_strided((3, H, page, D), (1 << 31, page * D, D, 1))
     g = torch.Generator().manual_seed(1)
-    k, v = (torch.randn(3, 1, page, D, generator=g).half().to(dev) for _ in range(2))
+    k, v = (torch.randn(3, H, page, D, generator=g).half().to(dev) for _ in range(2))
     kc.copy_(k)
     vc.copy_(v)
-    q = torch.randn(2, 1, D, generator=g).half().to(dev)
+    q = torch.randn(2, H, D, generator=g).half().to(dev)
     i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
-    seqs, x = m27q.Seqs(i32(0, 1, 2), i32(60, 40), i32(2, 0, 2, 1).view(2, 2), 2, 1, 64), m27q.Prefixes(i32(0, 2), i32(32), 2, 32)
+    seqs, x = m27q.Seqs(i32(0, 1, 2), i32(1084, 1064), i32(2, 0, 2, 1).view(2, 2), 2, 1, 1100), m27q.Prefixes(i32(0, 2), i32(1024), 2, 1024)
     outs = []
     for kk, vv in ((kc, vc), (k, v)):
         cache = m27q.KVCache(kk, vv)
-        out = torch.empty(2, 1, D, device=dev)
-        scratch = torch.empty(m27q.attn_shared_scratch_bytes(seqs, x, 1, cache), dtype=torch.uint8, device=dev)
+        out = torch.empty(2, H, D, device=dev)
+        scratch = torch.empty(m27q.attn_shared_scratch_bytes(seqs, x, H, cache), dtype=torch.uint8, device=dev)
+        assert scratch.numel() != m27q.attn_scratch_bytes(seqs, H, cache)  # the prefix by itself
         m27q.attn_shared(seqs, x, cache, q, out, scratch, 0.1)
         outs.append(out.cpu())
     assert torch.equal(outs[0], outs[1]) and bool(outs[0].abs().sum() > 0)

@@ -10,7 +10,7 @@ import pytest
 
 from gpu_util import say
 
-H, HK, D, ROT, PAGE, HIDDEN, VOCAB = 6, 1, 64, 32, 16, 256, 1000
+D, ROT, PAGE, HIDDEN, VOCAB = 64, 32, 16, 256, 1000
 
 
 def q8_0(rng, rows, cols):
@@ -21,8 +21,9 @@ def q8_0(rng, rows, cols):
 
 
 class Step:
-    def __init__(self, m, dev, n, prefix, seed=0):
+    def __init__(self, m, dev, n, prefix, H=6, HK=1, seed=0):
         import torch
+        self.H, self.HK = H, HK
         self.m, self.n, self.dev, self.prefix = m, n, dev, prefix
         rng = np.random.default_rng(seed)
         weight = lambda rows, cols=HIDDEN: m.Weight.upload(q8_0(rng, rows, cols), m.Q8_0, cols // 32, rows, device=dev)  # noqa: E731
@@ -49,6 +50,7 @@ class Step:
         self.out, self.logits = e(n, H, D), e(n, VOCAB)
         self.token, self.prob = torch.zeros(n, dtype=torch.int32, device=dev), e(n)
         self.scratch = e(m.attn_shared_scratch_bytes(self.seqs, self.prefixes, H, self.cache), dtype=torch.uint8)
+        self.apart = self.scratch.numel() != m.attn_scratch_bytes(self.seqs, H, self.cache)  # the prefix in a pass of its own
         self.plain = e(m.attn_scratch_bytes(self.seqs, H, self.cache), dtype=torch.uint8)
         self.pick = e(m.sample_rows_scratch_bytes(n, VOCAB), dtype=torch.uint8)
 
@@ -77,7 +79,7 @@ class Step:
     def without(self):
         """The same step by torch's norm, the paged attention, and candidates one row at a time: logits and tokens."""
         import torch
-        m, n = self.m, self.n
+        m, n, H = self.m, self.n, self.H
         norm = lambda x, w: x * (x.square().mean(-1, keepdim=True) + 1e-6).rsqrt() * w  # noqa: E731
         h = self.x + self.res
         act, act2 = m.Act(n, HIDDEN, self.dev), m.Act(n, H * D, self.dev)
@@ -94,10 +96,11 @@ class Step:
 
 
 @pytest.mark.gpu
-def test_step_beside_the_one_without(m27q, dev):
+@pytest.mark.parametrize("size", [(9, 160), (40, 4096, 32, 8)])
+def test_step_beside_the_one_without(m27q, dev, size):
     import torch
     say("batch step")
-    s = Step(m27q, dev, 9, 160)
+    s = Step(m27q, dev, *size)
     for i in range(4):
         s.inputs(i)
         s.run()
@@ -124,10 +127,12 @@ def test_step_beside_the_one_without(m27q, dev):
 
 
 @pytest.mark.gpu
-def test_step_captured_and_replayed(m27q, dev):
+@pytest.mark.parametrize("size,apart", [((9, 160), False), ((40, 4096, 32, 8), True), ((5, 3200, 24, 12), True)])
+def test_step_captured_and_replayed(m27q, dev, size, apart):
     import torch
     say("batch step graph")
-    s = Step(m27q, dev, 40, 480, seed=3)  # 240 rows of the prefix: the kernel of many
+    s = Step(m27q, dev, *size, seed=3)
+    assert s.apart == apart
     s.inputs(0)
     s.run()
     torch.cuda.synchronize()
@@ -151,7 +156,8 @@ def test_two_calls_on_two_streams(m27q, dev):
     """Two batches at once, each with scratch of its own."""
     import torch
     say("batch step streams")
-    steps = [Step(m27q, dev, 20, 320, seed=i) for i in (5, 6)]
+    steps = [Step(m27q, dev, 40, 4096, 32, 8, seed=i) for i in (5, 6)]
+    assert all(s.apart for s in steps)
     for i, s in enumerate(steps):
         s.inputs(i)
     want = []
