@@ -461,7 +461,7 @@ __device__ __forceinline__ int part_bin(int J, int off) {
     return J >= kBins ? -1 : J < kFine ? max(J - off, -1) : oct >= kOctaves ? kFine + oct - kOctaves : oct >= 0 ? kBins + 1 + oct : -1;
 }
 
-constexpr int kPlanThreads = 512;
+constexpr int kPlanThreads = 512, kHalves = 2;
 static_assert(kBins + 1 == kPlanThreads, "a thread a bin");
 
 // The largest of a wave's values, all above 0, for every lane.
@@ -497,25 +497,30 @@ __device__ __forceinline__ int first_of(const T *v, int n, F reaches) {
 // A row's bins from those of its parts, and the bins in which its borders can lie: of the top_k-th
 // token, of top_p, of min_p and of the pick.  What is not known before another border is found
 // leaves a range of bins.  A chain of steps that wait for each other bounds it: each wave does
-// for itself what is not a bin's (it took 11.4 us with the workgroup's threads looking for each border).
-__global__ __launch_bounds__(kPlanThreads) void k_sample_plan(const m27q_sampling p, const Scratch sc) {
+// for itself what is not a bin's (it took 11.4 us with the workgroup's threads looking for each border, 8.9
+// with all parts by the same threads; 8 now, of which loading and adding the parts' bins is a half).
+__global__ __launch_bounds__(kHalves * kPlanThreads) void k_sample_plan(const m27q_sampling p, const Scratch sc) {
     constexpr int W = kPlanThreads / 64;
     __shared__ unsigned long long mass_s[W], sum[kBins + 2];
     __shared__ uint32_t count_s[W], tokens_s[kBins + 2];  // down to a bin, without it
-    const int row = blockIdx.x, J = threadIdx.x, lane = J & 63, wave = J >> 6;
+    const int row = blockIdx.x, J = threadIdx.x & (kPlanThreads - 1), lane = J & 63, wave = J >> 6;
+    const int half = __builtin_amdgcn_readfirstlane(threadIdx.x / kPlanThreads);
     const Part *part = sc.part + (long long)row * sc.parts;
     const Rule r = row_rule(p, row);
     RowPlan &out = sc.plan[row];
     unsigned long long best = 0, high = 0;
+    double anchors = 0;  // of the first 64 parts, a lane each
     for (int i = lane; i < sc.parts; i += 64) {
-        high = max(high, ordered(part[i].anchor));
-        best = max(best, (unsigned long long)part[i].best);
+        const Part x = part[i];
+        if (i == lane) anchors = x.anchor;
+        high = max(high, ordered(x.anchor));
+        best = max(best, (unsigned long long)x.best);
     }
     best = max_wave(best);
     const double anchor = unordered(max_wave(high));
     const float top = key_value(best);
     if (r.greedy || !__builtin_isfinite(top)) {
-        if (J == 0) {
+        if (threadIdx.x == 0) {
             p.token[row] = key_index(best);
             if (p.prob) p.prob[row] = 1.0f;
             out.state = 0;
@@ -523,20 +528,24 @@ __global__ __launch_bounds__(kPlanThreads) void k_sample_plan(const m27q_samplin
         return;
     }
 
-    // this thread's bin, from one stored sum of each part
+    // this thread's bin, from one stored sum of each part; half of the threads have the one half of the parts
     unsigned long long mass = 0;
     uint32_t count = 0;
     constexpr unsigned long long kMask = (1ull << kSumBits) - 1;
-    constexpr int kSkip = 1 << 20, AT = 32;  // parts on their way at a time
-    for (int i0 = 0; i0 < sc.parts; i0 += AT) {
-        const double down = anchor - part[min(i0 + (lane & (AT - 1)), sc.parts - 1)].anchor;
-        const int offs = i0 + (lane & (AT - 1)) < sc.parts && down < kReach ? (int)down : kSkip;
+    constexpr int kSkip = 1 << 20, AT = 16;  // parts on their way at a time
+    int offs = kSkip;
+    for (int i0 = half * AT; i0 < sc.parts; i0 += kHalves * AT) {
+        if (i0 % 64 < kHalves * AT) {
+            const int i = i0 - i0 % 64 + lane;
+            if (i0 >= 64) anchors = part[min(i, sc.parts - 1)].anchor;
+            offs = i < sc.parts && anchor - anchors < kReach ? (int)(anchor - anchors) : kSkip;
+        }
         const unsigned long long *bins = sc.bins + ((long long)row * sc.parts + i0) * kStored;
         unsigned long long x[AT];
         bool ok[AT];
 #pragma unroll
         for (int k = 0; k < AT; ++k) {
-            const int off = __builtin_amdgcn_readlane(offs, k), from = part_bin(J, off);
+            const int off = __builtin_amdgcn_readlane(offs, i0 % 64 + k), from = part_bin(J, off);
             ok[k] = off != kSkip && from >= 0;
             x[k] = bins[(off != kSkip ? k * kStored : 0) + (ok[k] ? from : 0)];
         }
@@ -546,6 +555,14 @@ __global__ __launch_bounds__(kPlanThreads) void k_sample_plan(const m27q_samplin
             mass += ok[k] ? x[k] & kMask : 0ull;
         }
     }
+    if (half) {
+        sum[J] = mass;
+        tokens_s[J] = count;
+    }
+    __syncthreads();
+    if (half) return;
+    mass += sum[J];
+    count += tokens_s[J];
     const double unit = sum_unit(p.n) * bin_scale(J);
     mass = (unsigned long long)__builtin_rint((double)mass * unit);
     unsigned long long above = scan_wave(mass);
@@ -630,23 +647,31 @@ __global__ __launch_bounds__(kPlanThreads) void k_sample_plan(const m27q_samplin
     out.unit[J] = unit;
     out.before[J] = before;
     out.at[J] = at;
-    if (J == 0) {
+    // a lane a range
+    float lo = __builtin_inff();
+    if (J < kRanges) {
         const double c = kUnitsPerNat * r.inv_t;
-        float least = __builtin_inff();
+        int first = b0[0], last = b1[0];
 #pragma unroll
-        for (int j = 0; j < kRanges; ++j) {
-            // logits of the bins, and a little more than those
-            const double up = (anchor - bin_distance(b0[j]) + 0.5) / c;
-            const double down = (anchor - bin_distance(b1[j]) - (b1[j] < kFine ? 0.5 : kUnit - 0.5)) / c;
-            const bool none = b1[j] < b0[j], all = !(c > 1e-30);
-            const float lo = none ? __builtin_inff() : all ? -__builtin_inff() : (float)(down - fabs(down) * 0x1p-20);
-            out.first[j] = b0[j];
-            out.last[j] = b1[j];
-            out.lo[j] = lo;
-            out.hi[j] = none ? -__builtin_inff() : all ? __builtin_inff() : (float)(up + fabs(up) * 0x1p-20);
-            least = fminf(least, lo);
+        for (int j = 1; j < kRanges; ++j) {
+            first = J == j ? b0[j] : first;
+            last = J == j ? b1[j] : last;
         }
-        out.least = least;
+        // logits of the bins, and a little more than those
+        const double up = (anchor - bin_distance(first) + 0.5) / c;
+        const double down = (anchor - bin_distance(last) - (last < kFine ? 0.5 : kUnit - 0.5)) / c;
+        const bool none = last < first, all = !(c > 1e-30);
+        lo = none ? __builtin_inff() : all ? -__builtin_inff() : (float)(down - fabs(down) * 0x1p-20);
+        out.first[J] = first;
+        out.last[J] = last;
+        out.lo[J] = lo;
+        out.hi[J] = none ? -__builtin_inff() : all ? __builtin_inff() : (float)(up + fabs(up) * 0x1p-20);
+    }
+    static_assert(kRanges == 4, "lanes that meet");
+    lo = fminf(lo, __shfl_xor(lo, 1));
+    lo = fminf(lo, __shfl_xor(lo, 2));
+    if (J == 0) {
+        out.least = lo;
         out.anchor = anchor;
         out.best = best;
         out.min_p_sum = min_p_sum;
@@ -955,7 +980,7 @@ template <typename T>
 hipError_t launch_t(const m27q_sampling &p, const Scratch &sc, hipStream_t s) {
     const dim3 parts(sc.parts, p.rows);
     hipLaunchKernelGGL((k_sample_parts<T>), parts, dim3(kPartThreads), 0, s, p, sc);
-    hipLaunchKernelGGL(k_sample_plan, dim3(p.rows), dim3(kPlanThreads), 0, s, p, sc);
+    hipLaunchKernelGGL(k_sample_plan, dim3(p.rows), dim3(kHalves * kPlanThreads), 0, s, p, sc);
     hipLaunchKernelGGL((k_sample_list<T>), parts, dim3(kPartThreads), 0, s, p, sc);
     hipLaunchKernelGGL(k_sample_pick, dim3(p.rows), dim3(kRowThreads), 0, s, p, sc);
     return hipGetLastError();
