@@ -71,100 +71,6 @@ __device__ __forceinline__ Rule row_rule(const m27q_sampling &p, int row) {
     return r;
 }
 
-struct Found {
-    uint64_t key;    // of the token at the border
-    uint64_t sum;    // of the weights down to it, itself included
-};
-
-// What a workgroup that goes through a whole row keeps in LDS.
-struct WholeRow {
-    unsigned long long mass[256];
-    uint32_t count[256];
-    unsigned long long total;
-    uint64_t found_key, found_sum;
-    uint32_t found_count;
-};
-
-// A row whose borders lie among more tokens than a list holds (thousands of equal logits): the
-// token at which a count or a sum of weights in descending order reaches its target, by 8 bits of
-// the keys at a time, the row read once for each.
-__device__ void sample_whole_row(const m27q_sampling &p, int row, const Rule &r, uint64_t best, WholeRow &s) {
-    const int n = (int)p.n, tid = threadIdx.x;
-    const long long base = (long long)row * p.stride;
-    auto value = [&](int i) { return load1(p.logits, base + i, p.type); };
-    const float top = value(key_index(best));
-    if (tid == 0) s.total = 0;
-    const double one = (double)(1ull << (62 - (64 - __builtin_clzll((unsigned long long)n))));
-    auto weight = [&](float v) {
-        const double w = exp(((double)v - (double)top) * r.inv_t);
-        return w > 0.0 ? w : 0.0;  // (NaN: none)
-    };
-    auto fixed = [&](double w) { return (unsigned long long)__builtin_rint(w * one); };
-
-    // The first token in order at which the running count reaches `most` or the running sum `target`.
-    auto border = [&](uint32_t most, double target) {
-        uint64_t prefix = 0, sum = 0;
-        uint32_t seen = 0;
-        for (int shift = kKeyBits - 8; shift >= 0; shift -= 8) {
-            __syncthreads();
-            if (tid < 256) s.mass[tid] = 0, s.count[tid] = 0;
-            __syncthreads();
-            for (int i = tid; i < n; i += kRowThreads) {
-                const float v = value(i);
-                const uint64_t key = order_key(v, i);
-                if ((key >> (shift + 8)) != prefix) continue;
-                const int digit = (int)(key >> shift) & 255;
-                atomicAdd(&s.count[digit], 1u);
-                atomicAdd(&s.mass[digit], fixed(weight(v)));
-            }
-            __syncthreads();
-            if (tid == 0) {
-                int digit = 255, last = -1;
-                for (; digit >= 0; --digit) {
-                    if (s.count[digit] == 0) continue;
-                    last = digit;
-                    if (seen + s.count[digit] >= most || (double)(sum + s.mass[digit]) >= target) break;
-                    seen += s.count[digit];
-                    sum += s.mass[digit];
-                }
-                if (digit < 0) {  // never reached: the last one
-                    digit = last;
-                    seen -= s.count[digit];
-                    sum -= s.mass[digit];
-                }
-                s.found_key = prefix << 8 | (uint64_t)digit;
-                s.found_sum = sum;
-                s.found_count = seen;
-            }
-            __syncthreads();
-            prefix = s.found_key;
-            sum = s.found_sum;
-            seen = s.found_count;
-        }
-        return Found{prefix, sum + fixed(weight(value(key_index(prefix))))};
-    };
-
-    const Found all = border((uint32_t)r.k, __builtin_inf());
-    uint64_t cut = all.key;
-    if (r.top_p < 1.0) cut = max(cut, border(0xffffffffu, r.top_p * (double)all.sum).key);
-    unsigned long long part = 0;
-    for (int i = tid; i < n; i += kRowThreads) {
-        const float v = value(i);
-        const uint64_t key = order_key(v, i);
-        const double w = weight(v);
-        if (key == best || (key >= cut && w >= r.min_p)) part += fixed(w);
-    }
-    atomicAdd(&s.total, part);
-    __syncthreads();
-    const Found pick = border(0xffffffffu, r.u * (double)s.total);
-    if (tid == 0) {
-        const int i = key_index(pick.key);
-        p.token[row] = i;
-        if (p.prob) p.prob[row] = (float)(weight(value(i)) * one / (double)s.total);
-    }
-}
-
-
 // ------------------------------------------------------------------ bins --
 //
 // Weights are told apart by y = 16 log2(e) l / T, a sixteenth of an octave a unit.  The tokens of a
@@ -748,6 +654,204 @@ __global__ __launch_bounds__(kPartThreads) void k_sample_list(const m27q_samplin
     }
 }
 
+// The smallest of a workgroup's values that do not descend from thread to thread, but for the largest of
+// their type, which stands for none: that of each wave's first.
+template <typename T>
+__device__ __forceinline__ void min_of_first(T v, T &to) {
+    const T none = sizeof(T) == 8 ? (T)~0ull : (T)0x7fffffff;
+    const unsigned long long m = __ballot(v != none);
+    if (m && (int)(threadIdx.x & 63) == __builtin_ctzll(m)) atomicMin(&to, v);
+}
+
+// What a workgroup that goes through a whole row keeps in LDS.
+constexpr int kDigitBits = 11, kDigits = 1 << kDigitBits;
+struct WholeRow {
+    unsigned long long mass[kDigits];
+    uint64_t key[kDigits];               // of a digit's only token
+    uint32_t count[kDigits];
+    unsigned long long total;
+    uint64_t found_key;
+    unsigned long long found_sum, found_own;
+    uint32_t found_count, found_held;
+    int found;
+};
+struct Border {
+    uint64_t key;              // of the token at the border
+    unsigned long long sum;    // of the weights down to it, itself included
+    unsigned long long own;    // its weight
+};
+
+// U logits of a row, all on their way at once.
+template <int U>
+__device__ __forceinline__ void load_some(const m27q_sampling &p, long long base, int i0, float (&v)[U]) {
+    const int last = (int)p.n - 1;
+    if (p.type == M27Q_TYPE_F32) {
+#pragma unroll
+        for (int j = 0; j < U; ++j) v[j] = logit<float>(p.logits, base + min(i0 + j * kRowThreads, last));
+    } else if (p.type == M27Q_TYPE_F16) {
+#pragma unroll
+        for (int j = 0; j < U; ++j) v[j] = logit<_Float16>(p.logits, base + min(i0 + j * kRowThreads, last));
+    } else {
+#pragma unroll
+        for (int j = 0; j < U; ++j) v[j] = logit<__bf16>(p.logits, base + min(i0 + j * kRowThreads, last));
+    }
+}
+
+// A row whose borders lie among more tokens than a list holds (flat ones, thousands of equal logits): the
+// token at which a count or a sum of weights in descending order reaches its target, by 11 bits of the keys at
+// a time, the row read once for each, until one token is left.  Weights are those of the bins, in units of which the row's
+// sum has 61 bits.
+__device__ void sample_whole_row(const m27q_sampling &p, int row, const Rule &r, const RowPlan &plan, const double *octave,
+                                 WholeRow &s, uint32_t *scan32, unsigned long long *scan64) {
+    const int n = (int)p.n, tid = threadIdx.x, lane = tid & 63;
+    const long long base = (long long)row * p.stride;
+    const uint64_t best = plan.best;
+    const float top = key_value(best);
+    const Scale scale = row_scale(r, plan.anchor);
+    const Weights x(octave);
+    const int row_bits = 62 - (32 - __builtin_clz(p.n));  // of the anchor's weight in the plan's sums
+    const int up = 61 - kMassBits - max(0, 64 - __builtin_clzll(plan.sum[kBins] | 1) - row_bits);
+    const auto weight = [&](float v) -> unsigned long long {
+        const Place a = place_of(v, scale);
+        return a.bin < kBins ? x.mass(a.z, a.k, 0) << up >> (bin_distance(a.bin) / kUnit) : 0;
+    };
+    constexpr int U = 8;
+
+    // The first token in order at which the running count reaches `most` or the running sum `target`, a part
+    // of the sum of all if `of_all`; the last one if none does.
+    const auto border = [&](uint32_t most, double target, bool of_all) -> Border {
+        uint64_t prefix = 0;
+        unsigned long long sum = 0;
+        uint32_t seen = 0;
+        int above = kKeyBits;  // the key's bits above these are the prefix
+        while (true) {
+            const int shift = max(above - kDigitBits, 0), mask = (1 << (above - shift)) - 1;
+            for (int i = tid; i < kDigits; i += kRowThreads) s.mass[i] = 0, s.count[i] = 0;
+            if (tid == 0) s.found = 0x7fffffff;
+            __syncthreads();
+            for (int i0 = tid; i0 - tid < n; i0 += U * kRowThreads) {
+                float v[U];
+                load_some(p, base, i0, v);
+#pragma unroll 1
+                for (int j = 0; j < U; ++j) {
+                    const int i = i0 + j * kRowThreads;
+                    float l = v[0];
+#pragma unroll
+                    for (int k = 1; k < U; ++k) l = j == k ? v[k] : l;
+                    const uint64_t key = order_key(l, i);
+                    const bool in = i < n && key >> above == prefix;
+                    const unsigned long long some = __ballot(in);
+                    if (!some) continue;
+                    const int digit = (int)(key >> shift) & mask, first = __builtin_ctzll(some);
+                    const int same = __builtin_amdgcn_readlane(digit, first);
+                    unsigned long long w = in ? weight(l) : 0;
+                    if (__ballot(in && digit != same) == 0) {  // lanes that would meet in one place
+                        w = scan_wave(w);
+                        if (lane == 63) {
+                            atomicAdd(&s.mass[same], w);
+                            atomicAdd(&s.count[same], (uint32_t)__popcll(some));
+                        }
+                        if (lane == first) s.key[same] = key;
+                    } else if (in) {
+                        atomicAdd(&s.mass[digit], w);
+                        atomicAdd(&s.count[digit], 1u);
+                        s.key[digit] = key;
+                    }
+                }
+            }
+            __syncthreads();
+            // the digits in descending order, two a thread
+            constexpr int E = kDigits / kRowThreads;
+            static_assert(E == 2, "two digits a thread");
+            const int d0 = kDigits - 1 - E * tid, d1 = d0 - 1;
+            const uint32_t c0 = s.count[d0], c1 = s.count[d1];
+            const unsigned long long m0 = s.mass[d0], m1 = s.mass[d1];
+            uint32_t tokens;
+            unsigned long long all;
+            const uint32_t c = scan_group<kRowThreads>(c0 + c1, scan32, tokens);
+            const unsigned long long m = scan_group<kRowThreads>(m0 + m1, scan64, all);
+            if (of_all) {
+                if (tid == 0) s.total = all;
+                target *= (double)all;
+                of_all = false;
+            }
+            const auto reaches = [&](uint32_t count, unsigned long long mass) {
+                return seen + count >= most || (double)(sum + mass) >= target || count == tokens;
+            };
+            const int hit = c0 && reaches(c + c0, m + m0) ? E * tid : c1 && reaches(c + c0 + c1, m + m0 + m1) ? E * tid + 1 : 0x7fffffff;
+            min_of_first(hit, s.found);
+            __syncthreads();
+            if (s.found / E == tid) {
+                const bool second = s.found % E;
+                s.found_key = second ? s.key[d1] : s.key[d0];
+                s.found_count = seen + c + (second ? c0 : 0);
+                s.found_held = second ? c1 : c0;
+                s.found_sum = sum + m + (second ? m0 : 0);
+                s.found_own = second ? m1 : m0;
+            }
+            __syncthreads();
+            seen = s.found_count;
+            sum = s.found_sum;
+            prefix = s.found_key >> shift;
+            above = shift;
+            const Border found{s.found_key, sum + s.found_own, s.found_own};
+            const bool done = s.found_held == 1 || shift == 0;
+            __syncthreads();  // all have read it
+            if (done) return found;
+        }
+    };
+
+    uint64_t cut = 0;                // the last key that is kept
+    bool known = false;              // the sum of what is kept
+    unsigned long long total = 0;
+    if (r.k < n) {
+        const Border b = border((uint32_t)r.k, __builtin_inf(), false);
+        cut = b.key;
+        total = b.sum;
+        known = true;
+    }
+    if (r.top_p < 1.0) {
+        const Border b = border(0xffffffffu, known ? r.top_p * (double)total : r.top_p, !known);
+        if (b.key > cut || !known) {
+            cut = b.key;
+            total = b.sum;
+        }
+        known = true;
+    }
+    if (r.min_p > 0.0) {
+        // far from the weight min_p a logit tells by itself
+        const double limit = (double)top + log(r.min_p) / r.inv_t, near = 1e-9 * (fabs(limit) + fabs((double)top));
+        if (tid == 0) s.total = 0;
+        __syncthreads();
+        unsigned long long part = 0;
+        for (int i0 = tid; i0 < n; i0 += U * kRowThreads) {
+            float v[U];
+            load_some(p, base, i0, v);
+#pragma unroll 1
+            for (int j = 0; j < U; ++j) {
+                const int i = i0 + j * kRowThreads;
+                float l = v[0];
+#pragma unroll
+                for (int k = 1; k < U; ++k) l = j == k ? v[k] : l;
+                const uint64_t key = order_key(l, i);
+                if (i >= n || key < cut) continue;
+                const bool kept = (double)l > limit + near || (!((double)l < limit - near) && exp(((double)l - (double)top) * r.inv_t) >= r.min_p);
+                if (kept || key == best) part += weight(l);
+            }
+        }
+        atomicAdd(&s.total, part);
+        __syncthreads();
+        total = s.total;
+        known = true;
+        __syncthreads();
+    }
+    const Border pick = border(0xffffffffu, known ? r.u * (double)total : r.u, !known);
+    if (tid == 0) {
+        p.token[row] = key_index(pick.key);
+        if (p.prob) p.prob[row] = (float)((double)pick.own / (double)(known ? total : s.total));
+    }
+}
+
 constexpr int kCrowd = 1024;
 struct PickShared {
     union {
@@ -770,15 +874,6 @@ struct PickShared {
     uint32_t most;
     double octave[kUnit];
 };
-
-// The smallest of a workgroup's values that do not descend from thread to thread, but for the largest of
-// their type, which stands for none: that of each wave's first.
-template <typename T>
-__device__ __forceinline__ void min_of_first(T v, T &to) {
-    const T none = sizeof(T) == 8 ? (T)~0ull : (T)0x7fffffff;
-    const unsigned long long m = __ballot(v != none);
-    if (m && (int)(threadIdx.x & 63) == __builtin_ctzll(m)) atomicMin(&to, v);
-}
 
 // How far down in its bin a logit lies, of 1: by what it is off a whole unit.
 __device__ __forceinline__ float part_of(const Place &a) {
@@ -942,6 +1037,7 @@ __global__ __launch_bounds__(kRowThreads) void k_sample_pick(const m27q_sampling
     if (state == 0) return;
     const Rule r = row_rule(p, row);
     bool done = false;
+    if (threadIdx.x < kUnit) s.octave[threadIdx.x] = Weights::factor(threadIdx.x);
     if (state == 1) {
         if (threadIdx.x <= kBins) {
             s.before[threadIdx.x] = plan.before[threadIdx.x];
@@ -956,7 +1052,6 @@ __global__ __launch_bounds__(kRowThreads) void k_sample_pick(const m27q_sampling
             s.pick = 0x7fffffff;
             s.most = 0;
         }
-        if (threadIdx.x < kUnit) s.octave[threadIdx.x] = Weights::factor(threadIdx.x);
         const int n = (int)min(plan.listed, (uint32_t)kList);
         if (n <= kRowThreads) done = pick_from_list<1>(p, sc, plan, r, n, s);
         else if (n <= 2 * kRowThreads) done = pick_from_list<2>(p, sc, plan, r, n, s);
@@ -964,7 +1059,7 @@ __global__ __launch_bounds__(kRowThreads) void k_sample_pick(const m27q_sampling
         else done = pick_from_list<8>(p, sc, plan, r, n, s);
         if (!done) __syncthreads();
     }
-    if (!done) sample_whole_row(p, row, r, plan.best, s.whole);
+    if (!done) sample_whole_row(p, row, r, plan, s.octave, s.whole, s.scan32, s.scan);
 }
 
 struct Sizes {
