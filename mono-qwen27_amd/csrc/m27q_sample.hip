@@ -15,15 +15,16 @@
 //   plan   a row's bins from its parts', and those that can hold a border
 //   list   the tokens of these bins, from a second reading (parts without any are passed over)
 //   pick   a row's list in order, its running sums, the borders, the token
-// Where the list would be too long (thousands of equal logits at a border), pick goes through
-// the whole row by bits of its keys.
+// Where the list would be too long (flat rows, thousands of equal logits at a border), pick reads the whole
+// row once or twice more for each border, by pieces of its bin's keys.
 //
 // 200 rows of 248320 F32, top-p (199 MB): 101 us, of these 54 for parts, 9, 26 for list (7.6 TB/s:
 // what parts read last still lies in the caches) and 11.  parts is bound by the vector units: some 32 operations
 // of a wave for each 64 tokens, half of them on 64 bits, and the LDS additions beside them (a
 // plain read of the same bytes: 29).  64 rows of all rules 47.5 us (20, 9.3, 12, 9); one row
-// 25.7: four launches of 5.6, 8.9, 5.2 and 6, each the latency of its steps.  Whole rows by
-// bits of their keys take 2779 for the 64.
+// 23.6: four launches of 5.4, 8, 5.2 and 6, each the latency of its steps.  64 rows of normal logits
+// (deviation 2.2) at temperature 2 or 5 with top-p, 10000 tokens a bin, 342 and 402 (890 by 11 bits of all keys at a time,
+// 2100 and 2890 by 8); equal logits throughout 950 without cuts, up to 2800 with all.
 #include "m27q_mix.h"
 
 namespace m27q {
@@ -170,6 +171,17 @@ __device__ __forceinline__ Place place_of(float l, const Scale &s) {
 __device__ __forceinline__ int bin_distance(int bin) { return bin < kFine ? bin : kFine + kUnit * (bin - kFine); }
 __device__ __forceinline__ double bin_scale(int bin) { return __builtin_ldexp(1.0, -(bin_distance(bin) / kUnit)); }
 
+// The logits of a range of bins, and a little more than those.
+struct LogitRange {
+    float lo, hi;
+};
+__device__ __forceinline__ LogitRange logits_of(const Scale &s, int first, int last) {
+    if (!(s.c > 1e-30)) return {-__builtin_inff(), __builtin_inff()};
+    const double up = (s.anchor - bin_distance(first) + 0.5) / s.c;
+    const double down = (s.anchor - bin_distance(last) - (last < kFine ? 0.5 : kUnit - 0.5)) / s.c;
+    return {(float)(down - fabs(down) * 0x1p-20), (float)(up + fabs(up) * 0x1p-20)};
+}
+
 // What is kept of a part of a row, and of a row.
 struct Part {
     double anchor;        // -infinity: no token of any weight
@@ -177,12 +189,14 @@ struct Part {
 };
 constexpr int kList = 8192;
 constexpr int kRanges = 4;
+constexpr int kMinBins = 3;  // at most, in which min_p's border lies
 struct RowPlan {
     double anchor;
     uint64_t best;
     int state;            // 0: done; 1: the tokens of marked bins make a list; 2: the whole row is gone through
     uint32_t listed;      // tokens on the list
     unsigned long long min_p_sum;         // of the tokens that min_p leaves, where none of its border's bins cuts them
+    int min_first, min_last;              // those bins
     int first[kRanges], last[kRanges];    // the marked bins
     float lo[kRanges], hi[kRanges];       // their logits lie within these
     float least;                          // and above this
@@ -563,15 +577,13 @@ __global__ __launch_bounds__(kHalves * kPlanThreads) void k_sample_plan(const m2
             first = J == j ? b0[j] : first;
             last = J == j ? b1[j] : last;
         }
-        // logits of the bins, and a little more than those
-        const double up = (anchor - bin_distance(first) + 0.5) / c;
-        const double down = (anchor - bin_distance(last) - (last < kFine ? 0.5 : kUnit - 0.5)) / c;
-        const bool none = last < first, all = !(c > 1e-30);
-        lo = none ? __builtin_inff() : all ? -__builtin_inff() : (float)(down - fabs(down) * 0x1p-20);
+        const LogitRange near = logits_of({c, anchor, false}, first, last);
+        const bool none = last < first;
+        lo = none ? __builtin_inff() : near.lo;
         out.first[J] = first;
         out.last[J] = last;
         out.lo[J] = lo;
-        out.hi[J] = none ? -__builtin_inff() : all ? __builtin_inff() : (float)(up + fabs(up) * 0x1p-20);
+        out.hi[J] = none ? -__builtin_inff() : near.hi;
     }
     static_assert(kRanges == 4, "lanes that meet");
     lo = fminf(lo, __shfl_xor(lo, 1));
@@ -581,6 +593,8 @@ __global__ __launch_bounds__(kHalves * kPlanThreads) void k_sample_plan(const m2
         out.anchor = anchor;
         out.best = best;
         out.min_p_sum = min_p_sum;
+        out.min_first = m0;
+        out.min_last = m1;
         out.state = listed <= (uint32_t)kList ? 1 : 2;
         out.listed = 0;  // counted by the next launch
     }
@@ -667,9 +681,8 @@ __device__ __forceinline__ void min_of_first(T v, T &to) {
 constexpr int kDigitBits = 11, kDigits = 1 << kDigitBits;
 struct WholeRow {
     unsigned long long mass[kDigits];
-    uint64_t key[kDigits];               // of a digit's only token
+    uint64_t key[kDigits];               // of a piece's only token
     uint32_t count[kDigits];
-    unsigned long long total;
     uint64_t found_key;
     unsigned long long found_sum, found_own;
     uint32_t found_count, found_held;
@@ -677,180 +690,9 @@ struct WholeRow {
 };
 struct Border {
     uint64_t key;              // of the token at the border
-    unsigned long long sum;    // of the weights down to it, itself included
-    unsigned long long own;    // its weight
+    unsigned long long down;   // the running sum, itself included
+    double own;                // its weight in that sum's units
 };
-
-// U logits of a row, all on their way at once.
-template <int U>
-__device__ __forceinline__ void load_some(const m27q_sampling &p, long long base, int i0, float (&v)[U]) {
-    const int last = (int)p.n - 1;
-    if (p.type == M27Q_TYPE_F32) {
-#pragma unroll
-        for (int j = 0; j < U; ++j) v[j] = logit<float>(p.logits, base + min(i0 + j * kRowThreads, last));
-    } else if (p.type == M27Q_TYPE_F16) {
-#pragma unroll
-        for (int j = 0; j < U; ++j) v[j] = logit<_Float16>(p.logits, base + min(i0 + j * kRowThreads, last));
-    } else {
-#pragma unroll
-        for (int j = 0; j < U; ++j) v[j] = logit<__bf16>(p.logits, base + min(i0 + j * kRowThreads, last));
-    }
-}
-
-// A row whose borders lie among more tokens than a list holds (flat ones, thousands of equal logits): the
-// token at which a count or a sum of weights in descending order reaches its target, by 11 bits of the keys at
-// a time, the row read once for each, until one token is left.  Weights are those of the bins, in units of which the row's
-// sum has 61 bits.
-__device__ void sample_whole_row(const m27q_sampling &p, int row, const Rule &r, const RowPlan &plan, const double *octave,
-                                 WholeRow &s, uint32_t *scan32, unsigned long long *scan64) {
-    const int n = (int)p.n, tid = threadIdx.x, lane = tid & 63;
-    const long long base = (long long)row * p.stride;
-    const uint64_t best = plan.best;
-    const float top = key_value(best);
-    const Scale scale = row_scale(r, plan.anchor);
-    const Weights x(octave);
-    const int row_bits = 62 - (32 - __builtin_clz(p.n));  // of the anchor's weight in the plan's sums
-    const int up = 61 - kMassBits - max(0, 64 - __builtin_clzll(plan.sum[kBins] | 1) - row_bits);
-    const auto weight = [&](float v) -> unsigned long long {
-        const Place a = place_of(v, scale);
-        return a.bin < kBins ? x.mass(a.z, a.k, 0) << up >> (bin_distance(a.bin) / kUnit) : 0;
-    };
-    constexpr int U = 8;
-
-    // The first token in order at which the running count reaches `most` or the running sum `target`, a part
-    // of the sum of all if `of_all`; the last one if none does.
-    const auto border = [&](uint32_t most, double target, bool of_all) -> Border {
-        uint64_t prefix = 0;
-        unsigned long long sum = 0;
-        uint32_t seen = 0;
-        int above = kKeyBits;  // the key's bits above these are the prefix
-        while (true) {
-            const int shift = max(above - kDigitBits, 0), mask = (1 << (above - shift)) - 1;
-            for (int i = tid; i < kDigits; i += kRowThreads) s.mass[i] = 0, s.count[i] = 0;
-            if (tid == 0) s.found = 0x7fffffff;
-            __syncthreads();
-            for (int i0 = tid; i0 - tid < n; i0 += U * kRowThreads) {
-                float v[U];
-                load_some(p, base, i0, v);
-#pragma unroll 1
-                for (int j = 0; j < U; ++j) {
-                    const int i = i0 + j * kRowThreads;
-                    float l = v[0];
-#pragma unroll
-                    for (int k = 1; k < U; ++k) l = j == k ? v[k] : l;
-                    const uint64_t key = order_key(l, i);
-                    const bool in = i < n && key >> above == prefix;
-                    const unsigned long long some = __ballot(in);
-                    if (!some) continue;
-                    const int digit = (int)(key >> shift) & mask, first = __builtin_ctzll(some);
-                    const int same = __builtin_amdgcn_readlane(digit, first);
-                    unsigned long long w = in ? weight(l) : 0;
-                    if (__ballot(in && digit != same) == 0) {  // lanes that would meet in one place
-                        w = scan_wave(w);
-                        if (lane == 63) {
-                            atomicAdd(&s.mass[same], w);
-                            atomicAdd(&s.count[same], (uint32_t)__popcll(some));
-                        }
-                        if (lane == first) s.key[same] = key;
-                    } else if (in) {
-                        atomicAdd(&s.mass[digit], w);
-                        atomicAdd(&s.count[digit], 1u);
-                        s.key[digit] = key;
-                    }
-                }
-            }
-            __syncthreads();
-            // the digits in descending order, two a thread
-            constexpr int E = kDigits / kRowThreads;
-            static_assert(E == 2, "two digits a thread");
-            const int d0 = kDigits - 1 - E * tid, d1 = d0 - 1;
-            const uint32_t c0 = s.count[d0], c1 = s.count[d1];
-            const unsigned long long m0 = s.mass[d0], m1 = s.mass[d1];
-            uint32_t tokens;
-            unsigned long long all;
-            const uint32_t c = scan_group<kRowThreads>(c0 + c1, scan32, tokens);
-            const unsigned long long m = scan_group<kRowThreads>(m0 + m1, scan64, all);
-            if (of_all) {
-                if (tid == 0) s.total = all;
-                target *= (double)all;
-                of_all = false;
-            }
-            const auto reaches = [&](uint32_t count, unsigned long long mass) {
-                return seen + count >= most || (double)(sum + mass) >= target || count == tokens;
-            };
-            const int hit = c0 && reaches(c + c0, m + m0) ? E * tid : c1 && reaches(c + c0 + c1, m + m0 + m1) ? E * tid + 1 : 0x7fffffff;
-            min_of_first(hit, s.found);
-            __syncthreads();
-            if (s.found / E == tid) {
-                const bool second = s.found % E;
-                s.found_key = second ? s.key[d1] : s.key[d0];
-                s.found_count = seen + c + (second ? c0 : 0);
-                s.found_held = second ? c1 : c0;
-                s.found_sum = sum + m + (second ? m0 : 0);
-                s.found_own = second ? m1 : m0;
-            }
-            __syncthreads();
-            seen = s.found_count;
-            sum = s.found_sum;
-            prefix = s.found_key >> shift;
-            above = shift;
-            const Border found{s.found_key, sum + s.found_own, s.found_own};
-            const bool done = s.found_held == 1 || shift == 0;
-            __syncthreads();  // all have read it
-            if (done) return found;
-        }
-    };
-
-    uint64_t cut = 0;                // the last key that is kept
-    bool known = false;              // the sum of what is kept
-    unsigned long long total = 0;
-    if (r.k < n) {
-        const Border b = border((uint32_t)r.k, __builtin_inf(), false);
-        cut = b.key;
-        total = b.sum;
-        known = true;
-    }
-    if (r.top_p < 1.0) {
-        const Border b = border(0xffffffffu, known ? r.top_p * (double)total : r.top_p, !known);
-        if (b.key > cut || !known) {
-            cut = b.key;
-            total = b.sum;
-        }
-        known = true;
-    }
-    if (r.min_p > 0.0) {
-        // far from the weight min_p a logit tells by itself
-        const double limit = (double)top + log(r.min_p) / r.inv_t, near = 1e-9 * (fabs(limit) + fabs((double)top));
-        if (tid == 0) s.total = 0;
-        __syncthreads();
-        unsigned long long part = 0;
-        for (int i0 = tid; i0 < n; i0 += U * kRowThreads) {
-            float v[U];
-            load_some(p, base, i0, v);
-#pragma unroll 1
-            for (int j = 0; j < U; ++j) {
-                const int i = i0 + j * kRowThreads;
-                float l = v[0];
-#pragma unroll
-                for (int k = 1; k < U; ++k) l = j == k ? v[k] : l;
-                const uint64_t key = order_key(l, i);
-                if (i >= n || key < cut) continue;
-                const bool kept = (double)l > limit + near || (!((double)l < limit - near) && exp(((double)l - (double)top) * r.inv_t) >= r.min_p);
-                if (kept || key == best) part += weight(l);
-            }
-        }
-        atomicAdd(&s.total, part);
-        __syncthreads();
-        total = s.total;
-        known = true;
-        __syncthreads();
-    }
-    const Border pick = border(0xffffffffu, known ? r.u * (double)total : r.u, !known);
-    if (tid == 0) {
-        p.token[row] = key_index(pick.key);
-        if (p.prob) p.prob[row] = (float)((double)pick.own / (double)(known ? total : s.total));
-    }
-}
 
 constexpr int kCrowd = 1024;
 struct PickShared {
@@ -1029,6 +871,170 @@ __device__ __forceinline__ bool pick_from_list(const m27q_sampling &p, const Scr
     return true;
 }
 
+// U logits of a row, all on their way at once.
+template <int U>
+__device__ __forceinline__ void load_some(const m27q_sampling &p, long long base, int i0, float (&v)[U]) {
+    const int last = (int)p.n - 1;
+    if (p.type == M27Q_TYPE_F32) {
+#pragma unroll
+        for (int j = 0; j < U; ++j) v[j] = logit<float>(p.logits, base + min(i0 + j * kRowThreads, last));
+    } else if (p.type == M27Q_TYPE_F16) {
+#pragma unroll
+        for (int j = 0; j < U; ++j) v[j] = logit<_Float16>(p.logits, base + min(i0 + j * kRowThreads, last));
+    } else {
+#pragma unroll
+        for (int j = 0; j < U; ++j) v[j] = logit<__bf16>(p.logits, base + min(i0 + j * kRowThreads, last));
+    }
+}
+
+// A row whose borders lie among more tokens than a list holds (flat ones, thousands of equal logits): the
+// token of a border's bin at which a count or a sum of weights in descending order reaches its target, by 2048 pieces
+// of the keys that are left at a time, the row read once for each, until one token is left.
+__device__ __forceinline__ void sample_whole_row(const m27q_sampling &p, int row, const Rule &r, const RowPlan &plan, PickShared &s) {
+    const int n = (int)p.n, tid = threadIdx.x, lane = tid & 63;
+    const long long base_at = (long long)row * p.stride;
+    const float top = key_value(plan.best);
+    const Scale scale = row_scale(r, plan.anchor);
+    const Weights x(s.octave);
+    WholeRow &o = s.whole;
+    constexpr int U = 4;
+
+    // Among the tokens of a bin the first at which their count reaches `most` or the row's running sum `target`; the
+    // last one if none does.
+    const auto border = [&](int bin, uint32_t most, double target) -> Border {
+        const unsigned long long lo = s.sum[bin], hi = s.sum[bin + 1];
+        const uint32_t tokens = s.before[bin + 1] - s.before[bin];
+        const double unit = s.unit[bin];
+        const auto down = [&](uint32_t count, unsigned long long mass) {
+            return count == tokens ? hi : min(lo + (unsigned long long)__builtin_rint((double)mass * unit), hi);
+        };
+        const LogitRange near = logits_of(scale, bin, bin);
+        uint64_t first = (uint64_t)order_bits(near.lo) << 24, span = ((uint64_t)order_bits(near.hi) << 24 | 0xffffff) - first + 1;
+        unsigned long long sum = 0;
+        uint32_t seen = 0;
+        while (true) {
+            const int shift = max(64 - __builtin_clzll((span - 1) | 1) - kDigitBits, 0);
+            const float least = key_value(first), most_l = key_value(first + span - 1);
+            for (int i = tid; i < kDigits; i += kRowThreads) o.mass[i] = 0, o.count[i] = 0;
+            if (tid == 0) o.found = 0x7fffffff;
+            __syncthreads();
+            for (int i0 = tid; i0 - tid < n; i0 += U * kRowThreads) {
+                float v[U];
+                load_some(p, base_at, i0, v);
+#pragma unroll
+                for (int j = 0; j < U; ++j) {
+                    const int i = i0 + j * kRowThreads;
+                    if (__ballot(v[j] >= least && v[j] <= most_l) == 0) continue;
+                    const uint64_t key = order_key(v[j], i), at = key - first;
+                    const Place a = place_of(v[j], scale);
+                    const bool in = i < n && at < span && a.bin == bin;
+                    const unsigned long long some = __ballot(in);
+                    if (!some) continue;
+                    const int digit = (int)(at >> shift) & (kDigits - 1), one = __builtin_ctzll(some);
+                    const int same = __builtin_amdgcn_readlane(digit, one);
+                    unsigned long long w = in ? x.mass(a.z, a.k, 0) : 0;
+                    if (__ballot(in && digit != same) == 0) {  // lanes that would meet in one place
+                        w = scan_wave(w);
+                        if (lane == 63) {
+                            atomicAdd(&o.mass[same], w);
+                            atomicAdd(&o.count[same], (uint32_t)__popcll(some));
+                        }
+                        if (lane == one) o.key[same] = key;
+                    } else if (in) {
+                        atomicAdd(&o.mass[digit], w);
+                        atomicAdd(&o.count[digit], 1u);
+                        o.key[digit] = key;
+                    }
+                }
+            }
+            __syncthreads();
+            // the pieces in descending order, two a thread
+            constexpr int E = kDigits / kRowThreads;
+            static_assert(E == 2, "two pieces a thread");
+            const int d0 = kDigits - 1 - E * tid, d1 = d0 - 1;
+            const uint32_t c0 = o.count[d0], c1 = o.count[d1];
+            const unsigned long long m0 = o.mass[d0], m1 = o.mass[d1];
+            uint32_t left;
+            unsigned long long all;
+            const uint32_t c = scan_group<kRowThreads>(c0 + c1, s.scan32, left);
+            const unsigned long long m = scan_group<kRowThreads>(m0 + m1, s.scan, all);
+            const auto reaches = [&](uint32_t count, unsigned long long mass) {
+                return seen + count >= most || (double)down(seen + count, sum + mass) >= target || count == left;
+            };
+            const int hit = c0 && reaches(c + c0, m + m0) ? E * tid : c1 && reaches(c + c0 + c1, m + m0 + m1) ? E * tid + 1 : 0x7fffffff;
+            min_of_first(hit, o.found);
+            __syncthreads();
+            if (o.found / E == tid) {
+                const bool second = o.found % E;
+                o.found_key = second ? o.key[d1] : o.key[d0];
+                o.found_count = seen + c + (second ? c0 : 0);
+                o.found_held = second ? c1 : c0;
+                o.found_sum = sum + m + (second ? m0 : 0);
+                o.found_own = second ? m1 : m0;
+            }
+            __syncthreads();
+            seen = o.found_count;
+            sum = o.found_sum;
+            first += (uint64_t)(kDigits - 1 - o.found) << shift;
+            span = 1ull << shift;
+            const Border found{o.found_key, down(seen + 1, sum + o.found_own), (double)o.found_own * unit};
+            const bool done = o.found_held == 1 || shift == 0;
+            __syncthreads();  // all have read it
+            if (done) return found;
+        }
+    };
+    const auto bin_at = [&](double target) {  // as the plan's
+        const double t = fmax(target, 1.0);
+        return min(first_of(s.sum + 1, kBins, [&](unsigned long long v) { return (double)v >= t || v == s.sum[kBins]; }), kBins - 1);
+    };
+
+    unsigned long long among = s.sum[kBins], total;
+    if ((uint32_t)r.k < s.before[kBins]) {
+        const int bin = min(first_of(s.before + 1, kBins, [&](uint32_t v) { return v >= (uint32_t)r.k; }), kBins - 1);
+        among = border(bin, (uint32_t)r.k - s.before[bin], __builtin_inf()).down;
+    }
+    total = among;
+    if (r.top_p < 1.0) {
+        const double target = r.top_p * (double)among;
+        total = min(total, border(bin_at(target), 0xffffffffu, target).down);
+    }
+    if (r.min_p > 0.0) {
+        // in the bins where its border can lie
+        if (tid < kMinBins) o.mass[tid] = 0, o.count[tid] = 0;
+        __syncthreads();
+        const LogitRange near = logits_of(scale, plan.min_first, plan.min_last);
+        for (int i0 = tid; i0 - tid < n; i0 += U * kRowThreads) {
+            float v[U];
+            load_some(p, base_at, i0, v);
+#pragma unroll
+            for (int j = 0; j < U; ++j) {
+                if (!(i0 + j * kRowThreads < n && v[j] >= near.lo && v[j] <= near.hi)) continue;
+                const Place a = place_of(v[j], scale);
+                if (a.bin < plan.min_first || a.bin > plan.min_last) continue;
+                if (exp(((double)v[j] - (double)top) * r.inv_t) >= r.min_p) atomicAdd(&o.mass[a.bin - plan.min_first], x.mass(a.z, a.k, 0));
+                else o.count[a.bin - plan.min_first] = 1;
+            }
+        }
+        __syncthreads();
+        unsigned long long sum = plan.min_p_sum;
+        for (int i = plan.min_last - plan.min_first; i >= 0; --i) {
+            const int bin = plan.min_first + i;
+            if (o.count[i]) sum = min(s.sum[bin] + (unsigned long long)__builtin_rint((double)o.mass[i] * s.unit[bin]), s.sum[bin + 1]);
+        }
+        total = min(total, sum);
+        __syncthreads();
+    }
+    // the first token is kept whatever the rest says
+    const Place f = place_of(top, scale);
+    total = max(total, min((unsigned long long)__builtin_rint((double)x.mass(f.z, f.k, 0) * s.unit[f.bin]), s.sum[f.bin + 1]));
+    const double target = r.u * (double)total;
+    const Border pick = border(bin_at(target), 0xffffffffu, target);
+    if (tid == 0) {
+        p.token[row] = key_index(pick.key);
+        if (p.prob) p.prob[row] = (float)(pick.own / (double)total);
+    }
+}
+
 __global__ __launch_bounds__(kRowThreads) void k_sample_pick(const m27q_sampling p, const Scratch sc) {
     __shared__ PickShared s;
     const int row = blockIdx.x;
@@ -1038,13 +1044,13 @@ __global__ __launch_bounds__(kRowThreads) void k_sample_pick(const m27q_sampling
     const Rule r = row_rule(p, row);
     bool done = false;
     if (threadIdx.x < kUnit) s.octave[threadIdx.x] = Weights::factor(threadIdx.x);
+    if (threadIdx.x <= kBins) {
+        s.before[threadIdx.x] = plan.before[threadIdx.x];
+        s.at[threadIdx.x] = plan.at[threadIdx.x];
+        s.sum[threadIdx.x] = plan.sum[threadIdx.x];
+        s.unit[threadIdx.x] = plan.unit[threadIdx.x];
+    }
     if (state == 1) {
-        if (threadIdx.x <= kBins) {
-            s.before[threadIdx.x] = plan.before[threadIdx.x];
-            s.at[threadIdx.x] = plan.at[threadIdx.x];
-            s.sum[threadIdx.x] = plan.sum[threadIdx.x];
-            s.unit[threadIdx.x] = plan.unit[threadIdx.x];
-        }
         if (threadIdx.x == 0) {
             s.among = plan.sum[kBins];  // unless the top_k-th is on the list
             s.top_p = ~0ull;
@@ -1057,9 +1063,9 @@ __global__ __launch_bounds__(kRowThreads) void k_sample_pick(const m27q_sampling
         else if (n <= 2 * kRowThreads) done = pick_from_list<2>(p, sc, plan, r, n, s);
         else if (n <= 4 * kRowThreads) done = pick_from_list<4>(p, sc, plan, r, n, s);
         else done = pick_from_list<8>(p, sc, plan, r, n, s);
-        if (!done) __syncthreads();
     }
-    if (!done) sample_whole_row(p, row, r, plan, s.octave, s.whole, s.scan32, s.scan);
+    __syncthreads();
+    if (!done) sample_whole_row(p, row, r, plan, s);
 }
 
 struct Sizes {
