@@ -230,12 +230,16 @@ __device__ __forceinline__ int part_index(int i) { return i * kPartThreads + (in
 template <typename T>
 __device__ __forceinline__ void load_part(const m27q_sampling &p, int row, int first, float (&v)[kEach]) {
     const int count = min(kPart, (int)p.n - first);
-    const long long base = (long long)row * p.stride + first;
+    const T *const from = (const T *)p.logits + ((long long)row * p.stride + first);
+    if (count == kPart) {
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) v[i] = logit<T>(p.logits, base + min(part_index(i), count - 1));
-    if (count < kPart)
+        for (int i = 0; i < kEach; ++i) v[i] = (float)(from + i * kPartThreads)[threadIdx.x];
+        return;
+    }
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) v[i] = part_index(i) < count ? v[i] : -__builtin_inff();
+    for (int i = 0; i < kEach; ++i) v[i] = (float)from[min(part_index(i), count - 1)];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) v[i] = part_index(i) < count ? v[i] : -__builtin_inff();
 }
 
 // A part's bins, and its largest token.
