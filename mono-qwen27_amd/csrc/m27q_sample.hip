@@ -18,11 +18,11 @@
 // Where the list would be too long (flat rows, thousands of equal logits at a border), pick reads the whole
 // row once or twice more for each border, by pieces of its bin's keys.
 //
-// 200 rows of 248320 F32, top-p (199 MB): 101 us, of these 54 for parts, 9, 26 for list (7.6 TB/s:
-// what parts read last still lies in the caches) and 11.  parts is bound by the vector units: some 32 operations
+// 200 rows of 248320 F32, top-p (199 MB): 92 us, of these 50 for parts, 8, 26 for list (7.6 TB/s:
+// what parts read last still lies in the caches) and 10.  parts is bound by the vector units: some 30 operations
 // of a wave for each 64 tokens, half of them on 64 bits, and the LDS additions beside them (a
-// plain read of the same bytes: 29).  64 rows of all rules 47.5 us (20, 9.3, 12, 9); one row
-// 23.6: four launches of 5.4, 8, 5.2 and 6, each the latency of its steps.  64 rows of normal logits
+// plain read of the same bytes: 29).  64 rows of all rules 46 us (19, 8.5, 12, 8); one row
+// 23: four launches of 5.3, 8.1, 5.3 and 6, each the latency of its steps.  64 rows of normal logits
 // (deviation 2.2) at temperature 2 or 5 with top-p, 10000 tokens a bin, 342 and 402 (890 by 11 bits of all keys at a time,
 // 2100 and 2890 by 8); equal logits throughout 950 without cuts, up to 2800 with all.
 #include "m27q_mix.h"
