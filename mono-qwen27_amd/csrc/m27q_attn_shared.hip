@@ -9,10 +9,11 @@ namespace {
 
 long long tiles_of(long long rows) { return (rows + kWaves * kRows - 1) / (kWaves * kRows); }
 
-// A prefix of many rows and all sequences' own keys in one launch: the prefix's workgroups, bound by the matrix units,
-// come first, one on each CU, and beside them those of the own keys, bound by memory.  64 tokens behind 32768
-// places and up to 1021 own ones, 24 heads of 256 on 4, F16 to F32: 123 us and 6 of joining, of 45 for the bytes (300 MB) and
-// 67 for the products; 8 prompts of 301 tokens behind 8192, BF16: 444 us, 1.0 PFLOP/s of the pairs that count.
+// A prefix of many rows and all sequences' own keys in one launch: the prefix's workgroups, bound by the matrix
+// units, come first, one on each CU, and beside them those of the own keys, bound by memory.  64 tokens behind
+// 32768 places and up to 1021 own ones, 24 heads of 256 on 4, F16 to F32: 123 us and 6 of joining, of 45 for
+// the bytes (300 MB) and 67 for the products; 8 prompts of 301 tokens behind 8192, BF16: 444 us, 1.0 PFLOP/s of
+// the pairs that count.
 template <int D, bool BF, int NP>
 __global__ __launch_bounds__(kWaves * 64, 2) void k_attn_both(const AttnParams p, unsigned px, unsigned prefix, unsigned ox) {
     if (blockIdx.x < prefix) {
@@ -24,8 +25,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void k_attn_both(const AttnParams p
     }
 }
 
-// The same of few rows, bound by the latency of a part's steps: 4 tokens behind 32768 places and up to 300 own ones, 137
-// MB, 38.5 us with the join, 3.6 TB/s.
+// The same of few rows, bound by the latency of a part's steps: 4 tokens behind 32768 places and up to 300 own
+// ones, 137 MB, 38.5 us with the join, 3.6 TB/s.
 template <int D, bool BF, int NP, int PREFIX_ROWS, int OWN_ROWS>
 __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) void k_attn_few_both(const AttnParams p, unsigned px, unsigned prefix,
                                                                                   unsigned ox) {
@@ -43,12 +44,15 @@ void launch_parts(const AttnParams &p, const SharedPlan &plan, hipStream_t s) {
     const int group = (int)(p.q.heads / p.cache.heads);
     const long long pr = (long long)p.prefix.max_rows * group, orows = (long long)p.seqs.max_q * group;
     const unsigned tp = plan.prefix.few ? 1 : (unsigned)tiles_of(pr), to = plan.prefix.few ? 1 : (unsigned)tiles_of(orows);
-    const unsigned px = tp * p.prefix.groups * p.cache.heads, ox = to * p.seqs.n * p.cache.heads, prefix = px * plan.prefix.splits;
+    const unsigned px = tp * p.prefix.groups * p.cache.heads, ox = to * p.seqs.n * p.cache.heads;
+    const unsigned prefix = px * plan.prefix.splits;
     const dim3 grid(prefix + ox * plan.own), block(kWaves * 64);
-    if (!plan.prefix.few) hipLaunchKernelGGL((k_attn_both<D, BF, NP>), grid, block, 0, s, p, px, prefix, ox);
-    else if (std::max(pr, orows) <= 16) hipLaunchKernelGGL((k_attn_few_both<D, BF, NP, 16, 16>), grid, block, 0, s, p, px, prefix, ox);
-    else if (orows <= 16) hipLaunchKernelGGL((k_attn_few_both<D, BF, NP, kRows, 16>), grid, block, 0, s, p, px, prefix, ox);
-    else hipLaunchKernelGGL((k_attn_few_both<D, BF, NP, kRows, kRows>), grid, block, 0, s, p, px, prefix, ox);
+    auto k = k_attn_both<D, BF, NP>;
+    if (plan.prefix.few)
+        k = std::max(pr, orows) <= 16 ? k_attn_few_both<D, BF, NP, 16, 16>
+            : orows <= 16             ? k_attn_few_both<D, BF, NP, kRows, 16>
+                                      : k_attn_few_both<D, BF, NP, kRows, kRows>;
+    hipLaunchKernelGGL(k, grid, block, 0, s, p, px, prefix, ox);
 }
 
 template <int D, bool BF>
@@ -68,18 +72,21 @@ int parts_of(long long wgs, long long slots, long long keys, long long least, lo
     return (int)std::max(1ll, std::min({slots / wgs, (keys + least - 1) / least, limit}));
 }
 
-// Whether a prefix is read once for its group, or by each sequence as the rest of its keys (from the caches then, which hold
-// it after the first): what is saved against what a pass of its own costs, from the bounds, as if all sequences
-// shared.  In tiles of 32 places of 256 values, by times measured with 4 cache heads of 256 (24 query heads, F16 to F32):
-// 656 tiles a us of up to 16 rows and 496 of 32 by themselves, 160 of 128 rows of a group.  A few rows (of a group 32):
-// what is saved has to be 1200 tiles, for lengths, groups and places are looked up one after another; 4 tokens behind
-// 2048, 8192, 16384 and 32768 places 16.6, 24.3, 29.0 and 38.5 us, by themselves 13.0, 22.7, 31.1 and 48.3; 9 behind
-// 1560 (8 heads) 15.0 and 19.9.  More: 6 us, and 1 for 400 tiles of own keys, which have a wave of a workgroup here; 64 tokens and up
-// to 600 own places behind 1024, 2048, 8192 and 32768 41.7, 44.1, 66 and 117 and 35.0, 46.4, 117 and 403; 8 x 5 tokens behind 8192,
-// 16384 and 32768 37.9, 53.9 and 78.7 and 34.5, 50.5 and 83.4; 3 x 8 x 5 behind 12000 66 and 96.  Prompts save
-// what is left over of tiles of 128 rows: 4 of 200 tokens behind 512, 1024 and 4096 49, 61 and 147 and 48, 74 and 165.
-bool worth_sharing(const m27q_seqs &seqs, const m27q_prefixes &prefix, long long group, const m27q_cache &cache, long long shared) {
-    const double n = seqs.n, groups = prefix.groups, tile = (double)cache.heads * cache.dim / (256 * kKeys), tiles = shared * tile;
+// Whether a prefix is read once for its group, or by each sequence as the rest of its keys (from the caches
+// then, which hold it after the first): what is saved against what a pass of its own costs, from the bounds, as
+// if all sequences shared.  In tiles of 32 places of 256 values, by times measured with 4 cache heads of 256
+// (24 query heads, F16 to F32): 656 tiles a us of up to 16 rows and 496 of 32 by themselves, 160 of 128 rows of
+// a group.  A few rows (of a group 32): what is saved has to be 1200 tiles, for lengths, groups and places are
+// looked up one after another; 4 tokens behind 2048, 8192, 16384 and 32768 places 16.6, 24.3, 29.0 and 38.5 us,
+// by themselves 13.0, 22.7, 31.1 and 48.3; 9 behind 1560 (8 heads) 15.0 and 19.9.  More: 6 us, and 1 for 400
+// tiles of own keys, which have a wave of a workgroup here; 64 tokens and up to 600 own places behind 1024,
+// 2048, 8192 and 32768 41.7, 44.1, 66 and 117 and 35.0, 46.4, 117 and 403; 8 x 5 tokens behind 8192, 16384 and
+// 32768 37.9, 53.9 and 78.7 and 34.5, 50.5 and 83.4; 3 x 8 x 5 behind 12000 66 and 96.  Prompts save what is
+// left over of tiles of 128 rows: 4 of 200 tokens behind 512, 1024 and 4096 49, 61 and 147 and 48, 74 and 165.
+bool worth_sharing(const m27q_seqs &seqs, const m27q_prefixes &prefix, long long group, const m27q_cache &cache,
+                   long long shared) {
+    const double n = seqs.n, groups = prefix.groups;
+    const double tile = (double)cache.heads * cache.dim / (256 * kKeys), tiles = shared * tile;
     const long long rows = seqs.max_q * group, together = prefix.max_rows * group;
     const double others = groups * tiles * tiles_of(together) / 160;
     if (rows > kRows) return n * tiles * tiles_of(rows) / 160 - others >= 1.5;
@@ -99,13 +106,14 @@ long long shared_groups(const m27q_seqs &seqs, const m27q_prefixes &prefix, uint
 // The prefix's parts, at most 48 of the join's 64, and those of a sequence's own keys, of which there are as
 // many as the longest sequence has behind the longest prefix: what runs at once, in one launch.  Many rows: a
 // place on a CU for the own keys of each sequence and head, up to one of its two, and the others for the
-// prefix.  Few: up to half of the places for the own keys, in parts of 128, a tile a wave, at least.  Measured, with
-// other numbers of parts: 64 tokens behind 32768 places 130 us with 21 of the prefix, 161, 141, 138 and 150 with 14,
-// 17, 32 and 42; 3 groups of 8 x 5 tokens behind 12000 places 66 with 17, 62, 64, 75 and 72 with 16, 18, 10 and 21; 8
-// prompts of 301 behind 8192 places 438 with 1, 474, 500 and 433 with 2, 3 and 4.  (Each kind in a launch of its own:
-// 150, 80 and 473 us.)  Few rows: 4 tokens behind 2048 places 16.5 with 16, 17.2, 17.1 and 17.8 with 11, 22 and 32 (two
-// launches: 23.1); behind 32768 places 38.9 with 48, 40.6, 37.7 and 38.4 with 24, 32 and 40; 8 tokens, 8 cache heads of 128,
-// 4096 places and up to 1500 own ones 21.2, 18.5 with half as many parts of the own ones.
+// prefix.  Few: up to half of the places for the own keys, in parts of 128, a tile a wave, at least.  Measured,
+// with other numbers of parts: 64 tokens behind 32768 places 130 us with 21 of the prefix, 161, 141, 138 and
+// 150 with 14, 17, 32 and 42; 3 groups of 8 x 5 tokens behind 12000 places 66 with 17, 62, 64, 75 and 72 with
+// 16, 18, 10 and 21; 8 prompts of 301 behind 8192 places 438 with 1, 474, 500 and 433 with 2, 3 and 4.  (Each
+// kind in a launch of its own: 150, 80 and 473 us.)  Few rows: 4 tokens behind 2048 places 16.5 with 16, 17.2,
+// 17.1 and 17.8 with 11, 22 and 32 (two launches: 23.1); behind 32768 places 38.9 with 48, 40.6, 37.7 and 38.4
+// with 24, 32 and 40; 8 tokens, 8 cache heads of 128, 4096 places and up to 1500 own ones 21.2, 18.5 with half
+// as many parts of the own ones.
 SharedPlan shared_plan(const m27q_seqs &seqs, const m27q_prefixes &prefix, uint32_t q_heads, const m27q_cache &cache,
                        int cus) {
     const long long group = q_heads / cache.heads, slots = 2ll * cus;

@@ -79,7 +79,6 @@ inline bool attn_shape(const m27q_seqs *s, uint32_t q_heads, const m27q_cache *c
     return attn_groups(*s, q_heads, *c) <= kMaxGroups;
 }
 
-
 // What every attention over pages asks of its arguments.
 inline m27q_status check_attn(const m27q_seqs *seqs, const m27q_cache *cache, const m27q_rows &q, const m27q_rows &out,
                               float scale, const void *scratch) {

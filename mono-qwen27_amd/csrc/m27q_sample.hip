@@ -214,7 +214,13 @@ struct Scratch {
 };
 
 // 2^-36 of the anchor's weight, the unit of its octave's bins, in the units of a row's sums, which fit 62 bits.
-__device__ __forceinline__ double sum_unit(uint32_t n) { return (double)(1ull << (62 - (32 - __builtin_clz(n)))) / (double)(1ull << kMassBits); }
+__device__ __forceinline__ double sum_unit(uint32_t n) {
+    return (double)(1ull << (62 - (32 - __builtin_clz(n)))) / (double)(1ull << kMassBits);
+}
+// A bin's weights in the units of a row's sums.
+__device__ __forceinline__ unsigned long long row_mass(unsigned long long mass, double unit) {
+    return (unsigned long long)__builtin_rint((double)mass * unit);
+}
 
 template <typename T>
 __device__ __forceinline__ float logit(const void *p, long long at) { return (float)((const T *)p)[at]; }
@@ -382,7 +388,8 @@ __device__ __forceinline__ T scan_group(T v, T *lds, T &all) {
 // bin's, or, where an octave of the row lies among the part's fine bins, their octave's.  -1: it has none.
 __device__ __forceinline__ int part_bin(int J, int off) {
     const int oct = kOctaves + J - kFine - off / kUnit;
-    return J >= kBins ? -1 : J < kFine ? max(J - off, -1) : oct >= kOctaves ? kFine + oct - kOctaves : oct >= 0 ? kBins + 1 + oct : -1;
+    if (J < kFine) return max(J - off, -1);
+    return J >= kBins ? -1 : oct >= kOctaves ? kFine + oct - kOctaves : oct >= 0 ? kBins + 1 + oct : -1;
 }
 
 constexpr int kPlanThreads = 512, kHalves = 2;
@@ -396,7 +403,8 @@ __device__ __forceinline__ unsigned long long max_wave(unsigned long long v) {
     v = max(v, moved<0x118, 0xf>(v));
     v = max(v, moved<0x142, 0xa>(v));
     v = max(v, moved<0x143, 0xc>(v));
-    return (unsigned long long)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), 63) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+    const uint32_t high = (uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), 63);
+    return (unsigned long long)high << 32 | (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 // Numbers in their order as bits, and back.
 __device__ __forceinline__ unsigned long long ordered(double v) {
@@ -488,7 +496,7 @@ __global__ __launch_bounds__(kHalves * kPlanThreads) void k_sample_plan(const m2
     mass += sum[J];
     count += tokens_s[J];
     const double unit = sum_unit(p.n) * bin_scale(J);
-    mass = (unsigned long long)__builtin_rint((double)mass * unit);
+    mass = row_mass(mass, unit);
     unsigned long long above = scan_wave(mass);
     uint32_t before = scan_wave(count);
     if (lane == 63) {
@@ -513,7 +521,8 @@ __global__ __launch_bounds__(kHalves * kPlanThreads) void k_sample_plan(const m2
 
     const unsigned long long total = sum[kBins];
     const uint32_t tokens = tokens_s[kBins];
-    const auto bin_at = [&](double target) {  // the bin in which the running sum reaches it, the last one that holds a token if none does
+    // the bin in which the running sum reaches a target, the last one that holds a token if none does
+    const auto bin_at = [&](double target) {
         const double t = fmax(target, 1.0);   // (the first token's own bin holds far more)
         return first_of(sum + 1, kBins, [&](unsigned long long v) { return (double)v >= t || v == total; });
     };
@@ -741,8 +750,8 @@ __device__ __forceinline__ float part_of(uint64_t key, int bin, const Scale &s, 
 // token's place in its bucket is how many of it are larger.  False: some bucket holds so many
 // (equal logits of 32 bits) that this would take long.
 template <int E>
-__device__ __forceinline__ bool pick_from_list(const m27q_sampling &p, const Scratch &sc, const RowPlan &plan, const Rule &r, int n,
-                                               PickShared &s) {
+__device__ __forceinline__ bool pick_from_list(const m27q_sampling &p, const Scratch &sc, const RowPlan &plan, const Rule &r,
+                                               int n, PickShared &s) {
     const int row = blockIdx.x, tid = threadIdx.x, i0 = tid * E;
     const Scale scale = row_scale(r, plan.anchor);
     const Weights x(s.octave);
@@ -761,7 +770,8 @@ __device__ __forceinline__ bool pick_from_list(const m27q_sampling &p, const Scr
         if (e * kRowThreads + tid >= n) continue;
         const Place a = place_of(key_value(key[e]), scale);
         const uint32_t at = s.at[a.bin], count = s.at[a.bin + 1] - at;
-        const float part = p.type == M27Q_TYPE_F32 ? part_of(a) : part_of(key[e], a.bin, scale, p.type == M27Q_TYPE_BF16 ? 16 : 13, p.n);
+        const int low = p.type == M27Q_TYPE_BF16 ? 16 : 13;
+        const float part = p.type == M27Q_TYPE_F32 ? part_of(a) : part_of(key[e], a.bin, scale, low, p.n);
         // (below n even if somebody writes to the logits meanwhile)
         bucket[e] = min(at + min((uint32_t)fmaxf(part * (float)count, 0.0f), count - 1), (uint32_t)n - 1);
         slot[e] = atomicAdd(&s.count[bucket[e]], 1u);
@@ -835,7 +845,7 @@ __device__ __forceinline__ bool pick_from_list(const m27q_sampling &p, const Scr
     for (int e = 0; e < E; ++e) {
         const uint32_t i = (uint32_t)(i0 + e);
         const unsigned long long lo = s.sum[bin[e]], hi = s.sum[bin[e] + 1], in = run - s.start[bin[e]];
-        const auto to = [&](unsigned long long x) { return min(lo + (unsigned long long)__builtin_rint((double)x * s.unit[bin[e]]), hi); };
+        const auto to = [&](unsigned long long x) { return min(lo + row_mass(x, s.unit[bin[e]]), hi); };
         down[e] = i + 1 == s.at[bin[e] + 1] ? hi : to(in + own[e]);
         rank[e] = i < (uint32_t)n ? (int)(s.before[bin[e]] + i - s.at[bin[e]]) : 0x7fffffff;
         run += own[e];
@@ -857,7 +867,7 @@ __device__ __forceinline__ bool pick_from_list(const m27q_sampling &p, const Scr
     }
     // the first token is kept whatever the rest says
     const Place f = place_of(top, scale);
-    const unsigned long long one = min((unsigned long long)__builtin_rint((double)x.mass(f.z, f.k, 0) * s.unit[f.bin]), s.sum[f.bin + 1]);
+    const unsigned long long one = min(row_mass(x.mass(f.z, f.k, 0), s.unit[f.bin]), s.sum[f.bin + 1]);
     const unsigned long long total = max(one, min(s.among, min(s.top_p, s.min_p)));
     const double target = r.u * (double)total;
     int at = 0x7fffffff;
@@ -894,7 +904,8 @@ __device__ __forceinline__ void load_some(const m27q_sampling &p, long long base
 // A row whose borders lie among more tokens than a list holds (flat ones, thousands of equal logits): the
 // token of a border's bin at which a count or a sum of weights in descending order reaches its target, by 2048 pieces
 // of the keys that are left at a time, the row read once for each, until one token is left.
-__device__ __forceinline__ void sample_whole_row(const m27q_sampling &p, int row, const Rule &r, const RowPlan &plan, PickShared &s) {
+__device__ __forceinline__ void sample_whole_row(const m27q_sampling &p, int row, const Rule &r, const RowPlan &plan,
+                                                 PickShared &s) {
     const int n = (int)p.n, tid = threadIdx.x, lane = tid & 63;
     const long long base_at = (long long)row * p.stride;
     const float top = key_value(plan.best);
@@ -910,7 +921,7 @@ __device__ __forceinline__ void sample_whole_row(const m27q_sampling &p, int row
         const uint32_t tokens = s.before[bin + 1] - s.before[bin];
         const double unit = s.unit[bin];
         const auto down = [&](uint32_t count, unsigned long long mass) {
-            return count == tokens ? hi : min(lo + (unsigned long long)__builtin_rint((double)mass * unit), hi);
+            return count == tokens ? hi : min(lo + row_mass(mass, unit), hi);
         };
         const LogitRange near = logits_of(scale, bin, bin);
         uint64_t first = (uint64_t)order_bits(near.lo) << 24, span = ((uint64_t)order_bits(near.hi) << 24 | 0xffffff) - first + 1;
@@ -965,7 +976,9 @@ __device__ __forceinline__ void sample_whole_row(const m27q_sampling &p, int row
             const auto reaches = [&](uint32_t count, unsigned long long mass) {
                 return seen + count >= most || (double)down(seen + count, sum + mass) >= target || count == left;
             };
-            const int hit = c0 && reaches(c + c0, m + m0) ? E * tid : c1 && reaches(c + c0 + c1, m + m0 + m1) ? E * tid + 1 : 0x7fffffff;
+            int hit = 0x7fffffff;
+            if (c1 && reaches(c + c0 + c1, m + m0 + m1)) hit = E * tid + 1;
+            if (c0 && reaches(c + c0, m + m0)) hit = E * tid;
             min_of_first(hit, o.found);
             __syncthreads();
             if (o.found / E == tid) {
@@ -989,7 +1002,8 @@ __device__ __forceinline__ void sample_whole_row(const m27q_sampling &p, int row
     };
     const auto bin_at = [&](double target) {  // as the plan's
         const double t = fmax(target, 1.0);
-        return min(first_of(s.sum + 1, kBins, [&](unsigned long long v) { return (double)v >= t || v == s.sum[kBins]; }), kBins - 1);
+        const unsigned long long all = s.sum[kBins];
+        return min(first_of(s.sum + 1, kBins, [&](unsigned long long v) { return (double)v >= t || v == all; }), kBins - 1);
     };
 
     unsigned long long among = s.sum[kBins], total;
@@ -1015,22 +1029,23 @@ __device__ __forceinline__ void sample_whole_row(const m27q_sampling &p, int row
                 if (!(i0 + j * kRowThreads < n && v[j] >= near.lo && v[j] <= near.hi)) continue;
                 const Place a = place_of(v[j], scale);
                 if (a.bin < plan.min_first || a.bin > plan.min_last) continue;
-                if (exp(((double)v[j] - (double)top) * r.inv_t) >= r.min_p) atomicAdd(&o.mass[a.bin - plan.min_first], x.mass(a.z, a.k, 0));
-                else o.count[a.bin - plan.min_first] = 1;
+                const int at = a.bin - plan.min_first;
+                if (exp(((double)v[j] - (double)top) * r.inv_t) >= r.min_p) atomicAdd(&o.mass[at], x.mass(a.z, a.k, 0));
+                else o.count[at] = 1;
             }
         }
         __syncthreads();
         unsigned long long sum = plan.min_p_sum;
         for (int i = plan.min_last - plan.min_first; i >= 0; --i) {
             const int bin = plan.min_first + i;
-            if (o.count[i]) sum = min(s.sum[bin] + (unsigned long long)__builtin_rint((double)o.mass[i] * s.unit[bin]), s.sum[bin + 1]);
+            if (o.count[i]) sum = min(s.sum[bin] + row_mass(o.mass[i], s.unit[bin]), s.sum[bin + 1]);
         }
         total = min(total, sum);
         __syncthreads();
     }
     // the first token is kept whatever the rest says
     const Place f = place_of(top, scale);
-    total = max(total, min((unsigned long long)__builtin_rint((double)x.mass(f.z, f.k, 0) * s.unit[f.bin]), s.sum[f.bin + 1]));
+    total = max(total, min(row_mass(x.mass(f.z, f.k, 0), s.unit[f.bin]), s.sum[f.bin + 1]));
     const double target = r.u * (double)total;
     const Border pick = border(bin_at(target), 0xffffffffu, target);
     if (tid == 0) {

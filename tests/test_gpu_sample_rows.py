@@ -11,8 +11,6 @@ from gpu_util import say
 SLACK = 2.0 ** -35
 
 
-
-
 def allowed(x, T, k, top_p, min_p, u):
     """{token: probs} of the tokens that a row may give, and their shares of what may be kept."""
     x = x.astype(np.float64)
