@@ -11,9 +11,9 @@ long long tiles_of(long long rows) { return (rows + kWaves * kRows - 1) / (kWave
 
 // A prefix of many rows and all sequences' own keys in one launch: the prefix's workgroups, bound by the matrix
 // units, come first, one on each CU, and beside them those of the own keys, bound by memory.  64 tokens behind
-// 32768 places and up to 1021 own ones, 24 heads of 256 on 4, F16 to F32: 123 us and 6 of joining, of 45 for
-// the bytes (300 MB) and 67 for the products; 8 prompts of 301 tokens behind 8192, BF16: 444 us, 1.0 PFLOP/s of
-// the pairs that count.
+// 32768 places and up to 1021 own ones, 24 heads of 256 on 4, F16 to F32: 122 us and 9 of joining, of 62 for
+// the bytes (304 MB) and 63 for the products; 8 prompts of 301 tokens behind 8192, BF16: 449 us with 33 of joining,
+// 0.9 PFLOP/s of the pairs that count.
 template <int D, bool BF, int NP>
 __global__ __launch_bounds__(kWaves * 64, 2) void k_attn_both(const AttnParams p, unsigned px, unsigned prefix, unsigned ox) {
     if (blockIdx.x < prefix) {

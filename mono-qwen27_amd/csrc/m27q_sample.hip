@@ -23,8 +23,9 @@
 // of a wave for each 64 tokens, half of them on 64 bits, and the LDS additions beside them (a
 // plain read of the same bytes: 29).  64 rows of all rules 46 us (19, 8.5, 12, 8); one row
 // 23: four launches of 5.3, 8.1, 5.3 and 6, each the latency of its steps.  64 rows of normal logits
-// (deviation 2.2) at temperature 2 or 5 with top-p, 10000 tokens a bin, 342 and 402 (890 by 11 bits of all keys at a time,
-// 2100 and 2890 by 8); equal logits throughout 950 without cuts, up to 2800 with all.
+// (deviation 2.2) at temperature 2 or 5 with top-p, 10000 tokens a bin, 200 and 229 (342 and 402 where tokens near a border
+// do not wait until they fill a wave, 850 and 890 by 11 bits of all keys at a time, 2100 and 2890 by 8); equal logits
+// throughout 1070 without cuts, up to 3200 with all.
 #include "m27q_mix.h"
 
 namespace m27q {
@@ -696,6 +697,7 @@ struct WholeRow {
     unsigned long long mass[kDigits];
     uint64_t key[kDigits];               // of a piece's only token
     uint32_t count[kDigits];
+    float2 wait[kRowThreads / 64][128];  // a wave's tokens near a border: logit, and index as bits
     uint64_t found_key;
     unsigned long long found_sum, found_own;
     uint32_t found_count, found_held;
@@ -933,35 +935,55 @@ __device__ __forceinline__ void sample_whole_row(const m27q_sampling &p, int row
             for (int i = tid; i < kDigits; i += kRowThreads) o.mass[i] = 0, o.count[i] = 0;
             if (tid == 0) o.found = 0x7fffffff;
             __syncthreads();
+            // few tokens of most waves lie near: those wait until they fill one
+            float2 *const wait = o.wait[tid >> 6];
+            int waiting = 0;
+            const auto add = [&](bool there) {
+                const float2 e = wait[lane];
+                const uint64_t key = order_key(e.x, __float_as_int(e.y)), at = key - first;
+                const Place a = place_of(e.x, scale);
+                const bool in = there && at < span && a.bin == bin;
+                const unsigned long long some = __ballot(in);
+                if (!some) return;
+                const int digit = (int)(at >> shift) & (kDigits - 1), one = __builtin_ctzll(some);
+                const int same = __builtin_amdgcn_readlane(digit, one);
+                unsigned long long w = in ? x.mass(a.z, a.k, 0) : 0;
+                if (__ballot(in && digit != same) == 0) {  // lanes that would meet in one place
+                    w = scan_wave(w);
+                    if (lane == 63) {
+                        atomicAdd(&o.mass[same], w);
+                        atomicAdd(&o.count[same], (uint32_t)__popcll(some));
+                    }
+                    if (lane == one) o.key[same] = key;
+                } else if (in) {
+                    atomicAdd(&o.mass[digit], w);
+                    atomicAdd(&o.count[digit], 1u);
+                    o.key[digit] = key;
+                }
+            };
             for (int i0 = tid; i0 - tid < n; i0 += U * kRowThreads) {
                 float v[U];
                 load_some(p, base_at, i0, v);
 #pragma unroll
                 for (int j = 0; j < U; ++j) {
                     const int i = i0 + j * kRowThreads;
-                    if (__ballot(v[j] >= least && v[j] <= most_l) == 0) continue;
-                    const uint64_t key = order_key(v[j], i), at = key - first;
-                    const Place a = place_of(v[j], scale);
-                    const bool in = i < n && at < span && a.bin == bin;
-                    const unsigned long long some = __ballot(in);
+                    const bool close = i < n && v[j] >= least && v[j] <= most_l;
+                    const unsigned long long some = __ballot(close);
                     if (!some) continue;
-                    const int digit = (int)(at >> shift) & (kDigits - 1), one = __builtin_ctzll(some);
-                    const int same = __builtin_amdgcn_readlane(digit, one);
-                    unsigned long long w = in ? x.mass(a.z, a.k, 0) : 0;
-                    if (__ballot(in && digit != same) == 0) {  // lanes that would meet in one place
-                        w = scan_wave(w);
-                        if (lane == 63) {
-                            atomicAdd(&o.mass[same], w);
-                            atomicAdd(&o.count[same], (uint32_t)__popcll(some));
-                        }
-                        if (lane == one) o.key[same] = key;
-                    } else if (in) {
-                        atomicAdd(&o.mass[digit], w);
-                        atomicAdd(&o.count[digit], 1u);
-                        o.key[digit] = key;
+                    if (close) wait[waiting + __popcll(some & ((1ull << lane) - 1))] = make_float2(v[j], __int_as_float(i));
+                    waiting += (int)__popcll(some);
+                    __builtin_amdgcn_wave_barrier();
+                    if (waiting >= 64) {
+                        add(true);
+                        waiting -= 64;
+                        const float2 rest = wait[64 + lane];
+                        __builtin_amdgcn_wave_barrier();
+                        wait[lane] = rest;
+                        __builtin_amdgcn_wave_barrier();
                     }
                 }
             }
+            add(lane < waiting);
             __syncthreads();
             // the pieces in descending order, two a thread
             constexpr int E = kDigits / kRowThreads;
