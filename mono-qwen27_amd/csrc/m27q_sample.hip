@@ -44,7 +44,6 @@ __device__ __forceinline__ uint32_t order_bits(float v) {
 __device__ __forceinline__ uint64_t order_key(float v, int i) {
     return (uint64_t)order_bits(v) << 24 | (0xffffffu - (uint32_t)i);
 }
-constexpr int kKeyBits = 56;
 __device__ __forceinline__ int key_index(uint64_t key) { return (int)(0xffffffu - (uint32_t)(key & 0xffffffu)); }
 
 __device__ __forceinline__ float key_value(uint64_t key) {
