@@ -232,7 +232,8 @@ constexpr int kCopies = 4;  // of a part's bins: lanes that meet in a bin wait f
 // The i-th of a thread's tokens in a part.
 __device__ __forceinline__ int part_index(int i) { return i * kPartThreads + (int)threadIdx.x; }
 
-// A part's logits, all on their way at once; -infinity behind the end.
+// A part's logits, all on their way at once; NaN behind the end, which no comparison takes (a border's range may reach
+// down to -infinity).
 template <typename T>
 __device__ __forceinline__ void load_part(const m27q_sampling &p, int row, int first, float (&v)[kEach]) {
     const int count = min(kPart, (int)p.n - first);
@@ -245,7 +246,7 @@ __device__ __forceinline__ void load_part(const m27q_sampling &p, int row, int f
 #pragma unroll
     for (int i = 0; i < kEach; ++i) v[i] = (float)from[min(part_index(i), count - 1)];
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) v[i] = part_index(i) < count ? v[i] : -__builtin_inff();
+    for (int i = 0; i < kEach; ++i) v[i] = part_index(i) < count ? v[i] : __builtin_nanf("");
 }
 
 // A part's bins, and its largest token.

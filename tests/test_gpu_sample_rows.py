@@ -217,6 +217,34 @@ def test_values_at_the_ends(m27q, dev, n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 100, 900, 5000, 8193, 20000])
+def test_what_lies_behind_a_row_is_not_its(m27q, dev, n):
+    """Rows of the lowest number (all tokens masked with it), whose border's logits reach down to -infinity, and temperatures
+    that take every number: the values behind a row, as large or larger, are none of its tokens."""
+    import torch
+    say("sample behind rows", n)
+    low, inf = torch.finfo(torch.float32).min, float("inf")
+    buf = torch.full((4, n + 9000), low, device=dev)
+    buf[2, n:] = 5.0
+    buf[3] = 1.0
+    buf[3, 0] = -2.0
+    x = buf[:, :n]
+    seen = x.cpu().numpy()
+    token, prob = torch.empty(4, dtype=torch.int32, device=dev), torch.empty(4, device=dev)
+    scratch = torch.empty(m27q.sample_rows_scratch_bytes(4, n), dtype=torch.uint8, device=dev)
+    f32 = lambda v: torch.full((4,), v, device=dev)  # noqa: E731
+    for T in (1.0, 0.01, 3e31, inf):
+        for k, top_p, min_p in ((0, 1.0, 0.0), (n // 2 + 1, 1.0, 0.0), (0, 0.6, 0.0), (0, 1.0, 0.3)):
+            for u in (0.0, 0.45, 1.0):
+                m27q.sample_rows(x, f32(u), token, scratch, f32(T), torch.full((4,), k, dtype=torch.int32, device=dev), f32(top_p),
+                                 f32(min_p), prob)
+                for r, (t, p) in enumerate(zip(token.tolist(), prob.tolist())):
+                    ok = allowed(seen[r], np.float32(T), k, np.float32(top_p), np.float32(min_p), np.float32(u))
+                    assert t in ok, (T, k, top_p, min_p, u, r, t, list(ok)[:4])
+                    assert any(abs(p - q) <= (8 * SLACK + 2.0 ** -24) * q for q in ok[t]), (T, k, top_p, min_p, u, r, p, ok[t])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("T", [1e-3, 1e-5, 8e-6, 3e-6, 1e-6, 1e-9, 1e-11, 1e-13])
 def test_temperatures_near_0(m27q, dev, T):
     """Steps between logits from a few octaves to more than numbers of 32 and of 52 bits hold: several sizes of logits, rows with
