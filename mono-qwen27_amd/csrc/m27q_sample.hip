@@ -44,6 +44,7 @@ __device__ __forceinline__ uint32_t order_bits(float v) {
 __device__ __forceinline__ uint64_t order_key(float v, int i) {
     return (uint64_t)order_bits(v) << 24 | (0xffffffu - (uint32_t)i);
 }
+constexpr uint64_t kLastKey = (uint64_t)0xff800000 << 24 | 0xffffff;  // of infinity
 __device__ __forceinline__ int key_index(uint64_t key) { return (int)(0xffffffu - (uint32_t)(key & 0xffffffu)); }
 
 __device__ __forceinline__ float key_value(uint64_t key) {
@@ -931,7 +932,9 @@ __device__ __forceinline__ void sample_whole_row(const m27q_sampling &p, int row
         uint32_t seen = 0;
         while (true) {
             const int shift = max(64 - __builtin_clzll((span - 1) | 1) - kDigitBits, 0);
-            const float least = key_value(first), most_l = key_value(first + span - 1);
+            // (the piece of the largest numbers reaches past infinity, where keys stand for none)
+            const uint64_t last = first + span - 1;
+            const float least = key_value(first), most_l = key_value(last < kLastKey ? last : kLastKey);
             for (int i = tid; i < kDigits; i += kRowThreads) o.mass[i] = 0, o.count[i] = 0;
             if (tid == 0) o.found = 0x7fffffff;
             __syncthreads();

@@ -245,6 +245,28 @@ def test_what_lies_behind_a_row_is_not_its(m27q, dev, n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n", [2000, 9001, 40000])
+@pytest.mark.parametrize("T", [float("inf"), 1e35, 3e31])
+def test_largest_numbers_at_the_highest_temperatures(m27q, dev, n, T):
+    """Logits at the largest number of 32 bits, a few, half of them or all, where the temperature leaves every token its weight:
+    the borders' bin then holds all numbers, up to infinity."""
+    say("sample largest", n, T)
+    rng = np.random.default_rng(n)
+    top = np.float32(np.finfo(np.float32).max)
+    x = logits(rng, 6, n, "bulk")
+    x[0] = top
+    x[1, [3, n // 2, n - 1]] = top
+    x[2] = np.where(rng.random(n) < 0.5, top, -top)
+    x[3, ::2], x[3, 1::3] = top, -np.inf
+    x[4] = np.nextafter(top, np.float32(0)) * (1 - 2.0 ** -22 * rng.integers(0, 2, n))
+    x[4, 7] = top
+    x[5] = -top
+    for k, top_p, min_p in ((0, 1.0, 0.0), (n // 3, 1.0, 0.0), (0, 0.7, 0.0), (0, 1.0, 0.5), (2, 1.0, 0.0), (n // 2, 0.5, 0.1)):
+        for u in (0.0, 1e-4, 0.6, 1.0):
+            check(m27q, dev, x, T, k, top_p, min_p, u)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("T", [1e-3, 1e-5, 8e-6, 3e-6, 1e-6, 1e-9, 1e-11, 1e-13])
 def test_temperatures_near_0(m27q, dev, T):
     """Steps between logits from a few octaves to more than numbers of 32 and of 52 bits hold: several sizes of logits, rows with
