@@ -11,6 +11,14 @@ namespace m27q {
 
 constexpr int kWave = 64;  // CDNA wavefront width
 
+// Between a wave's LDS accesses that exchange values between its lanes.  The
+// hardware runs a wave's LDS operations in order, so no wait is needed; this
+// keeps the compiler, which sees each lane's own addresses, from moving them.
+__device__ __forceinline__ void wave_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // e^t, with t clamped to [-87, 87], so that 2^n and the result stay normal
 // floats; a NaN t gives NaN back (so gated() and silu() propagate it).  Cody-Waite range reduction (W. J. Cody and
 // W. Waite, Software Manual for the Elementary Functions, 1980):

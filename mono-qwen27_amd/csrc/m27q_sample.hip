@@ -26,6 +26,7 @@
 // (deviation 2.2) at temperature 2 or 5 with top-p, 10000 tokens a bin, 200 and 229 (342 and 402 where tokens near a border
 // do not wait until they fill a wave, 850 and 890 by 11 bits of all keys at a time, 2100 and 2890 by 8); equal logits
 // throughout 1070 without cuts, up to 3200 with all.
+#include "m27q_device.h"
 #include "m27q_mix.h"
 
 namespace m27q {
@@ -975,14 +976,14 @@ __device__ __forceinline__ void sample_whole_row(const m27q_sampling &p, int row
                     if (!some) continue;
                     if (close) wait[waiting + __popcll(some & ((1ull << lane) - 1))] = make_float2(v[j], __int_as_float(i));
                     waiting += (int)__popcll(some);
-                    __builtin_amdgcn_wave_barrier();
+                    wave_order();
                     if (waiting >= 64) {
                         add(true);
                         waiting -= 64;
                         const float2 rest = wait[64 + lane];
-                        __builtin_amdgcn_wave_barrier();
+                        wave_order();
                         wait[lane] = rest;
-                        __builtin_amdgcn_wave_barrier();
+                        wave_order();
                     }
                 }
             }

@@ -455,18 +455,11 @@ __device__ __forceinline__ void store_codes(uint8_t *dst, const u4 &v, int j, in
     }
 }
 
-// Between a wave's LDS accesses that exchange values between its lanes.  The
-// hardware runs a wave's LDS operations in order, so no wait is needed; this
-// keeps the compiler, which sees each lane's own addresses, from moving them.
-// It also keeps it from scheduling across: over 800 shapes of up to one set per
+// wave_order() also keeps the compiler from scheduling across: over 800 shapes of up to one set per
 // CU, M = 17 to 64, 0.1% slower on average and 5% at most (Q6_K 1024 x 5120 at
 // M = 32 12.9 us with and without, IQ4_XS 2560 x 5120 at M = 48 17.3 against
 // 16.6).  In the loop it stands before the step's loads for IQ4_XS, between them
 // for Q8_0 and after them for the others, where each type lost least.
-__device__ __forceinline__ void wave_order() {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-}
 
 template <int V>
 struct Int {

@@ -87,3 +87,13 @@ def test_one_wave_slices_order_their_lds_accesses(tmp_path, wt, nt, layout):
                 state[t] |= now
                 todo.append(t)
     assert accesses > 20 and not swaps, swaps[:4]
+
+
+def test_flat_rows_order_the_tokens_that_wait(tmp_path):
+    """Sampling of flat rows: a wave's lanes hand each other the tokens near a border through LDS without a barrier, so a
+    fence stands before each point at which they do (the wave barrier alone orders no memory accesses)."""
+    blocks = kernel_blocks(tmp_path, os.path.join(CSRC, "m27q_sample.hip"), "13k_sample_pick")
+    points = [(b, i) for b, lines in blocks.items() for i, line in enumerate(lines) if "@llvm.amdgcn.wave.barrier()" in line]
+    assert len(points) >= 3
+    for b, i in points:
+        assert i and re.match(r'fence syncscope\("wavefront"\) acq_rel', blocks[b][i - 1]), (b, blocks[b][max(0, i - 2):i + 1])
