@@ -546,7 +546,9 @@ M27Q_API m27q_status m27q_delta_rule(const m27q_delta *d, void *scratch, size_t 
  *   h = x + add;  y = weight h / sqrt(mean(h^2) + eps)
  * x, add, sum and out are rows of one shape (tokens of them), each of any type; add
  * may be NULL (h = x), weight (device, dim fp32 values, for every head the same) may
- * be NULL (ones); dim 1 .. 2^20, eps above 0.  Written are those that are not NULL,
+ * be NULL (ones); dim 1 .. 2^20, eps above 0; tokens up to 2^24, tokens * heads
+ * below 2^22 (dim up to 512: 2^24, and 2^26 for whole units of 8 values in rows and
+ * weights of 16-byte alignment).  Written are those that are not NULL,
  * one at least, of sum (h), out (y) and xq: y's codes in the format of
  * m27q_quant_act for tokens rows of K = heads * dim values, by its rule (dim % 32
  * == 0, tokens up to 2^16, K up to 2^20).  Computed in fp32, the squares' sum

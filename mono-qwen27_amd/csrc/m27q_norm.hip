@@ -178,42 +178,48 @@ static bool norm_vectorizes(const NormParams &p) {
            (uintptr_t)p.weight % 16 == 0;
 }
 
-// Work-items of a grid's x are less than 2^32: workgroups of at most 1024 a row, of 256 for short rows.
-bool norm_fits(const NormParams &p) {
-    const long long rows = (long long)p.tokens * p.x.heads;
-    return rows * (p.x.dim <= 512 ? kThreads : 1024) < (1ll << 32);
-}
-
-// A head's lanes for up to 512 values: 98304 heads of 96 15.8 us, a workgroup each 35.5; of 256 32.6 and 36.9 (65536 of
-// 512: 43.1 and 41.4).  Longer rows: a unit a thread, two of 16 bits (BF16, 4096 rows of 5120: two 30.5 us, one
-// 32.9, four 34.3; of 2048 12.9, 14.5 and 13.1; of 8192 46.4, 49.5 and 49.7.  F32: 63.9, 62.6 and 66.0, a
-// single row 3.7, 3.4 and 4.2).  Not by the number of rows: the squares are summed in one order in any batch.
-hipError_t launch_norm(const NormParams &p, hipStream_t s) {
-    const long long rows = (long long)p.tokens * p.x.heads;
+// The kernel for a call, and a row's threads.  A head's lanes for up to 512 values: 98304 heads of 96 15.8 us, a workgroup
+// each 35.5; of 256 32.6 and 36.9 (65536 of 512: 43.1 and 41.4).  Longer rows: a unit a thread, two of 16 bits (BF16, 4096
+// rows of 5120: two 30.5 us, one 32.9, four 34.3; of 2048 12.9, 14.5 and 13.1; of 8192 46.4, 49.5 and 49.7.  F32: 63.9, 62.6
+// and 66.0, a single row 3.7, 3.4 and 4.2).  Not by the number of rows: the squares are summed in one order in any batch.
+enum NormKind { kAny, kLanes, kUnits1, kUnits2, kUnits4 };
+struct NormForm {
+    NormKind kind;
+    int threads;
+};
+static NormForm norm_form(const NormParams &p) {
     const int units = (int)p.x.dim / 8;
-    if (!norm_vectorizes(p)) {
-        hipLaunchKernelGGL(k_norm_any, dim3((unsigned)rows), dim3(kThreads), 0, s, p);
-    } else if (units <= 64) {
+    if (!norm_vectorizes(p)) return {kAny, kThreads};
+    if (units <= 64) {
         int L = 4;
         while (L < units) L *= 2;
-        const dim3 grid((unsigned)((rows * L + kThreads - 1) / kThreads));
-        switch (L) {
-            case 4: hipLaunchKernelGGL((k_norm_heads<4>), grid, dim3(kThreads), 0, s, p, rows); break;
-            case 8: hipLaunchKernelGGL((k_norm_heads<8>), grid, dim3(kThreads), 0, s, p, rows); break;
-            case 16: hipLaunchKernelGGL((k_norm_heads<16>), grid, dim3(kThreads), 0, s, p, rows); break;
-            case 32: hipLaunchKernelGGL((k_norm_heads<32>), grid, dim3(kThreads), 0, s, p, rows); break;
-            default: hipLaunchKernelGGL((k_norm_heads<64>), grid, dim3(kThreads), 0, s, p, rows);
+        return {kLanes, L};
+    }
+    if (units > 128 && units <= 2048 && p.x.type != M27Q_TYPE_F32) return {kUnits2, (units + 127) / 128 * 64};
+    if (units <= 1024) return {kUnits1, (units + 63) / 64 * 64};
+    return {units <= 2048 ? kUnits2 : kUnits4, 1024};
+}
+
+// Work-items of a grid's x are less than 2^32.
+bool norm_fits(const NormParams &p) {
+    return (long long)p.tokens * p.x.heads * norm_form(p).threads <= (1ll << 32) - kThreads;
+}
+
+hipError_t launch_norm(const NormParams &p, hipStream_t s) {
+    const long long rows = (long long)p.tokens * p.x.heads;
+    const NormForm f = norm_form(p);
+    const dim3 grid((unsigned)(f.kind == kLanes ? (rows * f.threads + kThreads - 1) / kThreads : rows)), block(f.threads);
+    switch (f.kind) {
+        case kAny: hipLaunchKernelGGL(k_norm_any, grid, block, 0, s, p); break;
+        case kLanes: {
+            auto k = f.threads == 4 ? k_norm_heads<4> : f.threads == 8 ? k_norm_heads<8> : f.threads == 16 ? k_norm_heads<16>
+                     : f.threads == 32 ? k_norm_heads<32> : k_norm_heads<64>;
+            hipLaunchKernelGGL(k, grid, dim3(kThreads), 0, s, p, rows);
+            break;
         }
-    } else if (units > 128 && units <= 2048 && p.x.type != M27Q_TYPE_F32) {
-        const int threads = (units + 127) / 128 * 64;
-        hipLaunchKernelGGL((k_norm_row<2, 1024>), dim3((unsigned)rows), dim3(threads), 0, s, p, threads);
-    } else if (units <= 1024) {
-        const int threads = (units + 63) / 64 * 64;
-        hipLaunchKernelGGL((k_norm_row<1, 1024>), dim3((unsigned)rows), dim3(threads), 0, s, p, threads);
-    } else if (units <= 2048) {
-        hipLaunchKernelGGL((k_norm_row<2, 1024>), dim3((unsigned)rows), dim3(1024), 0, s, p, 1024);
-    } else {
-        hipLaunchKernelGGL((k_norm_row<4, 1024>), dim3((unsigned)rows), dim3(1024), 0, s, p, 1024);
+        case kUnits1: hipLaunchKernelGGL((k_norm_row<1, 1024>), grid, block, 0, s, p, f.threads); break;
+        case kUnits2: hipLaunchKernelGGL((k_norm_row<2, 1024>), grid, block, 0, s, p, f.threads); break;
+        default: hipLaunchKernelGGL((k_norm_row<4, 1024>), grid, block, 0, s, p, f.threads);
     }
     return hipGetLastError();
 }

@@ -205,3 +205,20 @@ def test_rows_past_32_bits(m27q, dev):
     m27q.rms_norm(x, None, 1e-6, out=a)
     m27q.rms_norm(v, None, 1e-6, out=b)
     assert torch.equal(a, b) and bool(a.abs().sum() > 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,heads,dim", [((1 << 24) // 17 + 5, 17, 8), ((1 << 22) // 3 + 7, 3, 520)])
+def test_more_rows_than_workgroups_of_the_largest_kind(m27q, dev, tokens, heads, dim):
+    """Past 2^32 / 256 short rows or 2^32 / 1024 longer ones, of kernels with fewer threads a row."""
+    import torch
+    say("norm many rows", tokens, heads, dim)
+    some = make(dev, 1000, heads, dim, "bf16", 3)
+    x = some.repeat(-(-tokens // 1000), 1, 1)[:tokens]
+    out, one = torch.empty_like(x), torch.empty_like(some)
+    m27q.rms_norm(x, None, 1e-6, out=out)
+    m27q.rms_norm(some, None, 1e-6, out=one)
+    assert bool(one.abs().sum() > 0)
+    for at in range(0, tokens, 1000):
+        if at % 100000 == 0 or at + 1000 >= tokens:
+            assert torch.equal(out[at: at + 1000], one[: tokens - at])
