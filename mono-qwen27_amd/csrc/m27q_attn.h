@@ -541,7 +541,8 @@ __device__ __forceinline__ int first_key(const AttnParams &p, int place) {
 
 // The keys of a workgroup whose rows stand at first .. last (of len >= 0 cached tokens, so none
 // of these sums passes 32 bits), and its part of them: lo a multiple of a tile, hi >= lo, and
-// hi <= max_kv where there are any.
+// hi <= max_kv where there are any.  Of own keys there are parts for the longest sequence that there
+// may be: one of a few keys takes the first of them, own_least keys each, and has none in the others.
 template <Kind KIND>
 __device__ __forceinline__ void set_keys(const AttnParams &p, Work &w, int len, int shared, int first, int last, int part) {
     // tiles lie whole within pages or the other way round
@@ -549,11 +550,20 @@ __device__ __forceinline__ void set_keys(const AttnParams &p, Work &w, int len, 
     w.hi = max(w.lo, min(min(len, (int)p.seqs.max_kv), last + 1));
     const int parts = KIND == kPrefix ? p.prefix_parts : KIND == kOwn ? p.splits - p.prefix_parts : p.splits;
     if (parts > 1) {
-        const int tiles = (w.hi - w.lo + kKeys - 1) / kKeys, each = (tiles + parts - 1) / parts;
+        const int tiles = (w.hi - w.lo + kKeys - 1) / kKeys;
+        int each = (tiles + parts - 1) / parts;
+        if constexpr (KIND == kOwn) each = max(each, p.own_least / kKeys);
         const int end = w.hi;
         w.lo += part * each * kKeys;
         w.hi = max(w.lo, min(end, w.lo + each * kKeys));
     }
+}
+
+// Of a row's own keys a part without any, and of a sequence of no group the prefix's parts: nothing for the join.
+__device__ __forceinline__ void put_none(const AttnParams &p, long long row0, int part, bool empty, bool alone) {
+    if (empty) p.stat[row0 + p.prefix_parts + part] = make_float2(0, 0);
+    if (alone && part == 0)
+        for (int i = 0; i < p.prefix_parts; ++i) p.stat[row0 + i] = make_float2(0, 0);
 }
 
 // Looks at every page of the keys once, the threads of a workgroup in turn: tiles trust them then.
@@ -624,6 +634,13 @@ __device__ __forceinline__ void attn_many(const AttnParams &p, unsigned bx, unsi
         __syncthreads();
     }
     set_keys<KIND>(p, w, len, sr.shared, first, last, (int)part_id);
+    if (KIND == kOwn && w.lo >= w.hi) {  // a part that this sequence does not need
+        const int row = w.row0 + (int)threadIdx.x;
+        if (threadIdx.x < kWaves * kRows && row < w.rows)
+            put_none(p, ((long long)(sr.first + row / group) * p.q.heads + w.head * group + row % group) * p.splits,
+                     (int)part_id, true, sr.shared < 0);
+        return;
+    }
 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
     const int wrow = w.row0 + wave * kRows;  // this wave's first row
@@ -724,8 +741,7 @@ __device__ __forceinline__ void attn_many(const AttnParams &p, unsigned bx, unsi
         const long long row0 = ((long long)token * p.q.heads + qh) * p.splits;
         const long long at = row0 + (KIND == kOwn ? p.prefix_parts : 0) + part_id;
         if (h == 0) p.stat[at] = make_float2(x.m * sc, x.l);
-        if (KIND == kOwn && sr.shared < 0 && part_id == 0 && h == 0)  // no prefix
-            for (int i = 0; i < p.prefix_parts; ++i) p.stat[row0 + i] = make_float2(0, 0);
+        if (KIND == kOwn && h == 0) put_none(p, row0, (int)part_id, false, sr.shared < 0);
         if (x.l == 0) return;
         float *o = p.part + at * D;
 #pragma unroll
@@ -808,6 +824,10 @@ __device__ __forceinline__ void attn_few(const AttnParams &p, unsigned bx, unsig
     const int token = sr.first + at, qh = w.head * group + row - at * group;
     const unsigned long long part0 = (unsigned long long)((uint32_t)token * p.q.heads + qh) * (uint32_t)p.splits;
     const unsigned long long part = part0 + (KIND == kOwn ? p.prefix_parts : 0) + by;
+    if (KIND == kOwn && w.lo >= w.hi) {  // a part that this sequence does not need
+        if (live && threadIdx.x < RW) put_none(p, part0, (int)by, true, sr.shared < 0);
+        return;
+    }
     // loads end in order: what is needed first is asked for first
     typename R::Raw q;
     R::load_q(p, token, qh, q);
@@ -996,8 +1016,7 @@ __device__ __forceinline__ void attn_few(const AttnParams &p, unsigned bx, unsig
     }
     if (KIND != kAll || p.splits > 1) {
         if (threadIdx.x < RW) p.stat[part] = make_float2(m * sc, l);
-        if (KIND == kOwn && sr.shared < 0 && by == 0 && threadIdx.x < RW)  // no prefix
-            for (int i = 0; i < p.prefix_parts; ++i) p.stat[part0 + i] = make_float2(0, 0);
+        if (KIND == kOwn && threadIdx.x < RW) put_none(p, part0, (int)by, false, sr.shared < 0);
         if (l == 0) return;
 #pragma unroll
         for (int u = 0; u < Q; ++u)
@@ -1039,10 +1058,13 @@ __global__ __launch_bounds__(256) void k_attn_join(const AttnParams p) {
 #pragma unroll
     for (int i = 0; i < AT; ++i) v[i] = *(const f32x4 *)(from + (long long)min(i, p.splits - 1) * D);
     float f[RPW], inv[RPW];  // lane i: part i's factor of each of the wave's rows
+    int parts = p.splits;    // own keys: up to the last that has any, as most sequences need few of theirs
+    unsigned long long there = 0;
 #pragma unroll
     for (int r = 0; r < RPW; ++r) {
         float2 st = p.stat[(base + min(first + r, rows - 1)) * p.splits + min(lane, p.splits - 1)];
         if (lane >= p.splits) st.y = 0;
+        there |= __ballot(st.y != 0);
         float m = st.y != 0 ? st.x : -__builtin_inff();
 #pragma unroll
         for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
@@ -1053,12 +1075,13 @@ __global__ __launch_bounds__(256) void k_attn_join(const AttnParams p) {
         for (int o = 1; o < 64; o <<= 1) l += __shfl_xor(l, o);
         inv[r] = l == 0 ? 0.0f : 1.0f / l;
     }
+    if constexpr (KIND == kOwn) parts = there ? 64 - __builtin_clzll(there) : 0;
     f32x4 o = {};
-    for (int i0 = 0; i0 < p.splits; i0 += AT) {
+    for (int i0 = 0; i0 < parts; i0 += AT) {
         f32x4 u[AT];
 #pragma unroll
         for (int i = 0; i < AT; ++i) u[i] = v[i];
-        if (i0 + AT < p.splits) {
+        if (i0 + AT < parts) {
 #pragma unroll
             for (int i = 0; i < AT; ++i) v[i] = *(const f32x4 *)(from + (long long)min(i0 + AT + i, p.splits - 1) * D);
         }
@@ -1070,7 +1093,7 @@ __global__ __launch_bounds__(256) void k_attn_join(const AttnParams p) {
                 const float y = __shfl(f[r], (i0 + i) & 63);
                 w = mine == r ? y : w;
             }
-            o = i0 + i >= p.splits || w == -1.0f ? o : o + u[i] * w;
+            o = i0 + i >= parts || w == -1.0f ? o : o + u[i] * w;
         }
     }
     if (!live) return;

@@ -83,6 +83,12 @@ int parts_of(long long wgs, long long slots, long long keys, long long least, lo
 // 2048, 8192 and 32768 41.7, 44.1, 66 and 117 and 35.0, 46.4, 117 and 403; 8 x 5 tokens behind 8192, 16384 and
 // 32768 37.9, 53.9 and 78.7 and 34.5, 50.5 and 83.4; 3 x 8 x 5 behind 12000 66 and 96.  Prompts save what is
 // left over of tiles of 128 rows: 4 of 200 tokens behind 512, 1024 and 4096 49, 61 and 147 and 48, 74 and 165.
+// Three numbers do not fit every shape.  Few rows: over 396 cases (2 to 32 sequences behind 1024 to 32768 places, 1 to
+// 16 cache heads of 64 to 256) the way taken is 2.8% slower than the other one on average, by more than 10% in 37 of
+// them, at most by 61% (5 tokens behind 1024 places, 8 heads of 256: by themselves 20.8 us, shared 12.9; 4 behind
+// 8192, 4 heads: 22.5 and 24.3).  Prompts count as if all were as long as the longest: 301, 195, 206, 200, 183, 198, 266
+// and 273 tokens behind 8192 places are shared for a saving of 34 of 120 tiles, of which they have 90, and take 445
+// us, by themselves 455; one of 2000 and seven of 20 778 and 2640.
 bool worth_sharing(const m27q_seqs &seqs, const m27q_prefixes &prefix, long long group, const m27q_cache &cache,
                    long long shared) {
     const double n = seqs.n, groups = prefix.groups;
@@ -103,17 +109,25 @@ long long shared_groups(const m27q_seqs &seqs, const m27q_prefixes &prefix, uint
     return a + b;
 }
 
-// The prefix's parts, at most 48 of the join's 64, and those of a sequence's own keys, of which there are as
-// many as the longest sequence has behind the longest prefix: what runs at once, in one launch.  Many rows: a
-// place on a CU for the own keys of each sequence and head, up to one of its two, and the others for the
-// prefix.  Few: up to half of the places for the own keys, in parts of 128, a tile a wave, at least.  Measured,
-// with other numbers of parts: 64 tokens behind 32768 places 130 us with 21 of the prefix, 161, 141, 138 and
-// 150 with 14, 17, 32 and 42; 3 groups of 8 x 5 tokens behind 12000 places 66 with 17, 62, 64, 75 and 72 with
-// 16, 18, 10 and 21; 8 prompts of 301 behind 8192 places 438 with 1, 474, 500 and 433 with 2, 3 and 4.  (Each
-// kind in a launch of its own: 150, 80 and 473 us.)  Few rows: 4 tokens behind 2048 places 16.5 with 16, 17.2,
-// 17.1 and 17.8 with 11, 22 and 32 (two launches: 23.1); behind 32768 places 38.9 with 48, 40.6, 37.7 and 38.4
-// with 24, 32 and 40; 8 tokens, 8 cache heads of 128, 4096 places and up to 1500 own ones 21.2, 18.5 with half
-// as many parts of the own ones.
+// The prefix's parts, at most 48 of the join's 64, and those of a sequence's own keys: what runs at once, in one
+// launch.  Many rows: a place on a CU for the own keys of each sequence and head, up to one of its two, and the
+// others for the prefix.  Few: up to half of the places for the own keys, in parts of 128, a tile a wave, at
+// least.  Measured, with other numbers of parts: 64 tokens behind 32768 places 130 us with 21 of the prefix, 161,
+// 141, 138 and 150 with 14, 17, 32 and 42; 3 groups of 8 x 5 tokens behind 12000 places 66 with 17, 62, 64, 75
+// and 72 with 16, 18, 10 and 21; 8 prompts of 301 behind 8192 places 438 with 1, 474, 500 and 433 with 2, 3 and 4.
+// (Each kind in a launch of its own: 150, 80 and 473 us.)  Few rows: 4 tokens behind 2048 places 16.5 with 16,
+// 17.2, 17.1 and 17.8 with 11, 22 and 32 (two launches: 23.1); behind 32768 places 38.9 with 48, 40.6, 37.7 and
+// 38.4 with 24, 32 and 40; 8 tokens, 8 cache heads of 128, 4096 places and up to 1500 own ones 21.2, 18.5 with
+// half as many parts of the own ones.
+//
+// A sequence usually has as many own keys as the longest has behind the longest prefix: `usual` parts.  But it may
+// share less than the bounds say, or nothing: there are parts then as for all of its keys, filling half of the places
+// (few rows) or all of them (many, whose tokens have a wave of four: two at least, for up to 32 rounds of workgroups).  A
+// sequence that does not need them leaves them at once: 4 tokens behind 32768 places 38 us with and without them, 64
+// behind 8192 63, the 3 x 8 x 5 71.2 and 69.9.  4 tokens of 32000 places that share 512 under bounds of 33000 take 113
+// us so, with the usual parts 579 (the paged attention 97); 8 x 5 tokens behind 16384 places and 5 of a sequence of 17000
+// by itself 112 and 313 (88); 64 tokens behind 32768 places and one of 33000 by itself 910 and 1715 (1110), as a group of
+// one 200.
 SharedPlan shared_plan(const m27q_seqs &seqs, const m27q_prefixes &prefix, uint32_t q_heads, const m27q_cache &cache,
                        int cus) {
     const long long group = q_heads / cache.heads, slots = 2ll * cus;
@@ -123,14 +137,18 @@ SharedPlan shared_plan(const m27q_seqs &seqs, const m27q_prefixes &prefix, uint3
     SharedPlan r{};
     if (!worth_sharing(seqs, prefix, group, cache, shared)) {
         const AttnPlan each = attn_plan(seqs, q_heads, cache, cus);
-        return {{each.few, 0}, each.splits};
+        return {{each.few, 0}, each.splits, 0};
     }
     r.prefix.few = rows <= kRows && seqs.max_q * group <= kRows;
     const int least = r.prefix.few ? 128 : 256;
     const long long places = r.prefix.few && cache.dim == 256 ? cus : slots;
     r.prefix.splits = parts_of(wgs, places - std::min(own, places / 2), shared, least, 48);
-    const long long left = r.prefix.few ? places - wgs * r.prefix.splits : slots;
-    r.own = parts_of(own, left, (long long)seqs.max_kv - shared, least, kMaxSplits - r.prefix.splits);
+    const long long left = r.prefix.few ? places - wgs * r.prefix.splits : slots, behind = seqs.max_kv - shared;
+    const long long limit = kMaxSplits - r.prefix.splits, usual = parts_of(own, left, behind, least, limit);
+    const long long most = r.prefix.few ? places / 2
+                           : tiles_of(seqs.max_q * group) > 1 ? places : std::max(places, std::min(2 * own, 64 * places));
+    r.own = (int)std::max(usual, (long long)parts_of(own, most, seqs.max_kv, least, limit));
+    r.own_least = (int)std::max((long long)least, ((behind + usual - 1) / usual + kKeys - 1) / kKeys * kKeys);
     return r;
 }
 

@@ -98,6 +98,7 @@ M27Q_API m27q_status m27q_attn_shared(const m27q_seqs *seqs, const m27q_prefixes
     p.prefix = *prefix;
     const SharedPlan plan = shared_plan(p.seqs, *prefix, q->heads, *cache, cu_count());
     p.prefix_parts = plan.prefix.splits;
+    p.own_least = plan.own_least;
     p.splits = plan.prefix.splits + plan.own;
     if (scratch_bytes < attn_scratch(p.seqs, q->heads, cache->dim, p.splits)) return M27Q_ERR_SCRATCH;
     p.part = (float *)scratch;

@@ -40,6 +40,7 @@ struct AttnParams {
     // behind shared prefixes: parts 0 .. prefix_parts - 1 are of the prefix, the others of a sequence's own keys
     m27q_prefixes prefix;
     int prefix_parts;
+    int own_least;  // keys of a part of those at least
 };
 struct AttnPlan {
     int few;        // the kernel for few rows
@@ -56,6 +57,7 @@ hipError_t launch_attn(const AttnParams &p, const AttnPlan &plan, hipStream_t s)
 struct SharedPlan {
     AttnPlan prefix;  // no parts: not worth a pass of its own, every sequence reads all of its keys
     int own;          // parts of a sequence's own keys
+    int own_least;    // keys of one of them at least, whole tiles
 };
 long long shared_groups(const m27q_seqs &seqs, const m27q_prefixes &prefix, uint32_t q_heads, const m27q_cache &cache);
 SharedPlan shared_plan(const m27q_seqs &seqs, const m27q_prefixes &prefix, uint32_t q_heads, const m27q_cache &cache,

@@ -70,6 +70,18 @@ def test_shared_attention_refuses(m27q):
     assert call(s=seqs(m, **wide), x=prefix(groups=65535, max_rows=1 << 24)) == SHAPE
 
 
+@pytest.mark.parametrize("n,max_q,max_rows,prefix,own", [(4, 1, 4, 48, 8), (9, 5, 40, 48, 14), (65, 1, 64, 21, 2)])
+def test_own_keys_have_parts_beside_a_prefix(m27q, n, max_q, max_rows, prefix, own):
+    """Bounds that let a sequence share anything from nothing to all of its keys: the scratch has room for the prefix's parts
+    and for as many of its own as fill the 256 CUs (two places on each; of few rows of 256 half of one), two at least."""
+    m = m27q
+    tokens, heads, dim = n * max_q, 24, 256
+    s = seqs(m, n=n, tokens=tokens, max_q=max_q, max_kv=33000, table_stride=600)
+    c = cache(m, heads=4, dim=dim, page_size=64, page_stride=4 * 64 * dim, pages=100)
+    x = m.PrefixesDesc(FAKE, FAKE, 1, max_rows, 33000, 0)
+    assert m.lib().m27q_attn_shared_scratch_bytes(ref(s), ref(x), heads, ref(c)) >= (prefix + own) * tokens * heads * (dim * 4 + 8)
+
+
 def test_sampling_refuses(m27q):
     m = m27q
 

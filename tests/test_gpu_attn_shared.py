@@ -147,6 +147,27 @@ def test_bounds(m27q, dev):
         p.check("f32", 0.125, **how)
 
 
+LOOSE = [
+    # lens, groups (first, sequences, shared), H, Hk, D, page, type, output; max_len as large as max_kv
+    ([(1, 300), (1, 290), (1, 6000)], [(0, 2, 256)], 6, 2, 256, 64, "f16", "f32"),              # a long one of no group: few rows
+    ([(1, 300), (1, 290), (1, 6000)], [(0, 2, 256), (2, 1, 5952)], 6, 2, 256, 64, "f16", "f32"),  # it is a group by itself
+    ([(1, 5000), (1, 4990), (1, 20), (1, 33)], [(0, 2, 64), (2, 2, 0)], 4, 1, 128, 16, "bf16", "bf16"),  # long behind little
+    ([(5, 400 + i) for i in range(9)] + [(5, 5000)], [(0, 9, 352)], 6, 1, 64, 16, "f16", "f32"),  # many rows
+    ([(1, 40)] * 50 + [(1, 3000)], [(0, 50, 32)], 4, 1, 128, 16, "bf16", "f32"),
+    ([(70, 470), (33, 433), (130, 4030)], [(0, 2, 384)], 2, 1, 64, 16, "f16", "f16"),           # prompts
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,groups,H,Hk,D,page,t,out", LOOSE)
+def test_sequences_longer_than_the_bounds_let_expect(m27q, dev, lens, groups, H, Hk, D, page, t, out):
+    """max_len as large as max_kv, as a step that is captured with the largest bounds has it."""
+    say("shared loose", lens[-2:], groups, H, Hk, D, page, t, out)
+    p = Shared(m27q, dev, lens, groups, H, Hk, D, page, t)
+    p.check(out, D ** -0.5, max_len=p.max_kv)
+    p.check(out, D ** -0.5, max_len=max(1, p.max_kv - 40), length=[0] * len(groups))
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("lens", [[(1, 333), (2, 370)], [(90, 433), (20, 370)]])
 def test_pages_that_are_none(m27q, dev, lens):
