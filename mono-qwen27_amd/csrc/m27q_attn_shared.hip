@@ -135,7 +135,9 @@ SharedPlan shared_plan(const m27q_seqs &seqs, const m27q_prefixes &prefix, uint3
     const long long own = attn_groups(seqs, q_heads, cache);
     const long long shared = prefix.max_len < seqs.max_kv ? prefix.max_len : seqs.max_kv;
     SharedPlan r{};
-    if (!worth_sharing(seqs, prefix, group, cache, shared)) {
+    // (work-items of the join's grid, 256 for 1024 / dim rows, are less than 2^32)
+    const bool joins = (long long)seqs.max_q * q_heads / (1024 / cache.dim) < (1ll << 24) - 1;
+    if (!joins || !worth_sharing(seqs, prefix, group, cache, shared)) {
         const AttnPlan each = attn_plan(seqs, q_heads, cache, cus);
         return {{each.few, 0}, each.splits, 0};
     }

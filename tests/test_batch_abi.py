@@ -82,6 +82,20 @@ def test_own_keys_have_parts_beside_a_prefix(m27q, n, max_q, max_rows, prefix, o
     assert m.lib().m27q_attn_shared_scratch_bytes(ref(s), ref(x), heads, ref(c)) >= (prefix + own) * tokens * heads * (dim * 4 + 8)
 
 
+@pytest.mark.parametrize("dim,tokens", [(256, 1 << 20), (256, (1 << 20) - 64), (64, 1 << 22), (64, (1 << 22) - 64)])
+def test_prefixes_of_more_rows_than_a_join_takes(m27q, dim, tokens):
+    """The join has a workgroup for 1024 / dim rows, of 2^24 workgroups at most: above that each sequence reads all of its
+    keys, in one part (the scratch is the paged attention's)."""
+    m = m27q
+    heads = 64
+    s = seqs(m, n=2, tokens=tokens, max_q=tokens, max_kv=1 << 22, table_stride=1 << 16)
+    c = cache(m, heads=heads, dim=dim, page_size=64, page_stride=heads * 64 * dim, pages=1 << 18)
+    x = m.PrefixesDesc(FAKE, FAKE, 1, tokens, 1 << 21, 0)
+    paged = m.lib().m27q_attn_scratch_bytes(ref(s), heads, ref(c))
+    shared = m.lib().m27q_attn_shared_scratch_bytes(ref(s), ref(x), heads, ref(c))
+    assert paged == 16 and (shared == paged) == (tokens * heads * dim // 1024 >= 1 << 24)
+
+
 def test_sampling_refuses(m27q):
     m = m27q
 
