@@ -9,6 +9,7 @@ import numpy as np
 import pytest
 
 from gpu_util import say
+from test_gpu_sample_rows import SLACK, allowed
 
 D, ROT, PAGE, HIDDEN, VOCAB = 64, 32, 16, 256, 1000
 
@@ -124,6 +125,25 @@ def test_step_beside_the_one_without(m27q, dev, size):
                 assert int(s.token[r]) in near
             else:
                 assert 0 <= int(s.token[r]) < VOCAB and 0 < float(s.prob[r]) <= 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [(9, 160), (40, 4096, 32, 8)])
+def test_tokens_of_a_step_against_the_definition(m27q, dev, size):
+    """Every row's token and share, those without a number of candidates too, from the step's own logits."""
+    import torch
+    say("batch step tokens", size)
+    s = Step(m27q, dev, *size, seed=1)
+    for i in range(3):
+        s.inputs(i)
+        s.run()
+        torch.cuda.synchronize()
+        logits, T, u = s.logits.cpu().numpy(), s.T.cpu().numpy(), s.u.cpu().numpy()
+        for r in range(s.n):
+            ok = allowed(logits[r], T[r], int(s.top_k[r]), np.float32(1), np.float32(0), u[r])
+            token, prob = int(s.token[r]), float(s.prob[r])
+            assert token in ok, (r, token, list(ok)[:4])
+            assert any(abs(prob - p) <= (8 * SLACK + 2.0 ** -24) * p + 2.0 ** -126 for p in ok[token]), (r, prob, ok[token])
 
 
 @pytest.mark.gpu
