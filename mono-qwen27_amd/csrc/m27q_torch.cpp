@@ -54,6 +54,16 @@ void *data(const at::Tensor &t) {
     return t.mutable_data_ptr();
 }
 
+struct Scratch {
+    void *ptr;
+    size_t bytes;
+    explicit Scratch(PyObject *o) {
+        const at::Tensor &t = *tensor(o);
+        ptr = data(t);
+        bytes = t.numel() * t.element_size();
+    }
+};
+
 m27q_rows rows(PyObject *o, int64_t tokens) {
     const at::Tensor &t = *tensor(o);
     if (t.dim() != 3 || t.size(0) != tokens || (t.stride(2) != 1 && t.size(2) != 1) || t.size(1) > 0xffff || t.size(2) > 0xffff)
@@ -115,7 +125,8 @@ struct Args {
         if (v < 0 || v > 0xffffffffll) throw Bad{M27Q_ERR_RANGE};
         return (uint32_t)v;
     }
-    // Last, when all other arguments are known to fit.
+    // Last, when all other arguments are known to fit: in a statement of its own, as a call's arguments are
+    // evaluated in any order, and a tensor that is looked at later is not refused.
     hipStream_t stream(int i) const {
         if (apart || (place != kPinned && place != c10::impl::getDeviceGuardImpl(at::kCUDA)->getDevice().index()))
             throw Bad{kNotHere};
@@ -153,7 +164,9 @@ PyObject *py_rope(PyObject *, PyObject *const *a, Py_ssize_t n) {
         if (tokens > 0x7fffffff) throw Bad{M27Q_ERR_SHAPE};
         const int32_t *pos = int32s(c.a[1], tokens);
         const m27q_rows x = rows(c.a[2], tokens), out = rows(c.a[3], tokens);
-        return m27q_rope(record<m27q_rope_plan>(c.a[0]), pos, (int)tokens, &x, &out, c.stream(4));
+        const m27q_rope_plan *plan = record<m27q_rope_plan>(c.a[0]);
+        const hipStream_t stream = c.stream(4);
+        return m27q_rope(plan, pos, (int)tokens, &x, &out, stream);
     });
 }
 
@@ -164,8 +177,10 @@ PyObject *py_rope_append(PyObject *, PyObject *const *a, Py_ssize_t n) {
         const int64_t t = s->tokens;
         const int32_t *pos = int32s(c.a[1], t);
         const m27q_rows q = rows(c.a[4], t), q_out = rows(c.a[5], t), k = rows(c.a[6], t), v = rows(c.a[7], t);
-        return m27q_rope_append(record<m27q_rope_plan>(c.a[0]), pos, s, record<m27q_cache>(c.a[3]), &q, &q_out, &k, &v,
-                                c.stream(8));
+        const m27q_rope_plan *plan = record<m27q_rope_plan>(c.a[0]);
+        const m27q_cache *cache = record<m27q_cache>(c.a[3]);
+        const hipStream_t stream = c.stream(8);
+        return m27q_rope_append(plan, pos, s, cache, &q, &q_out, &k, &v, stream);
     });
 }
 
@@ -174,11 +189,13 @@ PyObject *py_attn_paged(PyObject *, PyObject *const *a, Py_ssize_t n) {
     return call(a, n, 8, [](Args c) {
         const m27q_seqs *s = record<m27q_seqs>(c.a[0]);
         const m27q_rows q = rows(c.a[2], s->tokens), out = rows(c.a[3], s->tokens);
-        const at::Tensor &scratch = *tensor(c.a[4]);
+        const m27q_cache *cache = record<m27q_cache>(c.a[1]);
+        const Scratch scratch(c.a[4]);
+        const float scale = (float)c.real(5);
         const long long window = c.whole(6);
         if (window > 0x7fffffff || window < 0) throw Bad{M27Q_ERR_RANGE};
-        return m27q_attn_paged(s, record<m27q_cache>(c.a[1]), &q, &out, (float)c.real(5), (int)window, data(scratch),
-                               scratch.numel() * scratch.element_size(), c.stream(7));
+        const hipStream_t stream = c.stream(7);
+        return m27q_attn_paged(s, cache, &q, &out, scale, (int)window, scratch.ptr, scratch.bytes, stream);
     });
 }
 
@@ -188,9 +205,11 @@ PyObject *py_attn_shared(PyObject *, PyObject *const *a, Py_ssize_t n) {
         const m27q_seqs *s = record<m27q_seqs>(c.a[0]);
         const m27q_prefixes *x = record<m27q_prefixes>(c.a[1]);
         const m27q_rows q = rows(c.a[3], s->tokens), out = rows(c.a[4], s->tokens);
-        const at::Tensor &scratch = *tensor(c.a[5]);
-        return m27q_attn_shared(s, x, record<m27q_cache>(c.a[2]), &q, &out, (float)c.real(6), data(scratch),
-                                scratch.numel() * scratch.element_size(), c.stream(7));
+        const m27q_cache *cache = record<m27q_cache>(c.a[2]);
+        const Scratch scratch(c.a[5]);
+        const float scale = (float)c.real(6);
+        const hipStream_t stream = c.stream(7);
+        return m27q_attn_shared(s, x, cache, &q, &out, scale, scratch.ptr, scratch.bytes, stream);
     });
 }
 
@@ -211,8 +230,10 @@ PyObject *py_rms_norm(PyObject *, PyObject *const *a, Py_ssize_t n) {
                 throw Bad{M27Q_ERR_SHAPE};
             xq = data(*act);
         }
-        return m27q_rms_norm(&x, add.ptr ? &add : nullptr, (int)tokens, weight, (float)c.real(3), sum.ptr ? &sum : nullptr,
-                             out.ptr ? &out : nullptr, xq, c.stream(9));
+        const float eps = (float)c.real(3);
+        const hipStream_t stream = c.stream(9);
+        return m27q_rms_norm(&x, add.ptr ? &add : nullptr, (int)tokens, weight, eps, sum.ptr ? &sum : nullptr,
+                             out.ptr ? &out : nullptr, xq, stream);
     });
 }
 
@@ -236,8 +257,9 @@ PyObject *py_sample_rows(PyObject *, PyObject *const *a, Py_ssize_t n) {
         s.top_p = floats(c.a[6], rows, true);
         s.min_p = floats(c.a[7], rows, true);
         s.prob = floats(c.a[8], rows, true);
-        const at::Tensor &scratch = *tensor(c.a[3]);
-        return m27q_sample_rows(&s, data(scratch), scratch.numel() * scratch.element_size(), c.stream(9));
+        const Scratch scratch(c.a[3]);
+        const hipStream_t stream = c.stream(9);
+        return m27q_sample_rows(&s, scratch.ptr, scratch.bytes, stream);
     });
 }
 
@@ -271,8 +293,9 @@ PyObject *py_delta_rule(PyObject *, PyObject *const *a, Py_ssize_t n) {
         d.scale = (float)c.real(10);
         d.max_len = c.u32(11);
         d.head_map = c.u32(13);
-        const at::Tensor &scratch = *tensor(c.a[9]);
-        return m27q_delta_rule(&d, data(scratch), scratch.numel() * scratch.element_size(), c.stream(14));
+        const Scratch scratch(c.a[9]);
+        const hipStream_t stream = c.stream(14);
+        return m27q_delta_rule(&d, scratch.ptr, scratch.bytes, stream);
     });
 }
 
