@@ -127,12 +127,13 @@ constexpr int kReach = kFine + kUnit * kCoarse;  // units down to where weights 
 struct Scale {
     double c;       // units of a logit
     double anchor;
-    bool wide;      // distances from the anchor are not whole numbers of 2^26 at most, or T is infinite
+    bool wide;      // distances from the anchor are not whole numbers of 2^26 at most, T is infinite, or a step of the
+                    // smallest logits is no small part of a unit
 };
 __device__ __forceinline__ Scale row_scale(const Rule &r, double anchor) {
     const double far = fabs(anchor) + kReach;
     const double c = kUnitsPerNat * r.inv_t;
-    return {c, anchor, __builtin_amdgcn_readfirstlane(!(far < 0x1p26) || !(c > 0.0)) != 0};
+    return {c, anchor, __builtin_amdgcn_readfirstlane(!(far < 0x1p26) || !(c > 0.0) || c > 0x1p140) != 0};
 }
 
 // A logit in whole units, and what is left over: of the exact product, rounded once, whatever anchor it is
@@ -302,7 +303,8 @@ __global__ __launch_bounds__(kPartThreads) void k_sample_parts(const m27q_sampli
             }
         } else {
             // the same without branches, several tokens' chains beside each other.  A logit above this one is
-            // less than 16 units past the last bin: what is further down, -infinity and NaN are left out by it.
+            // less than 16 units past the last bin (rounded to a float it is off by 4 units at most, 2^-24 of 2^26
+            // or, among the smallest, c 2^-150): what is further down, -infinity and NaN are left out by it.
             const float least = fmaxf((float)((s.anchor - (kReach + kUnit / 2)) / s.c), -0x1.fffffep+127f);
             const double low = s.anchor + 0x1.8p52;
             constexpr int AT = 4;

@@ -285,6 +285,26 @@ def test_temperatures_near_0(m27q, dev, T):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("top", [0, 1, 2, 5])
+@pytest.mark.parametrize("T", [1, 2, 3, 40])
+def test_smallest_logits_and_temperatures(m27q, dev, T, top):
+    """Logits and temperatures of a few times the smallest number of 32 bits: most of a row's tokens stand around the end of
+    its bins, where a step of the logits is more than an octave."""
+    say("sample smallest", T, top)
+    rng = np.random.default_rng(T)
+    tiny = np.float32(2.0 ** -149)
+    x = np.empty((4, 20000), np.float32)
+    x[0] = (-rng.integers(100, 108, 20000) * T) * tiny
+    x[1] = (-rng.integers(0, 120, 20000) * T) * tiny
+    x[2] = (top - 105 * T) * tiny
+    x[3] = top * tiny
+    x[:, 9000] = top * tiny
+    for k, top_p, min_p in ((0, 1.0, 0.0), (0, 0.9, 0.0), (50, 1.0, 0.0), (0, 1.0, 0.1)):
+        for u in (0.0, 0.5, 0.999):
+            check(m27q, dev, x, T * tiny, k, top_p, min_p, u)
+
+
+@pytest.mark.gpu
 def test_agrees_with_sampling_of_candidates(m27q, ora, dev):
     """m27q_topk and m27q_sample give the same tokens where u is not beside a border (they sum in 32 bits)."""
     import torch
