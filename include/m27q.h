@@ -468,8 +468,8 @@ M27Q_API m27q_status m27q_attn_paged(const m27q_seqs *seqs, const m27q_cache *ca
                                      size_t scratch_bytes, hipStream_t stream);
 
 /* Groups of sequences that share a prefix: group g is the sequences first[g] ..
- * first[g + 1] - 1 of a call, whose places 0 .. len[g] - 1 hold the same tokens,
- * in pages that all of them name.  first does not descend and stays within
+ * first[g + 1] - 1 of a call, whose places 0 .. len[g] - 1, where they have them, hold the
+ * same tokens in pages that all of them name.  first does not descend and stays within
  * 0 .. n; a sequence before first[0] or from first[groups] on shares nothing.
  * Bounds of the launch: a group has at most max_rows rows, from the first of its
  * first sequence to the last of its last one (rows past them may be left as they are),
@@ -485,12 +485,14 @@ typedef struct m27q_prefixes {
 
 /* m27q_attn_paged without a window, for a batch whose sequences share long
  * prefixes: a prefix's keys and values are read once for all rows of its group,
- * through the page table of the group's first sequence.  Only whole tiles of 32
+ * through the page table of the group's sequence with most tokens (of those with rows in
+ * the call; the first of equal ones).  Only whole tiles of 32
  * places are taken so; the rest of a sequence's places come from its own table.
  * Where that saves nothing (by the bounds and the numbers of sequences and heads), all
- * places do.  The tables of a group name the same pages for its prefix: the results
- * are those of m27q_attn_paged, to the order of sums.  (Where they do not, which one is
- * read is not said.)  A len past a sequence's own tokens is fine: rows see what lies at or
+ * places do.  The tables of a group name the same pages for as much of its prefix as a
+ * sequence with rows has of it: the results are those of m27q_attn_paged, to the order of
+ * sums.  (Where they do not, which one is read is not said.)  A len past a sequence's own
+ * tokens is fine, and so is a sequence without rows: rows see what lies at or
  * before their own place.  scratch as in m27q_attn_paged, by its own size. */
 M27Q_API size_t m27q_attn_shared_scratch_bytes(const m27q_seqs *seqs, const m27q_prefixes *prefix, uint32_t q_heads,
                                                const m27q_cache *cache);

@@ -164,32 +164,40 @@ __device__ __forceinline__ Unit unit_rows(const AttnParams &p, int u) {
     return x;
 }
 
-// The lowest and the highest place of a group's rows (a workgroup's threads a sequence each).
-__device__ __forceinline__ int2 group_places(const AttnParams &p, const Unit &x, int *lds) {
-    int lo = 0x7ffffffe, hi = -1;
+// The lowest and the highest place of a group's rows (a workgroup's threads a sequence each), and whose page table
+// is read for the prefix: that of the sequence with most tokens among those that have rows, the first of equal ones, for a
+// sequence whose tokens end within the prefix, or that has left the batch, need not name its pages.
+__device__ __forceinline__ int2 group_places(const AttnParams &p, Unit &x, int *lds) {
+    int lo = 0x7ffffffe, hi = -1, most = 0, at_s = x.s;
     for (int s = x.s0 + (int)threadIdx.x; s < x.s1; s += (int)blockDim.x) {
         const SeqRows r = seq_rows(p.seqs.start, s, (int)p.seqs.tokens, (int)p.seqs.max_q);
         if (r.count == 0) continue;
-        const int at = max(p.seqs.kv_len[s], 0) - (r.end - r.first);
+        const int len = max(p.seqs.kv_len[s], 0), at = len - (r.end - r.first);
         lo = min(lo, at);
         hi = max(hi, at + r.count - 1);
+        at_s = len > most ? s : at_s;
+        most = max(most, len);
     }
 #pragma unroll
     for (int o = 32; o; o >>= 1) {
         lo = min(lo, __shfl_xor(lo, o));
         hi = max(hi, __shfl_xor(hi, o));
+        const int len = __shfl_xor(most, o), s = __shfl_xor(at_s, o);
+        at_s = len > most || (len == most && s < at_s) ? s : at_s;
+        most = max(most, len);
     }
     const int wave = threadIdx.x >> 6;
-    if ((threadIdx.x & 63) == 0) {
-        lds[2 * wave] = lo;
-        lds[2 * wave + 1] = hi;
-    }
+    if ((threadIdx.x & 63) == 0) *(int4 *)(lds + 4 * wave) = make_int4(lo, hi, most, at_s);
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        lo = min(lo, lds[2 * i]);
-        hi = max(hi, lds[2 * i + 1]);
+        const int4 v = *(const int4 *)(lds + 4 * i);
+        lo = min(lo, v.x);
+        hi = max(hi, v.y);
+        at_s = v.z > most || (v.z == most && v.w < at_s) ? v.w : at_s;
+        most = max(most, v.z);
     }
+    x.s = __builtin_amdgcn_readfirstlane(at_s);
     return make_int2(__builtin_amdgcn_readfirstlane(lo), __builtin_amdgcn_readfirstlane(hi));
 }
 // The place of one of a group's rows.
@@ -619,7 +627,7 @@ __device__ __forceinline__ void attn_many(const AttnParams &p, unsigned bx, unsi
     const int s = pair / p.cache.heads;
     Work w;
     w.head = pair - s * p.cache.heads;
-    const Unit sr = unit_rows<KIND>(p, s);
+    Unit sr = unit_rows<KIND>(p, s);
     w.s = sr.s;
     w.rows = sr.count * group;
     w.row0 = (int)(nx / pairs - 1 - fromlast) * kWaves * kRows;
@@ -631,6 +639,7 @@ __device__ __forceinline__ void attn_many(const AttnParams &p, unsigned bx, unsi
         const int2 at = group_places(p, sr, (int *)(char *)ka);
         first = at.x;
         last = at.y;
+        w.s = sr.s;
         __syncthreads();
     }
     set_keys<KIND>(p, w, len, sr.shared, first, last, (int)part_id);
@@ -805,7 +814,7 @@ __device__ __forceinline__ void attn_few(const AttnParams &p, unsigned bx, unsig
     const int s = bx / p.cache.heads;
     Work w;
     w.head = bx - s * p.cache.heads;
-    const Unit sr = unit_rows<KIND>(p, s);
+    Unit sr = unit_rows<KIND>(p, s);
     w.s = sr.s;
     w.rows = sr.count * group;
     if (w.rows == 0) return;
@@ -815,6 +824,7 @@ __device__ __forceinline__ void attn_few(const AttnParams &p, unsigned bx, unsig
         const int2 at = group_places(p, sr, (int *)kts);
         first = at.x;
         last = at.y;
+        w.s = sr.s;
         __syncthreads();
     }
     set_keys<KIND>(p, w, len, sr.shared, first, last, (int)by);

@@ -147,6 +147,22 @@ def test_bounds(m27q, dev):
         p.check("f32", 0.125, **how)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,n,H,Hk,D,page", [
+    ([(0, 2100), (1, 40)] + [(1, 2100 + 9 * i) for i in range(11)], 2048, 2, 2, 128, 64),  # few rows
+    ([(0, 1040), (1, 0), (5, 20)] + [(5, 1030 + i) for i in range(9)], 1024, 2, 2, 128, 32),
+    ([(0, 450), (60, 65), (90, 430), (20, 400)], 256, 6, 2, 64, 16)])
+def test_tables_that_end_within_the_prefix(m27q, dev, lens, n, H, Hk, D, page):
+    """A group's first sequence has left the batch, the next one's tokens end within the prefix: their tables name no page
+    that is not theirs."""
+    say("shared short tables", lens[:4])
+    p = Shared(m27q, dev, lens, [(0, len(lens), n)], H, Hk, D, page)
+    for s, (a, m) in enumerate(lens):
+        p.table[s, -(-m // page) if a else 0:] = -1
+    p.check("f32", 0.125)
+    assert p.apart
+
+
 LOOSE = [
     # lens, groups (first, sequences, shared), H, Hk, D, page, type, output; max_len as large as max_kv
     ([(1, 300), (1, 290), (1, 6000)], [(0, 2, 256)], 6, 2, 256, 64, "f16", "f32"),              # a long one of no group: few rows
