@@ -59,6 +59,7 @@ struct Scratch {
     size_t bytes;
     explicit Scratch(PyObject *o) {
         const at::Tensor &t = *tensor(o);
+        if (!t.is_contiguous()) throw Bad{M27Q_ERR_LAYOUT};  // its elements need not be as many bytes of memory
         ptr = data(t);
         bytes = t.numel() * t.element_size();
     }
@@ -225,6 +226,7 @@ PyObject *py_rms_norm(PyObject *, PyObject *const *a, Py_ssize_t n) {
         void *xq = nullptr;
         if (const at::Tensor *act = tensor(c.a[6], true)) {
             const long long M = c.whole(7), K = c.whole(8);
+            if (!act->is_contiguous()) throw Bad{M27Q_ERR_LAYOUT};
             if (M != tokens || K != (long long)x.heads * x.dim || M > 0xffff + 1 || K > (1 << 20) ||
                 (size_t)(act->numel() * act->element_size()) < m27q_act_bytes((int)M, (int)K))
                 throw Bad{M27Q_ERR_SHAPE};

@@ -158,3 +158,24 @@ def test_binding_refuses_tensors_that_do_not_fit(m27q, calls):
         m27q.Prefixes(torch.zeros(2, dtype=torch.int32), torch.zeros(2, dtype=torch.int32), 1, 1)
     with pytest.raises(m27q.M27QError):
         m27q.Prefixes(torch.zeros(2, dtype=torch.int64), torch.zeros(1, dtype=torch.int32), 1, 1)
+
+
+@pytest.mark.parametrize("name", ["attn_paged", "attn_shared", "sample_rows", "delta_rule", "rms_norm"])
+def test_binding_refuses_scratch_of_less_memory_than_elements(m27q, calls, name):
+    """Expanded tensors: a million elements in one byte of memory."""
+    import torch
+    m = m27q
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+    little = torch.zeros(1, dtype=torch.uint8).expand(1 << 20)
+    pages = torch.zeros(4, 2, 16, 64, dtype=torch.float16)
+    s, cache, q = m.Seqs(i32(0, 1, 2), i32(5, 6), i32(1, 2, 1, 3).view(2, 2), 2, 1, 20), m.KVCache(pages, pages), torch.zeros(2, 4, 64).half()
+    x, g, act = torch.zeros(2, 2, 64), torch.zeros(2, 2), m.Act(2, 64, "cpu")
+    act.buf = little
+    call = {"attn_paged": lambda: m.attn_paged(s, cache, q, q.clone(), little, 0.1),
+            "attn_shared": lambda: m.attn_shared(s, m.Prefixes(i32(0, 2), i32(16), 2, 16), cache, q, q.clone(), little, 0.1),
+            "sample_rows": lambda: calls["m27q_sample_rows"](scratch=little),
+            "delta_rule": lambda: m.delta_rule(i32(0, 2), x, x, x, g, g, torch.zeros(1, 2, 64, 64), None, x.clone(), little, 1.0, 2, slots=i32(0)),
+            "rms_norm": lambda: m.rms_norm(torch.zeros(2, 64), act=act)}[name]
+    with pytest.raises(m.M27QError) as e:
+        call()
+    assert e.value.status == LAYOUT and "current GPU" not in str(e.value)
