@@ -491,7 +491,8 @@ typedef struct m27q_prefixes {
  * Where that saves nothing (by the bounds and the numbers of sequences and heads), all
  * places do.  The tables of a group name the same pages for as much of its prefix as a
  * sequence with rows has of it: the results are those of m27q_attn_paged, to the order of
- * sums.  (Where they do not, which one is read is not said.)  A len past a sequence's own
+ * sums, and its weights are rounded as there, by the type of out.  (Where they do not, which one
+ * is read is not said.)  A len past a sequence's own
  * tokens is fine, and so is a sequence without rows: rows see what lies at or
  * before their own place.  scratch as in m27q_attn_paged, by its own size. */
 M27Q_API size_t m27q_attn_shared_scratch_bytes(const m27q_seqs *seqs, const m27q_prefixes *prefix, uint32_t q_heads,
@@ -577,6 +578,7 @@ M27Q_API m27q_status m27q_rms_norm(const m27q_rows *x, const m27q_rows *add, int
  * -infinity (weight 0 at any temperature).  Weights are computed in 64 bits (2^-36 of their size at most is
  * rounded off) and summed as integers: the same row gives the same token in any
  * batch.  rows up to 65535, n up to 2^24.
+ * For one row with at most 64 candidates m27q_topk and m27q_sample are the faster way.
  * scratch (16-byte aligned) >= m27q_sample_rows_scratch_bytes, what it holds is
  * of no matter. */
 typedef struct m27q_sampling {

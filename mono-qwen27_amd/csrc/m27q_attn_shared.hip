@@ -11,9 +11,11 @@ long long tiles_of(long long rows) { return (rows + kWaves * kRows - 1) / (kWave
 
 // A prefix of many rows and all sequences' own keys in one launch: the prefix's workgroups, bound by the matrix
 // units, come first, one on each CU, and beside them those of the own keys, bound by memory.  64 tokens behind
-// 32768 places and up to 1021 own ones, 24 heads of 256 on 4, F16 to F32: 122 us and 9 of joining, of 62 for
-// the bytes (304 MB) and 63 for the products; 8 prompts of 301 tokens behind 8192, BF16: 449 us with 33 of joining,
-// 0.9 PFLOP/s of the pairs that count.
+// 32768 places and up to 1021 own ones, 24 heads of 256 on 4, F16 to F32: 117 to 126 us with 9 of joining, where
+// 43 would do for the bytes (304 MB at a plain read's 7.15 TB/s) and 59 for the products (the second one in two pieces);
+// BF16 to F32, in three pieces, 165 (the paged attention 465), BF16 103 (418); 8 prompts of up to 301 tokens behind
+// 8192, BF16: 437 to 447 with 33 of joining, 0.85 PFLOP/s of the pairs that count.  Heads of 256 take all 256 registers:
+// BF16 to F32 spills 19 (64 bytes a lane), the others one.
 template <int D, bool BF, int NP>
 __global__ __launch_bounds__(kWaves * 64, 2) void k_attn_both(const AttnParams p, unsigned px, unsigned prefix, unsigned ox) {
     if (blockIdx.x < prefix) {

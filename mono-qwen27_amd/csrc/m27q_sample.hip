@@ -18,12 +18,13 @@
 // Where the list would be too long (flat rows, thousands of equal logits at a border), pick reads the whole
 // row once or twice more for each border, by pieces of its bin's keys.
 //
-// 200 rows of 248320 F32, top-p (199 MB): 92 us, of these 50 for parts, 8, 26 for list (7.6 TB/s:
-// what parts read last still lies in the caches) and 10.  parts is bound by the vector units: some 30 operations
-// of a wave for each 64 tokens, half of them on 64 bits, and the LDS additions beside them (a
-// plain read of the same bytes: 29).  64 rows of all rules 46 us (19, 8.5, 12, 8); one row
-// 23: four launches of 5.3, 8.1, 5.3 and 6, each the latency of its steps.  64 rows of normal logits
-// (deviation 2.2) at temperature 2 or 5 with top-p, 10000 tokens a bin, 200 and 229 (342 and 402 where tokens near a border
+// 200 rows of 248320 F32, top-p (199 MB): 92 to 103 us from card to card, of these 50 to 52 for parts, 8, 25 for
+// list (7.8 TB/s: what parts read last still lies in the caches) and 10.  parts is bound by the vector units: some 30
+// operations of a wave for each 64 tokens, half of them on 64 bits, and the LDS additions beside them (a
+// plain read of the same bytes: 28).  64 rows of all rules 45 to 48 us (19, 8.5, 12, 8); one row
+// 23 to 24: four launches of 5.3, 8, 5.3 and 6, each the latency of its steps (the 40 largest and the choice among them,
+// m27q_topk and m27q_sample, take 14).  64 rows of normal logits
+// (deviation 2.2) at temperature 2 or 5 with top-p, 10000 tokens a bin, 197 and 228 (342 and 402 where tokens near a border
 // do not wait until they fill a wave, 850 and 890 by 11 bits of all keys at a time, 2100 and 2890 by 8); equal logits
 // throughout 1070 without cuts, up to 3200 with all.
 #include "m27q_device.h"
